@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define MIMIR_PREFIXLM_ABI_VERSION 8
+#define MIMIR_PREFIXLM_ABI_VERSION 9
 
 /* Element types of q/k/v/out/dout/dq/dk/dv (lse and the workspace are float32). */
 enum MimirDType {
@@ -400,6 +400,169 @@ typedef struct MimirCacheAttnParams {
 } MimirCacheAttnParams;
 size_t mimir_prefixlm_cache_attn_workspace_bytes(const MimirCacheAttnParams* params);
 int mimir_prefixlm_cache_attn(const MimirCacheAttnParams* params, void* stream);
+
+/* Rotary positions from token positions and a frequency table: of each head of
+ * q [B, S, Hq, D] and (num_kv_heads > 0) k [B, S, Hkv, D], the pairs of the first
+ * rotary_dim columns are turned by the token's position times the pair's frequency,
+ *
+ *     a' = amplitude (a cos t - b sin t),  b' = amplitude (b cos t + a sin t),
+ *     t = 2 pi frac(positions[b, i] * turns[pair] / 2^64),
+ *
+ * in fp32 with one rounding; the other columns are copied.  Pair i is columns
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`.  inverse = 1 turns
+ * the other way (t -> -t): the gradient's map.  head_dim and rotary_dim even; each
+ * output may be its input (same pointer and strides).  Strides in elements. */
+typedef struct MimirRotaryParams {
+  const void* q;
+  const void* k;              /* NULL if num_kv_heads is 0 */
+  void* q_out;
+  void* k_out;
+  const int64_t* turns;       /* [rotary_dim / 2]: turn per position, in units of 2^-64 */
+  const void* positions;      /* device int32 or int64 (index_int64), by its strides [B, S] */
+  int64_t q_stride_batch, q_stride_token, q_stride_head;
+  int64_t k_stride_batch, k_stride_token, k_stride_head;
+  int64_t q_out_stride_batch, q_out_stride_token, q_out_stride_head;
+  int64_t k_out_stride_batch, k_out_stride_token, k_out_stride_head;
+  int64_t positions_stride_batch, positions_stride_token;
+  int32_t batch;              /* B */
+  int32_t seqlen;             /* S */
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;           /* D */
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t dtype;              /* enum MimirDType */
+  int32_t inverse;
+  int32_t index_int64;
+  float amplitude;
+} MimirRotaryParams;
+int mimir_prefixlm_rotary(const MimirRotaryParams* params, void* stream);
+
+/* Attention over a KV cache in pages of MIMIR_PAGE_TOKENS tokens, held in 8 bits (e4m3)
+ * under one power-of-two scale for each page and kv head.
+ *
+ *   cache_k      e4m3 [page][Hkv][64][D],  key   = code * 2^k_exponents[page][head]
+ *   cache_v      e4m3 [page][Hkv][D][64],  value = code * 2^v_exponents[page][head]
+ *   exponents    int8 [page][Hkv], in [-100, 120]
+ *
+ * with a stride between pages each (so that the layers of a model can lie side by side in
+ * a page).  Token t of batch row b lies in page page_table[row][t / 64], slot t % 64, where
+ * row = batch_indices ? batch_indices[b] : b.  With c = cache_lengths[b] and
+ * m = new_lengths ? new_lengths[b] : S:
+ *
+ *   1. k_new / v_new [b, i], i < m, are appended at tokens c + i.  Every page and head they
+ *      fall in takes the smallest exponent e >= -100 with |x| <= 448 * 2^e for its new
+ *      (finite) values, but not less than the one it has if it holds older tokens, whose
+ *      codes are rounded again where e grew.  Codes round to nearest even; infinite
+ *      values become NaN (e4m3 has no infinity).  Slots behind the row's last token keep
+ *      their codes.
+ *   2. query i < m of q [b, i, h] attends the tokens t < c + m of kv head h / (Hq / Hkv), and
+ *      if `causal` only t <= c + i; bf16 out [b, i, h].  Queries i >= m give zeros, and so do
+ *      those that see no token.
+ *
+ * Tokens past the table (t / 64 >= table_width) and pages outside [0, num_pages) are neither
+ * written nor attended; a batch row whose table row lies outside [0, table_rows), or whose
+ * length is negative, gives zeros.  No two batch rows of a call may append to one page.
+ * q, k_new, v_new and out are bf16 rows, 16-byte aligned, strides in elements; head_dim 64
+ * or 128.  The workspace holds partial results of split key ranges (nothing to clear: the
+ * call can be captured in a graph). */
+#define MIMIR_PAGE_TOKENS 64
+typedef struct MimirPagedAttnParams {
+  const void* q;              /* [B, S, Hq, D] */
+  const void* k_new;          /* [B, S, Hkv, D] */
+  const void* v_new;          /* [B, S, Hkv, D] */
+  void* out;                  /* [B, S, Hq, D] */
+  void* cache_k;
+  void* cache_v;
+  int8_t* k_exponents;
+  int8_t* v_exponents;
+  const int32_t* page_table;  /* [table_rows, table_width] */
+  const void* cache_lengths;  /* device int32 or int64 [B] (index_int64, as the next two) */
+  const void* batch_indices;  /* [B], or NULL (row b) */
+  const void* new_lengths;    /* [B], or NULL (S) */
+  int64_t q_stride_batch, q_stride_token, q_stride_head;
+  int64_t kn_stride_batch, kn_stride_token, kn_stride_head;
+  int64_t vn_stride_batch, vn_stride_token, vn_stride_head;
+  int64_t out_stride_batch, out_stride_token, out_stride_head;
+  int64_t k_stride_page, v_stride_page;      /* bytes */
+  int64_t ke_stride_page, ve_stride_page;    /* bytes */
+  int64_t table_stride;       /* int32 between rows of page_table */
+  int32_t batch;              /* B */
+  int32_t seqlen;             /* S */
+  int32_t num_pages;
+  int32_t table_rows;
+  int32_t table_width;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t causal;
+  int32_t dtype;              /* of q, k_new, v_new and out: MIMIR_DTYPE_BFLOAT16 */
+  int32_t index_int64;
+  float softmax_scale;
+  void* workspace;            /* >= mimir_prefixlm_paged_attn_workspace_bytes(params) */
+  size_t workspace_bytes;
+} MimirPagedAttnParams;
+size_t mimir_prefixlm_paged_attn_workspace_bytes(const MimirPagedAttnParams* params);
+int mimir_prefixlm_paged_attn(const MimirPagedAttnParams* params, void* stream);
+
+/* The rows of a paged cache and the pages they hold.
+ *
+ *   pages    int32 [rows][width]: the page of each run of 64 tokens, -1 where none
+ *   lengths  int32 [rows]: tokens held
+ *   counts   int32 [num_pages]: table entries that name the page (0: free)
+ *   missing  int32 [1]: pages asked for that the pool did not have, added up
+ *
+ * and the pool's four arrays, page by page (for the calls that move data): `bytes` per
+ * page each, a multiple of 16 for keys and values.  Entries outside [0, num_pages) are
+ * taken for none.  Pages are handed out lowest first, so results do not depend on
+ * timing.  Every call works on the device alone, without a host synchronisation.
+ *
+ * `workspace`: mimir_prefixlm_pages_workspace_bytes(params, items) bytes. */
+typedef struct MimirPagesParams {
+  int32_t* pages;
+  int32_t* lengths;
+  int32_t* counts;
+  int32_t* missing;
+  int64_t pages_stride;       /* int32 between rows of pages */
+  int32_t rows;
+  int32_t width;
+  int32_t num_pages;
+  void* data[4];              /* keys, values, key exponents, value exponents: page 0 */
+  int64_t data_bytes[4];      /* of a page */
+  int64_t data_stride[4];     /* bytes between pages */
+  void* workspace;
+  size_t workspace_bytes;
+} MimirPagesParams;
+size_t mimir_prefixlm_pages_workspace_bytes(const MimirPagesParams* params, int32_t items);
+
+/* Page destination[i] of the pool becomes a copy of page source[i], i < n.  Entries outside
+ * the pool are skipped; no destination may be named twice or be a source.  Uses the data
+ * fields and num_pages. */
+int mimir_prefixlm_pages_copy(const MimirPagesParams* params, const int32_t* source, const int32_t* destination,
+                              int32_t n, void* stream);
+
+/* Row destination[i] goes on from what row source[i] held before the call: it gives back its
+ * own pages, shares the full pages of the source and gets a copy of the source's last,
+ * partly filled page in a free one.  A source that is itself replaced by another row leaves
+ * that page to the first row (lowest i) that goes on from it, if no other row holds it.
+ * Entries with source = destination leave the row alone, entries outside the table are
+ * skipped, and of entries with one destination the last counts.  Where the pool has no
+ * free page the last page stays -1 and `missing` counts it. */
+int mimir_prefixlm_pages_fork(const MimirPagesParams* params, const int32_t* source, const int32_t* destination,
+                              int32_t n, void* stream);
+
+/* Moves the pages in use (counts > 0) to the front of the pool: those at or past their
+ * number, in ascending order, into the free pages before it, in ascending order; counts and
+ * pages follow.  used[0] (device) = their number. */
+int mimir_prefixlm_pages_compact(const MimirPagesParams* params, int32_t* used, void* stream);
+
+/* The listed rows (row_list int32 [n]; those outside the table are skipped, one may come
+ * twice) give back their pages and hold no tokens. */
+int mimir_prefixlm_pages_release(const MimirPagesParams* params, const int32_t* row_list, int32_t n, void* stream);
+
+/* Gives every row r with new_lengths[r] > 0 (int32 [rows]) the pages it lacks for
+ * lengths[r] + new_lengths[r] tokens, by row, then place; lengths stay. */
+int mimir_prefixlm_pages_reserve(const MimirPagesParams* params, const int32_t* new_lengths, void* stream);
 
 /* Device-side metadata check: writes to bad[0] (device int32 [2]) the first s in
  * [0, numseqs) whose lengths are invalid, or -1 if none, and to bad[1] why:

@@ -5,6 +5,10 @@ Drop-in replacement for ``mimir.model.layers.flash_attn_varlen_prefixlm``
 HIP kernels behind a C ABI (include/mimir_prefixlm.h), and the attention
 layer's core around it (``gated_attention``: gqkv split, RoPE, the operator and
 the sigmoid output gate of src/mimir/model/layers.py:182-239).
+
+Submodules for serving: ``mimir_amd.cache`` (attention against a static bf16 cache),
+``mimir_amd.paged`` (the same against 8-bit pages, and their bookkeeping) and
+``mimir_amd.rotary`` (rotary positions without tables, for training too).
 """
 
 from .metadata import (

@@ -21,7 +21,7 @@ from pathlib import Path
 # MIMIR_PREFIXLM_LIB overrides the in-tree library (e.g. to A/B two builds).
 LIB_PATH = Path(os.environ.get("MIMIR_PREFIXLM_LIB") or Path(__file__).resolve().parent / "_lib" / "libmimir_prefixlm.so")
 HOST_PATH = Path(__file__).resolve().parent / "_lib" / "_host_calls.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 DTYPE_FLOAT32 = 0
 DTYPE_BFLOAT16 = 1
@@ -118,6 +118,49 @@ class CacheAttnParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("turns", _vp), ("positions", _vp),
+        ("q_stride_batch", _i64), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("k_stride_batch", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("q_out_stride_batch", _i64), ("q_out_stride_token", _i64), ("q_out_stride_head", _i64),
+        ("k_out_stride_batch", _i64), ("k_out_stride_token", _i64), ("k_out_stride_head", _i64),
+        ("positions_stride_batch", _i64), ("positions_stride_token", _i64),
+        ("batch", _i32), ("seqlen", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("interleaved", _i32), ("dtype", _i32), ("inverse", _i32), ("index_int64", _i32),
+        ("amplitude", ctypes.c_float),
+    ]
+
+
+class PagedAttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k_new", _vp), ("v_new", _vp), ("out", _vp),
+        ("cache_k", _vp), ("cache_v", _vp), ("k_exponents", _vp), ("v_exponents", _vp),
+        ("page_table", _vp), ("cache_lengths", _vp), ("batch_indices", _vp), ("new_lengths", _vp),
+        ("q_stride_batch", _i64), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("kn_stride_batch", _i64), ("kn_stride_token", _i64), ("kn_stride_head", _i64),
+        ("vn_stride_batch", _i64), ("vn_stride_token", _i64), ("vn_stride_head", _i64),
+        ("out_stride_batch", _i64), ("out_stride_token", _i64), ("out_stride_head", _i64),
+        ("k_stride_page", _i64), ("v_stride_page", _i64), ("ke_stride_page", _i64), ("ve_stride_page", _i64),
+        ("table_stride", _i64),
+        ("batch", _i32), ("seqlen", _i32), ("num_pages", _i32), ("table_rows", _i32), ("table_width", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("causal", _i32), ("dtype", _i32),
+        ("index_int64", _i32), ("softmax_scale", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagesParams(ctypes.Structure):
+    _fields_ = [
+        ("pages", _vp), ("lengths", _vp), ("counts", _vp), ("missing", _vp), ("pages_stride", _i64),
+        ("rows", _i32), ("width", _i32), ("num_pages", _i32),
+        ("data", _vp * 4), ("data_bytes", _i64 * 4), ("data_stride", _i64 * 4),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+PAGE_TOKENS = 64  # MIMIR_PAGE_TOKENS
+
 BWD_STAGE_DELTA = 1
 BWD_STAGE_DKDV = 2
 BWD_STAGE_DQ = 4
@@ -137,6 +180,15 @@ EXPORTED_SYMBOLS = (
     "mimir_prefixlm_rope",
     "mimir_prefixlm_cache_attn",
     "mimir_prefixlm_cache_attn_workspace_bytes",
+    "mimir_prefixlm_rotary",
+    "mimir_prefixlm_paged_attn",
+    "mimir_prefixlm_paged_attn_workspace_bytes",
+    "mimir_prefixlm_pages_workspace_bytes",
+    "mimir_prefixlm_pages_copy",
+    "mimir_prefixlm_pages_fork",
+    "mimir_prefixlm_pages_compact",
+    "mimir_prefixlm_pages_release",
+    "mimir_prefixlm_pages_reserve",
     "mimir_prefixlm_check_metadata",
     "mimir_prefixlm_last_error",
     "mimir_prefixlm_abi_version",
@@ -188,6 +240,25 @@ def load() -> ctypes.CDLL:
         lib.mimir_prefixlm_cache_attn.restype = ctypes.c_int
         lib.mimir_prefixlm_cache_attn_workspace_bytes.argtypes = [ctypes.POINTER(CacheAttnParams)]
         lib.mimir_prefixlm_cache_attn_workspace_bytes.restype = ctypes.c_size_t
+        lib.mimir_prefixlm_rotary.argtypes = [ctypes.POINTER(RotaryParams), _vp]
+        lib.mimir_prefixlm_rotary.restype = ctypes.c_int
+        lib.mimir_prefixlm_paged_attn.argtypes = [ctypes.POINTER(PagedAttnParams), _vp]
+        lib.mimir_prefixlm_paged_attn.restype = ctypes.c_int
+        lib.mimir_prefixlm_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
+        lib.mimir_prefixlm_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+        pages = ctypes.POINTER(PagesParams)
+        lib.mimir_prefixlm_pages_workspace_bytes.argtypes = [pages, _i32]
+        lib.mimir_prefixlm_pages_workspace_bytes.restype = ctypes.c_size_t
+        lib.mimir_prefixlm_pages_copy.argtypes = [pages, _vp, _vp, _i32, _vp]
+        lib.mimir_prefixlm_pages_copy.restype = ctypes.c_int
+        lib.mimir_prefixlm_pages_fork.argtypes = [pages, _vp, _vp, _i32, _vp]
+        lib.mimir_prefixlm_pages_fork.restype = ctypes.c_int
+        lib.mimir_prefixlm_pages_compact.argtypes = [pages, _vp, _vp]
+        lib.mimir_prefixlm_pages_compact.restype = ctypes.c_int
+        lib.mimir_prefixlm_pages_release.argtypes = [pages, _vp, _i32, _vp]
+        lib.mimir_prefixlm_pages_release.restype = ctypes.c_int
+        lib.mimir_prefixlm_pages_reserve.argtypes = [pages, _vp, _vp]
+        lib.mimir_prefixlm_pages_reserve.restype = ctypes.c_int
         lib.mimir_prefixlm_check_metadata.argtypes = [_vp, _vp, _vp, _i32, _i32, _vp, _vp]
         lib.mimir_prefixlm_check_metadata.restype = ctypes.c_int
         lib.mimir_prefixlm_last_error.argtypes = []

@@ -54,6 +54,10 @@ SOURCES = [
     "prefixlm_layer.hip",
     "prefixlm_cache_bf16.hip",
     "prefixlm_noalloc.hip",
+    "prefixlm_rotary.hip",
+    "prefixlm_paged_append.hip",
+    "prefixlm_paged_attn.hip",
+    "prefixlm_pages.hip",
 ]
 
 

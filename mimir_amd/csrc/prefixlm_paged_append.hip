@@ -1,0 +1,157 @@
+// New keys / values into the pages of an 8-bit cache, for gfx950.
+//
+// One workgroup per (batch row, kv head, page that gets new tokens), for keys and for
+// values each.  The page and head take the smallest exponent e with |x| <= 448 * 2^e for
+// the new values, but not less than the one they have for older tokens, whose codes are
+// rounded again where e grew.  With scales of powers of two that costs them nothing
+// but the bits that fall below 2^(e - 9): an 8-bit float keeps its three fraction bits, so a finer
+// scale would not make the others more exact either.
+//
+// Bound by reading the new rows (bf16) and writing their codes; the page's older codes are
+// touched only where the exponent grew.  Values are turned to [D][token] through LDS.
+#include "prefixlm_paged.h"
+
+namespace mimir {
+namespace {
+
+constexpr int kThreads = 256;
+
+// The exponent that the largest finite magnitude needs, from its bf16 bits (448 = 1.75 * 2^8).
+__device__ __forceinline__ int exponent_for(int bits) {
+  const int e = (bits >> 7) - 127 - 8 + ((bits & 0x7f) > 96);
+  return e > kMinExponent ? e : kMinExponent;
+}
+
+// x / 2^e rounded to e4m3, four values to a word; infinities become NaN.
+__device__ __forceinline__ float coded_value(float x, int e) {
+  return __builtin_fabsf(x) <= 3.4028235e38f ? __builtin_amdgcn_ldexpf(x, -e) : __builtin_nanf("");
+}
+__device__ __forceinline__ int encode4(float a, float b, float c, float d) {
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+// Four codes times 2^shift, rounded to codes again.
+__device__ __forceinline__ int recode4(int x, int shift) {
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
+  return encode4(__builtin_amdgcn_ldexpf(lo[0], shift), __builtin_amdgcn_ldexpf(lo[1], shift),
+                 __builtin_amdgcn_ldexpf(hi[0], shift), __builtin_amdgcn_ldexpf(hi[1], shift));
+}
+
+template <int D>
+__device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touched) {
+  constexpr int kUnits = D / 8;                  // threads of a row
+  constexpr int kStep = kThreads / kUnits;       // rows at a time
+  constexpr int kPasses = kPage / kStep;
+  constexpr int kPitch = D + 4;
+  __shared__ uint8_t codes[kPage * kPitch];
+  __shared__ int top[kThreads / 64];
+  const int tid = threadIdx.x;
+  int u = blockIdx.x;
+  const int j = u % touched;
+  u /= touched;
+  const int hk = u % a.Hkv, b = u / a.Hkv;
+  const bool values = blockIdx.y == 1;
+  const PagedRow r(a, b);
+  if (r.m == 0) return;
+  const int at = r.n / kPage + j;                // of the row's pages
+  const int lo = max(r.n, at * kPage), hi = min(r.n + r.m, min(at + 1, a.width) * kPage);
+  if (lo >= hi) return;
+  const int page = page_id(a, r.row, at);
+  if (page < 0) return;
+  const int s0 = lo - at * kPage, s1 = hi - at * kPage;  // slots of the new tokens
+  const bf16_t* const x = values ? a.vn + (int64_t)b * a.vn_sb + (int64_t)hk * a.vn_sh + (int64_t)(lo - r.n) * a.vn_st
+                                 : a.kn + (int64_t)b * a.kn_sb + (int64_t)hk * a.kn_sh + (int64_t)(lo - r.n) * a.kn_st;
+  const int64_t x_st = values ? a.vn_st : a.kn_st;
+  uint8_t* const y = values ? a.cv + page * a.v_sp + (int64_t)hk * kPage * D : a.ck + page * a.k_sp + (int64_t)hk * kPage * D;
+  int8_t* const ey = values ? a.ve + page * a.ve_sp + hk : a.ke + page * a.ke_sp + hk;
+
+  const int row = tid / kUnits, c = tid % kUnits * 8;
+  bf16x8 v[kPasses];
+  int most = 0;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = p * kStep + row;
+    v[p] = bf16x8{};
+    if (t < s1 - s0) v[p] = *(const bf16x8*)&x[(int64_t)t * x_st + c];
+    const i32x4 words = __builtin_bit_cast(i32x4, v[p]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int bits = words[e >> 1] >> (16 * (e & 1)) & 0x7fff;
+      most = max(most, bits < 0x7f80 ? bits : 0);
+    }
+  }
+  const int had = s0 > 0 ? *ey : kMinExponent;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
+  if ((tid & 63) == 0) top[tid >> 6] = most;
+  __syncthreads();  // and every thread has read the old exponent
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) most = max(most, top[w]);
+  const int need = exponent_for(most);
+  const int e = s0 > 0 ? max(had, need) : need;
+  const int shift = had - e;
+  const bool grew = s0 > 0 && shift < 0;
+  if (tid == 0) *ey = (int8_t)e;
+
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = p * kStep + row;
+    if (t >= s1 - s0) break;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = coded_value((float)v[p][i], e);
+    const i32x2 w = {encode4(f[0], f[1], f[2], f[3]), encode4(f[4], f[5], f[6], f[7])};
+    if (values) {
+      *(int*)&codes[(s0 + t) * kPitch + c] = w[0];
+      *(int*)&codes[(s0 + t) * kPitch + c + 4] = w[1];
+    } else {
+      *(i32x2*)&y[(s0 + t) * D + c] = w;
+    }
+  }
+  if (!values) {
+    if (grew)
+      for (int i = tid * 4; i < s0 * D; i += kThreads * 4) *(int*)&y[i] = recode4(*(const int*)&y[i], shift);
+    return;
+  }
+  __syncthreads();
+  const int w0 = grew ? 0 : s0 / 4, words = (s1 + 3) / 4 - w0;  // words of four tokens to write, of each column
+  for (int i = tid; i < D * words; i += kThreads) {
+    const int d = i / words, t = (i - d * words + w0) * 4;
+    int out = 0;
+    if (t < s0 || t + 4 > s1) {
+      const int old = *(const int*)&y[d * kPage + t];
+      out = grew ? recode4(old, shift) : old;
+      // the word's slots behind the new tokens keep their codes
+      const int end = s1 - t;
+      if (end < 4) {
+        const unsigned keep = ~0u << (8 * end);
+        out = (int)(((unsigned)out & ~keep) | ((unsigned)old & keep));
+      }
+    }
+#pragma unroll
+    for (int e2 = 0; e2 < 4; ++e2)
+      if (t + e2 >= s0 && t + e2 < s1)
+        out = (int)(((unsigned)out & ~(0xffu << (8 * e2))) | (unsigned)codes[(t + e2) * kPitch + d] << (8 * e2));
+    *(int*)&y[d * kPage + t] = out;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void paged_append_d128_kernel(const PagedArgs a, int touched) {
+  paged_append_body<128>(a, touched);
+}
+__global__ __launch_bounds__(kThreads) void paged_append_d64_kernel(const PagedArgs a, int touched) {
+  paged_append_body<64>(a, touched);
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedArgs& a, hipStream_t stream) {
+  const int touched = (a.S + 2 * kPage - 2) / kPage;  // pages that S tokens may fall in
+  const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * touched), 2);
+  if (a.D == 128)
+    hipLaunchKernelGGL(paged_append_d128_kernel, grid, dim3(kThreads), 0, stream, a, touched);
+  else
+    hipLaunchKernelGGL(paged_append_d64_kernel, grid, dim3(kThreads), 0, stream, a, touched);
+  return hipGetLastError();
+}
+
+}  // namespace mimir

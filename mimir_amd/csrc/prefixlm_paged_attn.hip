@@ -1,0 +1,962 @@
+// Attention over an 8-bit paged KV cache, bf16 queries, for gfx950 (MI355X).
+//
+//   paged_append_*        the new rows into their pages (prefixlm_paged_append.hip)
+//   decode (at most 32 query rows per kv head, e.g. S = 1):
+//     paged_decode_*      the workgroups take equal shares of all pages of the call
+//     paged_merge_*       adds the partial rows of the shares
+//   otherwise:
+//     paged_prefill_*     one workgroup per (batch row, kv head, 128 query rows, key split)
+//     paged_merge_splits_* with several splits: adds their partial rows
+//
+// S^T = K Q^T and O^T += V^T P^T on bf16 MFMA with an online softmax in fp32.  Codes become
+// bf16 times their page's scale in the conversion instruction, exactly; P is rounded to
+// bf16 under the tile's own maximum, the one rounding before the output's.
+#include <algorithm>
+#include <cmath>
+
+#include "prefixlm_paged.h"
+
+namespace mimir {
+int fail_with(int code, const std::string& msg);
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kDecRows = 32;        // query rows of the decode kernel per kv head, at most
+constexpr float kRefRange = 30.f;   // how far (log2) a tile's reference may lie below the row's maximum
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Combine x over the four 16-lane groups of a wave.
+__device__ __forceinline__ float xor16_max(float x) {
+  const int xi = __float_as_int(x);
+  auto r = __builtin_amdgcn_permlane16_swap(xi, xi, false, false);
+  const int a = r[0], b = r[1];
+  return fmaxf(__int_as_float(a), __int_as_float(b));
+}
+__device__ __forceinline__ float xor16_sum(float x) {
+  const int xi = __float_as_int(x);
+  auto r = __builtin_amdgcn_permlane16_swap(xi, xi, false, false);
+  const int a = r[0], b = r[1];
+  return __int_as_float(a) + __int_as_float(b);
+}
+
+// bf16 1 where a bit of the lowest eight is set, 0 elsewhere.
+__device__ __forceinline__ bf16x8 ones_where(unsigned bits) {
+  i32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (int)((bits >> (2 * i) & 1) * 0x3f80u | (bits >> (2 * i + 1) & 1) * 0x3f800000u);
+  return __builtin_bit_cast(bf16x8, x);
+}
+
+// ------------------------------------------------------------------ partial rows
+
+// One output row from its n partial rows (maximum in the exp2 domain, sum, unnormalized O) at
+// slot(c), c < n: sum_c O_c 2^(m_c - M) / sum_c l_c 2^(m_c - M).  One wave; D / 4 lanes a part row,
+// four columns each, kChunk loads in flight.
+template <int D, typename Slot>
+__device__ __forceinline__ void merge_parts(const PagedArgs& a, int n, int lane, Slot&& slot, bf16_t* orow) {
+  constexpr int kChunk = 8, kLanes = D / 4, kParts = 64 / kLanes;
+  const int sub = lane / kLanes, col = lane % kLanes * 4;
+  float M = -INFINITY, lsum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < n; c0 += 64) {
+    const int in_chunk = min(n - c0, 64);
+    const int64_t row = slot(min(c0 + lane, n - 1));
+    f32x2 ml = *(const f32x2*)&a.part_ml[2 * row];
+    if (lane >= in_chunk) ml = f32x2{-INFINITY, 0.f};
+    float m = ml[0];
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const float m_new = fmaxf(M, m);
+    const float alpha = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+    // no allowed key in this part: its sum is 0 (or NaN, of scores that all were)
+    const float w = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - m_new);
+    float l = ml[1] * w;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
+    lsum = lsum * alpha + l;
+    acc *= alpha;
+    M = m_new;
+    for (int i0 = 0; i0 < in_chunk; i0 += kChunk * kParts) {
+      f32x4 v[kChunk];
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        const int src = min(i0 + i * kParts + sub, in_chunk - 1);
+        const int64_t at = __shfl(row, src, 64);
+        v[i] = *(const f32x4*)&a.part_o[at * D + col];
+      }
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        const int src = i0 + i * kParts + sub;
+        const float wi = __shfl(w, min(src, 63), 64);
+        if (src < in_chunk && wi != 0.f) acc += v[i] * wi;
+      }
+    }
+  }
+#pragma unroll
+  for (int off = kLanes; off < 64; off <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], off, 64);
+  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;  // NaN sums stay NaN
+  if (sub == 0) *(bf16x4*)&orow[col] = __builtin_convertvector(acc * inv, bf16x4);
+}
+
+// ------------------------------------------------------------------ decode
+//
+// Bound by the read of the pages.  Each wave streams its own pages straight into registers
+// (a page of one head is 16 loads of 16 bytes a lane at head_dim 128): the layouts make
+// every load an operand, so there is no LDS round trip and no barrier in the loop.  With the
+// matrix instruction's 16 x 16 x 32 form the 64 tokens of a page are dealt so that the
+// scores a lane group g holds are tokens 16 g .. 16 g + 15, in order: exactly the tokens of
+// the 16-byte load from a value column.  The next page's keys are requested once the scores
+// are formed and its values once they are used, so about a page per wave is in flight.
+//
+// The pages of all batch rows form a line, in units of four (one per wave), dealt evenly to
+// shares (one workgroup per share and kv head), so that rows of very different lengths
+// keep all CUs busy to the end.  A pair (batch row, kv head) inside one share is
+// finished there; the parts of the others are merged by a second kernel.  For batches of
+// more than kLineRows rows each pair takes a workgroup.
+
+constexpr int kLineRows = 256;  // batch rows of a line: one per thread
+constexpr int kUnit = kWaves;   // pages of a unit
+
+struct Line {
+  int incl[kLineRows];  // units up to and with batch row b
+  int kv[kLineRows];
+  int wave[kWaves];
+  int begin;            // batch row of the share's first unit
+};
+
+// All threads: the line into LDS; returns the total of units.
+__device__ __forceinline__ int line_scan(const PagedArgs& a, Line& line) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kv = tid < a.B ? PagedRow(a, tid).kv : 0;
+  int incl = (kv + kPage * kUnit - 1) / (kPage * kUnit);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += y;
+  }
+  if (lane == 63) line.wave[wave] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const int n = line.wave[w];
+    before += w < wave ? n : 0;
+    total += n;
+  }
+  line.incl[tid] = before + incl;
+  line.kv[tid] = kv;
+  return total;
+}
+
+// q units to each share, one more to the first r.
+struct Deal {
+  int q, r;
+  __device__ __forceinline__ Deal(int total, int shares) : q(total / shares), r(total - total / shares * shares) {}
+  __device__ __forceinline__ int begin(int share) const { return share * q + min(share, r); }
+  __device__ __forceinline__ int of(int u) const {  // the share of unit u
+    const int longer = r * (q + 1);
+    return u < longer ? u / (q + 1) : r + (u - longer) / q;
+  }
+};
+// Part slot (of two per share) of a segment: the one the share begins with, or a later one.
+__device__ __forceinline__ int part_slot(int share, bool first) { return 2 * share + !first; }
+
+// Zeros for `heads` heads from h0 on of batch row b.
+template <int D>
+__device__ __forceinline__ void zero_out(const PagedArgs& a, int b, int h0, int heads) {
+  for (int i = threadIdx.x; i < a.S * heads * (D / 8); i += blockDim.x) {
+    const int c = i % (D / 8), row = i / (D / 8);
+    *(bf16x8*)&a.out[(int64_t)b * a.o_sb + (int64_t)(row / heads) * a.o_st + (int64_t)(h0 + row % heads) * a.o_sh + c * 8] = bf16x8{};
+  }
+}
+
+template <int D, int NR, bool kPairs>
+__device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
+  constexpr int KH = D / 64;   // 16-byte loads of a key row per lane
+  constexpr int DT = D / 16;   // column tiles of the output
+  constexpr int kRowsMax = 16 * NR;
+  constexpr int kPitch = D + 4;
+  __shared__ Line line;
+  __shared__ float area[kWaves][kRowsMax * kPitch];
+  __shared__ f32x2 area_ml[kWaves][kRowsMax];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m16 = lane & 15, g = lane >> 4;
+  const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;  // share: the batch row, for pairs
+  const int R = a.S * a.G;
+
+  int b = share, u0 = 0, u_end = 1;
+  if constexpr (kPairs) {
+    if (PagedRow(a, b).kv == 0) {
+      zero_out<D>(a, b, hk * a.G, a.G);
+      return;
+    }
+  } else {
+    const int total = line_scan(a, line);
+    const Deal deal(total, a.shares);
+    u0 = deal.begin(share);
+    u_end = deal.begin(share + 1);
+    __syncthreads();
+    for (int r = blockIdx.x; r < a.B; r += gridDim.x)
+      if (line.kv[r] == 0) zero_out<D>(a, r, 0, a.Hkv * a.G);
+    if (u0 >= u_end) return;
+    if (tid < a.B && line.incl[tid] > u0 && (tid == 0 || line.incl[tid - 1] <= u0)) line.begin = tid;
+    __syncthreads();
+    b = line.begin;
+  }
+
+  // offsets of a lane in a page: key rows 16 (m16 / 4) + m16 % 4 (+ 4 per tile), value columns m16 (+ 16)
+  const int k_off = (16 * (m16 >> 2) + (m16 & 3)) * D + 16 * g;
+  const int v_off = m16 * kPage + 16 * g;
+  const float c2 = a.scale_log2;
+  const float ref_range = fminf(kRefRange / c2, 3e38f);
+  const int u_first = u0;
+
+  for (;;) {
+    // The segment: pages [t0, t1) of batch row b.
+    const PagedRow r(a, b);
+    int t0 = 0, t1 = (r.kv + kPage - 1) / kPage;
+    bool whole = true;
+    int u_next = u_end;
+    if constexpr (!kPairs) {
+      const int units = (t1 + kUnit - 1) / kUnit;
+      const int unit0 = u0 - (line.incl[b] - units), unit1 = min(units, unit0 + u_end - u0);
+      whole = unit0 == 0 && unit1 == units;
+      u_next = u0 + unit1 - unit0;
+      t0 = unit0 * kUnit;
+      t1 = min(t1, unit1 * kUnit);
+    }
+    const int n_my = t0 + wave < t1 ? (t1 - t0 - wave + kUnit - 1) / kUnit : 0;  // this wave's pages
+
+    // Q^T operands: lane holds query row m16 (+ 16), columns 64 h + 16 g + 8 s ..+7; rows past the
+    // last take the first (never read).  Each row's key limit; 0 for queries i >= m.
+    bf16x8 qf[NR][2 * KH];
+    int limit[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0;
+      const int i = row / a.G;
+      limit[nr] = 16 * nr + m16 < R && i < r.m ? (a.causal ? min(r.n + i + 1, r.kv) : r.kv) : 0;
+      const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)i * a.q_st + (int64_t)(hk * a.G + row - i * a.G) * a.q_sh + 16 * g;
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) qf[nr][2 * h + s] = *(const bf16x8*)&q[64 * h + 8 * s];
+    }
+    const int limit_min = a.causal ? min(r.n + 1, r.kv) : r.kv;
+
+    // The wave's pages, 64 at a time on its lanes: page id (-1: none) and exponents.
+    int ids = -1, ek = 0, ev = 0;
+    auto load_ids = [&](int i0) __attribute__((always_inline)) {
+      const int t = t0 + wave + kUnit * (i0 + lane);
+      ids = t < t1 ? page_id(a, r.row, t) : -1;
+      ek = ids >= 0 ? a.ke[ids * a.ke_sp + hk] : 0;
+      ev = ids >= 0 ? a.ve[ids * a.ve_sp + hk] : 0;
+    };
+    i32x4 kreg[4][KH], vreg[DT];
+    auto load_keys = [&](int i) __attribute__((always_inline)) {
+      const int id = max(__builtin_amdgcn_readlane(ids, i & 63), 0);  // none: page 0, masked
+      const uint8_t* p = a.ck + id * a.k_sp + (int64_t)hk * kPage * D;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int h = 0; h < KH; ++h) kreg[t][h] = *(const i32x4*)&p[k_off + 4 * t * D + 64 * h];
+    };
+    auto load_values = [&](int i) __attribute__((always_inline)) {
+      const int id = max(__builtin_amdgcn_readlane(ids, i & 63), 0);
+      const uint8_t* p = a.cv + id * a.v_sp + (int64_t)hk * kPage * D;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vreg[d] = *(const i32x4*)&p[v_off + 16 * kPage * d];
+    };
+
+    f32x4 oacc[NR][DT];
+    float m_run[NR], m_top[NR], l_run[NR];  // the sums' reference and the row's maximum so far (scores), the sum
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) oacc[nr][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[nr] = m_top[nr] = -INFINITY;
+      l_run[nr] = 0.f;
+    }
+    if (n_my > 0) {
+      load_ids(0);
+      load_keys(0);
+      load_values(0);
+    }
+    for (int i = 0; i < n_my; ++i) {
+      const int base = (t0 + wave + kUnit * i) * kPage;
+      const bool some = __builtin_amdgcn_readlane(ids, i & 63) >= 0;
+      const float ks = pow2(__builtin_amdgcn_readlane(ek, i & 63)), vs = pow2(__builtin_amdgcn_readlane(ev, i & 63));
+      f32x4 st[NR][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) st[nr][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < KH; ++h)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const bf16x8 kf = decode8(kreg[t][h][2 * s], kreg[t][h][2 * s + 1], ks);
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) st[nr][t] = mfma16(kf, qf[nr][2 * h + s], st[nr][t]);
+          }
+      }
+      const bool last_of_ids = (i & 63) == 63;
+      if (i + 1 < n_my) {
+        if (last_of_ids) load_ids(i + 1);
+        load_keys(i + 1);
+      }
+      // tokens 16 g + 4 t + e of the page
+      const bool edge = !some || base + kPage > limit_min;
+      bf16x8 pf[NR][2];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        if (edge) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!some || base + 16 * g + 4 * t + e >= limit[nr]) st[nr][t][e] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[nr][t][e]);
+        // Every page's probabilities under its own maximum (but not more than 2^30 below the row's so
+        // far, which bounds the sums): its largest is 1, exact in bf16.
+        mx = xor32_max(xor16_max(mx));
+        m_top[nr] = fmaxf(m_top[nr], mx);
+        const float m_new = fmaxf(mx, m_top[nr] - ref_range);
+        const float alpha = m_run[nr] == -INFINITY ? 1.f : fast_exp2((m_run[nr] - m_new) * c2);
+        m_run[nr] = m_new;
+        const float mb = m_new == -INFINITY ? 0.f : m_new;
+        float lsum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // the difference first: a scaled score of 2^30 is known to 2^6, and rounding it apart from the
+            // maximum would give probabilities up to 2^64
+            const float p = fast_exp2((st[nr][t][e] - mb) * c2);
+            st[nr][t][e] = p;
+            lsum += p;
+          }
+        l_run[nr] = l_run[nr] * alpha + lsum;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) oacc[nr][d] *= alpha;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f32x8 x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = st[nr][2 * c + (e >> 2)][e & 3];
+          pf[nr][c] = to_bf16x8(x);
+        }
+      }
+      if (edge) {
+        // What lies behind the last token is unwritten; a NaN among the values of tokens that only
+        // some of the rows see must not reach the others: it is taken out of the product
+        // and put into the rows that see it.
+        const int end = (some ? min(r.kv - base, kPage) : 0) - 16 * g;
+        unsigned nan = 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            vreg[d][w] = codes_before(vreg[d][w], 4 * w, end);
+            nan |= nan_codes(vreg[d][w]);
+          }
+        if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            unsigned at = 0;  // tokens 16 g + e whose code is NaN
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int w = e >> 2, sh = 8 * (e & 3);
+              if (((unsigned)vreg[d][w] >> sh & 0x7f) == 0x7f) {
+                at |= 1u << e;
+                vreg[d][w] &= (int)~(0xffu << sh);
+              }
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+              const int see = limit[nr] - base - 16 * g;  // of the lane group's tokens
+              const unsigned seen = see >= 16 ? 0xffffu : (see <= 0 ? 0u : (1u << see) - 1);
+              f32x4 hit = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int c = 0; c < 2; ++c) hit = mfma16(ones_where(at >> (8 * c)), ones_where(seen >> (8 * c)), hit);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (hit[e] > 0.f) oacc[nr][d][e] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const bf16x8 vf = decode8(vreg[d][2 * c], vreg[d][2 * c + 1], vs);
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) oacc[nr][d] = mfma16(vf, pf[nr][c], oacc[nr][d]);
+        }
+      if (i + 1 < n_my) load_values(i + 1);
+    }
+
+    // Merge the waves' rows through LDS.
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int row = 16 * nr + m16;
+      const float l = xor32_sum(xor16_sum(l_run[nr]));
+      if (row < R) {
+        if (g == 0) area_ml[wave][row] = f32x2{m_run[nr] == -INFINITY ? -INFINITY : m_run[nr] * c2, l};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *(f32x4*)&area[wave][row * kPitch + 16 * d + 4 * g] = oacc[nr][d];
+      }
+    }
+    __syncthreads();
+    constexpr int kLanes = D / 4, kRowsAt = kThreads / kLanes;
+    const int col = tid % kLanes * 4;
+    for (int row = tid / kLanes; row < R; row += kRowsAt) {
+      float M = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, area_ml[w][row][0]);
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const f32x2 ml = area_ml[w][row];
+        const float wt = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - M);  // no key: a sum of 0 (or NaN)
+        lsum += ml[1] * wt;
+        if (wt != 0.f) acc += *(const f32x4*)&area[w][row * kPitch + col] * wt;
+      }
+      if (whole) {
+        const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+        const int i = row / a.G;
+        *(bf16x4*)&a.out[(int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col] =
+            i < r.m ? __builtin_convertvector(acc * inv, bf16x4) : bf16x4{};
+      } else {
+        const int64_t slot = ((int64_t)part_slot(share, u0 == u_first) * a.Hkv + hk) * R + row;
+        *(f32x4*)&a.part_o[slot * D + col] = acc;
+        if (col == 0) *(f32x2*)&a.part_ml[slot * 2] = f32x2{M, lsum};
+      }
+    }
+    if (u_next >= u_end) return;
+    u0 = u_next;
+    if constexpr (!kPairs)
+      do ++b;
+      while (line.incl[b] <= u0);  // the next batch row with keys
+    __syncthreads();  // the merge's area is free again
+  }
+}
+
+#define DECODE(D, NR)                                                                                        \
+  __global__ __launch_bounds__(kThreads, 2) void paged_decode_d##D##_r##NR##_kernel(const PagedArgs a) {       \
+    paged_decode_body<D, NR, false>(a);                                                                      \
+  }                                                                                                          \
+  __global__ __launch_bounds__(kThreads, 2) void paged_decode_pairs_d##D##_r##NR##_kernel(const PagedArgs a) { \
+    paged_decode_body<D, NR, true>(a);                                                                       \
+  }
+DECODE(128, 1)
+DECODE(128, 2)
+DECODE(64, 1)
+DECODE(64, 2)
+#undef DECODE
+
+// Output rows of the pairs whose pages lie in several shares, one wave per row.
+template <int D>
+__device__ __forceinline__ void paged_merge_body(const PagedArgs& a) {
+  __shared__ Line line;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
+  const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  const int total = line_scan(a, line);
+  __syncthreads();
+  const int units = (line.kv[b] + kPage * kUnit - 1) / (kPage * kUnit), before = line.incl[b] - units;
+  if (units == 0 || row >= R) return;
+  const Deal deal(total, a.shares);
+  const int w0 = deal.of(before), n = deal.of(before + units - 1) - w0 + 1;
+  if (n == 1) return;  // written by its share
+  const int slot0 = part_slot(w0, before == deal.begin(w0));
+  const int i = row / a.G;
+  bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
+  if (i >= PagedRow(a, b).m) {  // a padding query
+    if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
+    return;
+  }
+  merge_parts<D>(a, n, lane, [&](int c) { return ((int64_t)(c == 0 ? slot0 : part_slot(w0 + c, true)) * a.Hkv + hk) * R + row; }, o);
+}
+__global__ __launch_bounds__(kThreads) void paged_merge_d128_kernel(const PagedArgs a) { paged_merge_body<128>(a); }
+__global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedArgs a) { paged_merge_body<64>(a); }
+
+// ------------------------------------------------------------------ prefill
+//
+// Rows are (token, head) pairs, token-major, 128 to a workgroup, so the G query heads of a
+// kv head share its pages.  A page's codes go through registers: requested while the page
+// before is computed, converted to bf16 by the workgroup once (not by each wave) and stored
+// to the other of two LDS stages.  The products run on the 32 x 32 x 16 form, whose scores of
+// a lane are tokens 4 hi .. and 8 + 4 hi .. of each 16; the values' tokens are stored in that
+// order, so that both operands are 16-byte LDS reads.
+
+constexpr int kRows = kWaves * 32;
+constexpr int kMaxSplits = 64;
+
+template <int D>
+__device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
+  constexpr int DT = D / 32, KS = D / 16;
+  constexpr int kPer = 4 * D / kThreads;  // 16-byte units of a page's keys (and values) per thread
+  using LK = TileLayout<D>;
+  using LV = TileLayout<64>;              // 64 columns of values by 64 tokens
+  __shared__ __attribute__((aligned(16))) bf16_t sK[2][LK::kElems];
+  __shared__ __attribute__((aligned(16))) bf16_t sV[2][D / 64 * LV::kElems];
+  __shared__ int s_nan[2][kWaves];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hi = lane >> 5;
+  int u = blockIdx.x;
+  const int split = u % a.splits;
+  u /= a.splits;
+  const int rt = a.n_rt - 1 - u % a.n_rt;  // later rows see more keys: first
+  u /= a.n_rt;
+  const int hk = u % a.Hkv, b = u / a.Hkv;
+  const PagedRow r(a, b);
+  const int R = a.S * a.G, Rm = r.kv > 0 ? r.m * a.G : 0;  // rows, and those that attend
+  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
+  const int n_valid = (tiles + per - 1) / per;  // splits that hold keys
+  if (split > 0 && split >= n_valid) return;
+
+  const int row = rt * kRows + wave * 32 + l32;
+  const bool row_ok = row < R;
+  const int ti = row_ok ? row / a.G : 0;
+  const int h = hk * a.G + (row_ok ? row - ti * a.G : 0);
+  auto limit_of = [&](int x) { return a.causal ? min(r.n + x / a.G + 1, r.kv) : r.kv; };
+  const int limit = row < Rm ? limit_of(row) : 0;
+  const int r0 = rt * kRows + wave * 32;
+  const bool active = r0 < Rm;
+  const int w_max = active ? limit_of(min(r0 + 31, Rm - 1)) : 0, w_min = active ? limit_of(r0) : 0;
+  const int wg0 = rt * kRows;
+  const int wg_max = wg0 < Rm ? limit_of(min(wg0 + kRows - 1, Rm - 1)) : 0, wg_min = wg0 < Rm ? limit_of(wg0) : 0;
+  const int kt0 = split * per;
+  const int kt1 = min((wg_max + kPage - 1) / kPage, kt0 + per);
+
+  i32x4 kreg[kPer], vreg[kPer];
+  int ek = 0, ev = 0;
+  bool some = false;
+  auto load_page = [&](int kt) __attribute__((always_inline)) {
+    const int id = load_const(a.table, (int64_t)r.row * a.t_st + kt);
+    some = id >= 0 && id < a.num_pages;
+    const int64_t p = some ? id : 0;  // none: page 0, masked
+    ek = a.ke[p * a.ke_sp + hk];
+    ev = a.ve[p * a.ve_sp + hk];
+    const uint8_t* kp = a.ck + p * a.k_sp + (int64_t)hk * kPage * D;
+    const uint8_t* vp = a.cv + p * a.v_sp + (int64_t)hk * kPage * D;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      kreg[i] = *(const i32x4*)&kp[(i * kThreads + tid) * 16];
+      vreg[i] = *(const i32x4*)&vp[(i * kThreads + tid) * 16];
+    }
+  };
+  auto stage_page = [&](int kt, int buf) __attribute__((always_inline)) {
+    const float ks = pow2(ek), vs = pow2(ev);
+    const int base = kt * kPage, end = some ? r.kv - base : 0;
+    unsigned nan = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int unit = i * kThreads + tid;
+      const int t = unit / (D / 16), c = unit % (D / 16) * 16;
+      bf16_t* const kd = &sK[buf][LK::off(t, c)];
+      *(bf16x8*)kd = decode8(kreg[i][0], kreg[i][1], ks);
+      *(bf16x8*)(kd + 8) = decode8(kreg[i][2], kreg[i][3], ks);
+      const int d = unit / 4, t16 = unit % 4 * 16;
+      i32x4 v = vreg[i];
+      if (end < kPage) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = codes_before(v[w], t16 + 4 * w, end);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) nan |= nan_codes(v[w]);
+      bf16_t* const vd = &sV[buf][(d >> 6) * LV::kElems + LV::off(d & 63, t16)];
+      *(bf16x8*)vd = decode8(v[0], v[2], vs);
+      *(bf16x8*)(vd + 8) = decode8(v[1], v[3], vs);
+    }
+    // NaN values matter apart only where rows of the workgroup see different tokens
+    const bool any = base + kPage > wg_min && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+    if (lane == 0) s_nan[buf][wave] = any | (some ? 0 : 2);
+  };
+
+  if (kt0 < kt1) load_page(kt0);
+  bf16x8 qf[KS];
+  {
+    const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)ti * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = row < Rm ? *(const bf16x8*)&q[16 * ks + 8 * hi] : bf16x8{};
+  }
+  f32x16 oacc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float c2 = a.scale_log2;
+  const int k_base = LK::off(l32, 8 * hi), v_base = LV::off(l32, 8 * hi);
+
+  auto compute = [&](int kt, int buf) __attribute__((always_inline)) {
+    const int base = kt * kPage;
+    if (!active || base >= w_max) return;
+    const int flags = s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3];
+    if (__builtin_amdgcn_readfirstlane(flags) & 2) return;  // no page here
+    f32x16 st[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      st[mt] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        st[mt] = mfma32(*(const bf16x8*)&sK[buf][k_base + mt * 32 * LK::kRowElems + ks * 16], qf[ks], st[mt]);
+    }
+    if (base + kPage > w_min) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (base + 32 * mt + 8 * (e >> 2) + 4 * hi + (e & 3) >= limit) st[mt][e] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[mt][e]);
+    mx = xor32_max(mx);
+    // The reference maximum moves only when it grows by more than 2^8 in probability terms.
+    const float m_cand = fmaxf(m_run, mx);
+    const bool grow = (m_cand - m_run) * c2 > 8.f;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+      const float m_new = grow ? m_cand : m_run;
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2((m_run - m_new) * c2);
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+      m_run = m_new;
+    }
+    const float ref = m_run == -INFINITY ? 0.f : m_run, mb = ref * c2;
+    float lsum = 0.f;
+    // Scaled scores past 2^24 are known to one only: their difference is formed before the scale,
+    // at an operation more each, or rounding them apart would give probabilities up to 2^(their ulp).
+    if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(mb) > 16777216.f) != 0) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[mt][e] = fast_exp2((st[mt][e] - ref) * c2);
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[mt][e] = fast_exp2(__builtin_fmaf(st[mt][e], c2, -mb));
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) lsum += st[mt][e];
+    l_run += lsum;
+    bf16x8 pf[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      f32x8 t;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = st[kk >> 1][8 * (kk & 1) + e];
+      pf[kk] = to_bf16x8(t);
+    }
+    if (flags & 1) {
+      // Values that are NaN: out of the product, and into the rows that see them.
+      bf16x8 see[4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        unsigned bits = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int f = 8 * (kk & 1) + e;
+          bits |= (base + 32 * (kk >> 1) + 8 * (f >> 2) + 4 * hi + (f & 3) < limit ? 1u : 0u) << e;
+        }
+        see[kk] = ones_where(bits);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        f32x16 hit = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          i32x4 v = *(const i32x4*)&sV[buf][(dt >> 1) * LV::kElems + v_base + (dt & 1) * 32 * LV::kRowElems + kk * 16];
+          unsigned bits = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((v[e >> 1] >> (16 * (e & 1)) & 0x7fff) > 0x7f80) {
+              bits |= 1u << e;
+              v[e >> 1] &= e & 1 ? 0xffff : (int)0xffff0000;
+            }
+          hit = mfma32(ones_where(bits), see[kk], hit);
+          oacc[dt] = mfma32(__builtin_bit_cast(bf16x8, v), pf[kk], oacc[dt]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (hit[e] > 0.f) oacc[dt][e] = __builtin_nanf("");
+      }
+      return;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        oacc[dt] = mfma32(*(const bf16x8*)&sV[buf][(dt >> 1) * LV::kElems + v_base + (dt & 1) * 32 * LV::kRowElems + kk * 16],
+                          pf[kk], oacc[dt]);
+  };
+
+  if (kt0 < kt1) stage_page(kt0, 0);
+  __syncthreads();
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int buf = (kt - kt0) & 1;
+    if (kt + 1 < kt1) load_page(kt + 1);
+    compute(kt, buf);
+    if (kt + 1 < kt1) stage_page(kt + 1, buf ^ 1);
+    __syncthreads();
+  }
+
+  const float l_tot = xor32_sum(l_run);
+  if (n_valid <= 1) {
+    if (!row_ok) return;
+    const float inv = row < Rm && l_tot != 0.f ? 1.f / l_tot : 0.f;
+    bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)ti * a.o_st + (int64_t)h * a.o_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        f32x4 t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = row < Rm ? oacc[dt][4 * rg + e] * inv : 0.f;
+        *(bf16x4*)&o[32 * dt + 8 * rg + 4 * hi] = __builtin_convertvector(t, bf16x4);
+      }
+    return;
+  }
+  const int64_t slot = ((((int64_t)b * a.Hkv + hk) * a.n_rt + rt) * a.splits + split) * kRows + wave * 32 + l32;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+      f32x4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = oacc[dt][4 * rg + e];
+      *(f32x4*)&a.part_o[slot * D + 32 * dt + 8 * rg + 4 * hi] = t;
+    }
+  if (hi == 0) *(f32x2*)&a.part_ml[slot * 2] = f32x2{m_run == -INFINITY ? -INFINITY : m_run * c2, l_tot};
+}
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d128_kernel(const PagedArgs a) { paged_prefill_body<128>(a); }
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d64_kernel(const PagedArgs a) { paged_prefill_body<64>(a); }
+
+template <int D>
+__device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
+  const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  if (row >= R) return;
+  const PagedRow r(a, b);
+  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
+  const int n = (tiles + per - 1) / per;
+  if (n <= 1) return;  // written by its split
+  const int i = row / a.G;
+  bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
+  if (i >= r.m) {  // a padding query
+    if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
+    return;
+  }
+  const int64_t unit0 = ((int64_t)pair * a.n_rt + row / kRows) * a.splits;
+  merge_parts<D>(a, n, lane, [&](int c) { return (unit0 + c) * kRows + row % kRows; }, o);
+}
+__global__ __launch_bounds__(kThreads) void paged_merge_splits_d128_kernel(const PagedArgs a) { paged_merge_splits_body<128>(a); }
+__global__ __launch_bounds__(kThreads) void paged_merge_splits_d64_kernel(const PagedArgs a) { paged_merge_splits_body<64>(a); }
+
+// ------------------------------------------------------------------ host side
+
+struct Plan {
+  bool decode, pairs;
+  int n_rt, splits;
+  int64_t units;  // workgroups of the attention kernel
+  size_t workspace_bytes;
+};
+
+Plan plan_of(const MimirPagedAttnParams& p) {
+  Plan s = {};
+  const int64_t cus = device_cu_count(), R = (int64_t)p.seqlen * (p.num_q_heads / p.num_kv_heads);
+  const int64_t pairs = (int64_t)p.batch * p.num_kv_heads;
+  s.decode = R <= kDecRows;
+  s.splits = 1;
+  if (s.decode) {
+    const int64_t most = (int64_t)p.batch * ((p.table_width + kUnit - 1) / kUnit);  // units of the line
+    s.pairs = p.batch > kLineRows || p.table_width <= kUnit;
+    if (s.pairs) {
+      s.units = pairs;
+    } else {
+      s.units = p.num_kv_heads * std::max<int64_t>(1, std::min(most, 2 * cus / p.num_kv_heads));
+      s.workspace_bytes = (size_t)s.units * 2 * (size_t)R * ((size_t)p.head_dim + 2) * sizeof(float);
+    }
+    return s;
+  }
+  s.n_rt = (int)((R + kRows - 1) / kRows);
+  const int64_t groups = pairs * s.n_rt;
+  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + groups - 1) / groups, p.table_width, kMaxSplits}));
+  s.units = groups * s.splits;
+  s.workspace_bytes = s.splits > 1 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
+  return s;
+}
+
+hipError_t launch_paged_attn(const MimirPagedAttnParams& p, const Plan& plan, hipStream_t stream) {
+  PagedArgs a = {};
+  a.q = (const bf16_t*)p.q;
+  a.kn = (const bf16_t*)p.k_new;
+  a.vn = (const bf16_t*)p.v_new;
+  a.out = (bf16_t*)p.out;
+  a.ck = (uint8_t*)p.cache_k;
+  a.cv = (uint8_t*)p.cache_v;
+  a.ke = p.k_exponents;
+  a.ve = p.v_exponents;
+  a.table = p.page_table;
+  a.lengths = p.cache_lengths;
+  a.indices = p.batch_indices;
+  a.fresh = p.new_lengths;
+  a.q_sb = p.q_stride_batch; a.q_st = p.q_stride_token; a.q_sh = p.q_stride_head;
+  a.kn_sb = p.kn_stride_batch; a.kn_st = p.kn_stride_token; a.kn_sh = p.kn_stride_head;
+  a.vn_sb = p.vn_stride_batch; a.vn_st = p.vn_stride_token; a.vn_sh = p.vn_stride_head;
+  a.o_sb = p.out_stride_batch; a.o_st = p.out_stride_token; a.o_sh = p.out_stride_head;
+  a.k_sp = p.k_stride_page; a.v_sp = p.v_stride_page; a.ke_sp = p.ke_stride_page; a.ve_sp = p.ve_stride_page;
+  a.t_st = p.table_stride;
+  a.B = p.batch;
+  a.S = p.seqlen;
+  a.num_pages = p.num_pages;
+  a.rows = p.table_rows;
+  a.width = p.table_width;
+  a.Hkv = p.num_kv_heads;
+  a.G = p.num_q_heads / p.num_kv_heads;
+  a.causal = p.causal != 0;
+  a.D = p.head_dim;
+  a.idx64 = p.index_int64 != 0;
+  a.scale_log2 = std::max(p.softmax_scale * kLog2e, 1.2e-38f);  // a normal number: masked scores times it stay -inf
+  a.n_rt = plan.n_rt;
+  a.splits = plan.splits;
+  a.cus = device_cu_count();
+  a.part_o = (float*)p.workspace;
+  const int64_t R = (int64_t)a.S * a.G;
+  hipError_t e = launch_paged_append(a, stream);
+  if (e != hipSuccess) return e;
+  const dim3 grid((unsigned)plan.units), block(kThreads);
+  const dim3 merge((unsigned)((int64_t)a.B * a.Hkv * ((R + kWaves - 1) / kWaves)));
+  if (plan.decode) {
+    a.shares = (int)(plan.units / a.Hkv);
+    a.part_ml = a.part_o + (size_t)plan.units * 2 * R * p.head_dim;
+#define DECODE(D, NR)                                                                                             \
+  if (plan.pairs)                                                                                                 \
+    hipLaunchKernelGGL(paged_decode_pairs_d##D##_r##NR##_kernel, grid, block, 0, stream, a);                        \
+  else                                                                                                            \
+    hipLaunchKernelGGL(paged_decode_d##D##_r##NR##_kernel, grid, block, 0, stream, a);
+    if (a.D == 128 && R <= 16) {
+      DECODE(128, 1)
+    } else if (a.D == 128) {
+      DECODE(128, 2)
+    } else if (R <= 16) {
+      DECODE(64, 1)
+    } else {
+      DECODE(64, 2)
+    }
+#undef DECODE
+    if (plan.pairs) return hipGetLastError();
+    if (a.D == 128)
+      hipLaunchKernelGGL(paged_merge_d128_kernel, merge, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL(paged_merge_d64_kernel, merge, block, 0, stream, a);
+    return hipGetLastError();
+  }
+  a.part_ml = a.part_o + (size_t)plan.units * kRows * p.head_dim;
+  if (a.D == 128)
+    hipLaunchKernelGGL(paged_prefill_d128_kernel, grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(paged_prefill_d64_kernel, grid, block, 0, stream, a);
+  if (plan.splits > 1) {
+    if (a.D == 128)
+      hipLaunchKernelGGL(paged_merge_splits_d128_kernel, merge, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL(paged_merge_splits_d64_kernel, merge, block, 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+// A bf16 operand of `heads` heads: pointer, then batch / token / head strides.
+int check_rows(const char* name, const void* x, int64_t sb, int64_t st, int64_t sh) {
+  if (x == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, std::string(name) + " is NULL");
+  if ((uintptr_t)x % 16 != 0 || sb < 0 || st < 0 || sh < 0 || sb % 8 != 0 || st % 8 != 0 || sh % 8 != 0)
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, std::string(name) + " must be 16-byte aligned with non-negative strides that are multiples of 8 elements");
+  return MIMIR_OK;
+}
+
+bool sizes_ok(const MimirPagedAttnParams* p) {
+  return p != nullptr && p->batch >= 0 && p->seqlen >= 0 && p->num_pages >= 0 && p->table_rows >= 0 && p->table_width >= 0 &&
+         p->num_q_heads > 0 && p->num_kv_heads > 0 && p->num_q_heads % p->num_kv_heads == 0;
+}
+
+}  // namespace
+}  // namespace mimir
+
+extern "C" {
+
+size_t mimir_prefixlm_paged_attn_workspace_bytes(const MimirPagedAttnParams* p) {
+  if (!mimir::sizes_ok(p) || p->batch == 0 || p->seqlen == 0) return 0;
+  return mimir::plan_of(*p).workspace_bytes;
+}
+
+int mimir_prefixlm_paged_attn(const MimirPagedAttnParams* p, void* stream) {
+  using namespace mimir;
+  fail_with(MIMIR_OK, "");
+  if (p == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->dtype != MIMIR_DTYPE_BFLOAT16)
+    return fail_with(MIMIR_ERR_UNSUPPORTED_DTYPE, "paged attention supports bfloat16 queries only (dtype code " + std::to_string(p->dtype) + ")");
+  if (!sizes_ok(p))
+    return fail_with(MIMIR_ERR_INVALID_ARGUMENT, p->num_kv_heads > 0 && p->num_q_heads > 0 && p->num_q_heads % p->num_kv_heads != 0
+                         ? "Query heads " + std::to_string(p->num_q_heads) + " must be divisible by key/value heads " + std::to_string(p->num_kv_heads) + "."
+                         : std::string("negative size or non-positive head count"));
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "head_dim " + std::to_string(p->head_dim) + " is not supported by paged attention (supported: 64, 128)");
+  if (!(p->softmax_scale > 0.f) || !std::isfinite(p->softmax_scale))
+    return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
+  if (p->batch == 0 || p->seqlen == 0) return MIMIR_OK;
+  if (p->num_pages == 0 || p->table_width == 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "the cache holds no pages");
+  if (p->table_width > (1 << 24)) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "page tables wider than 2^24 are not supported");
+  if (p->page_table == nullptr || p->cache_lengths == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "page_table or cache_lengths is NULL");
+  if (p->table_stride < 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "negative table_stride");
+  int rc;
+  if ((rc = check_rows("q", p->q, p->q_stride_batch, p->q_stride_token, p->q_stride_head)) ||
+      (rc = check_rows("k_new", p->k_new, p->kn_stride_batch, p->kn_stride_token, p->kn_stride_head)) ||
+      (rc = check_rows("v_new", p->v_new, p->vn_stride_batch, p->vn_stride_token, p->vn_stride_head)) ||
+      (rc = check_rows("out", p->out, p->out_stride_batch, p->out_stride_token, p->out_stride_head)))
+    return rc;
+  if (p->cache_k == nullptr || p->cache_v == nullptr || p->k_exponents == nullptr || p->v_exponents == nullptr)
+    return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "cache pointer is NULL");
+  const int64_t page = (int64_t)p->num_kv_heads * kPage * p->head_dim;
+  if ((uintptr_t)p->cache_k % 16 != 0 || (uintptr_t)p->cache_v % 16 != 0 || p->k_stride_page % 16 != 0 || p->v_stride_page % 16 != 0 ||
+      (p->num_pages > 1 && (p->k_stride_page < page || p->v_stride_page < page || p->ke_stride_page < p->num_kv_heads ||
+                            p->ve_stride_page < p->num_kv_heads)))
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "pages of the cache must be 16-byte aligned and apart");
+  const Plan plan = plan_of(*p);
+  const int64_t append = (int64_t)p->batch * p->num_kv_heads * ((p->seqlen + 2 * kPage - 2) / kPage);
+  const int64_t rows = (int64_t)p->seqlen * (p->num_q_heads / p->num_kv_heads);
+  if (rows > 0x7fffffff || plan.units > 0x7fffffff || append > 0x7fffffff || (int64_t)p->batch * p->num_kv_heads * ((rows + kWaves - 1) / kWaves) > 0x7fffffff)
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many query rows for one call; split the batch");
+  if (plan.workspace_bytes > 0 && (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || (uintptr_t)p->workspace % 16 != 0))
+    return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned and hold at least " + std::to_string(plan.workspace_bytes) + " bytes");
+  const hipError_t e = launch_paged_attn(*p, plan, (hipStream_t)stream);
+  return e == hipSuccess ? MIMIR_OK : fail_with(MIMIR_ERR_HIP, std::string("paged attention launch: ") + hipGetErrorString(e));
+}
+
+}  // extern "C"
