@@ -279,7 +279,7 @@ class _GeneralPath:
     def fwd(*args):
         return None
 
-    bwd = rope = cache_attn = fwd
+    bwd = rope = cache_attn = rotary = paged_attn = pages = fwd
 
 
 def _load_host():
@@ -311,8 +311,8 @@ _host = None
 def host():
     """The native host calls (csrc/host_calls.cpp), bound to the library.
 
-    ``fwd`` / ``bwd`` / ``rope`` / ``cache_attn`` check, allocate and launch a
-    well-formed call and return None for any other, which then takes the general path.
+    ``fwd`` / ``bwd`` / ``rope`` / ``cache_attn`` / ``rotary`` / ``paged_attn`` / ``pages`` check,
+    allocate and launch a well-formed call and return None for any other, which then takes the general path.
     Where the module is not built, or built for another torch or Python, they serve
     no call.  ImportError if the library itself is not built."""
     global _host
@@ -323,7 +323,10 @@ def host():
         if _host is None:
             module = _load_host()
             if module is not None:
+                import torch
+
                 module.bind(str(LIB_PATH))
+                module.streams(torch._C._cuda_getCurrentRawStream)
             _host = module or _GeneralPath
     return _host
 

@@ -1,6 +1,7 @@
 // The host side of the common calls in native code: argument checks, output
 // allocation, the parameter struct and the C-ABI launch of the forward, the
-// backward, RoPE and the KV-cache attention.
+// backward, RoPE and the KV-cache attention, and of rotary positions (with their
+// gradient), the paged attention and its pages' bookkeeping.
 //
 // Through ctypes these cost 24 us (forward), 32 us (backward) and 17 us (decode) of
 // Python per call, and the backward pays about twice that in a training step: the
@@ -20,7 +21,9 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/mimir_prefixlm.h"
@@ -38,6 +41,15 @@ struct Library {
   decltype(&mimir_prefixlm_cache_attn) cache_attn = nullptr;
   decltype(&mimir_prefixlm_cache_attn_workspace_bytes) cache_workspace = nullptr;
   decltype(&mimir_prefixlm_last_error) last_error = nullptr;
+  // null in a library without them: their calls then take the general path
+  decltype(&mimir_prefixlm_rotary) rotary = nullptr;
+  decltype(&mimir_prefixlm_paged_attn) paged_attn = nullptr;
+  decltype(&mimir_prefixlm_paged_attn_workspace_bytes) paged_workspace = nullptr;
+  decltype(&mimir_prefixlm_pages_workspace_bytes) pages_workspace = nullptr;
+  decltype(&mimir_prefixlm_pages_fork) pages_fork = nullptr;
+  decltype(&mimir_prefixlm_pages_compact) pages_compact = nullptr;
+  decltype(&mimir_prefixlm_pages_release) pages_release = nullptr;
+  decltype(&mimir_prefixlm_pages_reserve) pages_reserve = nullptr;
   c10::DeviceType device = c10::DeviceType::CUDA;  // of the tensors it takes
 } lib;
 
@@ -389,6 +401,326 @@ PyObject* py_cache_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------- rotary positions
+
+struct Rotary {
+  at::Tensor positions, turns;
+  double amplitude;
+  bool interleaved, inverse;
+};
+
+// A [.., tokens, heads, head_dim] operand that the kernel reads in place, like q but for its heads.
+bool rotary_operand(const at::Tensor& t, const at::Tensor& q) {
+  const int64_t n = q.dim();
+  if (t.dim() != n || t.scalar_type() != q.scalar_type() || t.device() != q.device() || t.stride(n - 1) != 1 || t.size(n - 1) != q.size(n - 1))
+    return false;
+  for (int64_t i = 0; i < n - 2; ++i)
+    if (t.size(i) != q.size(i)) return false;
+  return t.numel() > 0 && t.size(n - 2) <= 0x7fffffff;
+}
+bool rotary_served(const at::Tensor& q, const at::Tensor* k, const Rotary& r) {
+  if (lib.rotary == nullptr || !on_device(q) || (q.dim() != 3 && q.dim() != 4) ||
+      (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kFloat) || !rotary_operand(q, q) || (k != nullptr && !rotary_operand(*k, q)))
+    return false;
+  const int64_t n = q.dim(), d = q.size(n - 1), S = q.size(n - 3);
+  const at::Tensor &pos = r.positions, &turns = r.turns;
+  if (turns.dim() != 1 || turns.scalar_type() != at::kLong || turns.device() != q.device() || turns.size(0) < 1 || turns.size(0) > d / 2 ||
+      !turns.is_contiguous() || pos.device() != q.device() || (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt))
+    return false;
+  if (S > 0x7fffffff || (n == 4 && q.size(0) > 0x7fffffff)) return false;
+  // [tokens], or [batch, tokens]
+  return pos.size(pos.dim() - 1) == S && (pos.dim() == 1 || (pos.dim() == 2 && n == 4 && pos.size(0) == q.size(0)));
+}
+
+int launch_rotary(const at::Tensor& q, const at::Tensor* k, const Rotary& r, const at::Tensor& qo, const at::Tensor* ko, void* s) {
+  const int64_t n = q.dim();
+  MimirRotaryParams p = {};
+  auto strides = [n](const at::Tensor& t, int64_t& sb, int64_t& st, int64_t& sh) {
+    sb = n == 4 ? t.stride(0) : 0, st = t.stride(n - 3), sh = t.stride(n - 2);
+  };
+  p.q = q.const_data_ptr(), p.q_out = qo.mutable_data_ptr();
+  strides(q, p.q_stride_batch, p.q_stride_token, p.q_stride_head);
+  strides(qo, p.q_out_stride_batch, p.q_out_stride_token, p.q_out_stride_head);
+  if (k != nullptr) {
+    p.k = k->const_data_ptr(), p.k_out = ko->mutable_data_ptr();
+    strides(*k, p.k_stride_batch, p.k_stride_token, p.k_stride_head);
+    strides(*ko, p.k_out_stride_batch, p.k_out_stride_token, p.k_out_stride_head);
+    p.num_kv_heads = (int32_t)k->size(n - 2);
+  }
+  p.turns = r.turns.const_data_ptr<int64_t>(), p.positions = r.positions.const_data_ptr();
+  p.positions_stride_batch = r.positions.dim() == 2 ? r.positions.stride(0) : 0;
+  p.positions_stride_token = r.positions.stride(r.positions.dim() - 1);
+  p.batch = n == 4 ? (int32_t)q.size(0) : 1, p.seqlen = (int32_t)q.size(n - 3);
+  p.num_q_heads = (int32_t)q.size(n - 2), p.head_dim = (int32_t)q.size(n - 1), p.rotary_dim = (int32_t)(2 * r.turns.size(0));
+  p.interleaved = r.interleaved, p.inverse = r.inverse, p.amplitude = (float)r.amplitude;
+  p.dtype = q.scalar_type() == at::kBFloat16 ? MIMIR_DTYPE_BFLOAT16 : MIMIR_DTYPE_FLOAT32;
+  p.index_int64 = r.positions.scalar_type() == at::kLong;
+  const c10::DeviceGuard guard(q.device());
+  return lib.rotary(&p, s);
+}
+
+PyObject* current_stream = nullptr;  // torch's own function, device index -> raw handle
+
+// The stream of the thread that asks (the autograd engine's, for a backward).
+void* stream_of(const at::Tensor& t) {
+  const PyGILState_STATE gil = PyGILState_Ensure();
+  PyObject* o = current_stream != nullptr ? PyObject_CallFunction(current_stream, "i", (int)t.device().index()) : nullptr;
+  void* s = o != nullptr ? PyLong_AsVoidPtr(o) : nullptr;
+  const bool ok = o != nullptr && PyErr_Occurred() == nullptr;
+  Py_XDECREF(o);
+  if (!ok) PyErr_Clear();
+  PyGILState_Release(gil);
+  TORCH_CHECK(ok, "the current stream is not known");
+  return s;
+}
+
+// The gradient is the inverse turn, itself differentiable.  In a training step an autograd
+// function in Python took 150 us for a forward and backward of 15 us of GPU work.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const std::optional<at::Tensor>& k,
+                                                const at::Tensor& positions, const at::Tensor& turns, double amplitude, bool interleaved,
+                                                bool inverse, int64_t s) {
+    ctx->save_for_backward({positions, turns});
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["flags"] = (int64_t)interleaved | (int64_t)inverse << 1;
+    ctx->set_materialize_grads(false);
+    const Rotary r = {positions, turns, amplitude, interleaved, inverse};
+    const at::Tensor qo = at::empty(q.sizes(), q.options());
+    const at::Tensor ko = k.has_value() ? at::empty(k->sizes(), k->options()) : at::Tensor();
+    const int status = launch_rotary(q, k.has_value() ? &*k : nullptr, r, qo, &ko, (void*)s);
+    TORCH_CHECK(status == MIMIR_OK, lib.last_error());
+    if (!k.has_value()) return {qo};
+    return {qo, ko};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    torch::autograd::variable_list out(8), given;
+    std::vector<int> at;
+    for (int i = 0; i < (int)grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) {
+        given.push_back(grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous());
+        at.push_back(i);
+      }
+    if (given.empty()) return out;
+    const auto got = apply(given[0], given.size() > 1 ? std::optional<at::Tensor>(given[1]) : std::nullopt, saved[0], saved[1],
+                           ctx->saved_data["amplitude"].toDouble(), (flags & 1) != 0, (flags & 2) == 0, (int64_t)stream_of(given[0]));
+    for (size_t i = 0; i < at.size(); ++i) out[at[i]] = got[i];
+    return out;
+  }
+};
+
+// rotary(query, key or None, positions, turns, amplitude, interleaved, inverse, inplace, stream) -> (query, key or None)
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&](bool& raised) -> PyObject* {
+    TENSOR(q, a[0]);
+    const at::Tensor* k = nullptr;
+    if (!is_none(a[1])) NEED((k = tensor(a[1])) != nullptr);
+    TENSOR(positions, a[2]);
+    TENSOR(turns, a[3]);
+    const Rotary r = {positions, turns, PyFloat_AsDouble(a[4]), truth(a[5]), truth(a[6])};
+    NEED(PyErr_Occurred() == nullptr && rotary_served(q, k, r));
+    at::Tensor qo, ko;
+    const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || (k != nullptr && k->requires_grad()));
+    if (grad) {
+      NEED(!truth(a[7]) && current_stream != nullptr);
+      const auto out = RotaryFunction::apply(q, k != nullptr ? std::optional<at::Tensor>(*k) : std::nullopt, positions, turns, r.amplitude,
+                                             r.interleaved, r.inverse, (int64_t)stream(a[8]));
+      qo = out[0];
+      if (k != nullptr) ko = out[1];
+    } else {
+      if (truth(a[7])) {
+        for (const at::Tensor* t : {&q, k})
+          for (int64_t i = 0; t != nullptr && i < t->dim(); ++i) NEED(t->size(i) <= 1 || t->stride(i) > 0);
+        qo = q;
+        if (k != nullptr) ko = *k;
+      } else {
+        qo = at::empty(q.sizes(), q.options());
+        if (k != nullptr) ko = at::empty(k->sizes(), k->options());
+      }
+      const int status = launch_rotary(q, k, r, qo, &ko, stream(a[8]));
+      if (status == MIMIR_ERR_HIP) {
+        PyErr_SetString(PyExc_RuntimeError, lib.last_error());
+        raised = true;
+      }
+      NEED(status == MIMIR_OK);
+    }
+    PyObject* second = k != nullptr ? THPVariable_Wrap(ko) : Py_NewRef(Py_None);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(qo), second);
+  });
+}
+
+// ---------------------------------------------------------------- paged cache
+
+// The four arrays of a paged cache (a tuple): pages of contiguous [layers, heads, ..] apart.
+struct Paged {
+  const at::Tensor* t[4];
+  int64_t pages, layers, heads, d;
+};
+bool paged_cache(PyObject* o, Paged& c) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  for (int i = 0; i < 4; ++i) {
+    c.t[i] = tensor(PyTuple_GET_ITEM(o, i));
+    if (c.t[i] == nullptr || c.t[i]->dim() != (i < 2 ? 5 : 3) || c.t[i]->device() != c.t[0]->device() || !on_device(*c.t[i]) ||
+        c.t[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kChar))
+      return false;
+  }
+  c.pages = c.t[0]->size(0), c.layers = c.t[0]->size(1), c.heads = c.t[0]->size(2), c.d = c.t[0]->size(4);
+  if (c.pages < 1 || c.pages > (1 << 30) || c.t[0]->size(3) != MIMIR_PAGE_TOKENS || c.t[1]->size(3) != c.d || c.t[1]->size(4) != MIMIR_PAGE_TOKENS)
+    return false;
+  for (const at::Tensor* t : c.t) {
+    if (t->size(0) != c.pages || t->size(1) != c.layers || t->size(2) != c.heads) return false;
+    int64_t dense = 1;
+    for (int64_t i = t->dim() - 1; i > 0; --i) {
+      if (t->size(i) != 1 && t->stride(i) != dense) return false;
+      dense *= t->size(i);
+    }
+    if (dense == 0 || (c.pages > 1 && t->stride(0) < dense)) return false;
+  }
+  return true;
+}
+bool int_rows(const at::Tensor& t, const at::Device& device, int64_t dims) {
+  return t.dim() == dims && t.scalar_type() == at::kInt && t.device() == device && (t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1);
+}
+
+// paged_attn(query, key, value, cache, layer, page_table, cache_lengths, causal, batch_indices, new_lengths, softmax_scale,
+//            stream) -> out
+PyObject* py_paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 12, [&](bool& raised) -> PyObject* {
+    NEED(lib.paged_attn != nullptr && lib.paged_workspace != nullptr);
+    TENSOR(q, a[0]);
+    TENSOR(k, a[1]);
+    TENSOR(v, a[2]);
+    TENSOR(table, a[5]);
+    TENSOR(lens, a[6]);
+    NEED(on_device(q) && q.scalar_type() == at::kBFloat16 && q.dim() == 4 && k.dim() == 4 && v.dim() == 4);
+    const int64_t B = q.size(0), S = q.size(1), hq = q.size(2), d = q.size(3), hkv = k.size(2);
+    NEED(B > 0 && S > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && B <= 0x7fffffff && S <= 0x7fffffff && hq <= 0x7fffffff);
+    for (const at::Tensor* t : {&k, &v}) NEED(t->size(0) == B && t->size(1) == S && t->size(2) == hkv && t->size(3) == d);
+    for (const at::Tensor* t : {&q, &k, &v}) {
+      NEED(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->stride(3) == 1 && (uintptr_t)t->const_data_ptr() % 16 == 0);
+      for (int i = 0; i < 3; ++i) NEED(t->stride(i) % 8 == 0);
+    }
+    Paged c;
+    NEED(paged_cache(a[3], c) && c.heads == hkv && c.d == d && c.t[0]->device() == q.device());
+    int32_t layer;
+    NEED(PyLong_CheckExact(a[4]) && int32(a[4], layer) && layer < c.layers);
+    NEED(int_rows(table, q.device(), 2) && table.size(0) <= 0x7fffffff && table.size(1) <= 0x7fffffff);
+    MimirPagedAttnParams p = {};
+    for (PyObject* o : {a[6], a[8], a[9]}) {
+      if (is_none(o)) continue;
+      TENSOR(t, o);
+      NEED(t.dim() == 1 && t.size(0) == B && t.device() == q.device() && t.is_contiguous() && t.scalar_type() == lens.scalar_type() &&
+           (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt));
+    }
+    p.cache_lengths = lens.const_data_ptr();
+    if (!is_none(a[8])) p.batch_indices = tensor(a[8])->const_data_ptr();
+    if (!is_none(a[9])) p.new_lengths = tensor(a[9])->const_data_ptr();
+    p.index_int64 = lens.scalar_type() == at::kLong;
+    const at::Tensor out = empty({B, S, hq, d}, q, at::kBFloat16);
+    p.q = q.const_data_ptr(), p.k_new = k.const_data_ptr(), p.v_new = v.const_data_ptr(), p.out = out.mutable_data_ptr();
+    STRIDES4(q, q), STRIDES4(kn, k), STRIDES4(vn, v), STRIDES4(out, out);
+    p.cache_k = (char*)c.t[0]->mutable_data_ptr() + layer * hkv * MIMIR_PAGE_TOKENS * d;
+    p.cache_v = (char*)c.t[1]->mutable_data_ptr() + layer * hkv * MIMIR_PAGE_TOKENS * d;
+    p.k_exponents = (int8_t*)c.t[2]->mutable_data_ptr() + layer * hkv;
+    p.v_exponents = (int8_t*)c.t[3]->mutable_data_ptr() + layer * hkv;
+    p.k_stride_page = c.t[0]->stride(0), p.v_stride_page = c.t[1]->stride(0);
+    p.ke_stride_page = c.t[2]->stride(0), p.ve_stride_page = c.t[3]->stride(0);
+    p.page_table = table.const_data_ptr<int32_t>(), p.table_stride = table.stride(0);
+    p.batch = (int32_t)B, p.seqlen = (int32_t)S, p.num_pages = (int32_t)c.pages;
+    p.table_rows = (int32_t)table.size(0), p.table_width = (int32_t)table.size(1);
+    p.num_q_heads = (int32_t)hq, p.num_kv_heads = (int32_t)hkv, p.head_dim = (int32_t)d;
+    p.causal = truth(a[7]);
+    p.dtype = MIMIR_DTYPE_BFLOAT16;
+    p.softmax_scale = (float)PyFloat_AsDouble(a[10]);
+    p.workspace_bytes = lib.paged_workspace(&p);
+    at::Tensor ws;
+    if (p.workspace_bytes > 0) {
+      ws = empty({(int64_t)(p.workspace_bytes / 4)}, q, at::kFloat);
+      p.workspace = ws.mutable_data_ptr();
+    }
+    const c10::DeviceGuard guard(q.device());
+    NEED(launch(lib.paged_attn, p, stream(a[11]), raised));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// pages(call, table, cache or None, first, second or None, stream) -> what the call returns (True for nothing)
+//   "fork": source, destination rows; "compact": None; "release": rows; "reserve": new lengths
+PyObject* py_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&](bool& raised) -> PyObject* {
+    NEED(PyUnicode_Check(a[0]) && PyTuple_Check(a[1]) && PyTuple_GET_SIZE(a[1]) == 4);
+    const char* name = PyUnicode_AsUTF8(a[0]);
+    NEED(name != nullptr && lib.pages_workspace != nullptr);
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+      t[i] = tensor(PyTuple_GET_ITEM(a[1], i));
+      NEED(t[i] != nullptr && on_device(*t[i]) && int_rows(*t[i], t[0]->device(), i == 0 ? 2 : 1) && t[i]->size(0) <= 0x7fffffff);
+    }
+    const int64_t rows = t[0]->size(0), width = t[0]->size(1), pages = t[2]->size(0);
+    NEED(t[1]->size(0) == rows && t[3]->size(0) == 1 && pages <= (1 << 30) && rows > 0 && width > 0 && width <= 0x7fffffff &&
+         (rows == 1 || t[0]->stride(0) >= width));
+    MimirPagesParams p = {};
+    p.pages = t[0]->mutable_data_ptr<int32_t>(), p.lengths = t[1]->mutable_data_ptr<int32_t>();
+    p.counts = t[2]->mutable_data_ptr<int32_t>(), p.missing = t[3]->mutable_data_ptr<int32_t>();
+    p.pages_stride = rows == 1 ? width : t[0]->stride(0);
+    p.rows = (int32_t)rows, p.width = (int32_t)width, p.num_pages = (int32_t)pages;
+    if (!is_none(a[2])) {
+      Paged c;
+      NEED(paged_cache(a[2], c) && c.pages == pages && c.t[0]->device() == t[0]->device());
+      for (int i = 0; i < 4; ++i) {
+        p.data[i] = c.t[i]->mutable_data_ptr();
+        p.data_bytes[i] = c.t[i]->numel() / c.pages;
+        p.data_stride[i] = c.t[i]->stride(0);
+      }
+    }
+    const int32_t* list[2] = {nullptr, nullptr};
+    int64_t items = 0;
+    for (int i = 0; i < 2; ++i) {
+      if (is_none(a[3 + i])) continue;
+      TENSOR(x, a[3 + i]);
+      NEED(int_rows(x, t[0]->device(), 1) && (i == 0 || x.size(0) == items) && x.size(0) > 0 && x.size(0) <= 0x7fffffff);
+      items = x.size(0);
+      list[i] = x.const_data_ptr<int32_t>();
+    }
+    const std::string call = name;
+    at::Tensor ws, used;
+    if (call != "release") {
+      p.workspace_bytes = lib.pages_workspace(&p, call == "fork" ? (int32_t)items : 0);
+      ws = empty({(int64_t)(p.workspace_bytes / 4)}, *t[0], at::kInt);
+      p.workspace = ws.mutable_data_ptr();
+    }
+    const c10::DeviceGuard guard(t[0]->device());
+    void* const s = stream(a[5]);
+    NEED(PyErr_Occurred() == nullptr);
+    int status = MIMIR_ERR_INVALID_ARGUMENT;
+    if (call == "fork" && lib.pages_fork != nullptr && list[0] != nullptr && list[1] != nullptr) {
+      status = lib.pages_fork(&p, list[0], list[1], (int32_t)items, s);
+    } else if (call == "compact" && lib.pages_compact != nullptr) {
+      used = empty({1}, *t[0], at::kInt);
+      status = lib.pages_compact(&p, used.mutable_data_ptr<int32_t>(), s);
+    } else if (call == "release" && lib.pages_release != nullptr && list[0] != nullptr) {
+      status = lib.pages_release(&p, list[0], (int32_t)items, s);
+    } else if (call == "reserve" && lib.pages_reserve != nullptr && list[0] != nullptr && items == rows) {
+      status = lib.pages_reserve(&p, list[0], s);
+    }
+    if (status == MIMIR_ERR_HIP) {
+      PyErr_SetString(PyExc_RuntimeError, lib.last_error());
+      raised = true;
+    }
+    NEED(status == MIMIR_OK);
+    return used.defined() ? THPVariable_Wrap(used) : Py_NewRef(Py_True);
+  });
+}
+
+// streams(function): torch's function from a device index to the raw handle of its current stream.
+PyObject* py_streams(PyObject*, PyObject* f) {
+  PyObject* const old = current_stream;
+  current_stream = Py_NewRef(f);
+  Py_XDECREF(old);
+  Py_RETURN_NONE;
+}
+
 // bind(path, device="cuda"): the entry points of the (already loaded) C-ABI library, and
 // the type of device whose tensors it takes.
 PyObject* py_bind(PyObject*, PyObject* args) {
@@ -417,6 +749,14 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   get(lib.cache_workspace, "mimir_prefixlm_cache_attn_workspace_bytes");
   get(lib.last_error, "mimir_prefixlm_last_error");
   if (!ok) return PyErr_Format(PyExc_ImportError, "%s lacks an entry point", file);
+  get(lib.rotary, "mimir_prefixlm_rotary");
+  get(lib.paged_attn, "mimir_prefixlm_paged_attn");
+  get(lib.paged_workspace, "mimir_prefixlm_paged_attn_workspace_bytes");
+  get(lib.pages_workspace, "mimir_prefixlm_pages_workspace_bytes");
+  get(lib.pages_fork, "mimir_prefixlm_pages_fork");
+  get(lib.pages_compact, "mimir_prefixlm_pages_compact");
+  get(lib.pages_release, "mimir_prefixlm_pages_release");
+  get(lib.pages_reserve, "mimir_prefixlm_pages_reserve");
   Py_RETURN_NONE;
 }
 
@@ -426,6 +766,10 @@ PyMethodDef methods[] = {
     {"bwd", (PyCFunction)(void*)py_bwd, METH_FASTCALL, nullptr},
     {"rope", (PyCFunction)(void*)py_rope, METH_FASTCALL, nullptr},
     {"cache_attn", (PyCFunction)(void*)py_cache_attn, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void*)py_rotary, METH_FASTCALL, nullptr},
+    {"paged_attn", (PyCFunction)(void*)py_paged_attn, METH_FASTCALL, nullptr},
+    {"pages", (PyCFunction)(void*)py_pages, METH_FASTCALL, nullptr},
+    {"streams", py_streams, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods};

@@ -132,6 +132,13 @@ def _workspace(p: _capi.PagesParams, items: int, device) -> Tensor:
     return ws
 
 
+def _served(call: str, table: PageTable, cache: Optional[PagedCache], first=None, second=None):
+    """The call's result from the native host calls, None if it takes the general path."""
+    if not table.pages.is_cuda:
+        return None
+    return _capi.host().pages(call, table, cache, first, second, P._stream(table.pages.device))
+
+
 def _call(entry: str, device, p, *args) -> None:
     lib = _capi.load()
     with torch.cuda.device(device):
@@ -168,6 +175,8 @@ def fork_rows(cache: PagedCache, table: PageTable, source: Tensor, destination: 
     for one destination the last counts.  Pages reserved past the source's tokens are not
     forked.  Where no page is free the destination's last page stays -1 and ``table.missing``
     counts it."""
+    if _served("fork", table, cache, source, destination) is not None:
+        return
     p = _params(table, cache)
     device = table.pages.device
     src, dst = _row_list("source", source, device), _row_list("destination", destination, device)
@@ -180,6 +189,9 @@ def fork_rows(cache: PagedCache, table: PageTable, source: Tensor, destination: 
 def compact_pages(cache: PagedCache, table: PageTable) -> Tensor:
     """Move the pages in use to the front of the pool, all layers, and rename them in the table.
     Returns their number (int32 [1], on the device): the pool can be cut there."""
+    used = _served("compact", table, cache)
+    if used is not None:
+        return used
     p = _params(table, cache)
     device = table.pages.device
     used = torch.empty(1, dtype=torch.int32, device=device)
@@ -191,6 +203,8 @@ def compact_pages(cache: PagedCache, table: PageTable) -> Tensor:
 def release_rows(table: PageTable, rows: Tensor) -> None:
     """The listed rows give back their pages and hold no tokens (numbers outside the table are skipped,
     one may come twice)."""
+    if _served("release", table, None, rows) is not None:
+        return
     p = _params(table)
     device = table.pages.device
     rows = _row_list("rows", rows, device)
@@ -201,6 +215,8 @@ def reserve_pages(table: PageTable, new_lengths: Tensor) -> None:
     """Give every row the pages that it lacks for ``lengths + new_lengths`` tokens (none where
     ``new_lengths`` is 0), by row, then place, the lowest free page first.  The lengths stay: add the new ones
     when they have been appended.  Pages the pool does not have are counted in ``table.missing``."""
+    if _served("reserve", table, None, new_lengths) is not None:
+        return
     p = _params(table)
     device = table.pages.device
     new = _row_list("new_lengths", new_lengths, device)
@@ -266,6 +282,12 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
     Both raise with ``mimir_amd.set_validate_metadata(True)``, which costs a host read.  Infinite
     keys and values become NaN.
     """
+    scale = (1.0 / math.sqrt(query.shape[-1]) if query.shape[-1] else 1.0) if softmax_scale is None else float(softmax_scale)
+    if query.is_cuda and not P._validate_metadata:
+        out = _capi.host().paged_attn(query, key, value, cache, layer, page_table, cache_lengths, causal, cache_batch_indices,
+                                      new_lengths, scale, P._stream(query.device))
+        if out is not None:
+            return out
     if query.dtype != torch.bfloat16:
         raise TypeError(f"paged attention supports bfloat16 tensors only, got {query.dtype}")
     for name, t in (("query", query), ("key", key), ("value", value)):
@@ -313,7 +335,7 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
         ck.stride(0), cv.stride(0), ke.stride(0), ve.stride(0), page_table.stride(0),
         B, S, pages, *page_table.shape, hq, hkv, d, int(bool(causal)), _capi.DTYPE_BFLOAT16, int(index_dtype == torch.int64),
-        1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale), None, 0)
+        scale, None, 0)
     lib = _capi.load()
     ws_bytes = int(lib.mimir_prefixlm_paged_attn_workspace_bytes(ctypes.byref(p)))
     ws = torch.empty(max(ws_bytes // 4, 4), dtype=torch.float32, device=device)

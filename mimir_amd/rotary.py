@@ -183,6 +183,10 @@ def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
     the other way, which is also the gradient; any strides with a unit one on head_dim
     are read in place, so that the heads of a fused projection need no copy.
     """
+    if query.is_cuda:
+        res = _capi.host().rotary(query, key, positions, *frequencies, inverse, inplace, P._stream(query.device))
+        if res is not None:
+            return res
     positions = _check(query, key, positions, frequencies)
     grad = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
     if inplace:
