@@ -44,12 +44,11 @@ __device__ __forceinline__ float xor16_sum(float x) {
   return __int_as_float(a) + __int_as_float(b);
 }
 
-// bf16 1 where a bit of the lowest eight is set, 0 elsewhere.
-__device__ __forceinline__ bf16x8 ones_where(unsigned bits) {
-  i32x4 x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (int)((bits >> (2 * i) & 1) * 0x3f80u | (bits >> (2 * i + 1) & 1) * 0x3f800000u);
-  return __builtin_bit_cast(bf16x8, x);
+// Between LDS writes and reads of one wave's own: they complete in order, the compiler has to keep it.
+__device__ __forceinline__ void wave_lds_fence() {
+  __asm__ volatile("" ::: "memory");
+  wait_lds();
+  __asm__ volatile("" ::: "memory");
 }
 
 // ------------------------------------------------------------------ partial rows
@@ -184,8 +183,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
   constexpr int kRowsMax = 16 * NR;
   constexpr int kPitch = D + 4;
   __shared__ Line line;
-  __shared__ float area[kWaves][kRowsMax * kPitch];
+  __shared__ __attribute__((aligned(16))) float area[kWaves][kRowsMax * kPitch];
   __shared__ f32x2 area_ml[kWaves][kRowsMax];
+  __shared__ __attribute__((aligned(8))) unsigned short s_nan[kWaves][D * 4];  // NaN tokens of each column, by wave
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -239,8 +239,10 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 
     // Q^T operands: lane holds query row m16 (+ 16), columns 64 h + 16 g + 8 s ..+7; rows past the
     // last take the first (never read).  Each row's key limit; 0 for queries i >= m.
-    bf16x8 qf[NR][2 * KH];
+    // They wait in LDS, a copy for each wave in its part of the merge's area: registers for them would
+    // spill with two row tiles.
     int limit[NR];
+    i32x4* const q_lds = (i32x4*)area[wave] + lane;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0;
@@ -250,8 +252,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 #pragma unroll
       for (int h = 0; h < KH; ++h)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) qf[nr][2 * h + s] = *(const bf16x8*)&q[64 * h + 8 * s];
+        for (int s = 0; s < 2; ++s) q_lds[(nr * 2 * KH + 2 * h + s) * 64] = *(const i32x4*)&q[64 * h + 8 * s];
     }
+    wave_lds_fence();
     const int limit_min = a.causal ? min(r.n + 1, r.kv) : r.kv;
 
     // The wave's pages, 64 at a time on its lanes: page id (-1: none) and exponents.
@@ -298,18 +301,24 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       const float ks = pow2(__builtin_amdgcn_readlane(ek, i & 63)), vs = pow2(__builtin_amdgcn_readlane(ev, i & 63));
       f32x4 st[NR][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) st[nr][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) st[nr][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      __asm__ volatile("" ::: "memory");  // read again for every page
 #pragma unroll
-        for (int h = 0; h < KH; ++h)
+      for (int h = 0; h < KH; ++h)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < 2; ++s) {
+          bf16x8 qf[NR];
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) qf[nr] = __builtin_bit_cast(bf16x8, q_lds[(nr * 2 * KH + 2 * h + s) * 64]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
             const bf16x8 kf = decode8(kreg[t][h][2 * s], kreg[t][h][2 * s + 1], ks);
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) st[nr][t] = mfma16(kf, qf[nr][2 * h + s], st[nr][t]);
+            for (int nr = 0; nr < NR; ++nr) st[nr][t] = mfma16(kf, qf[nr], st[nr][t]);
           }
-      }
+        }
       const bool last_of_ids = (i & 63) == 63;
       if (i + 1 < n_my) {
         if (last_of_ids) load_ids(i + 1);
@@ -362,6 +371,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
           pf[nr][c] = to_bf16x8(x);
         }
       }
+      bool any_nan = false;
       if (edge) {
         // What lies behind the last token is unwritten; a NaN among the values of tokens that only
         // some of the rows see must not reach the others: it is taken out of the product
@@ -375,30 +385,20 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
             vreg[d][w] = codes_before(vreg[d][w], 4 * w, end);
             nan |= nan_codes(vreg[d][w]);
           }
-        if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+        any_nan = __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+        if (any_nan) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
             unsigned at = 0;  // tokens 16 g + e whose code is NaN
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int w = e >> 2, sh = 8 * (e & 3);
-              if (((unsigned)vreg[d][w] >> sh & 0x7f) == 0x7f) {
+            for (int e = 0; e < 16; ++e)
+              if (((unsigned)vreg[d][e >> 2] >> 8 * (e & 3) & 0x7f) == 0x7f) {
                 at |= 1u << e;
-                vreg[d][w] &= (int)~(0xffu << sh);
+                vreg[d][e >> 2] &= (int)~(0xffu << 8 * (e & 3));
               }
-            }
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-              const int see = limit[nr] - base - 16 * g;  // of the lane group's tokens
-              const unsigned seen = see >= 16 ? 0xffffu : (see <= 0 ? 0u : (1u << see) - 1);
-              f32x4 hit = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int c = 0; c < 2; ++c) hit = mfma16(ones_where(at >> (8 * c)), ones_where(seen >> (8 * c)), hit);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (hit[e] > 0.f) oacc[nr][d][e] = __builtin_nanf("");
-            }
+            s_nan[wave][(16 * d + m16) * 4 + g] = (unsigned short)at;
           }
+          wave_lds_fence();
         }
       }
 #pragma unroll
@@ -409,6 +409,19 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 #pragma unroll
           for (int nr = 0; nr < NR; ++nr) oacc[nr][d] = mfma16(vf, pf[nr][c], oacc[nr][d]);
         }
+      if (any_nan) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+          const int n = limit[nr] - base;
+          const uint64_t seen = n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (*(const uint64_t*)&s_nan[wave][(16 * d + 4 * g + e) * 4] & seen) oacc[nr][d][e] = __builtin_nanf("");
+        }
+        wave_lds_fence();
+      }
       if (i + 1 < n_my) load_values(i + 1);
     }
 
@@ -510,6 +523,15 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 constexpr int kRows = kWaves * 32;
 constexpr int kMaxSplits = 64;
 
+// Whether the batch rows hold about as many cached keys: none differs from the first by more
+// than an eighth of the chunk.
+__device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
+  if (a.B > 64) return false;
+  const int n = PagedRow(a, min((int)threadIdx.x & 63, a.B - 1)).n;
+  const int64_t off = n - __builtin_amdgcn_readfirstlane(n);
+  return __builtin_amdgcn_ballot_w64(8 * (off < 0 ? -off : off) > a.S) == 0;
+}
+
 template <int D>
 __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   constexpr int DT = D / 32, KS = D / 16;
@@ -518,16 +540,28 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   using LV = TileLayout<64>;              // 64 columns of values by 64 tokens
   __shared__ __attribute__((aligned(16))) bf16_t sK[2][LK::kElems];
   __shared__ __attribute__((aligned(16))) bf16_t sV[2][D / 64 * LV::kElems];
-  __shared__ int s_nan[2][kWaves];
+  // which tokens' values are NaN, for each column (a word of 64 bits), and whether any are, by wave
+  __shared__ __attribute__((aligned(8))) unsigned short s_nan[2][D * 4];
+  __shared__ int s_any[2][kWaves];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
-  int u = blockIdx.x;
-  const int split = u % a.splits;
-  u /= a.splits;
-  const int rt = a.n_rt - 1 - u % a.n_rt;  // later rows see more keys: first
-  u /= a.n_rt;
+  // Later row tiles of a causal chunk see more keys, and workgroups u and u + (CUs) share a CU.  On
+  // rows of about the same length they go by rank, the latest first over all pairs, and every
+  // other CU-sized run backwards, so that a CU's two are a long and a short one.
+  int u = blockIdx.x, split = 0, rt;
+  if (a.splits == 1 && a.causal && even_lengths(a)) {
+    const int run = u / a.cus, pairs = gridDim.x / a.n_rt;
+    if (run % 2 == 1 && (run + 1) * a.cus <= (int)gridDim.x) u = (2 * run + 1) * a.cus - 1 - u;
+    rt = a.n_rt - 1 - u / pairs;
+    u %= pairs;
+  } else {
+    split = u % a.splits;
+    u /= a.splits;
+    rt = a.n_rt - 1 - u % a.n_rt;
+    u /= a.n_rt;
+  }
   const int hk = u % a.Hkv, b = u / a.Hkv;
   const PagedRow r(a, b);
   const int R = a.S * a.G, Rm = r.kv > 0 ? r.m * a.G : 0;  // rows, and those that attend
@@ -550,12 +584,11 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const int kt1 = min((wg_max + kPage - 1) / kPage, kt0 + per);
 
   i32x4 kreg[kPer], vreg[kPer];
-  int ek = 0, ev = 0;
-  bool some = false;
+  int ek = 0, ev = 0, some = 0;
   auto load_page = [&](int kt) __attribute__((always_inline)) {
     const int id = load_const(a.table, (int64_t)r.row * a.t_st + kt);
     some = id >= 0 && id < a.num_pages;
-    const int64_t p = some ? id : 0;  // none: page 0, masked
+    const int64_t p = some ? id : 0;  // none: page 0, not attended
     ek = a.ke[p * a.ke_sp + hk];
     ev = a.ve[p * a.ve_sp + hk];
     const uint8_t* kp = a.ck + p * a.k_sp + (int64_t)hk * kPage * D;
@@ -566,10 +599,14 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       vreg[i] = *(const i32x4*)&vp[(i * kThreads + tid) * 16];
     }
   };
+  // Where a page holds tokens that some rows of the workgroup do not see: what lies behind
+  // the last one is unwritten, and a NaN value must not reach the rows that do not see it (0
+  // times NaN), so both are cleared and the NaN tokens noted.
   auto stage_page = [&](int kt, int buf) __attribute__((always_inline)) {
     const float ks = pow2(ek), vs = pow2(ev);
-    const int base = kt * kPage, end = some ? r.kv - base : 0;
-    unsigned nan = 0;
+    const int base = kt * kPage;
+    const bool edge = base + kPage > wg_min;
+    unsigned any = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int unit = i * kThreads + tid;
@@ -579,19 +616,33 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       *(bf16x8*)(kd + 8) = decode8(kreg[i][2], kreg[i][3], ks);
       const int d = unit / 4, t16 = unit % 4 * 16;
       i32x4 v = vreg[i];
-      if (end < kPage) {
+      if (edge) {
+        unsigned nan = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v[w] = codes_before(v[w], t16 + 4 * w, end);
+        for (int w = 0; w < 4; ++w) {
+          v[w] = codes_before(v[w], t16 + 4 * w, r.kv - base);
+          nan |= nan_codes(v[w]);
+        }
+        unsigned at = 0;
+        if (nan != 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (((unsigned)v[e >> 2] >> 8 * (e & 3) & 0x7f) == 0x7f) {
+              at |= 1u << e;
+              v[e >> 2] &= (int)~(0xffu << 8 * (e & 3));
+            }
+          any = 1;
+        }
+        s_nan[buf][unit] = (unsigned short)at;
       }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) nan |= nan_codes(v[w]);
       bf16_t* const vd = &sV[buf][(d >> 6) * LV::kElems + LV::off(d & 63, t16)];
       *(bf16x8*)vd = decode8(v[0], v[2], vs);
       *(bf16x8*)(vd + 8) = decode8(v[1], v[3], vs);
     }
-    // NaN values matter apart only where rows of the workgroup see different tokens
-    const bool any = base + kPage > wg_min && __builtin_amdgcn_ballot_w64(nan != 0) != 0;
-    if (lane == 0) s_nan[buf][wave] = any | (some ? 0 : 2);
+    if (edge) {
+      const int found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      if (lane == 0) s_any[buf][wave] = found;
+    }
   };
 
   if (kt0 < kt1) load_page(kt0);
@@ -608,11 +659,9 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const float c2 = a.scale_log2;
   const int k_base = LK::off(l32, 8 * hi), v_base = LV::off(l32, 8 * hi);
 
-  auto compute = [&](int kt, int buf) __attribute__((always_inline)) {
+  auto compute = [&](int kt, int buf, int there) __attribute__((always_inline)) {
     const int base = kt * kPage;
-    if (!active || base >= w_max) return;
-    const int flags = s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3];
-    if (__builtin_amdgcn_readfirstlane(flags) & 2) return;  // no page here
+    if (!active || base >= w_max || !there) return;
     f32x16 st[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -673,55 +722,32 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       for (int e = 0; e < 8; ++e) t[e] = st[kk >> 1][8 * (kk & 1) + e];
       pf[kk] = to_bf16x8(t);
     }
-    if (flags & 1) {
-      // Values that are NaN: out of the product, and into the rows that see them.
-      bf16x8 see[4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        unsigned bits = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int f = 8 * (kk & 1) + e;
-          bits |= (base + 32 * (kk >> 1) + 8 * (f >> 2) + 4 * hi + (f & 3) < limit ? 1u : 0u) << e;
-        }
-        see[kk] = ones_where(bits);
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        f32x16 hit = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          i32x4 v = *(const i32x4*)&sV[buf][(dt >> 1) * LV::kElems + v_base + (dt & 1) * 32 * LV::kRowElems + kk * 16];
-          unsigned bits = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if ((v[e >> 1] >> (16 * (e & 1)) & 0x7fff) > 0x7f80) {
-              bits |= 1u << e;
-              v[e >> 1] &= e & 1 ? 0xffff : (int)0xffff0000;
-            }
-          hit = mfma32(ones_where(bits), see[kk], hit);
-          oacc[dt] = mfma32(__builtin_bit_cast(bf16x8, v), pf[kk], oacc[dt]);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (hit[e] > 0.f) oacc[dt][e] = __builtin_nanf("");
-      }
-      return;
-    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         oacc[dt] = mfma32(*(const bf16x8*)&sV[buf][(dt >> 1) * LV::kElems + v_base + (dt & 1) * 32 * LV::kRowElems + kk * 16],
                           pf[kk], oacc[dt]);
+    if (base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[buf][0] | s_any[buf][1] | s_any[buf][2] | s_any[buf][3])) {
+      // NaN values into the rows that see them
+      const int n = limit - base;
+      const uint64_t seen = n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int d = 32 * dt + 8 * (e >> 2) + 4 * hi + (e & 3);
+          if (*(const uint64_t*)&s_nan[buf][4 * d] & seen) oacc[dt][e] = __builtin_nanf("");
+        }
+    }
   };
 
   if (kt0 < kt1) stage_page(kt0, 0);
   __syncthreads();
   for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1;
+    const int buf = (kt - kt0) & 1, there = some;
     if (kt + 1 < kt1) load_page(kt + 1);
-    compute(kt, buf);
+    compute(kt, buf, there);
     if (kt + 1 < kt1) stage_page(kt + 1, buf ^ 1);
     __syncthreads();
   }
@@ -808,7 +834,7 @@ Plan plan_of(const MimirPagedAttnParams& p) {
   }
   s.n_rt = (int)((R + kRows - 1) / kRows);
   const int64_t groups = pairs * s.n_rt;
-  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + groups - 1) / groups, p.table_width, kMaxSplits}));
+  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, p.table_width, kMaxSplits}));
   s.units = groups * s.splits;
   s.workspace_bytes = s.splits > 1 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
   return s;
