@@ -16,26 +16,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The exponent that the largest finite magnitude needs, from its bf16 bits (448 = 1.75 * 2^8).
-__device__ __forceinline__ int exponent_for(int bits) {
-  const int e = (bits >> 7) - 127 - 8 + ((bits & 0x7f) > 96);
-  return e > kMinExponent ? e : kMinExponent;
-}
-
-// x / 2^e rounded to e4m3, four values to a word; infinities become NaN.
-__device__ __forceinline__ float coded_value(float x, int e) {
-  return __builtin_fabsf(x) <= 3.4028235e38f ? __builtin_amdgcn_ldexpf(x, -e) : __builtin_nanf("");
-}
-__device__ __forceinline__ int encode4(float a, float b, float c, float d) {
-  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
-}
-// Four codes times 2^shift, rounded to codes again.
-__device__ __forceinline__ int recode4(int x, int shift) {
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-  return encode4(__builtin_amdgcn_ldexpf(lo[0], shift), __builtin_amdgcn_ldexpf(lo[1], shift),
-                 __builtin_amdgcn_ldexpf(hi[0], shift), __builtin_amdgcn_ldexpf(hi[1], shift));
-}
-
 template <int D>
 __device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touched) {
   constexpr int kUnits = D / 8;                  // threads of a row
@@ -72,12 +52,7 @@ __device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touche
     const int t = p * kStep + row;
     v[p] = bf16x8{};
     if (t < s1 - s0) v[p] = *(const bf16x8*)&x[(int64_t)t * x_st + c];
-    const i32x4 words = __builtin_bit_cast(i32x4, v[p]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int bits = words[e >> 1] >> (16 * (e & 1)) & 0x7fff;
-      most = max(most, bits < 0x7f80 ? bits : 0);
-    }
+    most = max(most, largest_bits(__builtin_bit_cast(i32x4, v[p])));
   }
   const int had = s0 > 0 ? *ey : kMinExponent;
 #pragma unroll

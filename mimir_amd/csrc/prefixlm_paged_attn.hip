@@ -1,10 +1,11 @@
 // Attention over an 8-bit paged KV cache, bf16 queries, for gfx950 (MI355X).
 //
-//   paged_append_*        the new rows into their pages (prefixlm_paged_append.hip)
 //   decode (at most 32 query rows per kv head, e.g. S = 1):
-//     paged_decode_*      the workgroups take equal shares of all pages of the call
+//     paged_decode_*      appends the new tokens and attends, the workgroups equal shares of all
+//                         pages of the call
 //     paged_merge_*       adds the partial rows of the shares
 //   otherwise:
+//     paged_append_*      the new tokens into their pages (prefixlm_paged_append.hip)
 //     paged_prefill_*     one workgroup per (batch row, kv head, 128 query rows, key split)
 //     paged_merge_splits_* with several splits: adds their partial rows
 //
@@ -42,6 +43,18 @@ __device__ __forceinline__ float xor16_sum(float x) {
   auto r = __builtin_amdgcn_permlane16_swap(xi, xi, false, false);
   const int a = r[0], b = r[1];
   return __int_as_float(a) + __int_as_float(b);
+}
+
+// The largest of the lanes' non-negative values, on every lane (DPP moves; six shuffles through LDS take
+// six round trips).
+__device__ __forceinline__ int wave_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr:1
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));  // row_shr:2
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));  // row_shr:4
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));  // row_shr:8
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15 into rows 1 and 3
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));  // row_bcast:31 into rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 // Between LDS writes and reads of one wave's own: they complete in order, the compiler has to keep it.
@@ -182,6 +195,9 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
   constexpr int DT = D / 16;   // column tiles of the output
   constexpr int kRowsMax = 16 * NR;
   constexpr int kPitch = D + 4;
+  // Two row tiles of head_dim 128 leave no registers for a page of keys and of values at once: the
+  // values are requested when the keys are used, and the other way round.
+  constexpr bool kTakeTurns = NR == 2 && D == 128;
   __shared__ Line line;
   __shared__ __attribute__((aligned(16))) float area[kWaves][kRowsMax * kPitch];
   __shared__ f32x2 area_ml[kWaves][kRowsMax];
@@ -237,24 +253,13 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
     }
     const int n_my = t0 + wave < t1 ? (t1 - t0 - wave + kUnit - 1) / kUnit : 0;  // this wave's pages
 
-    // Q^T operands: lane holds query row m16 (+ 16), columns 64 h + 16 g + 8 s ..+7; rows past the
-    // last take the first (never read).  Each row's key limit; 0 for queries i >= m.
-    // They wait in LDS, a copy for each wave in its part of the merge's area: registers for them would
-    // spill with two row tiles.
+    // Each row's key limit; 0 for queries i >= m.
     int limit[NR];
-    i32x4* const q_lds = (i32x4*)area[wave] + lane;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-      const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0;
-      const int i = row / a.G;
+      const int i = (16 * nr + m16) / a.G;
       limit[nr] = 16 * nr + m16 < R && i < r.m ? (a.causal ? min(r.n + i + 1, r.kv) : r.kv) : 0;
-      const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)i * a.q_st + (int64_t)(hk * a.G + row - i * a.G) * a.q_sh + 16 * g;
-#pragma unroll
-      for (int h = 0; h < KH; ++h)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) q_lds[(nr * 2 * KH + 2 * h + s) * 64] = *(const i32x4*)&q[64 * h + 8 * s];
     }
-    wave_lds_fence();
     const int limit_min = a.causal ? min(r.n + 1, r.kv) : r.kv;
 
     // The wave's pages, 64 at a time on its lanes: page id (-1: none) and exponents.
@@ -272,14 +277,135 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int h = 0; h < KH; ++h) kreg[t][h] = *(const i32x4*)&p[k_off + 4 * t * D + 64 * h];
+        for (int h = 0; h < KH; ++h) kreg[t][h] = __builtin_nontemporal_load((const i32x4*)&p[k_off + 4 * t * D + 64 * h]);
     };
     auto load_values = [&](int i) __attribute__((always_inline)) {
       const int id = max(__builtin_amdgcn_readlane(ids, i & 63), 0);
       const uint8_t* p = a.cv + id * a.v_sp + (int64_t)hk * kPage * D;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vreg[d] = *(const i32x4*)&p[v_off + 16 * kPage * d];
+      for (int d = 0; d < DT; ++d) vreg[d] = __builtin_nontemporal_load((const i32x4*)&p[v_off + 16 * kPage * d]);
     };
+
+    // The wave's page with new tokens, if any, is its last (they lie in two pages at most): tokens
+    // s0 .. s0 + cnt - 1 of it.  This wave alone reads and writes that page and head in the call, so the
+    // codes go to memory and, beside it, straight into the operands.
+    constexpr int kUnits = D / 8, kNewRows = 64 / kUnits;  // lanes of a new row, rows at a time
+    const int last = t0 + wave + kUnit * (n_my - 1);
+    const int new0 = max(r.n, last * kPage), s0 = new0 - last * kPage;
+    const int cnt = n_my > 0 ? max(min(r.n + r.m, min(last + 1, a.width) * kPage) - new0, 0) : 0;
+    const bf16_t* const x_k = a.kn + (int64_t)b * a.kn_sb + (int64_t)hk * a.kn_sh + (int64_t)(new0 - r.n) * a.kn_st;
+    const bf16_t* const x_v = a.vn + (int64_t)b * a.vn_sb + (int64_t)hk * a.vn_sh + (int64_t)(new0 - r.n) * a.vn_st;
+    i32x4 k_first = {0, 0, 0, 0}, v_first = {0, 0, 0, 0};  // the lane's first new row, requested with the queries
+    constexpr int kQueryBytes = NR * 2 * KH * 64 * 16;
+    static_assert(kQueryBytes + 2 * kRowsMax * D <= kRowsMax * kPitch * 4, "the queries and the new codes fit the wave's area");
+    uint8_t* const codes = (uint8_t*)area[wave] + kQueryBytes;  // [2][cnt][D]
+    auto append = [&](int i, int& e_k, int& e_v) __attribute__((always_inline)) {
+      // lane numbers that the compiler cannot see through: what is formed from them here would otherwise be
+      // held in registers through the loop over the pages (150 instead of 194 at head_dim 64)
+      const int lane = opaque_lane_id(), m16 = lane & 15, g = lane >> 4, x_row = lane / kUnits, x_col = lane % kUnits * 8;
+      const bf16_t* const xk = x_k + x_col;
+      const bf16_t* const xv = x_v + x_col;
+      const int page = __builtin_amdgcn_readlane(ids, i), had_k = e_k, had_v = e_v;
+      int most_k = largest_bits(k_first), most_v = largest_bits(v_first);
+      for (int t = x_row + kNewRows; t < cnt; t += kNewRows) {
+        most_k = max(most_k, largest_bits(*(const i32x4*)&xk[(int64_t)t * a.kn_st]));
+        most_v = max(most_v, largest_bits(*(const i32x4*)&xv[(int64_t)t * a.vn_st]));
+      }
+      e_k = exponent_for(wave_max(most_k));
+      e_v = exponent_for(wave_max(most_v));
+      if (s0 > 0) {
+        e_k = max(e_k, had_k);
+        e_v = max(e_v, had_v);
+      }
+      if (lane == 0) {
+        a.ke[page * a.ke_sp + hk] = (int8_t)e_k;
+        a.ve[page * a.ve_sp + hk] = (int8_t)e_v;
+      }
+      uint8_t* const yk = a.ck + page * a.k_sp + (int64_t)hk * kPage * D;
+      uint8_t* const yv = a.cv + page * a.v_sp + (int64_t)hk * kPage * D;
+      if (s0 > 0 && (e_k > had_k || e_v > had_v)) {
+        // Now and then (a larger magnitude than the page has seen): the older codes rounded again in memory,
+        // and the page read again.
+        for (int w = lane; w < s0 * D / 4; w += 64) ((int*)yk)[w] = recode4(((int*)yk)[w], had_k - e_k);
+        for (int w = lane; w < 16 * D; w += 64) {
+          const int old = ((int*)yv)[w], end = s0 - w % 16 * 4;  // older tokens of the word
+          const unsigned keep = end >= 4 ? 0u : (end <= 0 ? ~0u : ~0u << (8 * end));
+          ((int*)yv)[w] = (int)(((unsigned)recode4(old, had_v - e_v) & ~keep) | ((unsigned)old & keep));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        load_keys(i);
+        load_values(i);
+      }
+      for (int t = x_row; t < cnt; t += kNewRows) {
+        const i32x4 xs[2] = {t == x_row ? k_first : *(const i32x4*)&xk[(int64_t)t * a.kn_st],
+                             t == x_row ? v_first : *(const i32x4*)&xv[(int64_t)t * a.vn_st]};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const bf16x8 v = __builtin_bit_cast(bf16x8, xs[w]);
+          const int e = w ? e_v : e_k;
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] = coded_value((float)v[k], e);
+          const i32x2 c = {encode4(f[0], f[1], f[2], f[3]), encode4(f[4], f[5], f[6], f[7])};
+          *(i32x2*)&codes[(w * cnt + t) * D + x_col] = c;
+          if (w == 0) *(i32x2*)&yk[(s0 + t) * D + x_col] = c;
+        }
+      }
+      wave_lds_fence();
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int j = 16 * (m16 >> 2) + 4 * t + (m16 & 3) - s0;
+        if (j >= 0 && j < cnt) {
+#pragma unroll
+          for (int h = 0; h < KH; ++h) kreg[t][h] = *(const i32x4*)&codes[j * D + 64 * h + 16 * g];
+        }
+      }
+      for (int j = 0; j < cnt; ++j) {
+        const int slot = s0 + j, sh = 8 * (slot & 3);
+        if (g == slot >> 4) {
+          const uint8_t* const x = &codes[(cnt + j) * D + m16];
+          unsigned c[DT];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) c[d] = x[16 * d];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) yv[(16 * d + m16) * kPage + slot] = (uint8_t)c[d];
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (w == (slot & 15) >> 2) {  // uniform
+#pragma unroll
+              for (int d = 0; d < DT; ++d) vreg[d][w] = (int)(((unsigned)vreg[d][w] & ~(0xffu << sh)) | c[d] << sh);
+            }
+        }
+      }
+    };
+
+    // Q^T operands: lane holds query row m16 (+ 16), columns 64 h + 16 g + 8 s ..+7; rows past the last
+    // take the first (never read).  They wait in LDS, a copy for each wave in its part of the merge's area:
+    // registers for them would spill with two row tiles.
+    i32x4* const q_lds = (i32x4*)area[wave] + lane;
+    i32x4 q_in[NR][2 * KH];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0, i = row / a.G;
+      const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)i * a.q_st + (int64_t)(hk * a.G + row - i * a.G) * a.q_sh + 16 * g;
+#pragma unroll
+      for (int x = 0; x < 2 * KH; ++x) q_in[nr][x] = *(const i32x4*)&q[64 * (x >> 1) + 8 * (x & 1)];
+    }
+    if (n_my > 0) {
+      load_ids(0);
+      const int x_row = lane / kUnits, x_col = lane % kUnits * 8;
+      if (x_row < cnt) {
+        k_first = *(const i32x4*)&x_k[(int64_t)x_row * a.kn_st + x_col];
+        v_first = *(const i32x4*)&x_v[(int64_t)x_row * a.vn_st + x_col];
+      }
+      load_keys(0);
+      if (!kTakeTurns) load_values(0);
+    }
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int x = 0; x < 2 * KH; ++x) q_lds[(nr * 2 * KH + x) * 64] = q_in[nr][x];
+    wave_lds_fence();
 
     f32x4 oacc[NR][DT];
     float m_run[NR], m_top[NR], l_run[NR];  // the sums' reference and the row's maximum so far (scores), the sum
@@ -290,15 +416,16 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       m_run[nr] = m_top[nr] = -INFINITY;
       l_run[nr] = 0.f;
     }
-    if (n_my > 0) {
-      load_ids(0);
-      load_keys(0);
-      load_values(0);
-    }
     for (int i = 0; i < n_my; ++i) {
       const int base = (t0 + wave + kUnit * i) * kPage;
       const bool some = __builtin_amdgcn_readlane(ids, i & 63) >= 0;
-      const float ks = pow2(__builtin_amdgcn_readlane(ek, i & 63)), vs = pow2(__builtin_amdgcn_readlane(ev, i & 63));
+      int e_k = __builtin_amdgcn_readlane(ek, i & 63), e_v = __builtin_amdgcn_readlane(ev, i & 63);
+      const bool appends = cnt > 0 && i + 1 == n_my && some;
+      if (appends) {
+        if (kTakeTurns) load_values(i);
+        append(i & 63, e_k, e_v);
+      }
+      const float ks = pow2(e_k), vs = pow2(e_v);
       f32x4 st[NR][4];
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
@@ -319,9 +446,10 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
             for (int nr = 0; nr < NR; ++nr) st[nr][t] = mfma16(kf, qf[nr], st[nr][t]);
           }
         }
-      const bool last_of_ids = (i & 63) == 63;
-      if (i + 1 < n_my) {
-        if (last_of_ids) load_ids(i + 1);
+      if (kTakeTurns) {
+        if (!appends) load_values(i);
+      } else if (i + 1 < n_my) {
+        if ((i & 63) == 63) load_ids(i + 1);
         load_keys(i + 1);
       }
       // tokens 16 g + 4 t + e of the page
@@ -387,6 +515,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
           }
         any_nan = __builtin_amdgcn_ballot_w64(nan != 0) != 0;
         if (any_nan) {
+          const int lane = opaque_lane_id(), m16 = lane & 15, g = lane >> 4;
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
             unsigned at = 0;  // tokens 16 g + e whose code is NaN
@@ -410,6 +539,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
           for (int nr = 0; nr < NR; ++nr) oacc[nr][d] = mfma16(vf, pf[nr][c], oacc[nr][d]);
         }
       if (any_nan) {
+        const int g = opaque_lane_id() >> 4;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           const int n = limit[nr] - base;
@@ -422,10 +552,18 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
         }
         wave_lds_fence();
       }
-      if (i + 1 < n_my) load_values(i + 1);
+      if (i + 1 < n_my) {
+        if (kTakeTurns) {
+          if ((i & 63) == 63) load_ids(i + 1);
+          load_keys(i + 1);
+        } else {
+          load_values(i + 1);
+        }
+      }
     }
 
     // Merge the waves' rows through LDS.
+    const int lane_after = opaque_lane_id(), m16 = lane_after & 15, g = lane_after >> 4, tid = wave * 64 + lane_after;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       const int row = 16 * nr + m16;
@@ -827,7 +965,10 @@ Plan plan_of(const MimirPagedAttnParams& p) {
     if (s.pairs) {
       s.units = pairs;
     } else {
-      s.units = p.num_kv_heads * std::max<int64_t>(1, std::min(most, 2 * cus / p.num_kv_heads));
+      // Workgroups per CU: as many as fit at once (registers), two at head_dim 128 or with two row tiles, three
+      // else (64 rows of 500 to 4000 keys, 8 / 8 heads of 64: 42.3 -> 39.0 us; of 128 two are faster than three or four).
+      const int64_t per_cu = p.head_dim == 64 && R <= 16 ? 3 : 2;
+      s.units = p.num_kv_heads * std::max<int64_t>(1, std::min(most, per_cu * cus / p.num_kv_heads));
       s.workspace_bytes = (size_t)s.units * 2 * (size_t)R * ((size_t)p.head_dim + 2) * sizeof(float);
     }
     return s;
@@ -876,8 +1017,10 @@ hipError_t launch_paged_attn(const MimirPagedAttnParams& p, const Plan& plan, hi
   a.cus = device_cu_count();
   a.part_o = (float*)p.workspace;
   const int64_t R = (int64_t)a.S * a.G;
-  hipError_t e = launch_paged_append(a, stream);
-  if (e != hipSuccess) return e;
+  if (!plan.decode) {
+    const hipError_t e = launch_paged_append(a, stream);
+    if (e != hipSuccess) return e;
+  }
   const dim3 grid((unsigned)plan.units), block(kThreads);
   const dim3 merge((unsigned)((int64_t)a.B * a.Hkv * ((R + kWaves - 1) / kWaves)));
   if (plan.decode) {
