@@ -133,39 +133,56 @@ __device__ __forceinline__ void merge_parts(const PagedArgs& a, int n, int lane,
 // finished there; the parts of the others are merged by a second kernel.  For batches of
 // more than kLineRows rows each pair takes a workgroup.
 
-constexpr int kLineRows = 256;  // batch rows of a line: one per thread
-constexpr int kUnit = kWaves;   // pages of a unit
+constexpr int kUnit = kWaves;  // pages of a unit
+__device__ __forceinline__ int units_of(int kv) { return (kv + kPage * kUnit - 1) / (kPage * kUnit); }
 
+// The line as each wave sees it, 64 batch rows to a register, one per lane: neither LDS nor barriers,
+// whose round trips stood before a wave's first page (one row of 700 keys: 5000 of 18000 cycles).
+constexpr int kLineChunks = 4;
+constexpr int kLineRows = 64 * kLineChunks;
 struct Line {
-  int incl[kLineRows];  // units up to and with batch row b
-  int kv[kLineRows];
-  int wave[kWaves];
-  int begin;            // batch row of the share's first unit
+  PagedRow at[kLineChunks];
+  int incl[kLineChunks];  // units up to and with the lane's row
+  int total;
+  __device__ __forceinline__ Line(const PagedArgs& a, int lane) {
+#pragma unroll
+    for (int c = 0; c < kLineChunks; ++c) {
+      at[c].row = -1, at[c].n = at[c].m = at[c].kv = 0;
+      if (64 * c + lane < a.B) at[c] = PagedRow(a, 64 * c + lane);
+    }
+    total = 0;
+#pragma unroll
+    for (int c = 0; c < kLineChunks; ++c) {
+      incl[c] = total;
+      if (64 * c >= a.B) continue;  // uniform
+      incl[c] += wave_inclusive_sum(units_of(at[c].kv));
+      total = __builtin_amdgcn_readlane(incl[c], 63);
+    }
+  }
+  // The batch row that unit u < total lies in.
+  __device__ __forceinline__ int find(int u) const {
+#pragma unroll
+    for (int c = 0; c < kLineChunks; ++c) {
+      const uint64_t past = __builtin_amdgcn_ballot_w64(incl[c] > u);
+      if (past != 0) return 64 * c + __builtin_ctzll(past);
+    }
+    return 0;
+  }
+  // Of batch row b (uniform): its place, and the units up to and with it.
+  __device__ __forceinline__ PagedRow row(int b, int& upto) const {
+    PagedRow r;
+#pragma unroll
+    for (int c = 0; c < kLineChunks; ++c)
+      if (c == b >> 6) {
+        r.row = __builtin_amdgcn_readlane(at[c].row, b & 63);
+        r.n = __builtin_amdgcn_readlane(at[c].n, b & 63);
+        r.m = __builtin_amdgcn_readlane(at[c].m, b & 63);
+        r.kv = __builtin_amdgcn_readlane(at[c].kv, b & 63);
+        upto = __builtin_amdgcn_readlane(incl[c], b & 63);
+      }
+    return r;
+  }
 };
-
-// All threads: the line into LDS; returns the total of units.
-__device__ __forceinline__ int line_scan(const PagedArgs& a, Line& line) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int kv = tid < a.B ? PagedRow(a, tid).kv : 0;
-  int incl = (kv + kPage * kUnit - 1) / (kPage * kUnit);
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += y;
-  }
-  if (lane == 63) line.wave[wave] = incl;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const int n = line.wave[w];
-    before += w < wave ? n : 0;
-    total += n;
-  }
-  line.incl[tid] = before + incl;
-  line.kv[tid] = kv;
-  return total;
-}
 
 // q units to each share, one more to the first r.
 struct Deal {
@@ -198,7 +215,6 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
   // Two row tiles of head_dim 128 leave no registers for a page of keys and of values at once: the
   // values are requested when the keys are used, and the other way round.
   constexpr bool kTakeTurns = NR == 2 && D == 128;
-  __shared__ Line line;
   __shared__ __attribute__((aligned(16))) float area[kWaves][kRowsMax * kPitch];
   __shared__ f32x2 area_ml[kWaves][kRowsMax];
   __shared__ __attribute__((aligned(8))) unsigned short s_nan[kWaves][D * 4];  // NaN tokens of each column, by wave
@@ -210,24 +226,32 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
   const int share = blockIdx.x / a.Hkv, hk = blockIdx.x - share * a.Hkv;  // share: the batch row, for pairs
   const int R = a.S * a.G;
 
-  int b = share, u0 = 0, u_end = 1;
+  int b = share, u0 = 0, u_end = 1, upto = 0;
+  PagedRow r;
+  [[maybe_unused]] int incl[kLineChunks];  // of the line
   if constexpr (kPairs) {
-    if (PagedRow(a, b).kv == 0) {
+    r = PagedRow(a, b);
+    if (r.kv == 0) {
       zero_out<D>(a, b, hk * a.G, a.G);
       return;
     }
   } else {
-    const int total = line_scan(a, line);
-    const Deal deal(total, a.shares);
+    const Line line(a, lane);
+    const Deal deal(line.total, a.shares);
     u0 = deal.begin(share);
     u_end = deal.begin(share + 1);
-    __syncthreads();
-    for (int r = blockIdx.x; r < a.B; r += gridDim.x)
-      if (line.kv[r] == 0) zero_out<D>(a, r, 0, a.Hkv * a.G);
+#pragma unroll
+    for (int c = 0; c < kLineChunks; ++c) {
+      incl[c] = line.incl[c];
+      // batch rows without keys, dealt to the workgroups
+      for (uint64_t none = __builtin_amdgcn_ballot_w64(64 * c + lane < a.B && line.at[c].kv == 0); none != 0; none &= none - 1) {
+        const int z = 64 * c + __builtin_ctzll(none);
+        if (z % (int)gridDim.x == (int)blockIdx.x) zero_out<D>(a, z, 0, a.Hkv * a.G);
+      }
+    }
     if (u0 >= u_end) return;
-    if (tid < a.B && line.incl[tid] > u0 && (tid == 0 || line.incl[tid - 1] <= u0)) line.begin = tid;
-    __syncthreads();
-    b = line.begin;
+    b = line.find(u0);
+    r = line.row(b, upto);
   }
 
   // offsets of a lane in a page: key rows 16 (m16 / 4) + m16 % 4 (+ 4 per tile), value columns m16 (+ 16)
@@ -239,13 +263,12 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 
   for (;;) {
     // The segment: pages [t0, t1) of batch row b.
-    const PagedRow r(a, b);
     int t0 = 0, t1 = (r.kv + kPage - 1) / kPage;
     bool whole = true;
     int u_next = u_end;
     if constexpr (!kPairs) {
       const int units = (t1 + kUnit - 1) / kUnit;
-      const int unit0 = u0 - (line.incl[b] - units), unit1 = min(units, unit0 + u_end - u0);
+      const int unit0 = u0 - (upto - units), unit1 = min(units, unit0 + u_end - u0);
       whole = unit0 == 0 && unit1 == units;
       u_next = u0 + unit1 - unit0;
       t0 = unit0 * kUnit;
@@ -257,7 +280,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
     int limit[NR];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-      const int i = (16 * nr + m16) / a.G;
+      const int i = a.S == 1 ? 0 : (16 * nr + m16) / a.G;
       limit[nr] = 16 * nr + m16 < R && i < r.m ? (a.causal ? min(r.n + i + 1, r.kv) : r.kv) : 0;
     }
     const int limit_min = a.causal ? min(r.n + 1, r.kv) : r.kv;
@@ -386,7 +409,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
     i32x4 q_in[NR][2 * KH];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-      const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0, i = row / a.G;
+      const int row = 16 * nr + m16 < R ? 16 * nr + m16 : 0, i = a.S == 1 ? 0 : row / a.G;
       const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)i * a.q_st + (int64_t)(hk * a.G + row - i * a.G) * a.q_sh + 16 * g;
 #pragma unroll
       for (int x = 0; x < 2 * KH; ++x) q_in[nr][x] = *(const i32x4*)&q[64 * (x >> 1) + 8 * (x & 1)];
@@ -602,9 +625,18 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
     }
     if (u_next >= u_end) return;
     u0 = u_next;
-    if constexpr (!kPairs)
-      do ++b;
-      while (line.incl[b] <= u0);  // the next batch row with keys
+    if constexpr (!kPairs) {
+      // the next batch row with keys; its place is looked up again rather than held
+#pragma unroll
+      for (int c = kLineChunks - 1; c >= 0; --c) {
+        const uint64_t past = __builtin_amdgcn_ballot_w64(incl[c] > u0);
+        if (past != 0) {
+          b = 64 * c + __builtin_ctzll(past);
+          upto = __builtin_amdgcn_readlane(incl[c], b & 63);
+        }
+      }
+      r = PagedRow(a, b);
+    }
     __syncthreads();  // the merge's area is free again
   }
 }
@@ -625,22 +657,23 @@ DECODE(64, 2)
 // Output rows of the pairs whose pages lie in several shares, one wave per row.
 template <int D>
 __device__ __forceinline__ void paged_merge_body(const PagedArgs& a) {
-  __shared__ Line line;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
   const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
-  const int total = line_scan(a, line);
-  __syncthreads();
-  const int units = (line.kv[b] + kPage * kUnit - 1) / (kPage * kUnit), before = line.incl[b] - units;
-  if (units == 0 || row >= R) return;
-  const Deal deal(total, a.shares);
+  if (row >= R) return;
+  const Line line(a, lane);
+  int upto = 0;
+  const PagedRow r = line.row(b, upto);
+  const int units = units_of(r.kv), before = upto - units;
+  if (units == 0) return;
+  const Deal deal(line.total, a.shares);
   const int w0 = deal.of(before), n = deal.of(before + units - 1) - w0 + 1;
   if (n == 1) return;  // written by its share
   const int slot0 = part_slot(w0, before == deal.begin(w0));
   const int i = row / a.G;
   bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
-  if (i >= PagedRow(a, b).m) {  // a padding query
+  if (i >= r.m) {  // a padding query
     if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
     return;
   }
