@@ -705,6 +705,17 @@ __device__ __forceinline__ bool split_decision(int mode, const int* slots, const
 __device__ __forceinline__ uint64_t kernel_segment() {
   return (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
 }
+// Requests every 64 bytes of a kernel's arguments (kBytes, from the segment's start) at once.  The
+// compiler loads them where they are used, and each first touch of a cache line of the
+// segment is a round trip of its own.
+template <int kBytes>
+__device__ __forceinline__ void touch_args() {
+  const __attribute__((address_space(4))) int* seg = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+  int x = 0;
+#pragma unroll
+  for (int i = 0; i < kBytes; i += 64) x |= seg[i / 4];
+  __asm__ volatile("" ::"s"(x));
+}
 __device__ __forceinline__ uint64_t uniform_segment(uint64_t seg) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)seg);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(seg >> 32));

@@ -24,6 +24,7 @@ __device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touche
   constexpr int kPitch = D + 4;
   __shared__ uint8_t codes[kPage * kPitch];
   __shared__ int top[kThreads / 64];
+  touch_args<sizeof(PagedArgs)>();
   const int tid = threadIdx.x;
   int u = blockIdx.x;
   const int j = u % touched;

@@ -219,6 +219,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
   __shared__ f32x2 area_ml[kWaves][kRowsMax];
   __shared__ __attribute__((aligned(8))) unsigned short s_nan[kWaves][D * 4];  // NaN tokens of each column, by wave
 
+  touch_args<sizeof(PagedArgs)>();
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -657,6 +658,7 @@ DECODE(64, 2)
 // Output rows of the pairs whose pages lie in several shares, one wave per row.
 template <int D>
 __device__ __forceinline__ void paged_merge_body(const PagedArgs& a) {
+  touch_args<sizeof(PagedArgs)>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
   const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
@@ -715,6 +717,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   __shared__ __attribute__((aligned(8))) unsigned short s_nan[2][D * 4];
   __shared__ int s_any[2][kWaves];
 
+  touch_args<sizeof(PagedArgs)>();
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hi = lane >> 5;
@@ -956,6 +959,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prefill_d64_kernel(const Pa
 
 template <int D>
 __device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
+  touch_args<sizeof(PagedArgs)>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
   const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
