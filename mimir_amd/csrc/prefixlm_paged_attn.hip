@@ -242,14 +242,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
     u0 = deal.begin(share);
     u_end = deal.begin(share + 1);
 #pragma unroll
-    for (int c = 0; c < kLineChunks; ++c) {
-      incl[c] = line.incl[c];
-      // batch rows without keys, dealt to the workgroups
-      for (uint64_t none = __builtin_amdgcn_ballot_w64(64 * c + lane < a.B && line.at[c].kv == 0); none != 0; none &= none - 1) {
-        const int z = 64 * c + __builtin_ctzll(none);
-        if (z % (int)gridDim.x == (int)blockIdx.x) zero_out<D>(a, z, 0, a.Hkv * a.G);
-      }
-    }
+    for (int c = 0; c < kLineChunks; ++c) incl[c] = line.incl[c];
     if (u0 >= u_end) return;
     b = line.find(u0);
     r = line.row(b, upto);
@@ -347,7 +340,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       }
       uint8_t* const yk = a.ck + page * a.k_sp + (int64_t)hk * kPage * D;
       uint8_t* const yv = a.cv + page * a.v_sp + (int64_t)hk * kPage * D;
-      if (s0 > 0 && (e_k > had_k || e_v > had_v)) {
+      if (__builtin_expect(s0 > 0 && (e_k > had_k || e_v > had_v), 0)) {
         // Now and then (a larger magnitude than the page has seen): the older codes rounded again in memory,
         // and the page read again.
         for (int w = lane; w < s0 * D / 4; w += 64) ((int*)yk)[w] = recode4(((int*)yk)[w], had_k - e_k);
@@ -473,7 +466,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       if (kTakeTurns) {
         if (!appends) load_values(i);
       } else if (i + 1 < n_my) {
-        if ((i & 63) == 63) load_ids(i + 1);
+        if (__builtin_expect((i & 63) == 63, 0)) load_ids(i + 1);
         load_keys(i + 1);
       }
       // tokens 16 g + 4 t + e of the page
@@ -538,7 +531,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
             nan |= nan_codes(vreg[d][w]);
           }
         any_nan = __builtin_amdgcn_ballot_w64(nan != 0) != 0;
-        if (any_nan) {
+        if (__builtin_expect(any_nan, 0)) {
           const int lane = opaque_lane_id(), m16 = lane & 15, g = lane >> 4;
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
@@ -562,7 +555,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 #pragma unroll
           for (int nr = 0; nr < NR; ++nr) oacc[nr][d] = mfma16(vf, pf[nr][c], oacc[nr][d]);
         }
-      if (any_nan) {
+      if (__builtin_expect(any_nan, 0)) {
         const int g = opaque_lane_id() >> 4;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
@@ -578,7 +571,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       }
       if (i + 1 < n_my) {
         if (kTakeTurns) {
-          if ((i & 63) == 63) load_ids(i + 1);
+          if (__builtin_expect((i & 63) == 63, 0)) load_ids(i + 1);
           load_keys(i + 1);
         } else {
           load_values(i + 1);
@@ -615,7 +608,7 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
       }
       if (whole) {
         const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-        const int i = row / a.G;
+        const int i = a.S == 1 ? 0 : row / a.G;
         *(bf16x4*)&a.out[(int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col] =
             i < r.m ? __builtin_convertvector(acc * inv, bf16x4) : bf16x4{};
       } else {
@@ -668,17 +661,16 @@ __device__ __forceinline__ void paged_merge_body(const PagedArgs& a) {
   int upto = 0;
   const PagedRow r = line.row(b, upto);
   const int units = units_of(r.kv), before = upto - units;
-  if (units == 0) return;
+  const int i = a.S == 1 ? 0 : row / a.G;
+  bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
+  if (units == 0 || i >= r.m) {  // a batch row without keys, or a padding query
+    if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
+    return;
+  }
   const Deal deal(line.total, a.shares);
   const int w0 = deal.of(before), n = deal.of(before + units - 1) - w0 + 1;
   if (n == 1) return;  // written by its share
   const int slot0 = part_slot(w0, before == deal.begin(w0));
-  const int i = row / a.G;
-  bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
-  if (i >= r.m) {  // a padding query
-    if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
-    return;
-  }
   merge_parts<D>(a, n, lane, [&](int c) { return ((int64_t)(c == 0 ? slot0 : part_slot(w0 + c, true)) * a.Hkv + hk) * R + row; }, o);
 }
 __global__ __launch_bounds__(kThreads) void paged_merge_d128_kernel(const PagedArgs a) { paged_merge_body<128>(a); }
