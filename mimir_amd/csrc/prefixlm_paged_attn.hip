@@ -679,11 +679,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 // ------------------------------------------------------------------ prefill
 //
 // Rows are (token, head) pairs, token-major, 128 to a workgroup, so the G query heads of a
-// kv head share its pages.  A page's codes go through registers: requested while the page
-// before is computed, converted to bf16 by the workgroup once (not by each wave) and stored
-// to the other of two LDS stages.  The products run on the 32 x 32 x 16 form, whose scores of
-// a lane are tokens 4 hi .. and 8 + 4 hi .. of each 16; the values' tokens are stored in that
-// order, so that both operands are 16-byte LDS reads.
+// kv head share its pages.  A page's keys are copied to LDS as they are, its values go through
+// registers, converted to bf16 by the workgroup once (not by each wave): both requested while the
+// page before is computed, into the other of two stages.  S^T = K Q^T runs on the 8-bit matrix
+// instruction (the queries in two halves, below), O^T += V^T P^T on the bf16 one, whose probabilities a lane
+// holds as tokens 4 hi .. and 8 + 4 hi .. of each 16; the values' tokens are stored in that order, so
+// that every operand is a 16-byte LDS read.
 
 constexpr int kRows = kWaves * 32;
 constexpr int kMaxSplits = 64;
@@ -699,11 +700,11 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
 
 template <int D>
 __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
-  constexpr int DT = D / 32, KS = D / 16;
-  constexpr int kPer = 4 * D / kThreads;  // 16-byte units of a page's keys (and values) per thread
-  using LK = TileLayout<D>;
+  constexpr int DT = D / 32, KS = D / 64;
+  constexpr int kPer = 4 * D / kThreads;  // 16-byte units of a page's values per thread, and key copies per wave
+  constexpr int kUnits = D / 16;          // 16-byte units of a key
   using LV = TileLayout<64>;              // 64 columns of values by 64 tokens
-  __shared__ __attribute__((aligned(16))) bf16_t sK[2][LK::kElems];
+  __shared__ __attribute__((aligned(16))) uint8_t sK[2][kPage * D];
   __shared__ __attribute__((aligned(16))) bf16_t sV[2][D / 64 * LV::kElems];
   // which tokens' values are NaN, for each column (a word of 64 bits), and whether any are, by wave
   __shared__ __attribute__((aligned(8))) unsigned short s_nan[2][D * 4];
@@ -749,9 +750,12 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const int kt0 = split * per;
   const int kt1 = min((wg_max + kPage - 1) / kPage, kt0 + per);
 
-  i32x4 kreg[kPer], vreg[kPer];
+  // Keys go to LDS as they are, unit u of token t at place u ^ swizzle(t): sixteen tokens' reads of one
+  // column range then fall on sixteen different places of the banks.
+  auto swizzle = [](int t) { return D == 128 ? t >> 1 & 7 : t >> 2 & 3; };
+  i32x4 vreg[kPer];
   int ek = 0, ev = 0, some = 0;
-  auto load_page = [&](int kt) __attribute__((always_inline)) {
+  auto load_page = [&](int kt, int buf) __attribute__((always_inline)) {
     const int id = load_const(a.table, (int64_t)r.row * a.t_st + kt);
     some = id >= 0 && id < a.num_pages;
     const int64_t p = some ? id : 0;  // none: page 0, not attended
@@ -761,7 +765,9 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     const uint8_t* vp = a.cv + p * a.v_sp + (int64_t)hk * kPage * D;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      kreg[i] = *(const i32x4*)&kp[(i * kThreads + tid) * 16];
+      const int place = (wave * kPer + i) * 64 + lane, t = place / kUnits;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp + t * D + ((place % kUnits) ^ swizzle(t)) * 16),
+                                       (__attribute__((address_space(3))) void*)(sK[buf] + (wave * kPer + i) * 1024), 16, 0, 0);
       vreg[i] = *(const i32x4*)&vp[(i * kThreads + tid) * 16];
     }
   };
@@ -769,17 +775,13 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   // the last one is unwritten, and a NaN value must not reach the rows that do not see it (0
   // times NaN), so both are cleared and the NaN tokens noted.
   auto stage_page = [&](int kt, int buf) __attribute__((always_inline)) {
-    const float ks = pow2(ek), vs = pow2(ev);
+    const float vs = pow2(ev);
     const int base = kt * kPage;
     const bool edge = base + kPage > wg_min;
     unsigned any = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int unit = i * kThreads + tid;
-      const int t = unit / (D / 16), c = unit % (D / 16) * 16;
-      bf16_t* const kd = &sK[buf][LK::off(t, c)];
-      *(bf16x8*)kd = decode8(kreg[i][0], kreg[i][1], ks);
-      *(bf16x8*)(kd + 8) = decode8(kreg[i][2], kreg[i][3], ks);
       const int d = unit / 4, t16 = unit % 4 * 16;
       i32x4 v = vreg[i];
       if (edge) {
@@ -811,21 +813,49 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     }
   };
 
-  if (kt0 < kt1) load_page(kt0);
-  bf16x8 qf[KS];
+  if (kt0 < kt1) load_page(kt0, 0);
+  // The queries as two 8-bit halves under a power of two of each row, so that S^T = K Q^T runs on the keys'
+  // codes: q = (hi + lo) 2^e, hi the nearest code and lo that of the rest.  A code holds four
+  // significant bits and bf16 eight, so the two hold every element down to 2^-11 of the row's largest
+  // exactly and the smaller ones to 2^-19 of it.  Against bf16 keys, converted on their way to LDS: half
+  // the LDS reads for the same time on the matrix cores (twice the products at twice the rate).
+  i32x8 qh[KS], ql[KS];
+  int q_scale;
   {
-    const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)ti * a.q_st + (int64_t)h * a.q_sh;
+    const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)ti * a.q_st + (int64_t)h * a.q_sh + 32 * hi;
+    i32x4 x[KS][4];  // columns 64 s + 32 hi + 8 j ..+7
+    int most = 0;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = row < Rm ? *(const bf16x8*)&q[16 * ks + 8 * hi] : bf16x8{};
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[s][j] = row < Rm ? *(const i32x4*)&q[64 * s + 8 * j] : i32x4{0, 0, 0, 0};
+        most = max(most, largest_bits(x[s][j]));
+      }
+    most = max(most, __shfl_xor(most, 32, 64));
+    const int e = exponent_for(most);
+    q_scale = 127 + e;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int w0 = x[s][j >> 1][2 * (j & 1)], w1 = x[s][j >> 1][2 * (j & 1) + 1];
+        const float f0 = coded_value(__int_as_float(w0 << 16), e), f1 = coded_value(__int_as_float(w0 & 0xffff0000), e);
+        const float f2 = coded_value(__int_as_float(w1 << 16), e), f3 = coded_value(__int_as_float(w1 & 0xffff0000), e);
+        const int c = encode4(f0, f1, f2, f3);
+        const f32x2 a01 = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), a23 = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+        qh[s][j] = c;
+        ql[s][j] = encode4(f0 - a01[0], f1 - a01[1], f2 - a23[0], f3 - a23[1]);
+      }
   }
   f32x16 oacc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
   const float c2 = a.scale_log2;
-  const int k_base = LK::off(l32, 8 * hi), v_base = LV::off(l32, 8 * hi);
+  const int k_base = l32 * D, k_turn = 32 * hi ^ 16 * swizzle(l32), v_base = LV::off(l32, 8 * hi);
 
-  auto compute = [&](int kt, int buf, int there) __attribute__((always_inline)) {
+  auto compute = [&](int kt, int buf, int there, int k_scale) __attribute__((always_inline)) {
     const int base = kt * kPage;
     if (!active || base >= w_max || !there) return;
     f32x16 st[2];
@@ -833,8 +863,13 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     for (int mt = 0; mt < 2; ++mt) {
       st[mt] = f32x16{};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        st[mt] = mfma32(*(const bf16x8*)&sK[buf][k_base + mt * 32 * LK::kRowElems + ks * 16], qf[ks], st[mt]);
+      for (int s = 0; s < KS; ++s) {
+        const uint8_t* const kp = &sK[buf][k_base + mt * 32 * D];
+        const i32x4 k0 = *(const i32x4*)&kp[k_turn ^ (64 * s)], k1 = *(const i32x4*)&kp[k_turn ^ (64 * s + 16)];
+        const i32x8 k = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
+        st[mt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, ql[s], st[mt], 0, 0, 0, k_scale, 0, q_scale);
+        st[mt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qh[s], st[mt], 0, 0, 0, k_scale, 0, q_scale);
+      }
     }
     if (base + kPage > w_min) {
 #pragma unroll
@@ -909,13 +944,13 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   };
 
   if (kt0 < kt1) stage_page(kt0, 0);
-  __syncthreads();
   for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1, there = some;
-    if (kt + 1 < kt1) load_page(kt + 1);
-    compute(kt, buf, there);
-    if (kt + 1 < kt1) stage_page(kt + 1, buf ^ 1);
+    const int buf = (kt - kt0) & 1, there = some, k_scale = 127 + ek;
+    wait_vmem();  // the page's keys
     __syncthreads();
+    if (kt + 1 < kt1) load_page(kt + 1, buf ^ 1);
+    compute(kt, buf, there, k_scale);
+    if (kt + 1 < kt1) stage_page(kt + 1, buf ^ 1);
   }
 
   const float l_tot = xor32_sum(l_run);
