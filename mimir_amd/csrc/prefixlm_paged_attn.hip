@@ -9,9 +9,9 @@
 //     paged_prefill_*     one workgroup per (batch row, kv head, 128 query rows, key split)
 //     paged_merge_splits_* with several splits: adds their partial rows
 //
-// S^T = K Q^T and O^T += V^T P^T on bf16 MFMA with an online softmax in fp32.  Codes become
-// bf16 times their page's scale in the conversion instruction, exactly; P is rounded to
-// bf16 under the tile's own maximum, the one rounding before the output's.
+// S^T = K Q^T and O^T += V^T P^T on the matrix cores with an online softmax in fp32: decode in bf16 (codes
+// become bf16 times their page's scale in the conversion instruction, exactly), prefill on the
+// codes themselves.  P is rounded under the page's own maximum, to the eight bits of bf16.
 #include <algorithm>
 #include <cmath>
 
@@ -29,6 +29,25 @@ constexpr float kRefRange = 30.f;   // how far (log2) a tile's reference may lie
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// 8-bit operands, 32 consecutive columns a lane, under 2^(scale - 127) each.
+__device__ __forceinline__ f32x16 mfma8(i32x8 a, i32x8 b, f32x16 c, int a_scale, int b_scale) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, a_scale, 0, b_scale);
+}
+
+// Four values as codes hi and lo of x = hi + lo * 2^-4, |x| < 2^8: hi's rest is at most 2^4, so lo reaches
+// the scale's bottom sixteen times later than it would under hi's.
+constexpr int kLoShift = 4;
+__device__ __forceinline__ void halves8(float a, float b, float c, float d, int& hi, int& lo) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  constexpr float kLoScale = 1.f / (1 << kLoShift);
+  hi = encode4(a, b, c, d);
+  const f32x2 ab = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), cd = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+  s16x2 x = {0, 0};
+  x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, a - ab[0], b - ab[1], kLoScale, false);
+  x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, c - cd[0], d - cd[1], kLoScale, true);
+  lo = __builtin_bit_cast(int, x);
 }
 
 // Combine x over the four 16-lane groups of a wave.
@@ -679,12 +698,22 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 // ------------------------------------------------------------------ prefill
 //
 // Rows are (token, head) pairs, token-major, 128 to a workgroup, so the G query heads of a
-// kv head share its pages.  A page's keys are copied to LDS as they are, its values go through
-// registers, converted to bf16 by the workgroup once (not by each wave): both requested while the
-// page before is computed, into the other of two stages.  S^T = K Q^T runs on the 8-bit matrix
-// instruction (the queries in two halves, below), O^T += V^T P^T on the bf16 one, whose probabilities a lane
-// holds as tokens 4 hi .. and 8 + 4 hi .. of each 16; the values' tokens are stored in that order, so
-// that every operand is a 16-byte LDS read.
+// kv head share its pages, which are copied to LDS as they are while the page before is computed.
+//
+// Both products run on the 8-bit matrix instruction (32 x 32 x 64, twice the bf16 rate) with the codes
+// as one operand, their page's scale going into the instruction, and the other operand, queries or
+// probabilities, in two 8-bit halves: hi the nearest code, lo that of the rest (halves8).  A code holds
+// four significant bits, so the two hold the eight of bf16 in as much matrix time.
+//   queries        under a power of two of each row: exact down to 2^-15 of the row's largest element, the
+//                  smaller ones to 2^-22 of it
+//   probabilities  under a power of two of each row and page, 2^8 at most: to 2^-8 of themselves, as in
+//                  bf16, and to 2^-21 of the page's largest, so that a long tail of small ones
+//                  is rounded in its own pages only
+// Against bf16 operands (codes converted on their way to LDS, 1000 of 4600 cycles a page): half the LDS
+// reads, no conversions, no registers for them.
+//
+// The scores' rows are tokens 32 (m / 4 % 2) + 16 t + 4 (m / 8) + m % 4 for row m of tile t, so that the 32 a
+// lane holds are 32 hi .., in order: the 32 bytes of a value column that its half of the lanes reads.
 
 constexpr int kRows = kWaves * 32;
 constexpr int kMaxSplits = 64;
@@ -701,14 +730,13 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
 template <int D>
 __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   constexpr int DT = D / 32, KS = D / 64;
-  constexpr int kPer = 4 * D / kThreads;  // 16-byte units of a page's values per thread, and key copies per wave
-  constexpr int kUnits = D / 16;          // 16-byte units of a key
-  using LV = TileLayout<64>;              // 64 columns of values by 64 tokens
+  constexpr int kCopies = D / 64;  // 1 KiB copies of a page's keys, and of its values, per wave
   __shared__ __attribute__((aligned(16))) uint8_t sK[2][kPage * D];
-  __shared__ __attribute__((aligned(16))) bf16_t sV[2][D / 64 * LV::kElems];
-  // which tokens' values are NaN, for each column (a word of 64 bits), and whether any are, by wave
-  __shared__ __attribute__((aligned(8))) unsigned short s_nan[2][D * 4];
-  __shared__ int s_any[2][kWaves];
+  __shared__ __attribute__((aligned(16))) uint8_t sV[2][kPage * D];
+  // of a page that some rows see only part of: which tokens' values are NaN, for each column (64 bits),
+  // and whether any are, by wave
+  __shared__ __attribute__((aligned(8))) unsigned short s_nan[D * 4];
+  __shared__ int s_any[kWaves];
 
   touch_args<sizeof(PagedArgs)>();
   const int tid = threadIdx.x, lane = tid & 63;
@@ -750,75 +778,69 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const int kt0 = split * per;
   const int kt1 = min((wg_max + kPage - 1) / kPage, kt0 + per);
 
-  // Keys go to LDS as they are, unit u of token t at place u ^ swizzle(t): sixteen tokens' reads of one
-  // column range then fall on sixteen different places of the banks.
-  auto swizzle = [](int t) { return D == 128 ? t >> 1 & 7 : t >> 2 & 3; };
-  i32x4 vreg[kPer];
-  int ek = 0, ev = 0, some = 0;
+  // 16-byte unit u of token t's key lies at place u ^ k_place(t), of value column d at u ^ v_place(d): the
+  // sixteen rows of an operand read then fall on sixteen different places of the banks.
+  auto k_place = [](int t) { return D == 128 ? (t >> 1 & 3) | (t >> 3 & 4) : (t >> 2 & 1) | (t >> 4 & 2); };
+  auto v_place = [](int d) { return d >> 2 & 3; };
+  int id_next = 0, ek = 0, ev = 0, some = 0;
+  auto next_id = [&](int kt) { id_next = kt < kt1 ? load_const(a.table, (int64_t)r.row * a.t_st + kt) : -1; };
   auto load_page = [&](int kt, int buf) __attribute__((always_inline)) {
-    const int id = load_const(a.table, (int64_t)r.row * a.t_st + kt);
+    const int id = id_next;
+    next_id(kt + 1);  // a page ahead: the copies wait for no look at the table
     some = id >= 0 && id < a.num_pages;
     const int64_t p = some ? id : 0;  // none: page 0, not attended
-    ek = a.ke[p * a.ke_sp + hk];
-    ev = a.ve[p * a.ve_sp + hk];
     const uint8_t* kp = a.ck + p * a.k_sp + (int64_t)hk * kPage * D;
     const uint8_t* vp = a.cv + p * a.v_sp + (int64_t)hk * kPage * D;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int place = (wave * kPer + i) * 64 + lane, t = place / kUnits;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp + t * D + ((place % kUnits) ^ swizzle(t)) * 16),
-                                       (__attribute__((address_space(3))) void*)(sK[buf] + (wave * kPer + i) * 1024), 16, 0, 0);
-      vreg[i] = *(const i32x4*)&vp[(i * kThreads + tid) * 16];
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = wave * kCopies + i, place = at * 64 + lane;
+      const int t = place / (D / 16), d = place / 4;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kp + t * D + ((place % (D / 16)) ^ k_place(t)) * 16),
+                                       (__attribute__((address_space(3))) void*)(sK[buf] + at * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp + d * kPage + ((place & 3) ^ v_place(d)) * 16),
+                                       (__attribute__((address_space(3))) void*)(sV[buf] + at * 1024), 16, 0, 0);
     }
+    ek = a.ke[p * a.ke_sp + hk];
+    ev = a.ve[p * a.ve_sp + hk];
   };
-  // Where a page holds tokens that some rows of the workgroup do not see: what lies behind
-  // the last one is unwritten, and a NaN value must not reach the rows that do not see it (0
-  // times NaN), so both are cleared and the NaN tokens noted.
-  auto stage_page = [&](int kt, int buf) __attribute__((always_inline)) {
-    const float vs = pow2(ev);
-    const int base = kt * kPage;
-    const bool edge = base + kPage > wg_min;
+  // A page with tokens that some rows of the workgroup do not see: what lies behind the last one is
+  // unwritten, and a NaN value must not reach the rows that do not see it (0 times NaN), so
+  // both are cleared and the NaN tokens noted.
+  auto clean_page = [&](int kt, int buf) {
     unsigned any = 0;
+    for (int i = 0; i < kCopies; ++i) {
+      const int place = i * kThreads + tid, d = place / 4, t16 = ((place & 3) ^ v_place(d)) * 16;
+      i32x4* const at = (i32x4*)&sV[buf][place * 16];
+      i32x4 v = *at;
+      unsigned nan = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int unit = i * kThreads + tid;
-      const int d = unit / 4, t16 = unit % 4 * 16;
-      i32x4 v = vreg[i];
-      if (edge) {
-        unsigned nan = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          v[w] = codes_before(v[w], t16 + 4 * w, r.kv - base);
-          nan |= nan_codes(v[w]);
-        }
-        unsigned at = 0;
-        if (nan != 0) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (((unsigned)v[e >> 2] >> 8 * (e & 3) & 0x7f) == 0x7f) {
-              at |= 1u << e;
-              v[e >> 2] &= (int)~(0xffu << 8 * (e & 3));
-            }
-          any = 1;
-        }
-        s_nan[buf][unit] = (unsigned short)at;
+      for (int w = 0; w < 4; ++w) {
+        v[w] = codes_before(v[w], t16 + 4 * w, r.kv - kt * kPage);
+        nan |= nan_codes(v[w]);
       }
-      bf16_t* const vd = &sV[buf][(d >> 6) * LV::kElems + LV::off(d & 63, t16)];
-      *(bf16x8*)vd = decode8(v[0], v[2], vs);
-      *(bf16x8*)(vd + 8) = decode8(v[1], v[3], vs);
+      unsigned bits = 0;
+      if (nan != 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (((unsigned)v[e >> 2] >> 8 * (e & 3) & 0x7f) == 0x7f) {
+            bits |= 1u << e;
+            v[e >> 2] &= (int)~(0xffu << 8 * (e & 3));
+          }
+        any = 1;
+      }
+      s_nan[d * 4 + t16 / 16] = (unsigned short)bits;
+      *at = v;
     }
-    if (edge) {
-      const int found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-      if (lane == 0) s_any[buf][wave] = found;
-    }
+    const int found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+    if (lane == 0) s_any[wave] = found;
+    __syncthreads();
   };
 
-  if (kt0 < kt1) load_page(kt0, 0);
-  // The queries as two 8-bit halves under a power of two of each row, so that S^T = K Q^T runs on the keys'
-  // codes: q = (hi + lo) 2^e, hi the nearest code and lo that of the rest.  A code holds four
-  // significant bits and bf16 eight, so the two hold every element down to 2^-11 of the row's largest
-  // exactly and the smaller ones to 2^-19 of it.  Against bf16 keys, converted on their way to LDS: half
-  // the LDS reads for the same time on the matrix cores (twice the products at twice the rate).
+  if (kt0 < kt1) {
+    next_id(kt0);
+    load_page(kt0, 0);
+  }
+  // Q^T operands: the lane's row, columns 64 s + 32 hi ..+31, as codes under 2^(q_scale - 127).
   i32x8 qh[KS], ql[KS];
   int q_scale;
   {
@@ -842,10 +864,10 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
         const int w0 = x[s][j >> 1][2 * (j & 1)], w1 = x[s][j >> 1][2 * (j & 1) + 1];
         const float f0 = coded_value(__int_as_float(w0 << 16), e), f1 = coded_value(__int_as_float(w0 & 0xffff0000), e);
         const float f2 = coded_value(__int_as_float(w1 << 16), e), f3 = coded_value(__int_as_float(w1 & 0xffff0000), e);
-        const int c = encode4(f0, f1, f2, f3);
-        const f32x2 a01 = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), a23 = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-        qh[s][j] = c;
-        ql[s][j] = encode4(f0 - a01[0], f1 - a01[1], f2 - a23[0], f3 - a23[1]);
+        int c_hi, c_lo;
+        halves8(f0, f1, f2, f3, c_hi, c_lo);
+        qh[s][j] = c_hi;
+        ql[s][j] = c_lo;
       }
   }
   f32x16 oacc[DT];
@@ -853,36 +875,39 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   for (int dt = 0; dt < DT; ++dt) oacc[dt] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
   const float c2 = a.scale_log2;
-  const int k_base = l32 * D, k_turn = 32 * hi ^ 16 * swizzle(l32), v_base = LV::off(l32, 8 * hi);
+  const int k_token = 32 * (l32 >> 2 & 1) + 4 * (l32 >> 3) + (l32 & 3);  // + 16 t
+  const int k_base = k_token * D, k_turn = 32 * hi ^ 16 * k_place(k_token);
+  const int v_base = l32 * kPage, v_turn = 32 * hi ^ 16 * v_place(l32);
 
-  auto compute = [&](int kt, int buf, int there, int k_scale) __attribute__((always_inline)) {
+  auto compute = [&](int kt, int buf, int k_scale, int v_scale) __attribute__((always_inline)) {
     const int base = kt * kPage;
-    if (!active || base >= w_max || !there) return;
+    if (!active || base >= w_max) return;
     f32x16 st[2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      st[mt] = f32x16{};
+    for (int t = 0; t < 2; ++t) {
+      st[t] = f32x16{};
+      const uint8_t* const kp = &sK[buf][k_base + t * 16 * D];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const uint8_t* const kp = &sK[buf][k_base + mt * 32 * D];
         const i32x4 k0 = *(const i32x4*)&kp[k_turn ^ (64 * s)], k1 = *(const i32x4*)&kp[k_turn ^ (64 * s + 16)];
         const i32x8 k = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
-        st[mt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, ql[s], st[mt], 0, 0, 0, k_scale, 0, q_scale);
-        st[mt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, qh[s], st[mt], 0, 0, 0, k_scale, 0, q_scale);
+        st[t] = mfma8(k, ql[s], st[t], k_scale, q_scale - kLoShift);
+        st[t] = mfma8(k, qh[s], st[t], k_scale, q_scale);
       }
     }
+    // tokens 32 hi + 16 t + e
     if (base + kPage > w_min) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (base + 32 * mt + 8 * (e >> 2) + 4 * hi + (e & 3) >= limit) st[mt][e] = -INFINITY;
+          if (base + 32 * hi + 16 * t + e >= limit) st[t][e] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[mt][e]);
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[t][e]);
     mx = xor32_max(mx);
     // The reference maximum moves only when it grows by more than 2^8 in probability terms.
     const float m_cand = fmaxf(m_run, mx);
@@ -896,40 +921,44 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       m_run = m_new;
     }
     const float ref = m_run == -INFINITY ? 0.f : m_run, mb = ref * c2;
-    float lsum = 0.f;
-    // Scaled scores past 2^24 are known to one only: their difference is formed before the scale,
-    // at an operation more each, or rounding them apart would give probabilities up to 2^(their ulp).
-    if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(mb) > 16777216.f) != 0) {
+    // The page's probabilities times 2^-up, so that the largest lies in [2^7, 2^8).
+    const int up = (int)floorf(fmaxf((mx - ref) * c2, -100.f)) - 7;
+    // Scaled scores past 2^16 are known to 2^-8 only: their difference is formed before the scale, at an
+    // operation more each, or rounding them apart would give probabilities up to 2^(their ulp).
+    if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(mb) > 65536.f) != 0) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[mt][e] = fast_exp2((st[mt][e] - ref) * c2);
+        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2(__builtin_fmaf(st[t][e] - ref, c2, (float)-up));
     } else {
+      const float shift = -(mb + (float)up);
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[mt][e] = fast_exp2(__builtin_fmaf(st[mt][e], c2, -mb));
+        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2(__builtin_fmaf(st[t][e], c2, shift));
     }
+    float lsum = 0.f;
+    i32x8 ph, pl;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) lsum += st[mt][e];
-    l_run += lsum;
-    bf16x8 pf[4];
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      f32x8 t;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = st[kk >> 1][8 * (kk & 1) + e];
-      pf[kk] = to_bf16x8(t);
+    for (int w = 0; w < 8; ++w) {
+      const int t = w >> 2, e = 4 * (w & 3);
+      lsum += (st[t][e] + st[t][e + 1]) + (st[t][e + 2] + st[t][e + 3]);
+      int c_hi, c_lo;
+      halves8(st[t][e], st[t][e + 1], st[t][e + 2], st[t][e + 3], c_hi, c_lo);
+      ph[w] = c_hi;
+      pl[w] = c_lo;
     }
+    l_run += __builtin_amdgcn_ldexpf(lsum, up);
+    const int p_scale = 127 + up;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        oacc[dt] = mfma32(*(const bf16x8*)&sV[buf][(dt >> 1) * LV::kElems + v_base + (dt & 1) * 32 * LV::kRowElems + kk * 16],
-                          pf[kk], oacc[dt]);
-    if (base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[buf][0] | s_any[buf][1] | s_any[buf][2] | s_any[buf][3])) {
+    for (int dt = 0; dt < DT; ++dt) {
+      const uint8_t* const vp = &sV[buf][v_base + dt * 32 * kPage];
+      const i32x4 v0 = *(const i32x4*)&vp[v_turn], v1 = *(const i32x4*)&vp[v_turn ^ 16];
+      const i32x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+      oacc[dt] = mfma8(v, pl, oacc[dt], v_scale, p_scale - kLoShift);
+      oacc[dt] = mfma8(v, ph, oacc[dt], v_scale, p_scale);
+    }
+    if (__builtin_expect(base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[0] | s_any[1] | s_any[2] | s_any[3]), 0)) {
       // NaN values into the rows that see them
       const int n = limit - base;
       const uint64_t seen = n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
@@ -938,19 +967,19 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int d = 32 * dt + 8 * (e >> 2) + 4 * hi + (e & 3);
-          if (*(const uint64_t*)&s_nan[buf][4 * d] & seen) oacc[dt][e] = __builtin_nanf("");
+          if (*(const uint64_t*)&s_nan[4 * d] & seen) oacc[dt][e] = __builtin_nanf("");
         }
     }
   };
 
-  if (kt0 < kt1) stage_page(kt0, 0);
   for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1, there = some, k_scale = 127 + ek;
-    wait_vmem();  // the page's keys
+    const int buf = (kt - kt0) & 1, there = some;
+    wait_vmem();  // the page's copies
     __syncthreads();
+    const int k_scale = 127 + ek, v_scale = 127 + ev;
+    if (there && kt * kPage + kPage > wg_min) clean_page(kt, buf);  // uniform
     if (kt + 1 < kt1) load_page(kt + 1, buf ^ 1);
-    compute(kt, buf, there, k_scale);
-    if (kt + 1 < kt1) stage_page(kt + 1, buf ^ 1);
+    if (there) compute(kt, buf, k_scale, v_scale);
   }
 
   const float l_tot = xor32_sum(l_run);
