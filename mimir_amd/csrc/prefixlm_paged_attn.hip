@@ -716,6 +716,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 // lane holds are 32 hi .., in order: the 32 bytes of a value column that its half of the lanes reads.
 
 constexpr int kRows = kWaves * 32;
+constexpr int kTogether = 2;  // pages between two barriers
 constexpr int kMaxSplits = 64;
 
 // Whether the batch rows hold about as many cached keys: none differs from the first by more
@@ -731,12 +732,12 @@ template <int D>
 __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   constexpr int DT = D / 32, KS = D / 64;
   constexpr int kCopies = D / 64;  // 1 KiB copies of a page's keys, and of its values, per wave
-  __shared__ __attribute__((aligned(16))) uint8_t sK[2][kPage * D];
-  __shared__ __attribute__((aligned(16))) uint8_t sV[2][kPage * D];
+  __shared__ __attribute__((aligned(16))) uint8_t sK[2 * kTogether][kPage * D];
+  __shared__ __attribute__((aligned(16))) uint8_t sV[2 * kTogether][kPage * D];
   // of a page that some rows see only part of: which tokens' values are NaN, for each column (64 bits),
   // and whether any are, by wave
-  __shared__ __attribute__((aligned(8))) unsigned short s_nan[D * 4];
-  __shared__ int s_any[kWaves];
+  __shared__ __attribute__((aligned(8))) unsigned short s_nan[kTogether][D * 4];
+  __shared__ int s_any[kTogether][kWaves];
 
   touch_args<sizeof(PagedArgs)>();
   const int tid = threadIdx.x, lane = tid & 63;
@@ -782,13 +783,15 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   // sixteen rows of an operand read then fall on sixteen different places of the banks.
   auto k_place = [](int t) { return D == 128 ? (t >> 1 & 3) | (t >> 3 & 4) : (t >> 2 & 1) | (t >> 4 & 2); };
   auto v_place = [](int d) { return d >> 2 & 3; };
-  int id_next = 0, ek = 0, ev = 0, some = 0;
-  auto next_id = [&](int kt) { id_next = kt < kt1 ? load_const(a.table, (int64_t)r.row * a.t_st + kt) : -1; };
-  auto load_page = [&](int kt, int buf) __attribute__((always_inline)) {
-    const int id = id_next;
-    next_id(kt + 1);  // a page ahead: the copies wait for no look at the table
-    some = id >= 0 && id < a.num_pages;
-    const int64_t p = some ? id : 0;  // none: page 0, not attended
+  int id_next[kTogether], ek[kTogether], ev[kTogether];
+  bool some[kTogether];
+  auto next_id = [&](int kt, int j) { id_next[j] = kt < kt1 ? load_const(a.table, (int64_t)r.row * a.t_st + kt) : -1; };
+  auto load_page = [&](int kt, int j, int buf) __attribute__((always_inline)) {
+    const int id = id_next[j];
+    next_id(kt + kTogether, j);  // ahead: the copies wait for no look at the table
+    some[j] = id >= 0 && id < a.num_pages;
+    if (kt >= kt1) return;
+    const int64_t p = some[j] ? id : 0;  // none: page 0, not attended
     const uint8_t* kp = a.ck + p * a.k_sp + (int64_t)hk * kPage * D;
     const uint8_t* vp = a.cv + p * a.v_sp + (int64_t)hk * kPage * D;
 #pragma unroll
@@ -800,13 +803,13 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vp + d * kPage + ((place & 3) ^ v_place(d)) * 16),
                                        (__attribute__((address_space(3))) void*)(sV[buf] + at * 1024), 16, 0, 0);
     }
-    ek = a.ke[p * a.ke_sp + hk];
-    ev = a.ve[p * a.ve_sp + hk];
+    ek[j] = a.ke[p * a.ke_sp + hk];
+    ev[j] = a.ve[p * a.ve_sp + hk];
   };
   // A page with tokens that some rows of the workgroup do not see: what lies behind the last one is
   // unwritten, and a NaN value must not reach the rows that do not see it (0 times NaN), so
   // both are cleared and the NaN tokens noted.
-  auto clean_page = [&](int kt, int buf) {
+  auto clean_page = [&](int kt, int j, int buf) {
     unsigned any = 0;
     for (int i = 0; i < kCopies; ++i) {
       const int place = i * kThreads + tid, d = place / 4, t16 = ((place & 3) ^ v_place(d)) * 16;
@@ -828,17 +831,18 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
           }
         any = 1;
       }
-      s_nan[d * 4 + t16 / 16] = (unsigned short)bits;
+      s_nan[j][d * 4 + t16 / 16] = (unsigned short)bits;
       *at = v;
     }
     const int found = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-    if (lane == 0) s_any[wave] = found;
-    __syncthreads();
+    if (lane == 0) s_any[j][wave] = found;
   };
 
   if (kt0 < kt1) {
-    next_id(kt0);
-    load_page(kt0, 0);
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) next_id(kt0 + j, j);
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) load_page(kt0 + j, j, j);
   }
   // Q^T operands: the lane's row, columns 64 s + 32 hi ..+31, as codes under 2^(q_scale - 127).
   i32x8 qh[KS], ql[KS];
@@ -879,7 +883,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const int k_base = k_token * D, k_turn = 32 * hi ^ 16 * k_place(k_token);
   const int v_base = l32 * kPage, v_turn = 32 * hi ^ 16 * v_place(l32);
 
-  auto compute = [&](int kt, int buf, int k_scale, int v_scale) __attribute__((always_inline)) {
+  auto compute = [&](int kt, int j, int buf, int k_scale, int v_scale) __attribute__((always_inline)) {
     const int base = kt * kPage;
     if (!active || base >= w_max) return;
     f32x16 st[2];
@@ -958,7 +962,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       oacc[dt] = mfma8(v, pl, oacc[dt], v_scale, p_scale - kLoShift);
       oacc[dt] = mfma8(v, ph, oacc[dt], v_scale, p_scale);
     }
-    if (__builtin_expect(base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[0] | s_any[1] | s_any[2] | s_any[3]), 0)) {
+    if (__builtin_expect(base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[j][0] | s_any[j][1] | s_any[j][2] | s_any[j][3]), 0)) {
       // NaN values into the rows that see them
       const int n = limit - base;
       const uint64_t seen = n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
@@ -967,19 +971,30 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int d = 32 * dt + 8 * (e >> 2) + 4 * hi + (e & 3);
-          if (*(const uint64_t*)&s_nan[4 * d] & seen) oacc[dt][e] = __builtin_nanf("");
+          if (*(const uint64_t*)&s_nan[j][4 * d] & seen) oacc[dt][e] = __builtin_nanf("");
         }
     }
   };
 
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1, there = some;
-    wait_vmem();  // the page's copies
+  for (int kt = kt0, buf = 0; kt < kt1; kt += kTogether, buf ^= kTogether) {
+    wait_vmem();  // the pages' copies
     __syncthreads();
-    const int k_scale = 127 + ek, v_scale = 127 + ev;
-    if (there && kt * kPage + kPage > wg_min) clean_page(kt, buf);  // uniform
-    if (kt + 1 < kt1) load_page(kt + 1, buf ^ 1);
-    if (there) compute(kt, buf, k_scale, v_scale);
+    int k_scale[kTogether], v_scale[kTogether];
+    bool there[kTogether], cleaned = false;
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) {
+      k_scale[j] = 127 + ek[j], v_scale[j] = 127 + ev[j], there[j] = some[j];
+      if (there[j] && (kt + j) * kPage + kPage > wg_min) {  // uniform
+        clean_page(kt + j, j, buf + j);
+        cleaned = true;
+      }
+    }
+    if (cleaned) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) load_page(kt + kTogether + j, j, (buf ^ kTogether) + j);
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j)
+      if (there[j]) compute(kt + j, j, buf + j, k_scale[j], v_scale[j]);
   }
 
   const float l_tot = xor32_sum(l_run);
@@ -1013,8 +1028,9 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
 __global__ __launch_bounds__(kThreads, 2) void paged_prefill_d128_kernel(const PagedArgs a) { paged_prefill_body<128>(a); }
 __global__ __launch_bounds__(kThreads, 2) void paged_prefill_d64_kernel(const PagedArgs a) { paged_prefill_body<64>(a); }
 
+// Adds the partial rows of many key splits (short chunks on long rows), one wave to a row.
 template <int D>
-__device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
+__device__ __forceinline__ void paged_merge_many_body(const PagedArgs& a) {
   touch_args<sizeof(PagedArgs)>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = a.S * a.G, groups = (R + kWaves - 1) / kWaves;
@@ -1033,6 +1049,42 @@ __device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
   }
   const int64_t unit0 = ((int64_t)pair * a.n_rt + row / kRows) * a.splits;
   merge_parts<D>(a, n, lane, [&](int c) { return (unit0 + c) * kRows + row % kRows; }, o);
+}
+__global__ __launch_bounds__(kThreads) void paged_merge_many_d128_kernel(const PagedArgs a) { paged_merge_many_body<128>(a); }
+__global__ __launch_bounds__(kThreads) void paged_merge_many_d64_kernel(const PagedArgs a) { paged_merge_many_body<64>(a); }
+
+// The same for a few splits of many rows, D / 4 lanes to a row and four columns each, the parts in turn (a wave to
+// a row / so: 8 x 512 on 1536 keys, 8 / 8 heads of 64, two splits, 67.4 / 49.8 us; 100 on 3000, 16 / 4 heads
+// of 128, 32 splits, 35.7 / 39.6).
+constexpr int kFewSplits = 8;
+template <int D>
+__device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
+  touch_args<sizeof(PagedArgs)>();
+  constexpr int kLanes = D / 4, kRowsAt = kThreads / kLanes;
+  const int R = a.S * a.G, groups = (R + kRowsAt - 1) / kRowsAt;
+  const int pair = blockIdx.x / groups, row = (blockIdx.x - pair * groups) * kRowsAt + (int)threadIdx.x / kLanes;
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv, col = threadIdx.x % kLanes * 4;
+  const PagedRow r(a, b);
+  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
+  const int n = (tiles + per - 1) / per;
+  if (n <= 1 || row >= R) return;  // written by its split
+  const int i = row / a.G;
+  const int64_t part = (((int64_t)pair * a.n_rt + row / kRows) * a.splits) * kRows + row % kRows;  // + kRows each
+  float M = -INFINITY;
+  for (int c = 0; c < n; ++c) M = fmaxf(M, a.part_ml[2 * (part + c * kRows)]);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float lsum = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < n; ++c) {
+    const f32x2 ml = *(const f32x2*)&a.part_ml[2 * (part + c * kRows)];
+    const f32x4 o = *(const f32x4*)&a.part_o[(part + c * kRows) * D + col];
+    const float w = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - M);  // no key: a sum of 0 (or NaN)
+    lsum += ml[1] * w;
+    if (w != 0.f) acc += o * w;
+  }
+  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+  bf16_t* const out = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col;
+  *(bf16x4*)out = i < r.m ? __builtin_convertvector(acc * inv, bf16x4) : bf16x4{};  // zeros for padding queries
 }
 __global__ __launch_bounds__(kThreads) void paged_merge_splits_d128_kernel(const PagedArgs a) { paged_merge_splits_body<128>(a); }
 __global__ __launch_bounds__(kThreads) void paged_merge_splits_d64_kernel(const PagedArgs a) { paged_merge_splits_body<64>(a); }
@@ -1147,10 +1199,16 @@ hipError_t launch_paged_attn(const MimirPagedAttnParams& p, const Plan& plan, hi
   else
     hipLaunchKernelGGL(paged_prefill_d64_kernel, grid, block, 0, stream, a);
   if (plan.splits > 1) {
-    if (a.D == 128)
-      hipLaunchKernelGGL(paged_merge_splits_d128_kernel, merge, block, 0, stream, a);
+    const int rows_at = 4 * kThreads / a.D;
+    const dim3 joined((unsigned)((int64_t)a.B * a.Hkv * ((R + rows_at - 1) / rows_at)));
+    if (plan.splits > kFewSplits && a.D == 128)
+      hipLaunchKernelGGL(paged_merge_many_d128_kernel, merge, block, 0, stream, a);
+    else if (plan.splits > kFewSplits)
+      hipLaunchKernelGGL(paged_merge_many_d64_kernel, merge, block, 0, stream, a);
+    else if (a.D == 128)
+      hipLaunchKernelGGL(paged_merge_splits_d128_kernel, joined, block, 0, stream, a);
     else
-      hipLaunchKernelGGL(paged_merge_splits_d64_kernel, merge, block, 0, stream, a);
+      hipLaunchKernelGGL(paged_merge_splits_d64_kernel, joined, block, 0, stream, a);
   }
   return hipGetLastError();
 }
