@@ -103,7 +103,9 @@ __device__ __forceinline__ float coded_value(float x, int e) {
   return __builtin_fabsf(x) <= 3.4028235e38f ? __builtin_amdgcn_ldexpf(x, -e) : __builtin_nanf("");
 }
 __device__ __forceinline__ int encode4(float a, float b, float c, float d) {
-  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+  int x = __builtin_nondeterministic_value(x);  // both halves are written below
+  x = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, x, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, x, true);
 }
 // Four codes times 2^shift, rounded to codes again.
 __device__ __forceinline__ int recode4(int x, int shift) {

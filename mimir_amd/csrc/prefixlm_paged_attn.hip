@@ -44,7 +44,7 @@ __device__ __forceinline__ void halves8(float a, float b, float c, float d, int&
   constexpr float kLoScale = 1.f / (1 << kLoShift);
   hi = encode4(a, b, c, d);
   const f32x2 ab = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), cd = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-  s16x2 x = {0, 0};
+  s16x2 x = __builtin_nondeterministic_value(x);  // both halves are written below
   x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, a - ab[0], b - ab[1], kLoScale, false);
   x = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(x, c - cd[0], d - cd[1], kLoScale, true);
   lo = __builtin_bit_cast(int, x);
@@ -1120,7 +1120,7 @@ Plan plan_of(const MimirPagedAttnParams& p) {
   }
   s.n_rt = (int)((R + kRows - 1) / kRows);
   const int64_t groups = pairs * s.n_rt;
-  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / groups, p.table_width, kMaxSplits}));
+  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + groups * 3 / 4) / groups, p.table_width, kMaxSplits}));
   s.units = groups * s.splits;
   s.workspace_bytes = s.splits > 1 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
   return s;

@@ -59,24 +59,38 @@ __device__ __forceinline__ int block_exclusive(int x, int* shared, int& total) {
   return before + incl - x;
 }
 
+// A thread's kOwn consecutive counts from page p on, as a mask of those that hold(count); pages past the
+// last are left out.  Four 16-byte loads where the array allows it.
+constexpr int kOwn = 16;
+template <typename F>
+__device__ __forceinline__ unsigned count_mask(const Table& t, int p, F&& hold) {
+  unsigned mask = 0;
+  if (p + kOwn <= t.num_pages && (uintptr_t)t.counts % 16 == 0) {
+    i32x4 c[kOwn / 4];
+#pragma unroll
+    for (int e = 0; e < kOwn / 4; ++e) c[e] = ((const i32x4*)(t.counts + p))[e];
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) mask |= (hold(c[e / 4][e % 4]) ? 1u : 0u) << e;
+  } else {
+    for (int e = 0; e < kOwn && p + e < t.num_pages; ++e) mask |= (hold(t.counts[p + e]) ? 1u : 0u) << e;
+  }
+  return mask;
+}
+
 // The first `wanted` free pages, ascending, into list; returns how many there are (at most
-// wanted).  They count one from here on.  One workgroup of kScan threads.
+// wanted).  They count one from here on.  One workgroup of kScan threads, and no other at the time.
 __device__ int take_free(const Table& t, int wanted, int32_t* list, int* shared) {
   int found = 0;
-  for (int p0 = 0; p0 < t.num_pages && found < wanted; p0 += 4 * kScan) {
-    const int p = p0 + 4 * (int)threadIdx.x;
-    int free = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (p + e < t.num_pages && load_count(&t.counts[p + e]) == 0) free |= 1 << e;
+  for (int p0 = 0; p0 < t.num_pages && found < wanted; p0 += kOwn * kScan) {
+    const int p = p0 + kOwn * (int)threadIdx.x;
+    unsigned free = count_mask(t, p, [](int c) { return c == 0; });
     int total;
     int at = found + block_exclusive(__popc(free), shared, total);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((free >> e & 1) && at < wanted) {
-        list[at++] = p + e;
-        t.counts[p + e] = 1;
-      }
+    for (; free != 0 && at < wanted; free &= free - 1, ++at) {
+      const int page = p + __builtin_ctz(free);
+      list[at] = page;
+      t.counts[page] = 1;
+    }
     found += total;
   }
   __threadfence_block();
@@ -100,11 +114,12 @@ struct CopyArgs {
   // what the launch writes beside: fork's rows (entries with kept[i]) ...
   const int32_t *rowbuf, *kept, *dst_rows, *new_len;
   int entries;
-  // ... or compact's renamed pages
-  const int32_t* map;
+  // ... or compact's renamed pages, of those at or past used[0]
+  const int32_t *map, *used;
 };
 
 __global__ __launch_bounds__(kCopyThreads) void pages_move_kernel(const CopyArgs a) {
+  touch_args<sizeof(CopyArgs)>();
   const Table& t = a.table;
   const int64_t threads = (int64_t)gridDim.x * kCopyThreads, id = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
   const int n = a.n_dev != nullptr ? *a.n_dev : a.n;
@@ -117,11 +132,12 @@ __global__ __launch_bounds__(kCopyThreads) void pages_move_kernel(const CopyArgs
     }
   }
   if (a.map != nullptr) {
+    const int used = *a.used;
     for (int64_t i = id; i < (int64_t)t.rows * t.width; i += threads) {
       const int r = (int)(i / t.width);
       int32_t* const at = t.row(r) + (i - (int64_t)r * t.width);
       const int p = *at;
-      if (t.page_ok(p) && a.map[p] != p) *at = a.map[p];
+      if (p >= used && t.page_ok(p)) *at = a.map[p];
     }
     for (int64_t m = id; m < n; m += threads) {
       t.counts[a.dst[m]] = t.counts[a.src[m]];
@@ -245,18 +261,16 @@ __device__ __forceinline__ void fork_take(const ForkArgs& a, int* shared) {
   }
 }
 
-__global__ __launch_bounds__(kScan) void fork_small_kernel(const ForkArgs a) {
-  __shared__ int shared[kScan / 64];
+__global__ __launch_bounds__(kScan) void fork_plan_kernel(const ForkArgs a) {
+  touch_args<sizeof(ForkArgs)>();
   fork_plan(a);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = wave; i < a.n; i += kScan / 64) fork_gather(a, i, lane, 64);
-  __threadfence_block();
-  __syncthreads();
-  fork_take(a, shared);
 }
-__global__ __launch_bounds__(kScan) void fork_plan_kernel(const ForkArgs a) { fork_plan(a); }
-__global__ __launch_bounds__(256) void fork_gather_kernel(const ForkArgs a) { fork_gather(a, blockIdx.x, threadIdx.x, 256); }
+__global__ __launch_bounds__(256) void fork_gather_kernel(const ForkArgs a) {
+  touch_args<sizeof(ForkArgs)>();
+  fork_gather(a, blockIdx.x, threadIdx.x, 256);
+}
 __global__ __launch_bounds__(kScan) void fork_take_kernel(const ForkArgs a) {
+  touch_args<sizeof(ForkArgs)>();
   __shared__ int shared[kScan / 64];
   fork_take(a, shared);
 }
@@ -269,34 +283,31 @@ struct CompactArgs {
 };
 
 __global__ __launch_bounds__(kScan) void compact_plan_kernel(const CompactArgs a) {
+  touch_args<sizeof(CompactArgs)>();
   __shared__ int shared[kScan / 64];
   const Table& t = a.t;
-  int mine = 0, used;
-  for (int p = threadIdx.x; p < t.num_pages; p += kScan) mine += t.counts[p] > 0;
+  // the thread's pages of the first 16384, which it looks at once, and those behind them
+  const unsigned first = count_mask(t, kOwn * (int)threadIdx.x, [](int c) { return c > 0; });
+  int mine = __popc(first), used;
+  for (int p = kOwn * (kScan + (int)threadIdx.x); p < t.num_pages; p += kOwn * kScan)
+    mine += __popc(count_mask(t, p, [](int c) { return c > 0; }));
   block_exclusive(mine, shared, used);
   int holes = 0, moves = 0;
-  for (int p0 = 0; p0 < t.num_pages; p0 += 4 * kScan) {
-    const int p = p0 + 4 * (int)threadIdx.x;
-    int held = 0, inside = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (p + e < t.num_pages) {
-        inside |= 1 << e;
-        held |= (t.counts[p + e] > 0) << e;
-        a.map[p + e] = p + e;
-      }
-    const int front = used <= p ? 0 : (used - p >= 4 ? 15 : (1 << (used - p)) - 1);  // pages before `used`
-    const int hole = inside & ~held & front, late = held & ~front;
-    int total_h, total_m;
-    int ah = holes + block_exclusive(__popc(hole), shared, total_h);
-    int am = moves + block_exclusive(__popc(late), shared, total_m);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (hole >> e & 1) a.to[ah++] = p + e;
-      if (late >> e & 1) a.from[am++] = p + e;
-    }
-    holes += total_h;
-    moves += total_m;
+  for (int p0 = 0; p0 < t.num_pages; p0 += kOwn * kScan) {
+    const int p = p0 + kOwn * (int)threadIdx.x;
+    const unsigned held = p0 == 0 ? first : count_mask(t, p, [](int c) { return c > 0; });
+    const int left = t.num_pages - p;
+    const unsigned inside = left >= kOwn ? (1u << kOwn) - 1 : (left <= 0 ? 0u : (1u << left) - 1);
+    const unsigned front = used - p >= kOwn ? (1u << kOwn) - 1 : (used <= p ? 0u : (1u << (used - p)) - 1);  // pages before `used`
+    unsigned hole = inside & ~held & front, late = held & ~front;
+    // a free page behind `used` stays what it is, should a row name it all the same
+    for (unsigned rest = inside & ~held & ~front; rest != 0; rest &= rest - 1) a.map[p + __builtin_ctz(rest)] = p + __builtin_ctz(rest);
+    int total;  // of holes in the lower half, of late pages in the upper: at most kOwn * kScan each
+    const int before = block_exclusive(__popc(hole) | __popc(late) << 16, shared, total);
+    for (int at = holes + (before & 0xffff); hole != 0; hole &= hole - 1) a.to[at++] = p + __builtin_ctz(hole);
+    for (int at = moves + (before >> 16 & 0xffff); late != 0; late &= late - 1) a.from[at++] = p + __builtin_ctz(late);
+    holes += total & 0xffff;
+    moves += total >> 16 & 0xffff;
   }
   __threadfence_block();
   __syncthreads();
@@ -337,6 +348,7 @@ __device__ __forceinline__ int reserve_until(const ReserveArgs& a, int r) {
 
 // One wave per row: the pages it lacks.
 __global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs a) {
+  touch_args<sizeof(ReserveArgs)>();
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= a.t.rows) return;
   const int until = reserve_until(a, r);
@@ -349,6 +361,7 @@ __global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs a)
 
 // lack[r] becomes the rank of the row's first request; the free pages are listed.
 __global__ __launch_bounds__(kScan) void reserve_take_kernel(const ReserveArgs a) {
+  touch_args<sizeof(ReserveArgs)>();
   __shared__ int shared[kScan / 64];
   int64_t wanted = 0;
   for (int r0 = 0; r0 < a.t.rows; r0 += kScan) {
@@ -367,6 +380,7 @@ __global__ __launch_bounds__(kScan) void reserve_take_kernel(const ReserveArgs a
 }
 
 __global__ __launch_bounds__(256) void reserve_assign_kernel(const ReserveArgs a) {
+  touch_args<sizeof(ReserveArgs)>();
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= a.t.rows) return;
   const int until = reserve_until(a, r), got = *a.got;
@@ -490,14 +504,10 @@ int mimir_prefixlm_pages_fork(const MimirPagesParams* p, const int32_t* source, 
   f.kept = take(n); f.new_len = take(n); f.tail = take(n);
   f.from = take(n); f.to = take(n); f.free = take(n);
   f.rowbuf = take((int64_t)n * p->width);
-  // The rows' pages in one workgroup while they are few: one launch instead of three.
-  if ((int64_t)n * p->width <= 64 * kScan) {
-    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kScan), 0, s, f);
-  } else {
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kScan), 0, s, f);
-    hipLaunchKernelGGL(fork_gather_kernel, dim3((unsigned)n), dim3(256), 0, s, f);
-    hipLaunchKernelGGL(fork_take_kernel, dim3(1), dim3(kScan), 0, s, f);
-  }
+  // (All three in one workgroup took 26 us for 256 rows of up to 48 pages, a wave's rows one after another.)
+  hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kScan), 0, s, f);
+  hipLaunchKernelGGL(fork_gather_kernel, dim3((unsigned)n), dim3(256), 0, s, f);
+  hipLaunchKernelGGL(fork_take_kernel, dim3(1), dim3(kScan), 0, s, f);
   CopyArgs a = copy_args(*p);
   a.src = f.from;
   a.dst = f.to;
@@ -531,6 +541,7 @@ int mimir_prefixlm_pages_compact(const MimirPagesParams* p, int32_t* used, void*
   a.dst = c.to;
   a.n_dev = c.n_moves;
   a.map = c.map;
+  a.used = used;
   launch_move(a, std::max<int64_t>((int64_t)p->num_pages / 2 * a.chunks, ((int64_t)p->rows * p->width + kCopyThreads - 1) / kCopyThreads), s);
   return launched("compact launch");
 }

@@ -165,6 +165,30 @@ def test_compact(device, rows, width, pages, layers, heads, d):
         _same_cache(cache, pool)
 
 
+def test_compact_large_pools_and_odd_tables(device):
+    """More pages than the scan holds at once, counts that are not 16-byte aligned, and a row that names a
+    free page or none at all: such entries stay."""
+    for pages, offset in ((40_000, 0), (16_385, 1), (20_000, 3)):
+        cache = _random_cache(device, pages, 1, 1, 64, pages)
+        table = _random_table(device, 30, 60, pages, 7)
+        table.pages[3, 59], table.pages[4, 58], table.pages[5, 57] = pages - 1, pages + 5, -7
+        room = torch.zeros(pages + 4, dtype=torch.int32, device=device)
+        room[offset:offset + pages] = table.counts
+        room[offset + pages - 1] = 0
+        table = table._replace(counts=room[offset:offset + pages])
+        pool, want = O.Cache(*cache), O.Table(*table)
+        used = compact_pages(cache, table)
+        n, moves = want.compact()
+        pool.move(moves)
+        assert used.tolist() == [n] and len(moves) > 0
+        _same_table(table, want, pages)
+        _same_cache(cache, pool, pages)
+        new = torch.full((30,), 200, device=device)
+        reserve_pages(table, new)
+        want.reserve([200] * 30)
+        _same_table(table, want, pages)
+
+
 @pytest.mark.parametrize("n", [0, 1, 37, 600])
 def test_copy(device, n):
     cache = _random_cache(device, 1300, 2, 1, 64, n)
