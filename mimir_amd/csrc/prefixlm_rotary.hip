@@ -18,7 +18,7 @@
 // Bound by reading and writing the heads once.  A thread owns V pairs of columns of one
 // token, computes their angles once and takes every hp-th head of q and k with them, so
 // the series are shared by the heads and the loads of several heads are in flight
-// together; hp grows where the tokens alone do not fill the chip.
+// together.
 #include <algorithm>
 #include <cmath>
 
@@ -203,8 +203,12 @@ extern "C" int mimir_prefixlm_rotary(const MimirRotaryParams* p, void* stream) {
   // In place the columns past rotary_dim are there already.
   const bool in_place = a.q == a.qo && (!k || a.k == a.ko);
   a.items = in_place ? a.turning : p->head_dim / (2 * v);
-  // Threads for the whole chip (256 CUs x 16 waves): heads side by side until there are as many.
-  a.hp = 1;
+  // Four heads a thread, all in flight at once, or fewer until there are threads for the whole chip (256 CUs
+  // x 16 waves).  One thread for all heads while the tokens fill the chip / so: 16384 tokens, 20 heads of 128,
+  // 37.9 / 34.6 us (4.9 TB/s, a large copy's 5.1), 32768 tokens, 40 heads, half turned, 150 / 127 (5.3 TB/s),
+  // 24000 tokens, 4 heads, 13.8 / 10.4.  Two or eight heads are within 2%; non-temporal loads or stores slower
+  // (127 -> 136, 227).
+  a.hp = (a.H + 3) / 4;
   while (a.hp < a.H && a.tokens * a.items * a.hp < (int64_t)256 * 16 * 64) a.hp *= 2;
   a.hp = std::min(a.hp, a.H);
   if ((a.tokens * a.items * a.hp + 255) / 256 > 0x7fffffff) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many tokens for one launch");
