@@ -1106,7 +1106,15 @@ Plan plan_of(const MimirPagedAttnParams& p) {
   s.splits = 1;
   if (s.decode) {
     const int64_t most = (int64_t)p.batch * ((p.table_width + kUnit - 1) / kUnit);  // units of the line
-    s.pairs = p.batch > kLineRows || p.table_width <= kUnit;
+    // One workgroup per pair (nothing to merge, one launch) for short tables, and the longer the more pairs there
+    // are to even out, up to 1 MiB of keys and values: the longest pair runs alone.  Shares / pairs, 16 / 4
+    // heads of 128: one row of 450 keys 14.3 / 8.8 us, of 1000 14.1 / 12.1, of 2000 13.9 / 19.1; 8 rows of up to
+    // 1000 14.7 / 13.8, 1500 14.8 / 17.1; 64 of up to 1000 26.0 / 15.9, 2000 32.0 / 25.9, 8000 62 / 75; 200 of up
+    // to 2000 67 / 61; 128 of up to 6000, 32 / 8 heads, 168 / 175.  Heads of 64: 64 of up to 3000, 8 / 8, 32.5 /
+    // 25.1, 250 of up to 4000, 8 / 2, 39.1 / 31.6, 48 of up to 4000 17.4 / 29.4.  Twice as long with two row tiles,
+    // whose parts are larger (64 rows of up to 2000, 16 / 4 heads of 128, 5 tokens: 54 / 31).
+    const int64_t pair_pages = std::max<int64_t>(16, std::min<int64_t>(16 * pairs, 8192) / p.head_dim * (R > 16 ? 2 : 1));
+    s.pairs = p.batch > kLineRows || p.table_width <= pair_pages;
     if (s.pairs) {
       s.units = pairs;
     } else {

@@ -160,6 +160,33 @@ def test_many_rows(device, batch, hkv):
     _run(device, 1, 4 * hkv, hkv, 64, torch.randint(0, 700, (batch,), generator=gen).tolist(), seed=batch)
 
 
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("S", [1, 3, 8])
+def test_wide_tables(device, S, d):
+    """Tables much wider than the rows are long: their pages are dealt to shares whatever their number, with new
+    tokens in the last page of a share, padded rows, rows without keys, and NaN tokens."""
+    lens = [0, 1, 62, 63, 64, 65, 777, 1499, 255, 256, 257]
+    _run(device, S, 8, 2, d, lens, width=1100, seed=S)
+    _run(device, S, 8, 2, d, lens, False, new=[S, 0, 1, S, 0, S, S, max(S - 1, 1), S, 0, S], width=1100, seed=S)
+
+    def edit(x):
+        x["v"][6, S - 1, 1, 5] = float("nan")
+        x["k"][7, S // 2, 0] = float("inf")
+        x["order"][2] = -1
+        x["lengths"][5] = -1
+        x["table"][6, 3] = -1
+    _run(device, S, 8, 2, d, lens, rows=list(range(11)), width=1100, edit=edit, grow=20.0)
+
+
+@pytest.mark.parametrize("batch", [64, 65, 129, 256])
+def test_many_rows_in_a_wide_table(device, batch):
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 900, (batch,), generator=gen).tolist()
+    new = torch.randint(0, 2, (batch,), generator=gen).tolist()
+    _run(device, 1, 4, 1, 64, lens, seed=batch, width=600)
+    _run(device, 1, 4, 1, 64, lens, seed=batch, width=600, new=new)
+
+
 @pytest.mark.parametrize("S,hq", [(1, 8), (3, 8), (6, 8), (33, 8)])
 def test_long_rows(device, S, hq):
     """A long row cut into many shares (more than 64 pages for a wave), beside short ones."""
