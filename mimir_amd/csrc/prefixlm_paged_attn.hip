@@ -901,11 +901,12 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     }
     // tokens 32 hi + 16 t + e
     if (base + kPage > w_min) {
+      const int see = limit - base - 32 * hi;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (base + 32 * hi + 16 * t + e >= limit) st[t][e] = -INFINITY;
+          if (16 * t + e >= see) st[t][e] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
