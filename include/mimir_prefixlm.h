@@ -462,7 +462,8 @@ int mimir_prefixlm_rotary(const MimirRotaryParams* params, void* stream);
  *
  * Tokens past the table (t / 64 >= table_width) and pages outside [0, num_pages) are neither
  * written nor attended; a batch row whose table row lies outside [0, table_rows), or whose
- * length is negative, gives zeros.  No two batch rows of a call may append to one page.
+ * length is negative, gives zeros.  A page that a batch row appends to must be that row's
+ * alone in the call (neither appended to nor read for another): the rows run side by side.
  * q, k_new, v_new and out are bf16 rows, 16-byte aligned, strides in elements; head_dim 64
  * or 128.  The workspace holds partial results of split key ranges (nothing to clear: the
  * call can be captured in a graph). */

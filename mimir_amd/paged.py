@@ -236,6 +236,8 @@ def _rows4(name: str, t: Tensor) -> Tensor:
 
 def _validate(cache, table, lens, rows, new, S: int) -> None:
     """One host read for all checks of a call's indices."""
+    if table.shape[0] == 0:
+        raise IndexError("a page table without rows")
     n = lens.long()
     m = torch.full_like(n, S) if new is None else new.long()
     r = torch.arange(len(n), device=n.device) if rows is None else rows.long()
@@ -247,8 +249,9 @@ def _validate(cache, table, lens, rows, new, S: int) -> None:
     written = read & ((at + 1) * PAGE_TOKENS > n[:, None])
     bad = read & ((held < 0) | (held >= cache.keys.shape[0]))
     w = held[written & ~bad]
+    readers = torch.bincount(held[read & ~bad], minlength=1)  # of each page, in this call
     found = torch.stack([(n < 0).any(), ((m < 0) | (m > S)).any(), (~inside).any(), (end > table.shape[1] * PAGE_TOKENS).any(), bad.any(),
-                         torch.bincount(w, minlength=1).max() > 1 if len(w) else bad.new_zeros(())]).tolist()
+                         (readers[w] > 1).any()]).tolist()
     if found[0]:
         raise ValueError("cache_lengths must be non-negative")
     if found[1]:
@@ -260,7 +263,7 @@ def _validate(cache, table, lens, rows, new, S: int) -> None:
     if found[4]:
         raise IndexError("a row has no page for tokens that the call reads or writes")
     if found[5]:
-        raise ValueError("two batch rows append to one page")
+        raise ValueError("a page that a batch row appends to is held twice in the call")
 
 
 def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: PagedCache, layer: int, page_table: Tensor,
@@ -278,9 +281,10 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
     ``new_lengths`` [B]: of a padded batch, the tokens that count; the others are not appended and
     their outputs are zeros.  A row of 0 is left alone.  ``page_table`` is int32 [rows, max_pages]
     (``PageTable.pages``); the pages must be there (:func:`reserve_pages`): tokens without one are
-    dropped, and not attended.  No two batch rows may append to one page (fork_rows sees to that).
-    Both raise with ``mimir_amd.set_validate_metadata(True)``, which costs a host read.  Infinite
-    keys and values become NaN.
+    dropped, and not attended.  A page that a batch row appends to must be that row's alone in the
+    call, neither appended to nor read for another (fork_rows sees to that): the rows run side by
+    side.  Both raise with ``mimir_amd.set_validate_metadata(True)``, which costs a host read.
+    Infinite keys and values become NaN.  For inference: the result has no gradient.
     """
     scale = (1.0 / math.sqrt(query.shape[-1]) if query.shape[-1] else 1.0) if softmax_scale is None else float(softmax_scale)
     if query.is_cuda and not P._validate_metadata:
@@ -324,7 +328,7 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
 
     lens, rows, new = (index(n, t) for n, t in (("cache_lengths", cache_lengths), ("cache_batch_indices", cache_batch_indices),
                                                 ("new_lengths", new_lengths)))
-    if P._validate_metadata and B > 0 and S > 0 and page_table.shape[0] > 0:
+    if P._validate_metadata and B > 0 and S > 0:
         _validate(cache, page_table, lens, rows, new, S)
     q, k, v = _rows4("query", query), _rows4("key", key), _rows4("value", value)
     out = torch.empty((B, S, hq, d), dtype=q.dtype, device=device)

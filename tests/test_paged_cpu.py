@@ -148,3 +148,35 @@ def test_structs_match_the_header(cls, name):
     size, offsets = _c_layout(name, fields)
     assert ctypes.sizeof(cls) == size
     assert [getattr(cls, f).offset for f in fields] == list(offsets)
+
+
+@pytest.mark.parametrize("table,lens,new,bad", [
+    ([[0, 1], [0, 2]], [64, 65], None, None),           # page 0 is only read
+    ([[0, 1], [0, 2]], [3, 64], None, ValueError),      # appended to by row 0, read for row 1
+    ([[0, 1], [0, 2]], [64, 3], None, ValueError),
+    ([[0, 1], [0, 2]], [3, 64], [1, 0], None),          # row 1 is left alone
+    ([[0, 1], [2, 2]], [3, 64], None, ValueError),      # twice in one row
+    ([[0, 1], [2, 0]], [3, 5], None, None),             # behind row 1's last token: not looked at
+    ([[0, 1], [2, 3]], [63, 63], [2, 1], None),
+    ([[0, 1], [1, 3]], [63, 63], [2, 1], ValueError),   # row 0's second new token, row 1's page
+])
+def test_appended_pages_are_one_rows(table, lens, new, bad):
+    from mimir_amd.paged import _validate
+    ints = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    call = lambda rows=None: _validate(PagedCache.create(4, 1, 2, 64, device="cpu"), ints(table), ints(lens), rows,  # noqa: E731
+                                       None if new is None else ints(new), 2 if new else 1)
+    if bad is None:
+        call()
+    else:
+        with pytest.raises(bad, match="held twice"):
+            call()
+
+
+def test_validation_of_rows():
+    from mimir_amd.paged import _validate
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    cache, table = PagedCache.create(4, 1, 2, 64, device="cpu"), ints([0, 1], [2, 3])
+    with pytest.raises(ValueError, match="held twice"):
+        _validate(cache, table, ints(3, 3), ints(1, 1), None, 1)
+    with pytest.raises(IndexError, match="without rows"):
+        _validate(cache, table[:0], ints(3, 3), None, None, 1)
