@@ -530,6 +530,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (k != nullptr) ko = out[1];
     } else {
       if (truth(a[7])) {
+        NEED(k == nullptr || k->const_data_ptr() != q.const_data_ptr());
         for (const at::Tensor* t : {&q, k})
           for (int64_t i = 0; t != nullptr && i < t->dim(); ++i) NEED(t->size(i) <= 1 || t->stride(i) > 0);
         qo = q;

@@ -198,7 +198,7 @@ extern "C" int mimir_prefixlm_rotary(const MimirRotaryParams* p, void* stream) {
     return (uintptr_t)a.q % bytes == 0 && (uintptr_t)a.qo % bytes == 0 && (!k || ((uintptr_t)a.k % bytes == 0 && (uintptr_t)a.ko % bytes == 0));
   };
   while (v > 1 && !fits(v)) v /= 2;
-  if ((uintptr_t)a.q % es != 0 || (uintptr_t)a.qo % es != 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "rotary tensors must be aligned to their elements");
+  if ((uintptr_t)a.q % es != 0 || (uintptr_t)a.qo % es != 0 || (k && ((uintptr_t)a.k % es != 0 || (uintptr_t)a.ko % es != 0))) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "rotary tensors must be aligned to their elements");
   a.turning = p->rotary_dim / (2 * v);
   // In place the columns past rotary_dim are there already.
   const bool in_place = a.q == a.qo && (!k || a.k == a.ko);

@@ -32,6 +32,7 @@ from . import _capi
 from . import prefixlm as P
 
 PAGE_TOKENS = _capi.PAGE_TOKENS
+_INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
 class PagedCache(NamedTuple):
@@ -101,8 +102,10 @@ def _check_table(table: PageTable):
 
 
 def _row_list(name: str, t: Tensor, device) -> Tensor:
-    if t.dim() != 1 or t.is_floating_point() or t.is_complex():
+    if t.dim() != 1 or t.dtype not in _INTS:
         raise ValueError(f"{name} must be a vector of whole numbers, got {tuple(t.shape)} {t.dtype}")
+    if t.dtype == torch.int64:  # what 32 bits do not hold stays outside, rather than wrap to a row or page
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -322,7 +325,7 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
     def index(name, t):
         if t is None:
             return None
-        if t.shape != (B,) or t.is_floating_point():
+        if t.shape != (B,) or t.dtype not in _INTS:
             raise ValueError(f"{name} must be [{B}] whole numbers, got {tuple(t.shape)} {t.dtype}")
         return t.to(device=device, dtype=index_dtype).contiguous()
 

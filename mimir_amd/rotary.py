@@ -131,6 +131,8 @@ def _check(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
 def _turn(query, key, positions, frequencies, inverse: bool, inplace: bool = False):
     """Checked operands -> turned query and key (None without one)."""
     if inplace:
+        if key is not None and key.numel() > 0 and key.data_ptr() == query.data_ptr():
+            raise ValueError("an in-place query and key need memory of their own: the same tensor would be turned twice")
         for name, t in (("query", query), ("key", key)):
             if t is not None and (t.stride(-1) != 1 or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride()))):
                 raise ValueError(f"an in-place {name} needs a unit head_dim stride and memory of its own for every row")

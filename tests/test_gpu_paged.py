@@ -364,3 +364,30 @@ def test_validation(device):
             attention_with_pages(q, k, k, cache, 0, ints([0, 1], [3, -1]), ints(64, 65), True)
     finally:
         mimir_amd.set_validate_metadata(False)
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_two_streams_at_once(device, S):
+    """Calls of two layers that overlap on two streams, as the calls one after another."""
+    gen = torch.Generator().manual_seed(12)
+    lens = [900, 64, 5, 2030]
+    cache, table = _pool(lens, [8 * S] * 4, 2, 64, 2, gen)
+    one, two = (PagedCache(*(_move(x, device) for x in cache)) for _ in range(2))
+    table, lengths = table.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+    q, k, v = (torch.randn(4, S, h, 64, generator=gen).to(BF16).to(device) for h in (8, 2, 2))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs, wants = [[], []], [[], []]
+    torch.cuda.synchronize()
+    for step in range(6):
+        at = lengths + S * step
+        torch.cuda.synchronize()
+        for layer in range(2):
+            with torch.cuda.stream(streams[layer]):
+                outs[layer].append(attention_with_pages(q, k, v, one, layer, table, at, True))
+        for layer in range(2):
+            wants[layer].append(attention_with_pages(q, k, v, two, layer, table, at, True))
+    torch.cuda.synchronize()
+    for a, b in zip(outs[0] + outs[1], wants[0] + wants[1]):
+        assert torch.equal(a, b)
+    for a, b in zip(one, two):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

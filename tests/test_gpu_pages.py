@@ -335,3 +335,16 @@ def test_serving_run(device):
     for got, x in zip(cache[:2], (pool.keys, pool.values)):  # NaN codes of either sign are one
         g = got.cpu().view(torch.uint8).numpy()
         assert ((g == x) | ((g & 127 == 127) & (x & 127 == 127))).all()
+
+
+def test_numbers_past_32_bits_name_no_row(device):
+    table = _random_table(device, 4, 6, 40, 3)
+    want = O.Table(*table)
+    far = torch.tensor([1 << 32, (1 << 32) + 2, -(1 << 32)], device=device)
+    release_rows(table, far)
+    cache = PagedCache.create(40, 1, 1, 64, device=device)
+    fork_rows(cache, table, far, torch.tensor([0, 1, 2], device=device))
+    _same_table(table, want)
+    for bad in (torch.ones(4, dtype=torch.bool, device=device), torch.ones(4, device=device)):
+        with pytest.raises(ValueError, match="whole numbers"):
+            release_rows(table, bad)

@@ -174,3 +174,46 @@ def test_captured_and_on_another_stream(device):
         torch.cuda.synchronize()
         want = rotary(q, k, pos, table)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_one_tensor_in_place_as_query_and_key(device):
+    x = torch.randn(4, 3, 64, device=device)
+    table, pos = RotaryFrequencies.create(64, device=device), torch.arange(4, device=device)
+    for key in (x, x[:, :1]):
+        with pytest.raises(ValueError, match="memory of their own"):
+            rotary(x, key, pos, table, inplace=True)
+    want, _ = rotary(x, None, pos, table)
+    rotary(x[:, :2], x[:, 2:], pos, table, inplace=True)
+    assert torch.equal(x, want)
+
+
+def test_captured_forward_and_backward(device):
+    """The whole step in a graph, replayed beside eager steps of the same leaves, and a backward on a side stream."""
+    q, k = (torch.randn(3, 37, h, 64, device=device).bfloat16().requires_grad_(True) for h in (6, 2))
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    pos = torch.arange(37, device=device).expand(3, 37).contiguous()
+    table = RotaryFrequencies.create(48, interleaved=True, device=device)
+
+    def step():  # no graph of the leaves lives on after it
+        out = rotary(q, k, pos, table)
+        return (*torch.autograd.grad(out, (q, k), (dq, dk)), *(x.detach() for x in out))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step()
+    torch.cuda.synchronize()
+    for a, b in zip(eager, step()):
+        assert torch.equal(a, b)
+    for i in range(3):
+        pos.add_(1000 + i)
+        with torch.no_grad():
+            for x in (q, k, dq, dk):
+                x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b), i

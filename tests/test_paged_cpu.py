@@ -180,3 +180,13 @@ def test_validation_of_rows():
         _validate(cache, table, ints(3, 3), ints(1, 1), None, 1)
     with pytest.raises(IndexError, match="without rows"):
         _validate(cache, table[:0], ints(3, 3), None, None, 1)
+
+
+def test_lists_of_rows():
+    from mimir_amd.paged import _row_list
+    far = torch.tensor([0, 1 << 32, -(1 << 32), (1 << 32) + 1, -1])
+    assert _row_list("rows", far, "cpu").tolist() == [0, (1 << 31) - 1, -(1 << 31), (1 << 31) - 1, -1]  # none of them row 0 or 1 but the first
+    assert _row_list("rows", torch.tensor([3, 250], dtype=torch.uint8), "cpu").tolist() == [3, 250]
+    for bad in (torch.tensor([True, False]), torch.tensor([1.0]), torch.tensor([1j]), torch.tensor(1), torch.tensor([[1]])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            _row_list("rows", bad, "cpu")

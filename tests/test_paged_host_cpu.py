@@ -151,3 +151,12 @@ def test_left_to_the_general_path(bound):
                  ("release", table._replace(lengths=ints[:2]), None), ("release", table._replace(counts=ints.long()), None)):
         assert pages(*args) is None, args[0]
     assert calls.value == 0
+
+
+def test_one_tensor_in_place_as_query_and_key(bound):
+    host, _ = bound
+    x, pos, turns = torch.ones(5, 2, 8), torch.arange(5), torch.zeros(4, dtype=torch.int64)
+    assert host.rotary(x, x, pos, turns, 1.0, False, False, True, 0) is None
+    assert host.rotary(x, x[:, :1], pos, turns, 1.0, False, False, True, 0) is None
+    assert host.rotary(x[:, :1], x[:, 1:], pos, turns, 1.0, False, False, True, 0) is not None  # a fused projection's heads
+    assert host.rotary(x, x, pos, turns, 1.0, False, False, False, 0) is not None
