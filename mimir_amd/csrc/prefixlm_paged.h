@@ -30,6 +30,7 @@ struct PagedArgs {
   float *part_o, *part_ml;  // partial rows: unnormalized O [D]; maximum (exp2 domain) and sum
   int shares;               // decode: runs of pages, one workgroup per kv head each
   int n_rt, splits, cus;    // prefill: row tiles per (batch row, kv head), key splits of each
+  int slots;                // prefill of a padded batch: workgroups to deal its pages to; 0: the splits above
 };
 
 __device__ __forceinline__ int64_t paged_index(const void* p, int i, int idx64) {

@@ -36,15 +36,11 @@ __device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touche
   const int at = r.n / kPage + j;                // of the row's pages
   const int lo = max(r.n, at * kPage), hi = min(r.n + r.m, min(at + 1, a.width) * kPage);
   if (lo >= hi) return;
-  const int page = page_id(a, r.row, at);
-  if (page < 0) return;
+  const int page = page_id(a, r.row, at);  // looked at below, when the rows are on their way
   const int s0 = lo - at * kPage, s1 = hi - at * kPage;  // slots of the new tokens
   const bf16_t* const x = values ? a.vn + (int64_t)b * a.vn_sb + (int64_t)hk * a.vn_sh + (int64_t)(lo - r.n) * a.vn_st
                                  : a.kn + (int64_t)b * a.kn_sb + (int64_t)hk * a.kn_sh + (int64_t)(lo - r.n) * a.kn_st;
   const int64_t x_st = values ? a.vn_st : a.kn_st;
-  uint8_t* const y = values ? a.cv + page * a.v_sp + (int64_t)hk * kPage * D : a.ck + page * a.k_sp + (int64_t)hk * kPage * D;
-  int8_t* const ey = values ? a.ve + page * a.ve_sp + hk : a.ke + page * a.ke_sp + hk;
-
   const int row = tid / kUnits, c = tid % kUnits * 8;
   bf16x8 v[kPasses];
   int most = 0;
@@ -53,9 +49,15 @@ __device__ __forceinline__ void paged_append_body(const PagedArgs& a, int touche
     const int t = p * kStep + row;
     v[p] = bf16x8{};
     if (t < s1 - s0) v[p] = *(const bf16x8*)&x[(int64_t)t * x_st + c];
+  }
+  if (page < 0) return;
+  uint8_t* const y = values ? a.cv + page * a.v_sp + (int64_t)hk * kPage * D : a.ck + page * a.k_sp + (int64_t)hk * kPage * D;
+  int8_t* const ey = values ? a.ve + page * a.ve_sp + hk : a.ke + page * a.ke_sp + hk;
+  const int had = s0 > 0 ? *ey : kMinExponent;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
     most = max(most, largest_bits(__builtin_bit_cast(i32x4, v[p])));
   }
-  const int had = s0 > 0 ? *ey : kMinExponent;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) most = max(most, __shfl_xor(most, off, 64));
   if ((tid & 63) == 0) top[tid >> 6] = most;

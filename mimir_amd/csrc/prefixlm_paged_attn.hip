@@ -728,7 +728,46 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
   return __builtin_amdgcn_ballot_w64(8 * (off < 0 ? -off : off) > a.S) == 0;
 }
 
-template <int D>
+// A padded batch (new_lengths), whose row tiles with queries only the device knows: those alone are cut, each
+// into n runs of about as many pages, so that the runs of all are a.slots and one more for each row tile at
+// most.  Runs first, then the row tiles without queries.  64 batch rows, one per lane.  Against splits of the
+// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 82.7 us; 3 x up to 200 on 1000 to
+// 3000, 32 / 8, 42.0 -> 32.6; 8 x up to 700 on up to 2000, 8 / 8 heads of 64, 51.8 -> 43.0; 5 x up to 1339 on up to
+// 1000 49.4 -> 49.2 (more, shorter runs, and 9 us of merge).
+constexpr int kDealtRows = 64;
+struct Runs {
+  PagedRow at;      // of the lane's batch row
+  int act, n;       // its row tiles with queries, the runs of each
+  int incl, idle;   // up to and with it: runs of all kv heads, and row tiles without queries
+  __device__ __forceinline__ Runs(const PagedArgs& a, int lane) {
+    at.row = -1, at.n = at.m = at.kv = 0;
+    if (lane < a.B) at = PagedRow(a, lane);
+    const int tiles = (at.kv + kPage - 1) / kPage;
+    act = at.kv > 0 ? (at.m * a.G + kRows - 1) / kRows : 0;
+    const int pages = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv * tiles), 63);
+    const int most = max(kTogether, (pages + a.slots - 1) / a.slots);
+    n = max(1, (tiles + most - 1) / most);
+    n = (tiles + per(tiles, n) - 1) / per(tiles, n);
+    incl = wave_inclusive_sum(act * a.Hkv * n);
+    idle = wave_inclusive_sum(lane < a.B ? (a.n_rt - act) * a.Hkv : 0);
+  }
+  static __device__ __forceinline__ int per(int tiles, int n) { return max(1, (tiles + n - 1) / n); }
+  __device__ __forceinline__ PagedRow row(int b) const {
+    PagedRow r;
+    r.row = __builtin_amdgcn_readlane(at.row, b);
+    r.n = __builtin_amdgcn_readlane(at.n, b);
+    r.m = __builtin_amdgcn_readlane(at.m, b);
+    r.kv = __builtin_amdgcn_readlane(at.kv, b);
+    return r;
+  }
+  // The first run of row tile rt < act of (b, hk): the latest row tiles first, they see most.
+  __device__ __forceinline__ int first(const PagedArgs& a, int b, int hk, int rt) const {
+    const int tiles = __builtin_amdgcn_readlane(act, b), runs = __builtin_amdgcn_readlane(n, b);
+    return __builtin_amdgcn_readlane(incl, b) + ((hk - a.Hkv) * tiles + tiles - 1 - rt) * runs;
+  }
+};
+
+template <int D, bool kRuns>
 __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   constexpr int DT = D / 32, KS = D / 64;
   constexpr int kCopies = D / 64;  // 1 KiB copies of a page's keys, and of its values, per wave
@@ -746,24 +785,56 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   // Later row tiles of a causal chunk see more keys, and workgroups u and u + (CUs) share a CU.  On
   // rows of about the same length they go by rank, the latest first over all pairs, and every
   // other CU-sized run backwards, so that a CU's two are a long and a short one.
-  int u = blockIdx.x, split = 0, rt;
-  if (a.splits == 1 && a.causal && even_lengths(a)) {
-    const int run = u / a.cus, pairs = gridDim.x / a.n_rt;
-    if (run % 2 == 1 && (run + 1) * a.cus <= (int)gridDim.x) u = (2 * run + 1) * a.cus - 1 - u;
-    rt = a.n_rt - 1 - u / pairs;
-    u %= pairs;
+  int u = blockIdx.x, split = 0, rt, hk, b, n_valid, per;
+  int64_t unit;  // of partial rows
+  PagedRow r;
+  if constexpr (kRuns) {
+    const Runs runs(a, lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(runs.incl > u);
+    unit = u;
+    n_valid = 1;
+    if (past != 0) {
+      b = __builtin_ctzll(past);
+      n_valid = __builtin_amdgcn_readlane(runs.n, b);
+      const int act = __builtin_amdgcn_readlane(runs.act, b);
+      u -= __builtin_amdgcn_readlane(runs.incl, b) - act * a.Hkv * n_valid;
+      split = u % n_valid;
+      u /= n_valid;
+      rt = act - 1 - u % act;
+      hk = u / act;
+    } else {
+      u -= __builtin_amdgcn_readlane(runs.incl, 63);
+      const uint64_t rest = __builtin_amdgcn_ballot_w64(runs.idle > u);
+      if (rest == 0) return;
+      b = __builtin_ctzll(rest);
+      const int act = __builtin_amdgcn_readlane(runs.act, b), idle = a.n_rt - act;
+      u -= __builtin_amdgcn_readlane(runs.idle, b) - idle * a.Hkv;
+      rt = act + u % idle;
+      hk = u / idle;
+    }
+    r = runs.row(b);
+    per = Runs::per((r.kv + kPage - 1) / kPage, n_valid);
   } else {
-    split = u % a.splits;
-    u /= a.splits;
-    rt = a.n_rt - 1 - u % a.n_rt;
-    u /= a.n_rt;
+    if (a.splits == 1 && a.causal && even_lengths(a)) {
+      const int run = u / a.cus, pairs = gridDim.x / a.n_rt;
+      if (run % 2 == 1 && (run + 1) * a.cus <= (int)gridDim.x) u = (2 * run + 1) * a.cus - 1 - u;
+      rt = a.n_rt - 1 - u / pairs;
+      u %= pairs;
+    } else {
+      split = u % a.splits;
+      u /= a.splits;
+      rt = a.n_rt - 1 - u % a.n_rt;
+      u /= a.n_rt;
+    }
+    hk = u % a.Hkv, b = u / a.Hkv;
+    r = PagedRow(a, b);
+    const int tiles = (r.kv + kPage - 1) / kPage;
+    per = max(1, (tiles + a.splits - 1) / a.splits);
+    n_valid = (tiles + per - 1) / per;  // splits that hold keys
+    if (split > 0 && split >= n_valid) return;
+    unit = (((int64_t)b * a.Hkv + hk) * a.n_rt + rt) * a.splits + split;
   }
-  const int hk = u % a.Hkv, b = u / a.Hkv;
-  const PagedRow r(a, b);
   const int R = a.S * a.G, Rm = r.kv > 0 ? r.m * a.G : 0;  // rows, and those that attend
-  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
-  const int n_valid = (tiles + per - 1) / per;  // splits that hold keys
-  if (split > 0 && split >= n_valid) return;
 
   const int row = rt * kRows + wave * 32 + l32;
   const bool row_ok = row < R;
@@ -1014,7 +1085,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       }
     return;
   }
-  const int64_t slot = ((((int64_t)b * a.Hkv + hk) * a.n_rt + rt) * a.splits + split) * kRows + wave * 32 + l32;
+  const int64_t slot = unit * kRows + wave * 32 + l32;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1026,8 +1097,30 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     }
   if (hi == 0) *(f32x2*)&a.part_ml[slot * 2] = f32x2{m_run == -INFINITY ? -INFINITY : m_run * c2, l_tot};
 }
-__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d128_kernel(const PagedArgs a) { paged_prefill_body<128>(a); }
-__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d64_kernel(const PagedArgs a) { paged_prefill_body<64>(a); }
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d128_kernel(const PagedArgs a) { paged_prefill_body<128, false>(a); }
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_d64_kernel(const PagedArgs a) { paged_prefill_body<64, false>(a); }
+__global__ __launch_bounds__(kThreads, 2) void paged_prefill_runs_d128_kernel(const PagedArgs a) { paged_prefill_body<128, true>(a); }
+__global__ __launch_bounds__(kThreads, 3) void paged_prefill_runs_d64_kernel(const PagedArgs a) { paged_prefill_body<64, true>(a); }
+
+// Of a row tile: its batch row, the parts it is in, and the first of them.
+struct Parts {
+  PagedRow r;
+  int n;
+  int64_t first;
+  __device__ __forceinline__ Parts(const PagedArgs& a, int b, int hk, int rt) {
+    if (a.slots > 0) {
+      const Runs runs(a, threadIdx.x & 63);
+      r = runs.row(b);
+      n = __builtin_amdgcn_readlane(runs.n, b);
+      first = runs.first(a, b, hk, rt);
+    } else {
+      r = PagedRow(a, b);
+      const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
+      n = (tiles + per - 1) / per;
+      first = (((int64_t)b * a.Hkv + hk) * a.n_rt + rt) * a.splits;
+    }
+  }
+};
 
 // Adds the partial rows of many key splits (short chunks on long rows), one wave to a row.
 template <int D>
@@ -1038,9 +1131,9 @@ __device__ __forceinline__ void paged_merge_many_body(const PagedArgs& a) {
   const int row = blockIdx.x % groups * kWaves + wave, pair = blockIdx.x / groups;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
   if (row >= R) return;
-  const PagedRow r(a, b);
-  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
-  const int n = (tiles + per - 1) / per;
+  const Parts parts(a, b, hk, row / kRows);
+  const PagedRow& r = parts.r;
+  const int n = parts.n;
   if (n <= 1) return;  // written by its split
   const int i = row / a.G;
   bf16_t* const o = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh;
@@ -1048,44 +1141,62 @@ __device__ __forceinline__ void paged_merge_many_body(const PagedArgs& a) {
     if (lane < D / 8) *(bf16x8*)&o[lane * 8] = bf16x8{};
     return;
   }
-  const int64_t unit0 = ((int64_t)pair * a.n_rt + row / kRows) * a.splits;
-  merge_parts<D>(a, n, lane, [&](int c) { return (unit0 + c) * kRows + row % kRows; }, o);
+  merge_parts<D>(a, n, lane, [&](int c) { return (parts.first + c) * kRows + row % kRows; }, o);
 }
 __global__ __launch_bounds__(kThreads) void paged_merge_many_d128_kernel(const PagedArgs a) { paged_merge_many_body<128>(a); }
 __global__ __launch_bounds__(kThreads) void paged_merge_many_d64_kernel(const PagedArgs a) { paged_merge_many_body<64>(a); }
 
-// The same for a few splits of many rows, D / 4 lanes to a row and four columns each, the parts in turn (a wave to
+// The same for a few splits of many rows, D / 4 lanes to a row and four columns each, four parts at once (a wave to
 // a row / so: 8 x 512 on 1536 keys, 8 / 8 heads of 64, two splits, 67.4 / 49.8 us; 100 on 3000, 16 / 4 heads
 // of 128, 32 splits, 35.7 / 39.6).
 constexpr int kFewSplits = 8;
 template <int D>
 __device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
   touch_args<sizeof(PagedArgs)>();
-  constexpr int kLanes = D / 4, kRowsAt = kThreads / kLanes;
+  constexpr int kLanes = D / 4, kRowsAt = kThreads / kLanes, kChunk = 4;
   const int R = a.S * a.G, groups = (R + kRowsAt - 1) / kRowsAt;
-  const int pair = blockIdx.x / groups, row = (blockIdx.x - pair * groups) * kRowsAt + (int)threadIdx.x / kLanes;
+  const int pair = blockIdx.x / groups, row0 = (blockIdx.x - pair * groups) * kRowsAt, row = row0 + (int)threadIdx.x / kLanes;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv, col = threadIdx.x % kLanes * 4;
-  const PagedRow r(a, b);
-  const int tiles = (r.kv + kPage - 1) / kPage, per = max(1, (tiles + a.splits - 1) / a.splits);
-  const int n = (tiles + per - 1) / per;
+  const Parts parts(a, b, hk, row0 / kRows);  // a workgroup's rows lie in one row tile
+  const int n = parts.n;
   if (n <= 1 || row >= R) return;  // written by its split
   const int i = row / a.G;
-  const int64_t part = (((int64_t)pair * a.n_rt + row / kRows) * a.splits) * kRows + row % kRows;  // + kRows each
-  float M = -INFINITY;
-  for (int c = 0; c < n; ++c) M = fmaxf(M, a.part_ml[2 * (part + c * kRows)]);
+  bf16_t* const out = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col;
+  if (i >= parts.r.m) {  // a padding query
+    *(bf16x4*)out = bf16x4{};
+    return;
+  }
+  const int64_t part = parts.first * kRows + row % kRows;  // + kRows each
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float lsum = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < n; ++c) {
-    const f32x2 ml = *(const f32x2*)&a.part_ml[2 * (part + c * kRows)];
-    const f32x4 o = *(const f32x4*)&a.part_o[(part + c * kRows) * D + col];
-    const float w = ml[0] == -INFINITY ? ml[1] : fast_exp2(ml[0] - M);  // no key: a sum of 0 (or NaN)
-    lsum += ml[1] * w;
-    if (w != 0.f) acc += o * w;
+  float M = -INFINITY, lsum = 0.f;
+  for (int c0 = 0; c0 < n; c0 += kChunk) {
+    f32x2 ml[kChunk];
+    f32x4 o[kChunk];
+#pragma unroll
+    for (int c = 0; c < kChunk; ++c) {
+      const int64_t at = part + min(c0 + c, n - 1) * kRows;
+      ml[c] = *(const f32x2*)&a.part_ml[2 * at];
+      o[c] = *(const f32x4*)&a.part_o[at * D + col];
+    }
+    float m_new = M;
+#pragma unroll
+    for (int c = 0; c < kChunk; ++c) {
+      if (c0 + c >= n) ml[c] = f32x2{-INFINITY, 0.f};
+      m_new = fmaxf(m_new, ml[c][0]);
+    }
+    const float alpha = M == -INFINITY ? 1.f : fast_exp2(M - m_new);  // (what M = -inf has added is 0 or NaN)
+    acc *= alpha;
+    lsum *= alpha;
+    M = m_new;
+#pragma unroll
+    for (int c = 0; c < kChunk; ++c) {
+      const float w = ml[c][0] == -INFINITY ? ml[c][1] : fast_exp2(ml[c][0] - M);  // no key: a sum of 0 (or NaN)
+      lsum += ml[c][1] * w;
+      if (w != 0.f) acc += o[c] * w;
+    }
   }
   const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-  bf16_t* const out = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col;
-  *(bf16x4*)out = i < r.m ? __builtin_convertvector(acc * inv, bf16x4) : bf16x4{};  // zeros for padding queries
+  *(bf16x4*)out = __builtin_convertvector(acc * inv, bf16x4);
 }
 __global__ __launch_bounds__(kThreads) void paged_merge_splits_d128_kernel(const PagedArgs a) { paged_merge_splits_body<128>(a); }
 __global__ __launch_bounds__(kThreads) void paged_merge_splits_d64_kernel(const PagedArgs a) { paged_merge_splits_body<64>(a); }
@@ -1094,7 +1205,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_splits_d64_kernel(const 
 
 struct Plan {
   bool decode, pairs;
-  int n_rt, splits;
+  int n_rt, splits, slots;
   int64_t units;  // workgroups of the attention kernel
   size_t workspace_bytes;
 };
@@ -1131,7 +1242,12 @@ Plan plan_of(const MimirPagedAttnParams& p) {
   const int64_t groups = pairs * s.n_rt;
   s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + groups * 3 / 4) / groups, p.table_width, kMaxSplits}));
   s.units = groups * s.splits;
-  s.workspace_bytes = s.splits > 1 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
+  if (p.new_lengths != nullptr && p.batch <= kDealtRows && groups <= 4 * cus && p.table_width <= 1 << 20) {
+    // (one more per CU: the first three of those 90.7, 35.1 and 40.4 us)
+    s.slots = (int)((p.head_dim == 64 ? 2 : 1) * cus);
+    s.units = groups + s.slots;  // runs: pages / per <= slots, and one more for each row tile
+  }
+  s.workspace_bytes = s.splits > 1 || s.slots > 0 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
   return s;
 }
 
@@ -1168,6 +1284,7 @@ hipError_t launch_paged_attn(const MimirPagedAttnParams& p, const Plan& plan, hi
   a.scale_log2 = std::max(p.softmax_scale * kLog2e, 1.2e-38f);  // a normal number: masked scores times it stay -inf
   a.n_rt = plan.n_rt;
   a.splits = plan.splits;
+  a.slots = plan.slots;
   a.cus = device_cu_count();
   a.part_o = (float*)p.workspace;
   const int64_t R = (int64_t)a.S * a.G;
@@ -1203,11 +1320,15 @@ hipError_t launch_paged_attn(const MimirPagedAttnParams& p, const Plan& plan, hi
     return hipGetLastError();
   }
   a.part_ml = a.part_o + (size_t)plan.units * kRows * p.head_dim;
-  if (a.D == 128)
+  if (a.slots > 0 && a.D == 128)
+    hipLaunchKernelGGL(paged_prefill_runs_d128_kernel, grid, block, 0, stream, a);
+  else if (a.slots > 0)
+    hipLaunchKernelGGL(paged_prefill_runs_d64_kernel, grid, block, 0, stream, a);
+  else if (a.D == 128)
     hipLaunchKernelGGL(paged_prefill_d128_kernel, grid, block, 0, stream, a);
   else
     hipLaunchKernelGGL(paged_prefill_d64_kernel, grid, block, 0, stream, a);
-  if (plan.splits > 1) {
+  if (plan.splits > 1 || plan.slots > 0) {
     const int rows_at = 4 * kThreads / a.D;
     const dim3 joined((unsigned)((int64_t)a.B * a.Hkv * ((R + rows_at - 1) / rows_at)));
     if (plan.splits > kFewSplits && a.D == 128)

@@ -391,3 +391,26 @@ def test_two_streams_at_once(device, S):
         assert torch.equal(a, b)
     for a, b in zip(one, two):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 16, 4), (64, 8, 8), (128, 2, 2)])
+@pytest.mark.parametrize("lens,new,S", [
+    ([0, 0, 0, 0], [0, 0, 0, 0], 300), ([2000], [77], 200), ([3000, 5, 0, 640], [40, 0, 333, 64], 333),
+    ([130, 64, 900], [513, 0, 1], 513), ([0, 63, 64, 65, 200, 1], [128, 129, 127, 1, 0, 256], 256)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_padded_chunks(device, d, hq, hkv, lens, new, S, causal):
+    """Row tiles without queries, rows cut into many and into few runs of pages, lengths on both sides of a tile."""
+    def poison(x):
+        for b, n in enumerate(new):
+            for t in ("q", "k", "v"):
+                x[t][b, n:] = float("nan")
+    _run(device, S, hq, hkv, d, lens, causal, new=new, edit=poison, seed=S + d)
+
+
+@pytest.mark.parametrize("batch,S", [(64, 40), (65, 40), (63, 130), (64, 700)])
+def test_padded_batches_of_many_rows(device, batch, S):
+    """Up to 64 batch rows and 1024 row tiles are dealt by their pages, more are not: both as the oracle says."""
+    gen = torch.Generator().manual_seed(batch + S)
+    lens = torch.randint(0, 200, (batch,), generator=gen).tolist()
+    new = [[0, S, 1, n][n % 4] for n in torch.randint(0, S + 1, (batch,), generator=gen).tolist()]
+    _run(device, S, 8, 4, 64, lens, new=new, seed=batch)
