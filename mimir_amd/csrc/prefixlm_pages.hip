@@ -77,13 +77,17 @@ __device__ __forceinline__ unsigned count_mask(const Table& t, int p, F&& hold) 
   return mask;
 }
 
+// The free ones of the first pages, as take_free wants them: requested early, they are there by then.
+__device__ __forceinline__ unsigned first_free(const Table& t) {
+  return count_mask(t, kOwn * (int)threadIdx.x, [](int c) { return c == 0; });
+}
 // The first `wanted` free pages, ascending, into list; returns how many there are (at most
 // wanted).  They count one from here on.  One workgroup of kScan threads, and no other at the time.
-__device__ int take_free(const Table& t, int wanted, int32_t* list, int* shared) {
+__device__ __forceinline__ int take_free(const Table& t, unsigned first, int wanted, int32_t* list, int* shared) {
   int found = 0;
   for (int p0 = 0; p0 < t.num_pages && found < wanted; p0 += kOwn * kScan) {
     const int p = p0 + kOwn * (int)threadIdx.x;
-    unsigned free = count_mask(t, p, [](int c) { return c == 0; });
+    unsigned free = p0 == 0 ? first : count_mask(t, p, [](int c) { return c == 0; });
     int total;
     int at = found + block_exclusive(__popc(free), shared, total);
     for (; free != 0 && at < wanted; free &= free - 1, ++at) {
@@ -240,6 +244,7 @@ __device__ __forceinline__ void fork_gather(const ForkArgs& a, int i, int thread
 // Free pages for the last pages that are copied.  One workgroup.
 __device__ __forceinline__ void fork_take(const ForkArgs& a, int* shared) {
   const Table& t = a.t;
+  const unsigned first = first_free(t);
   int wanted = 0;
   for (int i0 = 0; i0 < a.n; i0 += kScan) {  // the rank of each request, in a.from for now
     const int i = i0 + threadIdx.x;
@@ -249,7 +254,7 @@ __device__ __forceinline__ void fork_take(const ForkArgs& a, int* shared) {
     if (i < a.n) a.from[i] = need ? rank : -1;
     wanted += total;
   }
-  const int got = take_free(t, wanted, a.free, shared);
+  const int got = take_free(t, first, wanted, a.free, shared);
   if (threadIdx.x == 0 && got < wanted) atomicAdd(t.missing, wanted - got);
   for (int i = threadIdx.x; i < a.n; i += kScan) {
     const int rank = a.from[i];
@@ -363,6 +368,7 @@ __global__ __launch_bounds__(256) void reserve_count_kernel(const ReserveArgs a)
 __global__ __launch_bounds__(kScan) void reserve_take_kernel(const ReserveArgs a) {
   touch_args<sizeof(ReserveArgs)>();
   __shared__ int shared[kScan / 64];
+  const unsigned first = first_free(a.t);
   int64_t wanted = 0;
   for (int r0 = 0; r0 < a.t.rows; r0 += kScan) {
     const int r = r0 + threadIdx.x;
@@ -372,7 +378,7 @@ __global__ __launch_bounds__(kScan) void reserve_take_kernel(const ReserveArgs a
     wanted += total;
   }
   const int most = wanted < a.t.num_pages ? (int)wanted : a.t.num_pages;
-  const int got = take_free(a.t, most, a.free, shared);
+  const int got = take_free(a.t, first, most, a.free, shared);
   if (threadIdx.x == 0) {
     *a.got = got;
     if (got < wanted) atomicAdd(a.t.missing, (int)(wanted - got));
@@ -394,6 +400,72 @@ __global__ __launch_bounds__(256) void reserve_assign_kernel(const ReserveArgs a
     rank += __builtin_popcountll(all);
   }
 }
+
+// Both for up to kScan rows in one launch of one workgroup: the waves go over the rows that lack pages,
+// kAtOnce of them in flight.  Or (kCounts) the count too, over all rows that ask for tokens.
+template <bool kCounts>
+__device__ __forceinline__ void reserve_place(const ReserveArgs& a) {
+  touch_args<sizeof(ReserveArgs)>();
+  constexpr int kAtOnce = 4, kWaves = kScan / 64;
+  __shared__ int shared[kWaves], s_row[kScan], s_until[kScan], s_rank[kScan];
+  const Table& t = a.t;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned first = first_free(t);
+  const int until = tid < t.rows ? reserve_until(a, tid) : 0;
+  const int lack = tid >= t.rows ? 0 : (kCounts ? until : a.lack[tid]);
+  int listed, wanted;
+  const int place = block_exclusive(lack > 0, shared, listed);
+  if constexpr (!kCounts) {
+    const int rank = block_exclusive(lack, shared, wanted);
+    if (lack > 0) s_rank[place] = rank;
+  }
+  if (lack > 0) {
+    s_row[place] = tid;
+    s_until[place] = until;
+  }
+  __syncthreads();
+  // each(e, rank, need, row, j): what lane's place j of listed row e needs, rank its requests so far
+  auto over_rows = [&](auto&& begin, auto&& each, auto&& end) __attribute__((always_inline)) {
+    for (int e0 = wave; e0 < listed; e0 += kAtOnce * kWaves) {
+      int row[kAtOnce], stop[kAtOnce], rank[kAtOnce], most = 0;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int e = min(e0 + k * kWaves, listed - 1);
+        row[k] = s_row[e];
+        stop[k] = e0 + k * kWaves < listed ? s_until[e] : 0;
+        rank[k] = begin(e);
+        most = max(most, stop[k]);
+      }
+      for (int j = lane; j - lane < most; j += 64) {
+        int p[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) p[k] = j < stop[k] ? t.row(row[k])[j] : 0;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const bool need = j < stop[k] && !t.page_ok(p[k]);
+          const uint64_t all = __builtin_amdgcn_ballot_w64(need);
+          each(rank[k] + __builtin_popcountll(all & ((1ull << lane) - 1)), need, row[k], j);
+          rank[k] += __builtin_popcountll(all);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (e0 + k * kWaves < listed) end(e0 + k * kWaves, rank[k]);
+    }
+  };
+  if constexpr (kCounts) {
+    over_rows([](int) { return 0; }, [](int, bool, int, int) {}, [&](int e, int n) { if (lane == 0) s_rank[e] = n; });
+    __syncthreads();
+    const int rank = block_exclusive(tid < listed ? s_rank[tid] : 0, shared, wanted);
+    if (tid < listed) s_rank[tid] = rank;
+  }
+  const int got = take_free(t, first, wanted, a.free, shared);  // (ends with a barrier)
+  if (tid == 0 && got < wanted) atomicAdd(t.missing, wanted - got);
+  over_rows([&](int e) { return s_rank[e]; },
+            [&](int mine, bool need, int row, int j) { if (need) t.row(row)[j] = mine < got ? a.free[mine] : -1; }, [](int, int) {});
+}
+__global__ __launch_bounds__(kScan) void reserve_place_kernel(const ReserveArgs a) { reserve_place<false>(a); }
+__global__ __launch_bounds__(kScan) void reserve_small_kernel(const ReserveArgs a) { reserve_place<true>(a); }
 
 // ------------------------------------------------------------------ host side
 
@@ -570,8 +642,21 @@ int mimir_prefixlm_pages_reserve(const MimirPagesParams* p, const int32_t* new_l
   a.got = w;
   a.lack = w + 16;
   a.free = a.lack + p->rows;
+  const int64_t entries = (int64_t)p->rows * p->width;
+  // One launch for small tables: 64 rows of 126 places, a page asked for here and there, in a graph 6.3 -> 5.7
+  // us, eagerly (the host's time) 19.6 -> 14.3; 256 rows of 126 in a graph 12.7.
+  if (p->rows <= 64 && entries <= 8192) {
+    hipLaunchKernelGGL(reserve_small_kernel, dim3(1), dim3(kScan), 0, s, a);
+    return launched("reserve launch");
+  }
   const unsigned grid = (unsigned)((p->rows + 3) / 4);
   hipLaunchKernelGGL(reserve_count_kernel, dim3(grid), dim3(256), 0, s, a);
+  // Two for up to 256 rows: 256 of 126 places, a page here and there, 6.3 -> 5.7 us in a graph, 40 rows admitted
+  // 19.6 -> 17.2 eagerly, all of them (16000 pages) 28.0 -> 35.0; 500 of 700 rows (11000 pages) 23.9 -> 33.2.
+  if (p->rows <= 256 && entries <= 1 << 30) {
+    hipLaunchKernelGGL(reserve_place_kernel, dim3(1), dim3(kScan), 0, s, a);
+    return launched("reserve launch");
+  }
   hipLaunchKernelGGL(reserve_take_kernel, dim3(1), dim3(kScan), 0, s, a);
   hipLaunchKernelGGL(reserve_assign_kernel, dim3(grid), dim3(256), 0, s, a);
   return launched("reserve launch");

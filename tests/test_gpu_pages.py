@@ -348,3 +348,19 @@ def test_numbers_past_32_bits_name_no_row(device):
     for bad in (torch.ones(4, dtype=torch.bool, device=device), torch.ones(4, device=device)):
         with pytest.raises(ValueError, match="whole numbers"):
             release_rows(table, bad)
+
+
+@pytest.mark.parametrize("rows,width,pages", [(257, 40, 12000), (256, 120, 30000), (1025, 5, 4000), (65, 9, 700),
+                                              (64, 128, 9000), (64, 129, 9000), (1, 700, 900), (60, 65, 70000)])
+def test_reserve_in_one_launch_two_and_three(device, rows, width, pages):
+    """On both sides of 64 and 256 rows and of 8192 table entries, from few asking rows to all, and out of pages."""
+    for seed in range(3):
+        table = _random_table(device, rows, width, pages, seed)
+        want = O.Table(*table)
+        rng = random.Random(seed)
+        for ask in (0.1, 1.0):
+            new = [rng.choice([1, 64, rng.randint(0, 64 * width)]) if rng.random() < ask else 0 for _ in range(rows)]
+            reserve_pages(table, torch.tensor(new, dtype=torch.int32, device=device))
+            want.reserve(new)
+            _same_table(table, want, (seed, ask))
+        assert _counted(table)
