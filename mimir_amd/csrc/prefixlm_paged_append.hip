@@ -7,8 +7,9 @@
 // but the bits that fall below 2^(e - 9): an 8-bit float keeps its three fraction bits, so a finer
 // scale would not make the others more exact either.
 //
-// Bound by reading the new rows (bf16) and writing their codes; the page's older codes are
-// touched only where the exponent grew.  Values are turned to [D][token] through LDS.
+// Reads the new rows (bf16) and writes their codes; the page's older codes are touched only where the
+// exponent grew.  8 x 512 tokens, 4 heads of 128 (13 MB): 7 us, where a copy's rate gives 2.5: bound by its
+// chain of round trips (arguments, lengths, page id and rows, exponent, codes).  Values are turned to [D][token] through LDS.
 #include "prefixlm_paged.h"
 
 namespace mimir {
