@@ -735,9 +735,9 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
 // A padded batch (new_lengths), whose row tiles with queries only the device knows: those alone are cut, each
 // into n runs of about as many pages, so that the runs of all are a.slots and one more for each row tile at
 // most.  Runs first, then the row tiles without queries.  64 batch rows, one per lane.  Against splits of the
-// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 82.7 us; 3 x up to 200 on 1000 to
+// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 82 us; 3 x up to 200 on 1000 to
 // 3000, 32 / 8, 42.0 -> 32.6; 8 x up to 700 on up to 2000, 8 / 8 heads of 64, 51.8 -> 43.0; 5 x up to 1339 on up to
-// 1000 49.4 -> 49.2 (more, shorter runs, and 9 us of merge).
+// 1000 49.4 -> 48.1 (42 -> 33 and 7.6 of merge).
 constexpr int kDealtRows = 64;
 struct Runs {
   PagedRow at;      // of the lane's batch row
@@ -747,15 +747,16 @@ struct Runs {
     at.row = -1, at.n = at.m = at.kv = 0;
     if (lane < a.B) at = PagedRow(a, lane);
     const int tiles = (at.kv + kPage - 1) / kPage;
-    act = at.kv > 0 ? (at.m * a.G + kRows - 1) / kRows : 0;
+    act = at.kv > 0 ? (int)((unsigned)(at.m * a.G + kRows - 1) / kRows) : 0;
     const int pages = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv * tiles), 63);
-    const int most = max(kTogether, (pages + a.slots - 1) / a.slots);
-    n = max(1, (tiles + most - 1) / most);
-    n = (tiles + per(tiles, n) - 1) / per(tiles, n);
+    const int most = max(kTogether, (int)((unsigned)(pages + a.slots - 1) / (unsigned)a.slots));
+    n = max(1, (int)((unsigned)(tiles + most - 1) / (unsigned)most));
+    const int runs = per(tiles, n);
+    n = max(1, (int)((unsigned)(tiles + runs - 1) / (unsigned)runs));
     incl = wave_inclusive_sum(act * a.Hkv * n);
     idle = wave_inclusive_sum(lane < a.B ? (a.n_rt - act) * a.Hkv : 0);
   }
-  static __device__ __forceinline__ int per(int tiles, int n) { return max(1, (tiles + n - 1) / n); }
+  static __device__ __forceinline__ int per(int tiles, int n) { return max(1, (int)((unsigned)(tiles + n - 1) / (unsigned)n)); }
   __device__ __forceinline__ PagedRow row(int b) const {
     PagedRow r;
     r.row = __builtin_amdgcn_readlane(at.row, b);
@@ -1161,16 +1162,28 @@ __device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
   const int R = a.S * a.G, groups = (R + kRowsAt - 1) / kRowsAt;
   const int pair = blockIdx.x / groups, row0 = (blockIdx.x - pair * groups) * kRowsAt, row = row0 + (int)threadIdx.x / kLanes;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv, col = threadIdx.x % kLanes * 4;
-  const Parts parts(a, b, hk, row0 / kRows);  // a workgroup's rows lie in one row tile
-  const int n = parts.n;
+  // A workgroup's rows lie in one row tile.  One wave looks it up: all four, each over 64 batch rows, made the
+  // launch VALU bound (5 x up to 1339 tokens, 8 heads of 64: 9.0 us).
+  __shared__ int s_n, s_m;
+  __shared__ int64_t s_first;
+  if (threadIdx.x < 64) {
+    const Parts parts(a, b, hk, row0 / kRows);
+    if (threadIdx.x == 0) {
+      s_n = parts.n;
+      s_m = parts.r.m;
+      s_first = parts.first;
+    }
+  }
+  __syncthreads();
+  const int n = s_n;
   if (n <= 1 || row >= R) return;  // written by its split
   const int i = row / a.G;
   bf16_t* const out = a.out + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)(hk * a.G + row - i * a.G) * a.o_sh + col;
-  if (i >= parts.r.m) {  // a padding query
+  if (i >= s_m) {  // a padding query
     *(bf16x4*)out = bf16x4{};
     return;
   }
-  const int64_t part = parts.first * kRows + row % kRows;  // + kRows each
+  const int64_t part = s_first * kRows + row % kRows;  // + kRows each
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float M = -INFINITY, lsum = 0.f;
   for (int c0 = 0; c0 < n; c0 += kChunk) {
