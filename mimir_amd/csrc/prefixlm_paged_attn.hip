@@ -735,9 +735,9 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
 // A padded batch (new_lengths), whose row tiles with queries only the device knows: those alone are cut, each
 // into n runs of about as many pages, so that the runs of all are a.slots and one more for each row tile at
 // most.  Runs first, then the row tiles without queries.  64 batch rows, one per lane.  Against splits of the
-// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 82 us; 3 x up to 200 on 1000 to
-// 3000, 32 / 8, 42.0 -> 32.6; 8 x up to 700 on up to 2000, 8 / 8 heads of 64, 51.8 -> 43.0; 5 x up to 1339 on up to
-// 1000 49.4 -> 48.1 (42 -> 33 and 7.6 of merge).
+// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 81 us; 3 x up to 200 on 1000 to
+// 3000, 32 / 8, 42.0 -> 32.6; 8 x up to 700 on up to 2000, 8 / 8 heads of 64, 51.8 -> 41.2; 5 x up to 1339 on up to
+// 1000 49.4 -> 46 (42 -> 31 and 7.8 of merge).
 constexpr int kDealtRows = 64;
 struct Runs {
   PagedRow at;      // of the lane's batch row
@@ -749,8 +749,16 @@ struct Runs {
     const int tiles = (at.kv + kPage - 1) / kPage;
     act = at.kv > 0 ? (int)((unsigned)(at.m * a.G + kRows - 1) / kRows) : 0;
     const int pages = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv * tiles), 63);
-    const int most = max(kTogether, (int)((unsigned)(pages + a.slots - 1) / (unsigned)a.slots));
-    n = max(1, (int)((unsigned)(tiles + most - 1) / (unsigned)most));
+    // At head_dim 64 all runs are to be on the chip at once, three per CU: a few more would be a second round (8 x up to
+    // 700 tokens on up to 2000 keys 43.3 -> 41.2 us).  At 128 one per CU and the remainders (all at once, two per CU:
+    // 8 x up to 512 on up to 3000 80 -> 77.5, 4 x up to 100 on up to 3000 31.8 -> 35.6).
+    const int all = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv), 63);
+    int most = max(kTogether, (int)((unsigned)(pages + a.slots - 1) / (unsigned)a.slots));
+    for (int tries = a.D == 64 && all <= a.slots ? 12 : 0;; --tries) {
+      n = max(1, (int)((unsigned)(tiles + most - 1) / (unsigned)most));
+      if (tries == 0 || __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv * n), 63) <= a.slots) break;
+      most += max(1, most / 16);
+    }
     const int runs = per(tiles, n);
     n = max(1, (int)((unsigned)(tiles + runs - 1) / (unsigned)runs));
     incl = wave_inclusive_sum(act * a.Hkv * n);
@@ -1260,8 +1268,7 @@ Plan plan_of(const MimirPagedAttnParams& p) {
   s.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + groups * 3 / 4) / groups, p.table_width, kMaxSplits}));
   s.units = groups * s.splits;
   if (p.new_lengths != nullptr && p.batch <= kDealtRows && groups <= 4 * cus && p.table_width <= 1 << 20) {
-    // (one more per CU: the first three of those 90.7, 35.1 and 40.4 us)
-    s.slots = (int)((p.head_dim == 64 ? 2 : 1) * cus);
+    s.slots = (int)((p.head_dim == 64 ? 3 : 1) * cus);
     s.units = groups + s.slots;  // runs: pages / per <= slots, and one more for each row tile
   }
   s.workspace_bytes = s.splits > 1 || s.slots > 0 ? (size_t)s.units * kRows * ((size_t)p.head_dim + 2) * sizeof(float) : 0;
