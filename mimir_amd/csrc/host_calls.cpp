@@ -535,6 +535,9 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
           for (int64_t i = 0; t != nullptr && i < t->dim(); ++i) NEED(t->size(i) <= 1 || t->stride(i) > 0);
         qo = q;
         if (k != nullptr) ko = *k;
+        // what autograd has saved of them is no longer what it was
+        for (const at::Tensor* t : {&q, k})
+          if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
       } else {
         qo = at::empty(q.sizes(), q.options());
         if (k != nullptr) ko = at::empty(k->sizes(), k->options());

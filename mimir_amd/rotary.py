@@ -136,6 +136,8 @@ def _turn(query, key, positions, frequencies, inverse: bool, inplace: bool = Fal
         for name, t in (("query", query), ("key", key)):
             if t is not None and (t.stride(-1) != 1 or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride()))):
                 raise ValueError(f"an in-place {name} needs a unit head_dim stride and memory of its own for every row")
+            if t is not None and not t.is_inference():  # what autograd has saved of it is no longer what it was
+                torch.autograd.graph.increment_version(t)
         q, k, qo, ko = query, key, query, key
     else:
         q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (query, key))

@@ -217,3 +217,16 @@ def test_captured_forward_and_backward(device):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b), i
+
+
+def test_in_place_is_seen_by_autograd(device):
+    pos, table = torch.arange(5, device=device), RotaryFrequencies.create(64, device=device)
+    for at in (pos, pos[3:4]):  # one position for all tokens: the general path
+        x = torch.randn(5, 2, 64, device=device, requires_grad=True) * 1
+        y = (x * x).sum()
+        want, _ = rotary(x.detach().clone(), None, at, table)
+        with torch.no_grad():
+            rotary(x, None, at, table, inplace=True)
+        assert torch.equal(x.detach(), want)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()

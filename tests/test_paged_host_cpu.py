@@ -160,3 +160,17 @@ def test_one_tensor_in_place_as_query_and_key(bound):
     assert host.rotary(x, x[:, :1], pos, turns, 1.0, False, False, True, 0) is None
     assert host.rotary(x[:, :1], x[:, 1:], pos, turns, 1.0, False, False, True, 0) is not None  # a fused projection's heads
     assert host.rotary(x, x, pos, turns, 1.0, False, False, False, 0) is not None
+
+
+def test_in_place_is_seen_by_autograd(bound):
+    host, _ = bound
+    pos, turns = torch.arange(5), torch.zeros(4, dtype=torch.int64)
+    x = torch.ones(5, 2, 8, requires_grad=True) * 1
+    y = (x * x).sum()
+    with torch.no_grad():
+        assert host.rotary(x, None, pos, turns, 1.0, False, False, True, 0) is not None
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        z = torch.ones(5, 2, 8)
+        assert host.rotary(z, z.clone(), pos, turns, 1.0, False, False, True, 0) is not None
