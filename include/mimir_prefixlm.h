@@ -544,8 +544,10 @@ int mimir_prefixlm_pages_copy(const MimirPagesParams* params, const int32_t* sou
 
 /* Row destination[i] goes on from what row source[i] held before the call: it gives back its
  * own pages, shares the full pages of the source and gets a copy of the source's last,
- * partly filled page in a free one.  A source that is itself replaced by another row leaves
- * that page to the first row (lowest i) that goes on from it, if no other row holds it.
+ * partly filled page in a free one.  Such a page that every row holding it gives back in the call
+ * (its sources are themselves replaced) goes uncopied to the first row (lowest i) that goes on
+ * from it, unless a row now holds it as a full one.  So a page that is copied is held after the
+ * call, and never one of those handed out.
  * Entries with source = destination leave the row alone, entries outside the table are
  * skipped, and of entries with one destination the last counts.  Where the pool has no
  * free page the last page stays -1 and `missing` counts it. */

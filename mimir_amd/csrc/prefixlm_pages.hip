@@ -188,16 +188,20 @@ struct ForkArgs {
   int32_t *last, *first;  // [rows]: the last entry for a destination, the first kept one of a source
   int32_t *kept, *new_len, *tail, *rowbuf;  // [n], rowbuf [n][width]
   int32_t *from, *to, *free;  // [n]
+  int32_t* given_up;          // [1]: whether a last page that several rows hold may have been given up by all
 };
 
 // What each entry takes: kept, its length, and its last page (>= 0: an heir's; < -1: a copy of
-// page -2 - tail; -1: none).  One workgroup.
+// page -2 - tail; -1: none).  One workgroup.  The only holder's heir is known here, and then the page
+// is held; one that several entries of the table name is looked at again once all have given theirs
+// back (fork_heirs): a page that is copied from must not be handed out as another's destination.
 __device__ __forceinline__ void fork_plan(const ForkArgs& a) {
   const Table& t = a.t;
   for (int r = threadIdx.x; r < t.rows; r += kScan) {
     a.last[r] = -1;
     a.first[r] = 0x7fffffff;
   }
+  if (threadIdx.x == 0) *a.given_up = 0;
   __threadfence_block();
   __syncthreads();
   for (int i = threadIdx.x; i < a.n; i += kScan)
@@ -218,8 +222,10 @@ __device__ __forceinline__ void fork_plan(const ForkArgs& a) {
     if (len % kPageTokens != 0 && full < t.width && t.page_ok(t.row(s)[full])) {
       const int p = t.row(s)[full];
       const int by = load_count(&a.last[s]);  // the entry that replaces the source
-      const bool heir = by >= 0 && a.src[by] != s && load_count(&a.first[s]) == i && load_count(&t.counts[p]) == 1;
+      const bool replaced = by >= 0 && a.src[by] != s, alone = load_count(&t.counts[p]) == 1;
+      const bool heir = replaced && alone && load_count(&a.first[s]) == i;
       tail = heir ? p : -2 - p;
+      if (replaced && !alone) *a.given_up = 1;  // every writer's value
     }
     a.tail[i] = tail;
     a.new_len[i] = t.lengths[s];
@@ -245,10 +251,33 @@ __device__ __forceinline__ void fork_gather(const ForkArgs& a, int i, int thread
   }
 }
 
+// Of last pages that no row holds any more, the first entry that would copy one takes it as it is: the lowest
+// entry i leaves i - n in the page's count.  One workgroup.
+__device__ __forceinline__ void fork_heirs(const ForkArgs& a) {
+  const Table& t = a.t;
+  auto unheld = [&](int i) { return a.kept[i] && a.tail[i] < -1 && load_count(&t.counts[-2 - a.tail[i]]) <= 0; };
+  for (int i = threadIdx.x; i < a.n; i += kScan)
+    if (unheld(i)) atomicMin(&t.counts[-2 - a.tail[i]], i - a.n);
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kScan)
+    if (unheld(i) && load_count(&t.counts[-2 - a.tail[i]]) == i - a.n) {
+      const int p = -2 - a.tail[i];
+      atomicExch(&t.counts[p], 1);
+      a.rowbuf[(int64_t)i * t.width + max(a.new_len[i], 0) / kPageTokens] = p;
+      a.tail[i] = p;
+    }
+  __threadfence();  // counts are read through the L1 from here on
+  __syncthreads();
+}
+
 // Free pages for the last pages that are copied.  One workgroup.
 __device__ __forceinline__ void fork_take(const ForkArgs& a, int* shared) {
   const Table& t = a.t;
-  const unsigned first = first_free(t);
+  unsigned first = first_free(t);
+  if (__builtin_expect(*a.given_up != 0, 0)) {  // uniform
+    fork_heirs(a);
+    first = first_free(t);
+  }
   int wanted = 0;
   for (int i0 = 0; i0 < a.n; i0 += kScan) {  // the rank of each request, in a.from for now
     const int i = i0 + threadIdx.x;
@@ -580,6 +609,7 @@ int mimir_prefixlm_pages_fork(const MimirPagesParams* p, const int32_t* source, 
   f.kept = take(n); f.new_len = take(n); f.tail = take(n);
   f.from = take(n); f.to = take(n); f.free = take(n);
   f.rowbuf = take((int64_t)n * p->width);
+  f.given_up = take(1);
   // (All three in one workgroup took 26 us for 256 rows of up to 48 pages, a wave's rows one after another.)
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kScan), 0, s, f);
   hipLaunchKernelGGL(fork_gather_kernel, dim3((unsigned)n), dim3(256), 0, s, f);

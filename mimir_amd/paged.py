@@ -172,8 +172,9 @@ def fork_rows(cache: PagedCache, table: PageTable, source: Tensor, destination: 
     samples, a shared prompt): it gives back its own pages, shares the source's full ones and gets a
     copy of the last, partly filled one, which it can then append to.
 
-    All entries at once, so a permutation of beams is one call.  A row that is itself replaced
-    leaves its last page to the first row that goes on from it, uncopied.  Entries with equal source
+    All entries at once, so a permutation of beams is one call.  A last page that all rows holding
+    it give back in the call (they are replaced themselves) is left to the first row that goes on from
+    it, uncopied.  Entries with equal source
     and destination leave the row as it is, entries outside the table are skipped, of several
     for one destination the last counts.  Pages reserved past the source's tokens are not
     forked.  Where no page is free the destination's last page stays -1 and ``table.missing``

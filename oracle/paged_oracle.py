@@ -190,19 +190,12 @@ class Table:
         last = {d: s for s, d in zip(src, dst) if 0 <= s < n and 0 <= d < n}
         at = {d: i for i, (s, d) in enumerate(zip(src, dst)) if 0 <= s < n and 0 <= d < n}
         kept = sorted((at[d], s, d) for d, s in last.items() if s != d)
-        replaced = {d for _, _, d in kept}
-        before, lengths, counts = [list(p) for p in self.pages], list(self.lengths), list(self.counts)
-        heirs, plan = set(), []
+        before, lengths, plan = [list(p) for p in self.pages], list(self.lengths), []
         for _, s, d in kept:
             full, tail = max(lengths[s], 0) // PAGE, -1
             if lengths[s] > 0 and lengths[s] % PAGE and full < len(before[s]):
                 tail = before[s][full]
-            heir = self.ok(tail) and s in replaced and s not in heirs and counts[tail] == 1
-            heirs.add(s)
-            row = [p if i < full and self.ok(p) else -1 for i, p in enumerate(before[s])]
-            if heir:
-                row[full] = tail
-            plan.append((d, row, lengths[s], full, -1 if heir or not self.ok(tail) else tail))
+            plan.append((d, [p if i < full and self.ok(p) else -1 for i, p in enumerate(before[s])], lengths[s], full, tail))
         for d, row, *_ in plan:
             for p in before[d]:
                 if self.ok(p):
@@ -210,13 +203,19 @@ class Table:
             for p in row:
                 if p >= 0:
                     self.counts[p] += 1
-        moves = []
+        copies = []
         for d, row, length, full, tail in plan:
-            if tail >= 0:
-                row[full] = self.free()
-                if row[full] >= 0:
-                    moves.append((tail, row[full]))
+            if self.ok(tail) and self.counts[tail] == 0:  # given back by all: the first to go on from it
+                row[full], self.counts[tail] = tail, 1
+            elif self.ok(tail):
+                copies.append((tail, row, full))
             self.pages[d], self.lengths[d] = row, length
+        moves = []
+        for tail, row, full in copies:
+            row[full] = self.free()
+            if row[full] >= 0:
+                moves.append((tail, row[full]))
+        assert not {a for a, _ in moves} & {b for _, b in moves}, moves
         return moves
 
     def compact(self):

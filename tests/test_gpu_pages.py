@@ -364,3 +364,42 @@ def test_reserve_in_one_launch_two_and_three(device, rows, width, pages):
             want.reserve(new)
             _same_table(table, want, (seed, ask))
         assert _counted(table)
+
+
+def _forked(device, rows, width, pages, layers, seed, table, lens, counts, src, dst):
+    cache = _random_cache(device, pages, layers, 1, 64, seed)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    table = PageTable(t(table), t(lens), t(counts), t([0]))
+    pool, want = O.Cache(*cache), O.Table(*table)
+    fork_rows(cache, table, t(src), t(dst))
+    pool.move(want.fork(src, dst))
+    _same_table(table, want, (seed, rows))
+    _same_cache(cache, pool, (seed, rows))
+    assert _counted(table)
+
+
+@pytest.mark.parametrize("rows,width,pages", [(2, 1, 3), (7, 3, 20), (40, 6, 150), (1300, 2, 2400)])
+def test_fork_of_shared_last_pages(device, rows, width, pages):
+    """Lengths set back into pages that several rows share: one that all give back goes to the first that goes on from
+    it, and no page that is copied is handed out.  More entries than a workgroup has threads, pools nearly full."""
+    from test_paged_cpu import _entries, _set_back
+
+    for seed in range(6):
+        for layers in (1, 5):
+            _forked(device, rows, width, pages, layers, seed, *_set_back(rows, width, pages, seed), *_entries(rows, seed))
+
+
+def test_fork_after_lengths_set_back(device):
+    """By the package's own calls: a fork, lengths set back into its shared page, and every holder replaced."""
+    cache, table = _random_cache(device, 8, 3, 2, 64, 1), PageTable.create(4, 2, 8, device=device)
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    reserve_pages(table, t(128, 0, 0, 100))
+    table.lengths.copy_(t(128, 0, 0, 100))
+    fork_rows(cache, table, t(0), t(1))
+    table.lengths.copy_(t(100, 100, 0, 100))
+    pool, want = O.Cache(*cache), O.Table(*table)
+    fork_rows(cache, table, t(3, 0, 3), t(0, 2, 1))
+    pool.move(want.fork([3, 0, 3], [0, 2, 1]))
+    _same_table(table, want)
+    _same_cache(cache, pool)
+    assert _counted(table) and int(table.missing[0]) == 0

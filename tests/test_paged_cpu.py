@@ -190,3 +190,78 @@ def test_lists_of_rows():
     for bad in (torch.tensor([True, False]), torch.tensor([1.0]), torch.tensor([1j]), torch.tensor(1), torch.tensor([[1]])):
         with pytest.raises(ValueError, match="whole numbers"):
             _row_list("rows", bad, "cpu")
+
+
+def _set_back(rows, width, pages, seed):
+    """A table of rows whose partly filled last pages several rows share, as after a fork and lengths set back."""
+    import random
+    rng = random.Random(seed)
+    free = list(range(pages))
+    rng.shuffle(free)
+    table, lens, counts = [], [], [0] * pages
+    for r in range(rows):
+        if r and rng.random() < 0.7:  # another's pages, all or the first ones, and within their last one
+            o = rng.randrange(r)
+            held = [p for p in table[o] if p >= 0]
+            row = held[:rng.randint(0, len(held))]
+        else:
+            row = [free.pop() for _ in range(min(rng.randint(0, width), len(free)))]
+        n = rng.randint(max(0, 64 * len(row) - 63), 64 * len(row))
+        if rng.random() < 0.2:
+            n = rng.randint(0, n)
+        for p in row:
+            counts[p] += 1
+        table.append(row + [-1] * (width - len(row)))
+        lens.append(n)
+    return table, lens, counts
+
+
+def _entries(rows, seed):
+    """All rows replaced in some order, or a few, some by each other, with repeats and numbers outside."""
+    import random
+    rng = random.Random(seed)
+    dst = list(range(rows))
+    rng.shuffle(dst)
+    if seed % 3 == 0:
+        return [rng.randrange(rows) for _ in dst], dst
+    if seed % 3 == 1:
+        return sorted(dst), dst
+    n = rng.randint(1, 2 * rows)
+    return [rng.randint(-1, rows) for _ in range(n)], [rng.randint(-1, rows) for _ in range(n)]
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_no_page_of_a_fork_is_read_and_written(seed):
+    """A page that a fork copies is held after the call, so it is none of those handed out, and every row's tokens
+    are the source's."""
+    rows, width, pages = 7, 3, 18 + seed % 7
+    t = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    table, lens, counts = _set_back(rows, width, pages, seed)
+    want = O.Table(t(table), t(lens), t(counts), t([0]))
+    src, dst = _entries(rows, seed)
+    moves = want.fork(src, dst)
+    assert not {a for a, _ in moves} & {b for _, b in moves}
+    assert all(want.counts[a] > 0 and want.counts[b] == 1 for a, b in moves)
+    named = [p for row in want.pages for p in row if p >= 0]
+    assert want.counts == [named.count(p) for p in range(pages)]
+    origin = dict((b, a) for a, b in moves)
+    last = {d: s for s, d in zip(src, dst) if 0 <= s < rows and 0 <= d < rows}
+    lost = 0
+    for d, s in last.items():
+        for i in range(-(-lens[s] // 64)):
+            p = want.pages[d][i]
+            lost += p < 0
+            assert p < 0 or origin.get(p, p) == table[s][i], (d, s, i)
+    assert lost == want.missing  # (no row here lacks a page that its tokens need)
+
+
+def test_a_last_page_given_up_by_all_goes_to_the_first():
+    t = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    # rows 0 and 2 hold page 0, 40 tokens of it; every row that held it goes on from another
+    want = O.Table(t([[0], [3], [0], [-1]]), t([40, 10, 40, 0]), t([2, 0, 0, 1]), t([0]))
+    # row 0 goes on in page 3, which row 1 alone held; row 2 in page 0; rows 3 and 1 in copies of it
+    assert want.fork([1, 0, 2, 2], [0, 2, 3, 1]) == [(0, 1), (0, 2)]
+    assert want.pages == [[3], [2], [0], [1]] and want.counts == [1, 1, 1, 1] and want.missing == 0
+    # no page left: the first still has it
+    want = O.Table(t([[0], [0]]), t([40, 40]), t([2]), t([0]))
+    assert want.fork([1, 0], [0, 1]) == [] and want.pages == [[0], [-1]] and want.missing == 1 and want.counts == [1]
