@@ -411,7 +411,9 @@ int mimir_prefixlm_cache_attn(const MimirCacheAttnParams* params, void* stream);
  * in fp32 with one rounding; the other columns are copied.  Pair i is columns
  * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`.  inverse = 1 turns
  * the other way (t -> -t): the gradient's map.  head_dim and rotary_dim even; each
- * output may be its input (same pointer and strides).  Strides in elements. */
+ * output may be its input (same pointer and strides), else the outputs share no memory
+ * with an input, each other or themselves (in place: the columns that are turned);
+ * MIMIR_ERR_UNSUPPORTED_SHAPE if they do.  Strides in elements. */
 typedef struct MimirRotaryParams {
   const void* q;
   const void* k;              /* NULL if num_kv_heads is 0 */

@@ -27,6 +27,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/mimir_prefixlm.h"
+#include "strided_overlap.h"
 
 namespace {
 
@@ -432,6 +433,17 @@ bool rotary_served(const at::Tensor& q, const at::Tensor* k, const Rotary& r) {
   return pos.size(pos.dim() - 1) == S && (pos.dim() == 1 || (pos.dim() == 2 && n == 4 && pos.size(0) == q.size(0)));
 }
 
+// Whether elements that an in-place call turns would be turned twice.
+bool turned_twice(const at::Tensor& q, const at::Tensor* k, const Rotary& r) {
+  const int64_t n = q.dim(), es = (int64_t)q.element_size();
+  auto region = [&](const at::Tensor& t) {
+    return mimir::Region{t.const_data_ptr(), 2 * r.turns.size(0) * es, {n == 4 ? t.size(0) : 1, t.size(n - 3), t.size(n - 2)},
+                         {n == 4 ? t.stride(0) * es : 0, t.stride(n - 3) * es, t.stride(n - 2) * es}};
+  };
+  const mimir::Region a = region(q);
+  return overlaps_itself(a) || (k != nullptr && (overlaps_itself(region(*k)) || overlap_each_other(a, region(*k))));
+}
+
 int launch_rotary(const at::Tensor& q, const at::Tensor* k, const Rotary& r, const at::Tensor& qo, const at::Tensor* ko, void* s) {
   const int64_t n = q.dim();
   MimirRotaryParams p = {};
@@ -530,9 +542,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (k != nullptr) ko = out[1];
     } else {
       if (truth(a[7])) {
-        NEED(k == nullptr || k->const_data_ptr() != q.const_data_ptr());
-        for (const at::Tensor* t : {&q, k})
-          for (int64_t i = 0; t != nullptr && i < t->dim(); ++i) NEED(t->size(i) <= 1 || t->stride(i) > 0);
+        NEED(!turned_twice(q, k, r));
         qo = q;
         if (k != nullptr) ko = *k;
         // what autograd has saved of them is no longer what it was

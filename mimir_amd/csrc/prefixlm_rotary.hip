@@ -23,6 +23,7 @@
 #include <cmath>
 
 #include "prefixlm_common.h"
+#include "strided_overlap.h"
 
 namespace mimir {
 int fail_with(int code, const std::string& msg);
@@ -202,6 +203,24 @@ extern "C" int mimir_prefixlm_rotary(const MimirRotaryParams* p, void* stream) {
   a.turning = p->rotary_dim / (2 * v);
   // In place the columns past rotary_dim are there already.
   const bool in_place = a.q == a.qo && (!k || a.k == a.ko);
+  // Threads write what others read: an output is its own input, element by element, or shares nothing with
+  // one, with the other output or with itself.
+  const int64_t run = (int64_t)(in_place ? p->rotary_dim : p->head_dim) * es;
+  auto region = [&](const void* x, int64_t sb, int64_t st, int64_t sh, int heads) {
+    return mimir::Region{x, run, {p->batch, p->seqlen, heads}, {sb * es, st * es, sh * es}};
+  };
+  const mimir::Region q_in = region(a.q, a.q_sb, a.q_st, a.q_sh, a.Hq), k_in = region(a.k, a.k_sb, a.k_st, a.k_sh, a.H - a.Hq);
+  const mimir::Region q_out = region(a.qo, a.qo_sb, a.qo_st, a.qo_sh, a.Hq), k_out = region(a.ko, a.ko_sb, a.ko_st, a.ko_sh, a.H - a.Hq);
+  auto same = [](const mimir::Region& x, const mimir::Region& y) {
+    bool all = x.base == y.base;
+    for (int i = 0; i < mimir::Region::kDims; ++i) all = all && (x.size[i] == 1 || x.stride[i] == y.stride[i]);
+    return all;
+  };
+  auto apart = [&](const mimir::Region& out, const mimir::Region& own, const mimir::Region& others) {
+    return !overlaps_itself(out) && (same(out, own) || !overlap_each_other(out, own)) && !overlap_each_other(out, others);
+  };
+  if (!apart(q_out, q_in, k_in) || (k && (!apart(k_out, k_in, q_in) || overlap_each_other(q_out, k_out))))
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "rotary outputs need memory of their own: elements that overlap would be turned twice");
   a.items = in_place ? a.turning : p->head_dim / (2 * v);
   // Four heads a thread, all in flight at once, or fewer until there are threads for the whole chip (256 CUs
   // x 16 waves).  One thread for all heads while the tokens fill the chip / so: 16384 tokens, 20 heads of 128,

@@ -136,8 +136,6 @@ def _turn(query, key, positions, frequencies, inverse: bool, inplace: bool = Fal
         for name, t in (("query", query), ("key", key)):
             if t is not None and (t.stride(-1) != 1 or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride()))):
                 raise ValueError(f"an in-place {name} needs a unit head_dim stride and memory of its own for every row")
-            if t is not None and not t.is_inference():  # what autograd has saved of it is no longer what it was
-                torch.autograd.graph.increment_version(t)
         q, k, qo, ko = query, key, query, key
     else:
         q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (query, key))
@@ -157,6 +155,9 @@ def _turn(query, key, positions, frequencies, inverse: bool, inplace: bool = Fal
     lib = _capi.load()
     with torch.cuda.device(query.device):
         _capi.raise_for_status(lib, lib.mimir_prefixlm_rotary(ctypes.byref(p), P._stream(query.device)))
+    for t in (query, key) if inplace else ():
+        if t is not None and not t.is_inference():  # what autograd has saved of it is no longer what it was
+            torch.autograd.graph.increment_version(t)
     return qo, ko
 
 
@@ -182,7 +183,7 @@ def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
     ``positions`` ([tokens] or [batch, tokens], or what broadcasts to them) times ``frequencies``.
 
     Returns ``(query, key)``, new tensors, or the given ones written in place (``inplace``; not
-    for tensors that need a gradient).  The first ``2 * len(frequencies.turns)`` columns of a
+    for tensors that need a gradient, nor where an element to turn lies in both or twice in one).  The first ``2 * len(frequencies.turns)`` columns of a
     head are turned, the others passed on.  fp32 arithmetic, one rounding.  ``inverse`` turns
     the other way, which is also the gradient; any strides with a unit one on head_dim
     are read in place, so that the heads of a fused projection need no copy.

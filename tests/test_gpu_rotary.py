@@ -230,3 +230,22 @@ def test_in_place_is_seen_by_autograd(device):
         assert torch.equal(x.detach(), want)
         with pytest.raises(RuntimeError, match="inplace"):
             y.backward()
+
+
+def test_in_place_views_that_overlap(device):
+    base = torch.randn(6, 5, 64, device=device)
+    table, pos = RotaryFrequencies.create(64, device=device), torch.arange(6, device=device)
+    half = RotaryFrequencies.create(32, device=device)
+    for at, freq, views in ((pos, table, lambda x: (x[:, :3], x[:, 2:])), (pos[:5], table, lambda x: (x[:5], x[1:])),
+                            (pos[3:4], table, lambda x: (x[:, :3], x[:, 2:])),  # one position for all: the general path
+                            (pos, half, lambda x: (x[:, :2, :32], x[:, :2, 16:48])),
+                            (pos, table, lambda x: (torch.as_strided(x, (6, 2, 64), (128, 32, 1)), None))):
+        x = base.clone()
+        with pytest.raises(ValueError, match="memory of their own"):
+            rotary(*views(x), at, freq, inplace=True)
+        assert torch.equal(x, base) and x._version == 0
+    for at in (pos, pos[3:4]):  # heads in turn share no element
+        x = base.clone()
+        want, _ = rotary(x, None, at, table)
+        rotary(x[:, ::2], x[:, 1::2], at, table, inplace=True)
+        assert torch.equal(x, want)
