@@ -532,6 +532,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TENSOR(turns, a[3]);
     const Rotary r = {positions, turns, PyFloat_AsDouble(a[4]), truth(a[5]), truth(a[6])};
     NEED(PyErr_Occurred() == nullptr && rotary_served(q, k, r));
+    for (const at::Tensor* t : {&q, k}) NEED(t == nullptr || !t->_fw_grad(0).defined());  // forward mode: the general path
     at::Tensor qo, ko;
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || (k != nullptr && k->requires_grad()));
     if (grad) {

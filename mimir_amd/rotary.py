@@ -165,6 +165,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, positions, turns, amplitude, interleaved, inverse):
         ctx.save_for_backward(positions, turns)
+        ctx.save_for_forward(positions, turns)
         ctx.meta = (amplitude, interleaved, inverse, key is not None)
         return _turn(query, key, positions, RotaryFrequencies(turns, amplitude, interleaved), inverse)
 
@@ -176,6 +177,21 @@ class _Rotary(torch.autograd.Function):
         dquery, dkey = _Rotary.apply(dquery, dkey if has_key else None, positions, turns, amplitude, interleaved, not inverse)
         return dquery, dkey, None, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tquery, tkey, *_):
+        positions, turns = ctx.saved_tensors
+        amplitude, interleaved, inverse, _ = ctx.meta
+        # the turn is linear: a tangent turns like its tensor
+        turned = iter(())
+        given = [t for t in (tquery, tkey) if t is not None]
+        if given:
+            turned = iter(_Rotary.apply(given[0], given[1] if len(given) > 1 else None, positions, turns, amplitude, interleaved, inverse))
+        return tuple(None if t is None else next(turned) for t in (tquery, tkey))
+
+
+def _has_tangent(t: Optional[Tensor]) -> bool:
+    return t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
 
 def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies: RotaryFrequencies, *,
            inverse: bool = False, inplace: bool = False):
@@ -183,10 +199,11 @@ def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
     ``positions`` ([tokens] or [batch, tokens], or what broadcasts to them) times ``frequencies``.
 
     Returns ``(query, key)``, new tensors, or the given ones written in place (``inplace``; not
-    for tensors that need a gradient, nor where an element to turn lies in both or twice in one).  The first ``2 * len(frequencies.turns)`` columns of a
-    head are turned, the others passed on.  fp32 arithmetic, one rounding.  ``inverse`` turns
-    the other way, which is also the gradient; any strides with a unit one on head_dim
-    are read in place, so that the heads of a fused projection need no copy.
+    for tensors that need a gradient, nor where an element to turn lies in both or twice in one).
+    The first ``2 * len(frequencies.turns)`` columns of a head are turned, the others passed on.
+    fp32 arithmetic, one rounding.  ``inverse`` turns the other way, which is also the gradient; in
+    forward mode tangents are turned like their tensors.  Any strides with a unit one on head_dim are
+    read in place, so that the heads of a fused projection need no copy.
     """
     if query.is_cuda:
         res = _capi.host().rotary(query, key, positions, *frequencies, inverse, inplace, P._stream(query.device))
@@ -194,6 +211,7 @@ def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
             return res
     positions = _check(query, key, positions, frequencies)
     grad = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
+    grad = grad or _has_tangent(query) or _has_tangent(key)
     if inplace:
         if grad:
             raise ValueError("an in-place rotary has no gradient: leave inplace off")

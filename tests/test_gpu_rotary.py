@@ -249,3 +249,18 @@ def test_in_place_views_that_overlap(device):
         want, _ = rotary(x, None, at, table)
         rotary(x[:, ::2], x[:, 1::2], at, table, inplace=True)
         assert torch.equal(x, want)
+
+
+def test_forward_mode(device):
+    import torch.autograd.forward_ad as fwd
+
+    table, pos = RotaryFrequencies.create(48, interleaved=True, scaling="yarn", factor=4.0, device=device), torch.arange(9, device=device) * 50
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, tq, tk = (torch.randn(9, h, 64, device=device, dtype=dtype) for h in (4, 2, 4, 2))
+        want, value = rotary(tq, tk, pos, table), rotary(q, k, pos, table)
+        for needs in (False, True):  # beside a reverse gradient too
+            with fwd.dual_level():
+                out = rotary(*(fwd.make_dual(x.detach().clone().requires_grad_(needs), t) for x, t in ((q, tq), (k, tk))), pos, table)
+                for got, y, t in zip(out, value, want):
+                    primal, tangent = fwd.unpack_dual(got)
+                    assert torch.equal(primal, y) and torch.equal(tangent, t) and primal.requires_grad == needs

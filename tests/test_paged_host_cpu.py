@@ -174,3 +174,18 @@ def test_in_place_is_seen_by_autograd(bound):
     with torch.inference_mode():
         z = torch.ones(5, 2, 8)
         assert host.rotary(z, z.clone(), pos, turns, 1.0, False, False, True, 0) is not None
+
+
+def test_tangents_take_the_general_path(bound):
+    import torch.autograd.forward_ad as fwd
+
+    host, stub = bound
+    x, pos, turns = torch.ones(5, 2, 8), torch.arange(5), torch.zeros(4, dtype=torch.int64)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, x)
+        ctypes.c_int.in_dll(stub, "stub_calls").value = 0
+        for q, k in ((d, None), (d, x), (x, d), (d, d)):
+            for inplace in (False, True):
+                assert host.rotary(q, k, pos, turns, 1.0, False, False, inplace, 0) is None
+        assert ctypes.c_int.in_dll(stub, "stub_calls").value == 0
+        assert host.rotary(x, None, pos, turns, 1.0, False, False, False, 0) is not None

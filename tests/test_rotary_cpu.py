@@ -105,3 +105,51 @@ def test_c_abi_empty_calls():
     for kw in (dict(batch=0), dict(seqlen=0)):
         assert lib.mimir_prefixlm_rotary(ctypes.byref(_params(**kw)), None) == _capi.OK
     assert lib.mimir_prefixlm_rotary(None, None) == _capi.ERR_INVALID_ARGUMENT
+
+
+@pytest.fixture
+def turned_on_the_cpu(monkeypatch):
+    """``rotary`` with the general path's launch replaced by the formula (64-bit angles, interleaved layout or halves)."""
+    import mimir_amd.rotary as R
+
+    def turn(query, key, positions, frequencies, inverse, inplace=False):
+        angle = positions[..., None, None] * (frequencies.turns.double() * 2.0 ** -64 * 2 * math.pi) * (-1 if inverse else 1)
+        z = torch.polar(torch.full_like(angle, frequencies.amplitude), angle)
+        out = []
+        for x in (query, key):
+            if x is None:
+                out.append(None)
+                continue
+            y = torch.view_as_real(torch.complex(*(x.detach().double().unflatten(-1, (2, -1)).unbind(-2))) * z)
+            out.append(y.mT.flatten(-2).to(x.dtype))
+        return tuple(out)
+
+    monkeypatch.setattr(R, "_turn", turn)
+    monkeypatch.setattr(R.P, "_check_device_tensor", lambda name, t: None)
+
+
+def test_tangents_are_turned(turned_on_the_cpu):
+    import torch.autograd.forward_ad as fwd
+
+    table, pos = RotaryFrequencies.create(8, amplitude=1.5, device="cpu"), torch.arange(5) * 100
+    gen = torch.Generator().manual_seed(0)
+    q, k, tq, tk = (torch.randn(5, h, 8, generator=gen) for h in (3, 2, 3, 2))
+    want = rotary(tq, tk, pos, table)
+    with fwd.dual_level():
+        dual = lambda x, t: fwd.make_dual(x, t)  # noqa: E731
+        tangent = lambda x: fwd.unpack_dual(x).tangent  # noqa: E731
+        a, b = rotary(dual(q, tq), dual(k, tk), pos, table)
+        assert torch.equal(tangent(a), want[0]) and torch.equal(tangent(b), want[1])
+        assert torch.equal(fwd.unpack_dual(a).primal, rotary(q, k, pos, table)[0])
+        a, none = rotary(dual(q, tq), None, pos, table, inverse=True)
+        assert none is None and torch.equal(tangent(a), rotary(tq, None, pos, table, inverse=True)[0])
+        a, b = rotary(q, dual(k, tk), pos, table)  # one side alone
+        assert (tangent(a) is None or not tangent(a).any()) and torch.equal(tangent(b), want[1])
+        with torch.no_grad():
+            assert torch.equal(tangent(rotary(dual(q, tq), k, pos, table)[0]), want[0])
+        with pytest.raises(ValueError, match="gradient"):
+            rotary(dual(q, tq), None, pos, table, inplace=True)
+        w = tq.clone().requires_grad_(True)  # the tangent's own gradient is the turn back
+        a, _ = rotary(dual(q, w), None, pos, table)
+        g, = torch.autograd.grad(tangent(a), w, want[0])
+        assert torch.equal(g, rotary(want[0], None, pos, table, inverse=True)[0])
