@@ -19,6 +19,9 @@
 #include <Python.h>
 #include <dlfcn.h>
 
+#include <stdexcept>
+#include <string>
+
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
@@ -123,6 +126,19 @@ at::Tensor workspace(PyObject* torch_empty, size_t bytes, PyObject* like) {
   return out;
 }
 
+// Other Python threads run while a call launches.  (A backward's thread may not hold the lock.)
+struct Unlocked {
+  PyThreadState* const state = PyGILState_Check() ? PyEval_SaveThread() : nullptr;
+  ~Unlocked() {
+    if (state != nullptr) PyEval_RestoreThread(state);
+  }
+};
+
+// A HIP error inside an autograd function: kernels may have run.
+struct LaunchError : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
 // Whether the call was launched; after a HIP error `raised` and the Python error are set.
 template <typename P>
 bool launch(int (*entry)(const P*, void*), const P& p, void* s, bool& raised) {
@@ -171,6 +187,9 @@ PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F&& body) {
   bool raised = false;
   try {
     out = body(raised);
+  } catch (const LaunchError& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    raised = true;
   } catch (const std::exception&) {  // e.g. out of memory: the general path raises it
   }
   if (out != nullptr || raised) return out;
@@ -468,6 +487,7 @@ int launch_rotary(const at::Tensor& q, const at::Tensor* k, const Rotary& r, con
   p.dtype = q.scalar_type() == at::kBFloat16 ? MIMIR_DTYPE_BFLOAT16 : MIMIR_DTYPE_FLOAT32;
   p.index_int64 = r.positions.scalar_type() == at::kLong;
   const c10::DeviceGuard guard(q.device());
+  const Unlocked unlocked;
   return lib.rotary(&p, s);
 }
 
@@ -500,7 +520,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
     const at::Tensor qo = at::empty(q.sizes(), q.options());
     const at::Tensor ko = k.has_value() ? at::empty(k->sizes(), k->options()) : at::Tensor();
     const int status = launch_rotary(q, k.has_value() ? &*k : nullptr, r, qo, &ko, (void*)s);
-    TORCH_CHECK(status == MIMIR_OK, lib.last_error());
+    if (status == MIMIR_ERR_HIP) throw LaunchError(lib.last_error());
+    TORCH_CHECK(status == MIMIR_OK, lib.last_error());  // a refusal: nothing launched
     if (!k.has_value()) return {qo};
     return {qo, ko};
   }
@@ -709,15 +730,18 @@ PyObject* py_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* const s = stream(a[5]);
     NEED(PyErr_Occurred() == nullptr);
     int status = MIMIR_ERR_INVALID_ARGUMENT;
-    if (call == "fork" && lib.pages_fork != nullptr && list[0] != nullptr && list[1] != nullptr) {
-      status = lib.pages_fork(&p, list[0], list[1], (int32_t)items, s);
-    } else if (call == "compact" && lib.pages_compact != nullptr) {
-      used = empty({1}, *t[0], at::kInt);
-      status = lib.pages_compact(&p, used.mutable_data_ptr<int32_t>(), s);
-    } else if (call == "release" && lib.pages_release != nullptr && list[0] != nullptr) {
-      status = lib.pages_release(&p, list[0], (int32_t)items, s);
-    } else if (call == "reserve" && lib.pages_reserve != nullptr && list[0] != nullptr && items == rows) {
-      status = lib.pages_reserve(&p, list[0], s);
+    if (call == "compact") used = empty({1}, *t[0], at::kInt);
+    {
+      const Unlocked unlocked;
+      if (call == "fork" && lib.pages_fork != nullptr && list[0] != nullptr && list[1] != nullptr) {
+        status = lib.pages_fork(&p, list[0], list[1], (int32_t)items, s);
+      } else if (call == "compact" && lib.pages_compact != nullptr) {
+        status = lib.pages_compact(&p, used.mutable_data_ptr<int32_t>(), s);
+      } else if (call == "release" && lib.pages_release != nullptr && list[0] != nullptr) {
+        status = lib.pages_release(&p, list[0], (int32_t)items, s);
+      } else if (call == "reserve" && lib.pages_reserve != nullptr && list[0] != nullptr && items == rows) {
+        status = lib.pages_reserve(&p, list[0], s);
+      }
     }
     if (status == MIMIR_ERR_HIP) {
       PyErr_SetString(PyExc_RuntimeError, lib.last_error());

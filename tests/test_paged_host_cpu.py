@@ -189,3 +189,44 @@ def test_tangents_take_the_general_path(bound):
                 assert host.rotary(q, k, pos, turns, 1.0, False, False, inplace, 0) is None
         assert ctypes.c_int.in_dll(stub, "stub_calls").value == 0
         assert host.rotary(x, None, pos, turns, 1.0, False, False, False, 0) is not None
+
+
+def test_a_failed_launch_under_autograd_is_not_run_again(bound):
+    host, stub = bound
+    status, calls = (ctypes.c_int.in_dll(stub, x) for x in ("stub_status", "stub_calls"))
+    x, pos, turns = torch.ones(5, 2, 8, requires_grad=True), torch.arange(5), torch.zeros(4, dtype=torch.int64)
+    call = lambda: host.rotary(x, None, pos, turns, 1.0, False, False, False, 0)  # noqa: E731
+    out, _ = call()
+    try:
+        calls.value, status.value = 0, _capi.ERR_HIP
+        with pytest.raises(RuntimeError, match="stub launch failed"):
+            call()
+        assert calls.value == 1
+        with pytest.raises(RuntimeError, match="stub launch failed"):
+            out.sum().backward()
+        assert calls.value == 2
+        status.value = _capi.ERR_UNSUPPORTED_SHAPE  # nothing launched: the general path raises it
+        assert call() is None
+    finally:
+        status.value = _capi.OK
+
+
+def test_launches_release_the_interpreter(tmp_path):
+    source = (STUB + MORE).replace("static int launched() {", "int PyGILState_Check(void);\nint stub_locked = 0;\n"
+                                   "static int launched() { stub_locked += PyGILState_Check();")
+    subprocess.run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-x", "c++", "-", "-o", str(tmp_path / "stub.so")],
+                   input=source, text=True, check=True)
+    copy = shutil.copy(_capi.HOST_PATH, tmp_path / "_host_calls.so")
+    loader = importlib.machinery.ExtensionFileLoader("_host_calls", str(copy))
+    host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_calls", loader))
+    loader.exec_module(host)
+    host.bind(str(tmp_path / "stub.so"), "cpu")
+    host.streams(lambda device: 0)
+    stub = ctypes.CDLL(str(tmp_path / "stub.so"))
+    calls, locked = (ctypes.c_int.in_dll(stub, x) for x in ("stub_calls", "stub_locked"))
+    for name, call in _calls(host).items():
+        assert call() is not None and locked.value == 0, name
+    x = torch.ones(5, 2, 8, requires_grad=True)
+    y, _ = host.rotary(x, None, torch.arange(5), torch.zeros(4, dtype=torch.int64), 1.0, False, False, False, 0)
+    y.sum().backward()
+    assert locked.value == 0 and calls.value == 8
