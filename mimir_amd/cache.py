@@ -40,7 +40,7 @@ def _rows4(name: str, t: Tensor) -> Tensor:
         raise ValueError(f"{name} must be [batch, tokens, heads, head_dim], got shape {tuple(t.shape)}")
     P._check_device_tensor(name, t)
     if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(2) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
+        t = P._own_copy(t)
     return t
 
 

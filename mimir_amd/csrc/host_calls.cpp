@@ -635,7 +635,7 @@ PyObject* py_paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (const at::Tensor* t : {&k, &v}) NEED(t->size(0) == B && t->size(1) == S && t->size(2) == hkv && t->size(3) == d);
     for (const at::Tensor* t : {&q, &k, &v}) {
       NEED(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->stride(3) == 1 && (uintptr_t)t->const_data_ptr() % 16 == 0);
-      for (int i = 0; i < 3; ++i) NEED(t->stride(i) % 8 == 0);
+      for (int i = 0; i < 3; ++i) NEED(t->size(i) == 1 || t->stride(i) % 8 == 0);
     }
     Paged c;
     NEED(paged_cache(a[3], c) && c.heads == hkv && c.d == d && c.t[0]->device() == q.device());
@@ -655,7 +655,10 @@ PyObject* py_paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.index_int64 = lens.scalar_type() == at::kLong;
     const at::Tensor out = empty({B, S, hq, d}, q, at::kBFloat16);
     p.q = q.const_data_ptr(), p.k_new = k.const_data_ptr(), p.v_new = v.const_data_ptr(), p.out = out.mutable_data_ptr();
-    STRIDES4(q, q), STRIDES4(kn, k), STRIDES4(vn, v), STRIDES4(out, out);
+    // a dim of one entry has no stride to speak of
+    auto step = [](const at::Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); };
+#define STEPS(name, t) p.name##_stride_batch = step(t, 0), p.name##_stride_token = step(t, 1), p.name##_stride_head = step(t, 2)
+    STEPS(q, q), STEPS(kn, k), STEPS(vn, v), STEPS(out, out);
     p.cache_k = (char*)c.t[0]->mutable_data_ptr() + layer * hkv * MIMIR_PAGE_TOKENS * d;
     p.cache_v = (char*)c.t[1]->mutable_data_ptr() + layer * hkv * MIMIR_PAGE_TOKENS * d;
     p.k_exponents = (int8_t*)c.t[2]->mutable_data_ptr() + layer * hkv;

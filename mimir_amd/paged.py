@@ -232,10 +232,13 @@ def reserve_pages(table: PageTable, new_lengths: Tensor) -> None:
 
 # ---------------------------------------------------------------- attention
 
-def _rows4(name: str, t: Tensor) -> Tensor:
-    if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(2) % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-    return t
+def _strides(t: Tensor):
+    """Of batch, tokens and heads; a dim of one entry has none to speak of."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()))
+
+
+def _rows4(t: Tensor) -> Tensor:
+    return P._own_copy(t) if t.stride(-1) != 1 or any(s % 8 for s in _strides(t)) or t.data_ptr() % 16 else t
 
 
 def _validate(cache, table, lens, rows, new, S: int) -> None:
@@ -334,13 +337,13 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
                                                 ("new_lengths", new_lengths)))
     if P._validate_metadata and B > 0 and S > 0:
         _validate(cache, page_table, lens, rows, new, S)
-    q, k, v = _rows4("query", query), _rows4("key", key), _rows4("value", value)
+    q, k, v = _rows4(query), _rows4(key), _rows4(value)
     out = torch.empty((B, S, hq, d), dtype=q.dtype, device=device)
     ck, cv, ke, ve = (t[:, layer] for t in cache)
     p = _capi.PagedAttnParams(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ck.data_ptr(), cv.data_ptr(), ke.data_ptr(), ve.data_ptr(),
         page_table.data_ptr(), lens.data_ptr(), None if rows is None else rows.data_ptr(), None if new is None else new.data_ptr(),
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
+        *_strides(q), *_strides(k), *_strides(v), *out.stride()[:3],
         ck.stride(0), cv.stride(0), ke.stride(0), ve.stride(0), page_table.stride(0),
         B, S, pages, *page_table.shape, hq, hkv, d, int(bool(causal)), _capi.DTYPE_BFLOAT16, int(index_dtype == torch.int64),
         scale, None, 0)

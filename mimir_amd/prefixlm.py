@@ -148,6 +148,12 @@ def _check_device_tensor(name: str, t: Tensor) -> None:
         )
 
 
+def _own_copy(t: Tensor) -> Tensor:
+    """A contiguous copy in memory of its own, which starts on 16 bytes: ``contiguous()`` returns a tensor
+    that torch calls contiguous as it is, whatever its address and the strides of dims of one entry."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _kernel_layout(t: Tensor) -> Tensor:
     """Unit stride on head_dim, 16-byte aligned rows; copies otherwise."""
     vec = 16 // t.element_size()
@@ -158,7 +164,7 @@ def _kernel_layout(t: Tensor) -> Tensor:
         or t.data_ptr() % 16
         or t.stride(0) < t.shape[-1]
     ):
-        t = t.contiguous()
+        t = _own_copy(t)
     return t
 
 
@@ -226,8 +232,9 @@ def rope_rows(t: Tensor, T: int, d: int, device, name: str) -> Tensor:
     t = t.reshape(-1, t.shape[-1])
     if t.shape != (T, d):
         raise ValueError(f"{name} must hold one [head_dim] row per token: expected {(T, d)}, got {tuple(t.shape)}")
-    if t.device != device or t.dtype != torch.float32 or t.stride(-1) != 1 or t.stride(0) % 4 or t.data_ptr() % 16:
-        t = t.to(device=device, dtype=torch.float32).contiguous()
+    t = t.to(device=device, dtype=torch.float32)
+    if t.stride(-1) != 1 or t.stride(0) % 4 or t.data_ptr() % 16:
+        t = _own_copy(t)
     return t
 
 
