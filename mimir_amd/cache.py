@@ -81,8 +81,10 @@ def attention_with_cache(query: Tensor, key: Tensor, value: Tensor, cache: Cache
         raise ValueError("cache tensors need a unit head_dim stride")
     q, k, v = _rows4("query", query), _rows4("key", key), _rows4("value", value)
     device = q.device
-    # int32 and int64 indices are read as they are (no conversion launch)
-    index_dtype = cache_lengths.dtype if cache_lengths.dtype in (torch.int32, torch.int64) else torch.int64
+    # int32 and int64 indices are read as they are (no conversion launch); of both, as int64: a row number past
+    # 32 bits must not wrap to a row of the cache
+    narrow = cache_lengths.dtype == torch.int32 and (cache_batch_indices is None or cache_batch_indices.dtype != torch.int64)
+    index_dtype = torch.int32 if narrow else torch.int64
     lens = cache_lengths.to(device=device, dtype=index_dtype).contiguous()
     if lens.shape != (B,):
         raise ValueError(f"cache_lengths must be [{B}], got {tuple(lens.shape)}")

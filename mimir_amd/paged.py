@@ -324,7 +324,9 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
             (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError(f"page_table must be int32 [rows, max_pages] on {device}, laid out row by row, got {tuple(page_table.shape)} "
                          f"{page_table.dtype} on {page_table.device}")
-    index_dtype = cache_lengths.dtype if cache_lengths.dtype in (torch.int32, torch.int64) else torch.int64
+    # one type for all three, wide enough for each: a row number past 32 bits must not wrap to a row of the table
+    index_dtype = torch.int64 if any(t is not None and t.dtype == torch.int64
+                                     for t in (cache_lengths, cache_batch_indices, new_lengths)) else torch.int32
 
     def index(name, t):
         if t is None:

@@ -52,3 +52,19 @@ def test_operator(device, T, dtype):
             grads.append((out, *torch.autograd.grad(out.float().sum(), ops)))
         for a, b in zip(*grads):
             assert torch.equal(a, b)
+
+
+def test_row_numbers_past_32_bits_beside_narrow_lengths(device):
+    """They name no row: zeros, and nothing is written."""
+    q, k = torch.randn(2, 1, 4, 64, device=device).bfloat16(), torch.randn(2, 1, 2, 64, device=device).bfloat16()
+    lens = torch.tensor([3, 5], dtype=torch.int32, device=device)
+    far = torch.tensor([1 << 32, 1], device=device)
+    paged, table = PagedCache.create(4, 1, 2, 64, device=device), PageTable.create(2, 1, 4, device=device)
+    reserve_pages(table, lens + 1)
+    out = attention_with_pages(q, k, k, paged, 0, table.pages, lens, True, far)
+    assert not out[0].any() and out[1].any() and not paged.keys[0].view(torch.uint8).any() and paged.keys[1].view(torch.uint8).any()
+    new = torch.tensor([1, (1 << 32) + 1], device=device)  # more than the call's one token: that one
+    assert torch.equal(attention_with_pages(q, k, k, paged, 0, table.pages, lens, True, far, new_lengths=new), out)
+    bf16 = Cache.create(2, 16, 2, 64, dtype=torch.bfloat16, device=device)
+    out = attention_with_cache(q, k, k, bf16, lens, True, far)
+    assert not out[0].any() and out[1].any() and not bf16.keys[0].any()
