@@ -48,7 +48,8 @@ class RotaryFrequencies(NamedTuple):
         * ``"wavelength"``: by the turns t that a pair makes in ``original_positions``: divided by ``factor``
           below ``low_turns``, kept above ``high_turns``, between them mixed by (t - low) / (high - low);
         * ``"yarn"``: mixed by the pair's index, linearly from the (rounded down) one of ``fast_turns``,
-          kept, to the (rounded up) one of ``slow_turns``, divided; amplitude 0.1 ln(factor) + 1.
+          kept, to the (rounded up) one of ``slow_turns``, divided; amplitude 0.1 ln(factor) + 1, and
+          1 for a factor below 1.
         """
         n = int(rotary_dim)
         if n < 2 or n % 2:
@@ -81,7 +82,7 @@ class RotaryFrequencies(NamedTuple):
 
             low, high = max(math.floor(index(fast_turns)), 0), min(math.ceil(index(slow_turns)), n - 1)
             slow = [min(1.0, max(0.0, (i - low) / max(high - low, 0.001))) for i in range(n // 2)]
-            return [f / factor * s + f * (1.0 - s) for s, f in zip(slow, freq)], 0.1 * math.log(factor) + 1.0
+            return [f / factor * s + f * (1.0 - s) for s, f in zip(slow, freq)], 0.1 * math.log(max(factor, 1.0)) + 1.0
         return freq, 1.0
 
     @classmethod

@@ -153,3 +153,11 @@ def test_tangents_are_turned(turned_on_the_cpu):
         a, _ = rotary(dual(q, w), None, pos, table)
         g, = torch.autograd.grad(tangent(a), w, want[0])
         assert torch.equal(g, rotary(want[0], None, pos, table, inverse=True)[0])
+
+
+@pytest.mark.parametrize("factor,amplitude", [(0.25, 1.0), (0.999, 1.0), (1.0, 1.0), (math.e, 1.1), (40.0, 0.1 * math.log(40.0) + 1.0)])
+def test_yarn_amplitude(factor, amplitude):
+    """A range that is not stretched is not amplified, nor damped."""
+    freq, got = RotaryFrequencies.inverse_frequencies(64, scaling="yarn", factor=factor, original_positions=4096)
+    assert math.isclose(got, amplitude)
+    assert RotaryFrequencies.create(64, scaling="yarn", factor=factor, device="cpu").amplitude == got
