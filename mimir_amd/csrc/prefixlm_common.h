@@ -748,6 +748,8 @@ struct Prologue {
 PlanArgs plan_args(const int32_t* cu_seqlens, const int32_t* prefix_lens, int numseqs, int total_seqlen,
                    int is_causal, int total_tokens, int max_seqlen_all, int kind, int group, int cap, void* items);
 // Compute units of the current device (cached per device).
+// Workgroups of 256 threads that one launch takes along a dimension: HIP's work items there stay below 2^32.
+constexpr int64_t kMaxGroups = 0xffffffffll / 256;
 int device_cu_count();
 
 // A second stream of the current device with fork / join events (created once

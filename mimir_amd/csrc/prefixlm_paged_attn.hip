@@ -1423,9 +1423,10 @@ int mimir_prefixlm_paged_attn(const MimirPagedAttnParams* p, void* stream) {
                             p->ve_stride_page < p->num_kv_heads)))
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "pages of the cache must be 16-byte aligned and apart");
   const Plan plan = plan_of(*p);
-  const int64_t append = (int64_t)p->batch * p->num_kv_heads * ((p->seqlen + 2 * kPage - 2) / kPage);
-  const int64_t rows = (int64_t)p->seqlen * (p->num_q_heads / p->num_kv_heads);
-  if (rows > 0x7fffffff || plan.units > 0x7fffffff || append > 0x7fffffff || (int64_t)p->batch * p->num_kv_heads * ((rows + kWaves - 1) / kWaves) > 0x7fffffff)
+  const int64_t rows = (int64_t)p->seqlen * (p->num_q_heads / p->num_kv_heads), pairs = (int64_t)p->batch * p->num_kv_heads;
+  const int64_t append = plan.decode ? 0 : pairs * (((int64_t)p->seqlen + 2 * kPage - 2) / kPage);
+  const int64_t merge = plan.workspace_bytes > 0 ? pairs * ((rows + kWaves - 1) / kWaves) : 0;
+  if (rows > 0x7fffffff || plan.units > kMaxGroups || append > kMaxGroups || merge > kMaxGroups)
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many query rows for one call; split the batch");
   if (plan.workspace_bytes > 0 && (p->workspace == nullptr || p->workspace_bytes < plan.workspace_bytes || (uintptr_t)p->workspace % 16 != 0))
     return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned and hold at least " + std::to_string(plan.workspace_bytes) + " bytes");

@@ -594,6 +594,7 @@ int mimir_prefixlm_pages_fork(const MimirPagesParams* p, const int32_t* source, 
   int rc;
   if ((rc = check_table(p, true)) || (rc = check_pool(p))) return rc;
   if (n < 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "negative size");
+  if (n > kMaxGroups) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one call");
   if (n == 0 || p->rows == 0) return MIMIR_OK;
   if (source == nullptr || destination == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "row list is NULL");
   if ((rc = check_workspace(p, n))) return rc;
@@ -656,6 +657,7 @@ int mimir_prefixlm_pages_release(const MimirPagesParams* p, const int32_t* row_l
   int rc;
   if ((rc = check_table(p, true))) return rc;
   if (n < 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "negative size");
+  if (n > kMaxGroups) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one call");
   if (n == 0 || p->rows == 0) return MIMIR_OK;
   if (row_list == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "row list is NULL");
   hipLaunchKernelGGL(release_kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, table_of(*p), row_list);
@@ -666,6 +668,7 @@ int mimir_prefixlm_pages_reserve(const MimirPagesParams* p, const int32_t* new_l
   int rc;
   if ((rc = check_table(p, true))) return rc;
   if (p->rows == 0) return MIMIR_OK;
+  if (p->rows > 4 * kMaxGroups) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one call");
   if (new_lengths == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "new_lengths is NULL");
   if ((rc = check_workspace(p, 0))) return rc;
   const hipStream_t s = (hipStream_t)stream;

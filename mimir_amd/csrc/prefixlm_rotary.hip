@@ -230,7 +230,7 @@ extern "C" int mimir_prefixlm_rotary(const MimirRotaryParams* p, void* stream) {
   a.hp = (a.H + 3) / 4;
   while (a.hp < a.H && a.tokens * a.items * a.hp < (int64_t)256 * 16 * 64) a.hp *= 2;
   a.hp = std::min(a.hp, a.H);
-  if ((a.tokens * a.items * a.hp + 255) / 256 > 0x7fffffff) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many tokens for one launch");
+  if ((a.tokens * a.items * a.hp + 255) / 256 > mimir::kMaxGroups) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many tokens for one launch");
   const hipStream_t s = (hipStream_t)stream;
   const bool il = p->interleaved != 0;
   if (es == 2) {

@@ -265,3 +265,25 @@ def test_a_last_page_given_up_by_all_goes_to_the_first():
     # no page left: the first still has it
     want = O.Table(t([[0], [0]]), t([40, 40]), t([2]), t([0]))
     assert want.fork([1, 0], [0, 1]) == [] and want.pages == [[0], [-1]] and want.missing == 1 and want.counts == [1]
+
+
+@pytest.mark.parametrize("kw", [
+    dict(batch=1 << 22, num_kv_heads=4),                            # decode: a workgroup of 256 threads for each row and head
+    dict(batch=1 << 24, num_q_heads=1, num_kv_heads=1),
+    dict(batch=1 << 18, seqlen=2000, num_q_heads=4, num_kv_heads=4),   # prefill: its append, and its row tiles
+])
+def test_attention_refuses_launches_of_2_to_32_threads(kw):
+    lib, p = _capi.load(), _attn(**kw)
+    page = p.num_kv_heads * 64 * 64
+    p.k_stride_page, p.v_stride_page, p.ke_stride_page, p.ve_stride_page = page, page, p.num_kv_heads, p.num_kv_heads
+    with pytest.raises(ValueError, match="too many"):
+        _capi.raise_for_status(lib, lib.mimir_prefixlm_paged_attn(ctypes.byref(p), None))
+
+
+def test_page_calls_refuse_launches_of_2_to_32_threads():
+    lib, n = _capi.load(), 1 << 24
+    for status in (lib.mimir_prefixlm_pages_fork(ctypes.byref(_pages(workspace_bytes=1 << 40)), 4096, 4096, n, None),
+                   lib.mimir_prefixlm_pages_release(ctypes.byref(_pages()), 4096, n, None),
+                   lib.mimir_prefixlm_pages_reserve(ctypes.byref(_pages(rows=1 << 26, workspace_bytes=1 << 40)), 4096, None)):
+        with pytest.raises(ValueError, match="too many rows"):
+            _capi.raise_for_status(lib, status)

@@ -161,3 +161,13 @@ def test_yarn_amplitude(factor, amplitude):
     freq, got = RotaryFrequencies.inverse_frequencies(64, scaling="yarn", factor=factor, original_positions=4096)
     assert math.isclose(got, amplitude)
     assert RotaryFrequencies.create(64, scaling="yarn", factor=factor, device="cpu").amplitude == got
+
+
+@pytest.mark.parametrize("kw", [dict(batch=1 << 15, seqlen=1 << 15), dict(seqlen=(1 << 31) - 1, dtype=0)])
+def test_launches_of_2_to_32_threads_are_refused(kw):
+    p = _params(num_q_heads=1, num_kv_heads=0, q_out=1 << 50, **kw)
+    p.q_stride_head = p.q_stride_token = p.q_out_stride_head = p.q_out_stride_token = 64
+    p.q_stride_batch = p.q_out_stride_batch = 64 * p.seqlen
+    lib = _capi.load()
+    with pytest.raises(ValueError, match="too many tokens"):
+        _capi.raise_for_status(lib, lib.mimir_prefixlm_rotary(ctypes.byref(p), None))
