@@ -9,9 +9,11 @@
 //     paged_prefill_*     one workgroup per (batch row, kv head, 128 query rows, key split)
 //     paged_merge_splits_* with several splits: adds their partial rows
 //
-// S^T = K Q^T and O^T += V^T P^T on the matrix cores with an online softmax in fp32: decode in bf16 (codes
-// become bf16 times their page's scale in the conversion instruction, exactly), prefill on the
-// codes themselves.  P is rounded under the page's own maximum, to the eight bits of bf16.
+// S^T = K Q^T and O^T += V^T P^T on the matrix cores with an online softmax in fp32: in bf16 (codes
+// become bf16 times their page's scale in the conversion instruction, exactly), prefill's first
+// product on the codes themselves.  P is rounded to bf16, as everywhere in this library: the one rounding
+// between the codes and the output that is not fp32's (and, in prefill, of query elements below 2^-15
+// of their row's largest).  The sums of P are those of the unrounded ones.
 #include <algorithm>
 #include <cmath>
 
@@ -702,22 +704,24 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 // Rows are (token, head) pairs, token-major, 128 to a workgroup, so the G query heads of a
 // kv head share its pages, which are copied to LDS as they are while the page before is computed.
 //
-// Both products run on the 8-bit matrix instruction (32 x 32 x 64, twice the bf16 rate) with the codes
-// as one operand, their page's scale going into the instruction, and the other operand, queries or
-// probabilities, in two 8-bit halves: hi the nearest code, lo that of the rest (halves8).  A code holds
-// four significant bits, so the two hold the eight of bf16 in as much matrix time.
-//   queries        under a power of two of each row: exact down to 2^-15 of the row's largest element, the
-//                  smaller ones to 2^-22 of it
-//   probabilities  under a power of two of each row and page, 2^8 at most: to 2^-8 of themselves, as in
-//                  bf16, and to 2^-21 of the page's largest, so that a long tail of small ones
-//                  is rounded in its own pages only
-// Against bf16 operands (codes converted on their way to LDS, 1000 of 4600 cycles a page): half the LDS
-// reads, no conversions, no registers for them.  8 x 512 tokens on 1536 keys, 16 / 4 heads of 128: 70 to 81 us
-// (warm and cool clocks) for 60 GFLOP counted, with the halves 120 executed; bound by the softmax's vector
-// instructions (busy 63% of the time, the matrix units 38%, two waves a SIMD).
+// The scores run on the 8-bit matrix instruction (32 x 32 x 64, twice the bf16 rate) with the keys' codes as one
+// operand, their page's scale going into the instruction, and the queries in two 8-bit halves as the other: hi the
+// nearest code, lo that of the rest (halves8), under a power of two of each row.  A code holds four significant
+// bits, so the two hold the eight of bf16 in as much matrix time, exactly down to 2^-15 of the row's largest element,
+// the smaller ones to 2^-22 of it: two fp32 half steps of the largest term.  (A third code for what they leave,
+// multiplied where a wave's queries leave anything: 8 to 12% slower.)  Against keys converted to bf16: half the LDS reads,
+// no conversions, and the queries are split once.
+// The output takes P in bf16 and the values' codes converted on their way into the operands, once for each wave.
+// P in two halves under its page's maximum, on the codes, lost small probabilities below 2^-21 of the page's
+// largest and was slower: it takes ten vector instructions for four, where a conversion of two takes one.  Halves /
+// bf16: 8 x 512 tokens on 1024 keys, 16 / 4 heads of 128, 66.6 / 66.4 us, 8 x up to 512 on up to 3000 85.2 / 81.8;
+// 8 / 8 heads of 64, 8 x 512 on 1024, 44.5 / 42.0, 4096 on 8192, 8 / 2, 167.7 / 144.9.
+// 8 x 512 tokens on 1536 keys, 16 / 4 heads of 128: 68 to 79 us (warm and cool clocks; 77.1 under the counters) for 60
+// GFLOP; the vector units are busy 56% and the matrix units 41% of the time, which two waves a SIMD overlap little.
 //
 // The scores' rows are tokens 32 (m / 4 % 2) + 16 t + 4 (m / 8) + m % 4 for row m of tile t, so that the 32 a
-// lane holds are 32 hi .., in order: the 32 bytes of a value column that its half of the lanes reads.
+// lane holds are 32 hi .., in order: the 32 bytes of a value column that its half of the lanes reads, eight of them
+// for each step of the second product.
 
 constexpr int kRows = kWaves * 32;
 constexpr int kTogether = 2;  // pages between two barriers
@@ -735,9 +739,8 @@ __device__ __forceinline__ bool even_lengths(const PagedArgs& a) {
 // A padded batch (new_lengths), whose row tiles with queries only the device knows: those alone are cut, each
 // into n runs of about as many pages, so that the runs of all are a.slots and one more for each row tile at
 // most.  Runs first, then the row tiles without queries.  64 batch rows, one per lane.  Against splits of the
-// full batch's tiles: 8 x up to 512 on up to 3000 keys, 16 / 4 heads of 128, 99.1 -> 81 us; 3 x up to 200 on 1000 to
-// 3000, 32 / 8, 42.0 -> 32.6; 8 x up to 700 on up to 2000, 8 / 8 heads of 64, 51.8 -> 41.2; 5 x up to 1339 on up to
-// 1000 49.4 -> 46 (42 -> 31 and 7.8 of merge).
+// full batch's tiles, on 1 to so many keys: 8 x up to 512 on 3000 keys, 16 / 4 heads of 128, 97 -> 80.5 us; 3 x up to 200
+// on 3000, 32 / 8, 54.6 -> 51.0; 8 x up to 700 on 2000, 8 / 8 heads of 64, 48.7 -> 43.5; 5 x up to 1339 on 1000 58.4 -> 47.0.
 constexpr int kDealtRows = 64;
 struct Runs {
   PagedRow at;      // of the lane's batch row
@@ -750,8 +753,9 @@ struct Runs {
     act = at.kv > 0 ? (int)((unsigned)(at.m * a.G + kRows - 1) / kRows) : 0;
     const int pages = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv * tiles), 63);
     // At head_dim 64 all runs are to be on the chip at once, three per CU: a few more would be a second round (8 x up to
-    // 700 tokens on up to 2000 keys 43.3 -> 41.2 us).  At 128 one per CU and the remainders (all at once, two per CU:
-    // 8 x up to 512 on up to 3000 80 -> 77.5, 4 x up to 100 on up to 3000 31.8 -> 35.6).
+    // 700 tokens on up to 2000 keys 48.6 -> 43.5 us, 5 x up to 1339 on 1000 50.1 -> 47.0, where two per CU take 43.4 and
+    // 49.9).  At 128 one per CU and the remainders (two per CU: 8 x up to 512 on up to 3000 80.5 -> 85.6, 4 x up to 100 on
+    // up to 3000 29.2 -> 31.0).
     const int all = __builtin_amdgcn_readlane(wave_inclusive_sum(act * a.Hkv), 63);
     int most = max(kTogether, (int)((unsigned)(pages + a.slots - 1) / (unsigned)a.slots));
     for (int tries = a.D == 64 && all <= a.slots ? 12 : 0;; --tries) {
@@ -967,7 +971,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   const int k_base = k_token * D, k_turn = 32 * hi ^ 16 * k_place(k_token);
   const int v_base = l32 * kPage, v_turn = 32 * hi ^ 16 * v_place(l32);
 
-  auto compute = [&](int kt, int j, int buf, int k_scale, int v_scale) __attribute__((always_inline)) {
+  auto compute = [&](int kt, int j, int buf, int k_scale, int e_v) __attribute__((always_inline)) {
     const int base = kt * kPage;
     if (!active || base >= w_max) return;
     f32x16 st[2];
@@ -1010,42 +1014,40 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       m_run = m_new;
     }
     const float ref = m_run == -INFINITY ? 0.f : m_run, mb = ref * c2;
-    // The page's probabilities times 2^-up, so that the largest lies in [2^7, 2^8).
-    const int up = (int)floorf(fmaxf((mx - ref) * c2, -100.f)) - 7;
     // Scaled scores past 2^16 are known to 2^-8 only: their difference is formed before the scale, at an
     // operation more each, or rounding them apart would give probabilities up to 2^(their ulp).
     if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(mb) > 65536.f) != 0) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2(__builtin_fmaf(st[t][e] - ref, c2, (float)-up));
+        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2((st[t][e] - ref) * c2);
     } else {
-      const float shift = -(mb + (float)up);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2(__builtin_fmaf(st[t][e], c2, shift));
+        for (int e = 0; e < 16; ++e) st[t][e] = fast_exp2(__builtin_fmaf(st[t][e], c2, -mb));
     }
     float lsum = 0.f;
-    i32x8 ph, pl;
+    bf16x8 pf[4];  // tokens 32 hi + 8 s ..+7
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const int t = w >> 2, e = 4 * (w & 3);
-      lsum += (st[t][e] + st[t][e + 1]) + (st[t][e + 2] + st[t][e + 3]);
-      int c_hi, c_lo;
-      halves8(st[t][e], st[t][e + 1], st[t][e + 2], st[t][e + 3], c_hi, c_lo);
-      ph[w] = c_hi;
-      pl[w] = c_lo;
+    for (int s = 0; s < 4; ++s) {
+      f32x8 x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = st[s >> 1][8 * (s & 1) + e];
+      lsum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      pf[s] = to_bf16x8(x);
     }
-    l_run += __builtin_amdgcn_ldexpf(lsum, up);
-    const int p_scale = 127 + up;
+    l_run += lsum;
+    const float vs = pow2(e_v);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const uint8_t* const vp = &sV[buf][v_base + dt * 32 * kPage];
-      const i32x4 v0 = *(const i32x4*)&vp[v_turn], v1 = *(const i32x4*)&vp[v_turn ^ 16];
-      const i32x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-      oacc[dt] = mfma8(v, pl, oacc[dt], v_scale, p_scale - kLoShift);
-      oacc[dt] = mfma8(v, ph, oacc[dt], v_scale, p_scale);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const i32x4 v = *(const i32x4*)&vp[half ? v_turn ^ 16 : v_turn];
+        oacc[dt] = mfma32(decode8(v[0], v[1], vs), pf[2 * half], oacc[dt]);
+        oacc[dt] = mfma32(decode8(v[2], v[3], vs), pf[2 * half + 1], oacc[dt]);
+      }
     }
     if (__builtin_expect(base + kPage > wg_min && __builtin_amdgcn_readfirstlane(s_any[j][0] | s_any[j][1] | s_any[j][2] | s_any[j][3]), 0)) {
       // NaN values into the rows that see them
@@ -1064,11 +1066,11 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
   for (int kt = kt0, buf = 0; kt < kt1; kt += kTogether, buf ^= kTogether) {
     wait_vmem();  // the pages' copies
     __syncthreads();
-    int k_scale[kTogether], v_scale[kTogether];
+    int k_scale[kTogether], e_v[kTogether];
     bool there[kTogether], cleaned = false;
 #pragma unroll
     for (int j = 0; j < kTogether; ++j) {
-      k_scale[j] = 127 + ek[j], v_scale[j] = 127 + ev[j], there[j] = some[j];
+      k_scale[j] = 127 + ek[j], e_v[j] = ev[j], there[j] = some[j];
       if (there[j] && (kt + j) * kPage + kPage > wg_min) {  // uniform
         clean_page(kt + j, j, buf + j);
         cleaned = true;
@@ -1079,7 +1081,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
     for (int j = 0; j < kTogether; ++j) load_page(kt + kTogether + j, j, (buf ^ kTogether) + j);
 #pragma unroll
     for (int j = 0; j < kTogether; ++j)
-      if (there[j]) compute(kt + j, j, buf + j, k_scale[j], v_scale[j]);
+      if (there[j]) compute(kt + j, j, buf + j, k_scale[j], e_v[j]);
   }
 
   const float l_tot = xor32_sum(l_run);
@@ -1160,8 +1162,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_many_d128_kernel(const P
 __global__ __launch_bounds__(kThreads) void paged_merge_many_d64_kernel(const PagedArgs a) { paged_merge_many_body<64>(a); }
 
 // The same for a few splits of many rows, D / 4 lanes to a row and four columns each, four parts at once (a wave to
-// a row / so: 8 x 512 on 1536 keys, 8 / 8 heads of 64, two splits, 67.4 / 49.8 us; 100 on 3000, 16 / 4 heads
-// of 128, 32 splits, 35.7 / 39.6).
+// a row / so: 8 x 512 on 1536 keys, 8 / 8 heads of 64, two splits, 64.4 / 47.6 us; 100 on 3000, 16 / 4 heads
+// of 128, 32 splits, 32.6 / 33.0).
 constexpr int kFewSplits = 8;
 template <int D>
 __device__ __forceinline__ void paged_merge_splits_body(const PagedArgs& a) {
@@ -1256,7 +1258,8 @@ Plan plan_of(const MimirPagedAttnParams& p) {
       s.units = pairs;
     } else {
       // Workgroups per CU: as many as fit at once (registers), two at head_dim 128 or with two row tiles, three
-      // else (64 rows of 500 to 4000 keys, 8 / 8 heads of 64: 42.3 -> 39.0 us; of 128 two are faster than three or four).
+      // else.  Two / three / four, heads of 64: 64 rows of 2000 to 16000 keys, 8 / 8, 90.5 / 89.6 / 95.1 us; 200 rows of
+      // 1100 to 9000, 8 / 2, 57.6 / 57.0 / 63.1.  Of 128 two are faster than three or four.
       const int64_t per_cu = p.head_dim == 64 && R <= 16 ? 3 : 2;
       s.units = p.num_kv_heads * std::max<int64_t>(1, std::min(most, per_cu * cus / p.num_kv_heads));
       s.workspace_bytes = (size_t)s.units * 2 * (size_t)R * ((size_t)p.head_dim + 2) * sizeof(float);

@@ -68,18 +68,16 @@ class Cache:
     def attend(self, q, k, v, layer, table, lengths, causal, rows=None, new=None, scale=None):
         """Appends, then the output in 64 bits and how far a kernel may be from it, element by element.
 
-        A kernel may hold queries and probabilities as two 8-bit halves hi + lo 2^-4 under a power of two: with |x|
-        at most 2^8.8, hi is off by at most 2^-4 of x, lo by 2^-4 of that rest, 2^-8 of x together (the half step
-        of bf16), or by half the smallest code step, 2^-10, times 2^-4.
-        Queries: the row's largest element lies above 224 = 2^7.8 under its power of two, bf16 elements are
-        exact but for the second kind, 2^-14 / 2^7.8 < 2^-21 of the largest.
-        Probabilities: the page's largest lies in [2^7, 2^8), so 2^-8 of each, or 2^-14 / 2^7 = 2^-21 of the largest.
+        A kernel may hold queries as two 8-bit halves hi + lo 2^-4 under a power of two of each row, and
+        probabilities as bf16.  With |x| at most 2^8.8, hi is off by at most 2^-4 of x, lo by 2^-4 of that rest, 2^-8 of x
+        together, which bf16 elements do not need (their bits end there), or by half the smallest code step,
+        2^-10, times 2^-4.  The row's largest element lies above 224 = 2^7.8 under its power of two, so that is
+        2^-14 / 2^7.8 < 2^-21 of the largest.  Rounding to bf16 is off by at most 2^-8.
 
         So a score is off by at most s = (d + 8) 2^-24 sum |q k| (its fp32 sums and the exponent's argument) + 2^-21
         (the exponential's own approximation) + 2^-21 max |q| sum |k|; an output by (2 s + 2^-8) sum p |v| / sum p
-        (the sum of the probabilities moves by s as well) + 2^-21 max p sum |v| / sum p, by (n / 32 + 64) 2^-24
-        of the first for the fp32 sums over n tokens (partial sums of 32 tokens a product, joined), and by its own
-        rounding, 2^-8 of it."""
+        (the sum of the probabilities moves by s as well), by (n / 32 + 64) 2^-24 of that for the fp32 sums over n
+        tokens (partial sums of 32 tokens a product, joined), and by its own rounding, 2^-8 of it."""
         q, k, v = (x.detach().cpu().double().numpy() for x in (q, k, v))
         B, S, hq, d = q.shape
         hkv = k.shape[2]
@@ -135,7 +133,6 @@ class Cache:
                         off = (d + 8) * 2.0 ** -24 * (np.abs(qq) @ np.abs(ks).T * scale).max(1, keepdims=True) + 2.0 ** -21
                         off = off + 2.0 ** -21 * scale * np.abs(qq).max(1, keepdims=True) * np.abs(ks).sum(1).max()
                         slack = (2 * off + 2.0 ** -8 + (kv / 32 + 64) * 2.0 ** -24) * spread
-                        slack = slack + 2.0 ** -21 * np.abs(vs).sum(0) / total  # the largest probability here is 1
                     out[b, i, h * (hq // hkv):(h + 1) * (hq // hkv)] = o
                     tol[b, i, h * (hq // hkv):(h + 1) * (hq // hkv)] = slack + 2.0 ** -8 * (np.abs(o) + slack)
         return out, tol
