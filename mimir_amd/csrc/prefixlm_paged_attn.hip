@@ -510,7 +510,8 @@ __device__ __forceinline__ void paged_decode_body(const PagedArgs& a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[nr][t][e]);
         // Every page's probabilities under its own maximum (but not more than 2^30 below the row's so
-        // far, which bounds the sums): its largest is 1, exact in bf16.
+        // far, which bounds the sums): its largest is 1, exact in bf16.  (P as the sum of two bf16 numbers, which would
+        // leave the output's own rounding alone: 1 to 4% slower with one row tile, up to 8% with two.)
         mx = xor32_max(xor16_max(mx));
         m_top[nr] = fmaxf(m_top[nr], mx);
         const float m_new = fmaxf(mx, m_top[nr] - ref_range);

@@ -414,3 +414,31 @@ def test_padded_batches_of_many_rows(device, batch, S):
     lens = torch.randint(0, 200, (batch,), generator=gen).tolist()
     new = [[0, S, 1, n][n % 4] for n in torch.randint(0, S + 1, (batch,), generator=gen).tolist()]
     _run(device, S, 8, 4, 64, lens, new=new, seed=batch)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("S", [1, 40, 300])
+def test_small_probabilities_that_carry_the_output(device, d, S):
+    """One token of each page takes nearly all of the softmax and holds zeros; the others, e^-16 of it, hold the output."""
+    from mimir_amd.paged import PagedCache, PageTable, reserve_pages
+
+    n, hkv = 192, 1
+    cache, table = PagedCache.create(12, 1, hkv, d, device=device), PageTable.create(1, 12, 12, device=device)
+    k, v = torch.zeros(1, n, hkv, d), torch.full((1, n, hkv, d), 2.0 ** 23)
+    k[..., 0] = -16.0
+    k[:, ::64], v[:, ::64] = 0.0, 0.0
+    v[:, 1::2] *= 1.5
+    k, v = (x.bfloat16().to(device) for x in (k, v))
+    lens = torch.zeros(1, dtype=torch.int32, device=device)
+    reserve_pages(table, torch.tensor([n + S], device=device))
+    attention_with_pages(torch.zeros(1, n, 2, d, device=device).bfloat16(), k, v, cache, 0, table.pages, lens, True)
+    q = torch.zeros(1, S, 2, d, device=device).bfloat16()
+    q[..., 0] = 1.0
+    far = torch.zeros(1, S, hkv, d, device=device).bfloat16()
+    far[..., 0] = -240.0  # the call's own tokens: nothing
+    lens.fill_(n)
+    pool = O.Cache(*cache)
+    got = attention_with_pages(q, far, far * 0, cache, 0, table.pages, lens, True, softmax_scale=1.0)
+    want, tol = pool.attend(q, far, far * 0, 0, table.pages, lens, True, scale=1.0)
+    assert want.min() > 50 and tol.max() < 1
+    assert (abs(got.cpu().double().numpy() - want) <= tol).all()
