@@ -12,8 +12,8 @@
 // S^T = K Q^T and O^T += V^T P^T on the matrix cores with an online softmax in fp32: in bf16 (codes
 // become bf16 times their page's scale in the conversion instruction, exactly), prefill's first
 // product on the codes themselves.  P is rounded to bf16, as everywhere in this library: the one rounding
-// between the codes and the output that is not fp32's (and, in prefill, of query elements below 2^-15
-// of their row's largest).  The sums of P are those of the unrounded ones.
+// between the codes and the output that is not fp32's (and, in prefill, of query elements below 2^-15 of the
+// largest of 32 columns).  The sums of P are those of the unrounded ones.
 #include <algorithm>
 #include <cmath>
 
@@ -33,7 +33,8 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 8-bit operands, 32 consecutive columns a lane, under 2^(scale - 127) each.
+// 8-bit operands, 32 columns a lane.  Of each row the first four registers of both lane halves stand under
+// 2^(scale - 127) of the lower half's lane, the other four under the upper's.
 __device__ __forceinline__ f32x16 mfma8(i32x8 a, i32x8 b, f32x16 c, int a_scale, int b_scale) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, a_scale, 0, b_scale);
 }
@@ -707,11 +708,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge_d64_kernel(const PagedAr
 //
 // The scores run on the 8-bit matrix instruction (32 x 32 x 64, twice the bf16 rate) with the keys' codes as one
 // operand, their page's scale going into the instruction, and the queries in two 8-bit halves as the other: hi the
-// nearest code, lo that of the rest (halves8), under a power of two of each row.  A code holds four significant
-// bits, so the two hold the eight of bf16 in as much matrix time, exactly down to 2^-15 of the row's largest element,
-// the smaller ones to 2^-22 of it: two fp32 half steps of the largest term.  (A third code for what they leave,
-// multiplied where a wave's queries leave anything: 8 to 12% slower.)  Against keys converted to bf16: half the LDS reads,
-// no conversions, and the queries are split once.
+// nearest code, lo that of the rest (halves8), under a power of two of each row and 32 columns.  A code holds four
+// significant bits, so the two hold the eight of bf16 in as much matrix time, exactly down to 2^-15 of the largest of
+// the 32, the smaller ones to 2^-22 of it: two fp32 half steps of the largest term.  (A third code for what they
+// leave, multiplied where a wave's queries leave anything: 8 to 12% slower.)  Against keys converted to bf16: half the
+// LDS reads, no conversions, and the queries are split once.
 // The output takes P in bf16 and the values' codes converted on their way into the operands, once for each wave.
 // P in two halves under its page's maximum, on the codes, lost small probabilities below 2^-21 of the page's
 // largest and was slower: it takes ten vector instructions for four, where a conversion of two takes one.  Halves /
@@ -933,27 +934,29 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
 #pragma unroll
     for (int j = 0; j < kTogether; ++j) load_page(kt0 + j, j, j);
   }
-  // Q^T operands: the lane's row, columns 64 s + 32 hi ..+31, as codes under 2^(q_scale - 127).
+  // Q^T operands: the lane's row, columns 64 s + 32 hi ..+31, as codes under 2^(q_scale[s] - 127).
   i32x8 qh[KS], ql[KS];
-  int q_scale;
+  int q_scale[KS];
   {
     const bf16_t* q = a.q + (int64_t)b * a.q_sb + (int64_t)ti * a.q_st + (int64_t)h * a.q_sh + 32 * hi;
     i32x4 x[KS][4];  // columns 64 s + 32 hi + 8 j ..+7
-    int most = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[s][j] = row < Rm ? *(const i32x4*)&q[64 * s + 8 * j] : i32x4{0, 0, 0, 0};
-        most = max(most, largest_bits(x[s][j]));
+      for (int j = 0; j < 4; ++j) x[s][j] = row < Rm ? *(const i32x4*)&q[64 * s + 8 * j] : i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      int e01[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int most = max(largest_bits(x[s][2 * c]), largest_bits(x[s][2 * c + 1]));
+        const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+        e01[c] = exponent_for(max((int)both[0], (int)both[1]));
       }
-    most = max(most, __shfl_xor(most, 32, 64));
-    const int e = exponent_for(most);
-    q_scale = 127 + e;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
+      q_scale[s] = 127 + (hi ? e01[1] : e01[0]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        const int e = e01[j >> 2];
         const int w0 = x[s][j >> 1][2 * (j & 1)], w1 = x[s][j >> 1][2 * (j & 1) + 1];
         const float f0 = coded_value(__int_as_float(w0 << 16), e), f1 = coded_value(__int_as_float(w0 & 0xffff0000), e);
         const float f2 = coded_value(__int_as_float(w1 << 16), e), f3 = coded_value(__int_as_float(w1 & 0xffff0000), e);
@@ -962,6 +965,7 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
         qh[s][j] = c_hi;
         ql[s][j] = c_lo;
       }
+    }
   }
   f32x16 oacc[DT];
 #pragma unroll
@@ -984,8 +988,8 @@ __device__ __forceinline__ void paged_prefill_body(const PagedArgs& a) {
       for (int s = 0; s < KS; ++s) {
         const i32x4 k0 = *(const i32x4*)&kp[k_turn ^ (64 * s)], k1 = *(const i32x4*)&kp[k_turn ^ (64 * s + 16)];
         const i32x8 k = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
-        st[t] = mfma8(k, ql[s], st[t], k_scale, q_scale - kLoShift);
-        st[t] = mfma8(k, qh[s], st[t], k_scale, q_scale);
+        st[t] = mfma8(k, ql[s], st[t], k_scale, q_scale[s] - kLoShift);
+        st[t] = mfma8(k, qh[s], st[t], k_scale, q_scale[s]);
       }
     }
     // tokens 32 hi + 16 t + e

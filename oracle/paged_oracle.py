@@ -68,14 +68,14 @@ class Cache:
     def attend(self, q, k, v, layer, table, lengths, causal, rows=None, new=None, scale=None):
         """Appends, then the output in 64 bits and how far a kernel may be from it, element by element.
 
-        A kernel may hold queries as two 8-bit halves hi + lo 2^-4 under a power of two of each row, and
-        probabilities as bf16.  With |x| at most 2^8.8, hi is off by at most 2^-4 of x, lo by 2^-4 of that rest, 2^-8 of x
-        together, which bf16 elements do not need (their bits end there), or by half the smallest code step,
-        2^-10, times 2^-4.  The row's largest element lies above 224 = 2^7.8 under its power of two, so that is
-        2^-14 / 2^7.8 < 2^-21 of the largest.  Rounding to bf16 is off by at most 2^-8.
+        A kernel may hold queries as two 8-bit halves hi + lo 2^-4 under a power of two of each row and 32 columns (two
+        runs of 16, 32 apart), and probabilities as bf16.  With |x| at most 2^8.8, hi is off by at most 2^-4 of x, lo by
+        2^-4 of that rest, 2^-8 of x together, which bf16 elements do not need (their bits end there), or by half the
+        smallest code step, 2^-10, times 2^-4.  The largest of the 32 lies above 224 = 2^7.8 under its power of two, so
+        that is 2^-14 / 2^7.8 < 2^-21 of it.  Rounding to bf16 is off by at most 2^-8.
 
         So a score is off by at most s = (d + 8) 2^-24 sum |q k| (its fp32 sums and the exponent's argument) + 2^-21
-        (the exponential's own approximation) + 2^-21 max |q| sum |k|; an output by (2 s + 2^-8) sum p |v| / sum p
+        (the exponential's own approximation) + 2^-21 sum max |q| sum |k| over the 32s; an output by (2 s + 2^-8) sum p |v| / sum p
         (the sum of the probabilities moves by s as well), by (n / 32 + 64) 2^-24 of that for the fp32 sums over n
         tokens (partial sums of 32 tokens a product, joined), and by its own rounding, 2^-8 of it."""
         q, k, v = (x.detach().cpu().double().numpy() for x in (q, k, v))
@@ -131,7 +131,9 @@ class Cache:
                         o = (p @ vs) / total
                         spread = (p @ np.abs(vs)) / total
                         off = (d + 8) * 2.0 ** -24 * (np.abs(qq) @ np.abs(ks).T * scale).max(1, keepdims=True) + 2.0 ** -21
-                        off = off + 2.0 ** -21 * scale * np.abs(qq).max(1, keepdims=True) * np.abs(ks).sum(1).max()
+                        blocks = lambda x: np.abs(x).reshape(len(x), d // 64, 2, 2, 16)  # noqa: E731
+                        rest = np.einsum("qsb,ksb->qk", blocks(qq).max((2, 4)), blocks(ks).sum((2, 4)))
+                        off = off + 2.0 ** -21 * scale * rest.max(1, keepdims=True)
                         slack = (2 * off + 2.0 ** -8 + (kv / 32 + 64) * 2.0 ** -24) * spread
                     out[b, i, h * (hq // hkv):(h + 1) * (hq // hkv)] = o
                     tol[b, i, h * (hq // hkv):(h + 1) * (hq // hkv)] = slack + 2.0 ** -8 * (np.abs(o) + slack)

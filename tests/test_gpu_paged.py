@@ -442,3 +442,35 @@ def test_small_probabilities_that_carry_the_output(device, d, S):
     want, tol = pool.attend(q, far, far * 0, 0, table.pages, lens, True, scale=1.0)
     assert want.min() > 50 and tol.max() < 1
     assert (abs(got.cpu().double().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("S", [1, 40, 300])
+def test_small_query_elements_beside_far_larger_ones(device, d, S):
+    """A column 2^20 times the others, at which every key is zero: the others decide, also in prefill, whose queries are
+    scaled by the largest of 32 columns (two runs of 16, 32 apart)."""
+    from mimir_amd.paged import PagedCache, PageTable, reserve_pages
+
+    n, hkv = 130, 2
+    gen = torch.Generator().manual_seed(d + S)
+    for big in (0, 37, d - 1):
+        cache, table = PagedCache.create(8, 1, hkv, d, device=device), PageTable.create(1, 8, 8, device=device)
+        q, k, v = (torch.randn(1, S, h, d, generator=gen) for h in (4, hkv, hkv))
+        block = lambda c: (c // 64, c // 16 % 2)  # noqa: E731
+        small = torch.tensor([block(c) != block(big) for c in range(d)])  # the columns that decide
+        q = torch.where(small, q, 0.0)
+        q[..., big] = 2.0 ** 20
+        k[..., big] = 0.0
+        lens = torch.zeros(1, dtype=torch.int32, device=device)
+        kn, vn = (torch.randn(1, n, hkv, d, generator=gen) for _ in range(2))
+        kn[..., big] = 0.0
+        reserve_pages(table, torch.tensor([n + S], device=device))
+        q, k, v, kn, vn = (x.bfloat16().to(device) for x in (q, k, v, kn, vn))
+        attention_with_pages(torch.zeros(1, n, 4, d, device=device).bfloat16(), kn, vn, cache, 0, table.pages, lens, True)
+        lens.fill_(n)
+        pool = O.Cache(*cache)
+        got = attention_with_pages(q, k, v, cache, 0, table.pages, lens, True)
+        plain = q.clone()
+        plain[..., big] = 0.0  # what the large column adds is zero: the bound of a call without it
+        want, tol = pool.attend(plain, k, v, 0, table.pages, lens, True)
+        assert (abs(got.cpu().double().numpy() - want) <= tol).all(), big
