@@ -10,7 +10,7 @@
 // take (move, 16 KiB chunk) units in turn until the list's count ends them.
 //
 // Measured: 1000 pages of 4 layers, 4 heads of 128 moved (530 MB) 99 us, 5.3 TB/s, after 5.7 of planning; a
-// fork of 256 rows of up to 48 pages 28 us: plan 4.0, gather 3.2, take 4.8 and the copies (79 MB) 16.5; each
+// fork of 256 rows of up to 48 pages 28 us: plan 4.1, gather 3.1, take 4.8 and the copies (79 MB) 17; each
 // planning launch is 2 us and a few round trips of 0.7.
 #include <algorithm>
 

@@ -11,9 +11,9 @@
 //
 // A frequency is held as the fraction of a turn per position in units of 2^-64, so the
 // 64-bit product position * turns, which wraps at whole turns, is the range reduction:
-// exact for any position, where a product in fp32 is a radian off at a million.  The
-// nearest quarter turn comes off as integer bits; what is left, at most pi / 4, goes
-// through the Taylor series (truncated below 2e-9) of sine and cosine.
+// exact for any position and the given turns, where a product in fp32 is a radian off at a million.  The
+// nearest quarter turn comes off as integer bits; what is left, at most pi / 4, is rounded to
+// fp32 (2^-28 of a turn at most) and goes through the Taylor series (truncated below 2e-9) of sine and cosine.
 //
 // Bound by reading and writing the heads once.  A thread owns V pairs of columns of one
 // token, computes their angles once and takes every hp-th head of q and k with them, so

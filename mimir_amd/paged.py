@@ -291,7 +291,9 @@ def attention_with_pages(query: Tensor, key: Tensor, value: Tensor, cache: Paged
     dropped, and not attended.  A page that a batch row appends to must be that row's alone in the
     call, neither appended to nor read for another (fork_rows sees to that): the rows run side by
     side.  Both raise with ``mimir_amd.set_validate_metadata(True)``, which costs a host read.
-    Infinite keys and values become NaN.  For inference: the result has no gradient.
+    Infinite keys and values become NaN.  Scores and sums are fp32; probabilities are rounded to bf16 for
+    the product with the values, and with more than 32 query rows per kv head the queries are read to 2^-22 of
+    the largest of 32 columns.  For inference: the result has no gradient.
     """
     scale = (1.0 / math.sqrt(query.shape[-1]) if query.shape[-1] else 1.0) if softmax_scale is None else float(softmax_scale)
     if query.is_cuda and not P._validate_metadata:

@@ -7,8 +7,11 @@ int64, restarting per document, or far along in a decode) and a table of frequen
 keys are turned in one launch, and the gradient is the inverse turn.
 
 Frequencies are fractions of a turn per position in units of 2^-64, so that the 64-bit
-product with a position wraps at whole turns: angles are exact to 2^-34 of a turn at
-any position.  float32 and bfloat16; no CPU fallback.
+product with a position wraps at whole turns: for the given ``turns`` the range reduction is
+exact at any position.  The rest, within an eighth of a turn, is then rounded to fp32: 2^-28 of
+a turn at most.  ``create`` forms its table in 64-bit floats, off by up to 3 * 2^-53 of a
+frequency, which far positions multiply: of the fastest pair that stays below 2^-28 of a turn up to
+position 7e7.  float32 and bfloat16; no CPU fallback.
 """
 
 from __future__ import annotations
