@@ -440,6 +440,52 @@ typedef struct MimirRotaryParams {
 } MimirRotaryParams;
 int mimir_prefixlm_rotary(const MimirRotaryParams* params, void* stream);
 
+/* Heads normed, scaled by a learned weight and turned by their position, in one pass:
+ * for each head's row x of q [B, S, Hq, D] and (num_kv_heads > 0) k [B, S, Hkv, D],
+ *
+ *     y = R (r w x),  r = 1 / sqrt(mean(x^2) + eps),  w = q_weight or k_weight [D],
+ *
+ * R the turn of mimir_prefixlm_rotary (amplitude, pair layout and rotary_dim as there), in
+ * fp32 with one rounding.  A weight may be NULL: ones.  weight_dtype: that of the heads, or
+ * float32.  The outputs share no memory with an input, each other or themselves.
+ *
+ * mimir_prefixlm_norm_rotary_bwd: from dq / dk, the gradients of the outputs, those of q and
+ * k in q_out / k_out and (not NULL) of the weights in dq_weight / dk_weight:
+ *     g = R^T dy,  dw = sum over the rows of r g x,  dx = r (w g - x r^2 mean(w g x)).
+ * The workspace is needed for weight gradients only and needs no clearing. */
+typedef struct MimirNormRotaryParams {
+  const void* q;
+  const void* k;              /* NULL if num_kv_heads is 0 */
+  void* q_out;
+  void* k_out;
+  const void* dq;             /* gradient: of q's output; else not read */
+  const void* dk;
+  const void* q_weight;       /* [D], or NULL */
+  const void* k_weight;
+  void* dq_weight;            /* gradient: [D], or NULL; else not read */
+  void* dk_weight;
+  const int64_t* turns;       /* [rotary_dim / 2] */
+  const void* positions;      /* int32 or int64 (index_int64) [B, S] */
+  int64_t q_stride_batch, q_stride_token, q_stride_head;
+  int64_t k_stride_batch, k_stride_token, k_stride_head;
+  int64_t q_out_stride_batch, q_out_stride_token, q_out_stride_head;
+  int64_t k_out_stride_batch, k_out_stride_token, k_out_stride_head;
+  int64_t dq_stride_batch, dq_stride_token, dq_stride_head;
+  int64_t dk_stride_batch, dk_stride_token, dk_stride_head;
+  int64_t positions_stride_batch, positions_stride_token;
+  int32_t batch, seqlen, num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  int32_t interleaved;
+  int32_t dtype;              /* MIMIR_DTYPE_FLOAT32 or MIMIR_DTYPE_BFLOAT16 */
+  int32_t weight_dtype;
+  int32_t index_int64;
+  float amplitude, eps;
+  void* workspace;            /* gradient: >= mimir_prefixlm_norm_rotary_workspace_bytes(params) */
+  size_t workspace_bytes;
+} MimirNormRotaryParams;
+size_t mimir_prefixlm_norm_rotary_workspace_bytes(const MimirNormRotaryParams* params);
+int mimir_prefixlm_norm_rotary(const MimirNormRotaryParams* params, void* stream);
+int mimir_prefixlm_norm_rotary_bwd(const MimirNormRotaryParams* params, void* stream);
+
 /* Attention over a KV cache in pages of MIMIR_PAGE_TOKENS tokens, held in 8 bits (e4m3)
  * under one power-of-two scale for each page and kv head.
  *

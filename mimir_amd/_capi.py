@@ -132,6 +132,24 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class NormRotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("dq", _vp), ("dk", _vp),
+        ("q_weight", _vp), ("k_weight", _vp), ("dq_weight", _vp), ("dk_weight", _vp), ("turns", _vp), ("positions", _vp),
+        ("q_stride_batch", _i64), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("k_stride_batch", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("q_out_stride_batch", _i64), ("q_out_stride_token", _i64), ("q_out_stride_head", _i64),
+        ("k_out_stride_batch", _i64), ("k_out_stride_token", _i64), ("k_out_stride_head", _i64),
+        ("dq_stride_batch", _i64), ("dq_stride_token", _i64), ("dq_stride_head", _i64),
+        ("dk_stride_batch", _i64), ("dk_stride_token", _i64), ("dk_stride_head", _i64),
+        ("positions_stride_batch", _i64), ("positions_stride_token", _i64),
+        ("batch", _i32), ("seqlen", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("interleaved", _i32), ("dtype", _i32), ("weight_dtype", _i32), ("index_int64", _i32),
+        ("amplitude", ctypes.c_float), ("eps", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class PagedAttnParams(ctypes.Structure):
     _fields_ = [
         ("q", _vp), ("k_new", _vp), ("v_new", _vp), ("out", _vp),
@@ -181,6 +199,9 @@ EXPORTED_SYMBOLS = (
     "mimir_prefixlm_cache_attn",
     "mimir_prefixlm_cache_attn_workspace_bytes",
     "mimir_prefixlm_rotary",
+    "mimir_prefixlm_norm_rotary",
+    "mimir_prefixlm_norm_rotary_bwd",
+    "mimir_prefixlm_norm_rotary_workspace_bytes",
     "mimir_prefixlm_paged_attn",
     "mimir_prefixlm_paged_attn_workspace_bytes",
     "mimir_prefixlm_pages_workspace_bytes",
@@ -242,6 +263,11 @@ def load() -> ctypes.CDLL:
         lib.mimir_prefixlm_cache_attn_workspace_bytes.restype = ctypes.c_size_t
         lib.mimir_prefixlm_rotary.argtypes = [ctypes.POINTER(RotaryParams), _vp]
         lib.mimir_prefixlm_rotary.restype = ctypes.c_int
+        for entry in (lib.mimir_prefixlm_norm_rotary, lib.mimir_prefixlm_norm_rotary_bwd):
+            entry.argtypes = [ctypes.POINTER(NormRotaryParams), _vp]
+            entry.restype = ctypes.c_int
+        lib.mimir_prefixlm_norm_rotary_workspace_bytes.argtypes = [ctypes.POINTER(NormRotaryParams)]
+        lib.mimir_prefixlm_norm_rotary_workspace_bytes.restype = ctypes.c_size_t
         lib.mimir_prefixlm_paged_attn.argtypes = [ctypes.POINTER(PagedAttnParams), _vp]
         lib.mimir_prefixlm_paged_attn.restype = ctypes.c_int
         lib.mimir_prefixlm_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]

@@ -55,6 +55,7 @@ SOURCES = [
     "prefixlm_cache_bf16.hip",
     "prefixlm_noalloc.hip",
     "prefixlm_rotary.hip",
+    "prefixlm_norm_rotary.hip",
     "prefixlm_paged_append.hip",
     "prefixlm_paged_attn.hip",
     "prefixlm_pages.hip",

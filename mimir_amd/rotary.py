@@ -224,3 +224,106 @@ def rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies:
         return _Rotary.apply(query, key, positions, frequencies.turns, frequencies.amplitude, frequencies.interleaved,
                              inverse)
     return _turn(query, key, positions, frequencies, inverse)
+
+
+# ---------------------------------------------------------------- heads normed and turned
+
+def _norm_weight(name: str, w: Optional[Tensor], like: Tensor) -> Optional[Tensor]:
+    if w is None:
+        return None
+    if w.dtype not in (torch.float32, like.dtype):
+        raise TypeError(f"{name} must be float32 or of the heads' type {like.dtype}, got {w.dtype}")
+    if w.shape != like.shape[-1:] or w.device != like.device:
+        raise ValueError(f"{name} must be [{like.shape[-1]}] on {like.device}, got {tuple(w.shape)} on {w.device}")
+    return w.contiguous()
+
+
+def _norm_params(query, key, positions, frequencies, query_weight, key_weight, eps, outputs, grads=(None, None)):
+    """The C struct of checked operands with unit head_dim strides, their outputs and (backward) gradients."""
+    weight = query_weight if query_weight is not None else key_weight
+    lead = query.shape[:-2]
+    four = lambda t: (0, 0, 0) if t is None else (0, *t.stride()[:2]) if t.dim() == 3 else t.stride()[:3]  # noqa: E731
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    pos = positions.stride()
+    return _capi.NormRotaryParams(
+        query.data_ptr(), ptr(key), *map(ptr, outputs), *map(ptr, grads), ptr(query_weight), ptr(key_weight), None, None,
+        frequencies.turns.data_ptr(), positions.data_ptr(),
+        *four(query), *four(key), *four(outputs[0]), *four(outputs[1]), *four(grads[0]), *four(grads[1]),
+        *((0, *pos) if len(lead) == 1 else pos),
+        1 if len(lead) == 1 else lead[0], lead[-1], query.shape[-2], 0 if key is None else key.shape[-2], query.shape[-1],
+        2 * frequencies.turns.shape[0], int(bool(frequencies.interleaved)), _DTYPES[query.dtype],
+        _DTYPES[query.dtype if weight is None else weight.dtype], int(positions.dtype == torch.int64),
+        float(frequencies.amplitude), eps, None, 0)
+
+
+def _launch_norm(entry: str, device, p) -> None:
+    lib = _capi.load()
+    with torch.cuda.device(device):
+        _capi.raise_for_status(lib, getattr(lib, entry)(ctypes.byref(p), P._stream(device)))
+
+
+def _unit(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def _norm_forward(query, key, positions, frequencies, query_weight, key_weight, eps):
+    query, key = _unit(query), _unit(key)
+    out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key))
+    _launch_norm("mimir_prefixlm_norm_rotary", query.device,
+                 _norm_params(query, key, positions, frequencies, query_weight, key_weight, eps, out))
+    return out
+
+
+class _NormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, positions, turns, amplitude, interleaved, eps):
+        ctx.save_for_backward(query, key, query_weight, key_weight, positions, turns)
+        ctx.meta = (amplitude, interleaved, eps)
+        return _norm_forward(query, key, positions, RotaryFrequencies(turns, amplitude, interleaved), query_weight, key_weight, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dquery, dkey):
+        query, key, query_weight, key_weight, positions, turns = ctx.saved_tensors
+        amplitude, interleaved, eps = ctx.meta
+        query, key, dquery, dkey = map(_unit, (query, key, dquery, dkey if key is not None else None))
+        out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key))
+        p = _norm_params(query, key, positions, RotaryFrequencies(turns, amplitude, interleaved), query_weight, key_weight, eps,
+                         out, (dquery, dkey))
+        weights = [torch.empty_like(w) if w is not None and needed else None
+                   for w, needed in zip((query_weight, key_weight), ctx.needs_input_grad[2:4])]
+        p.dq_weight, p.dk_weight = (None if w is None else w.data_ptr() for w in weights)
+        p.workspace_bytes = _capi.load().mimir_prefixlm_norm_rotary_workspace_bytes(ctypes.byref(p))
+        workspace = torch.empty(p.workspace_bytes // 4, dtype=torch.float32, device=query.device)
+        p.workspace = workspace.data_ptr()
+        _launch_norm("mimir_prefixlm_norm_rotary_bwd", query.device, p)
+        return (*out, *weights, None, None, None, None, None)
+
+
+def norm_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequencies: RotaryFrequencies,
+                query_weight: Optional[Tensor] = None, key_weight: Optional[Tensor] = None, *, eps: float = 1e-6):
+    """Norm each head of ``query`` [..., tokens, Hq, D] and ``key`` [..., tokens, Hkv, D] (or None) by its root
+    mean square, scale it by a learned weight [D] (or None) and turn it as :func:`rotary` does, in one pass:
+    ``turn(x / sqrt(mean(x^2) + eps) * weight)`` with the mean over all of the head.
+
+    Returns ``(query, key)``, new tensors; gradients for the heads and the weights, which are float32 or of the
+    heads' type, both the same.  fp32 arithmetic, one rounding; the weights' gradients are fp32 sums in a fixed
+    order.  Positions, frequencies and strides as for :func:`rotary`.
+    """
+    positions = _check(query, key, positions, frequencies)
+    if query.shape[-1] % 2:
+        raise ValueError(f"head_dim must be even, got {query.shape[-1]}")
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if key is None and key_weight is not None:
+        raise ValueError("a key_weight needs a key")
+    if query_weight is not None and key_weight is not None and query_weight.dtype != key_weight.dtype:
+        raise TypeError(f"query_weight and key_weight must be of one type, got {query_weight.dtype} and {key_weight.dtype}")
+    query_weight, key_weight = _norm_weight("query_weight", query_weight, query), _norm_weight("key_weight", key_weight, query)
+    given = (query, key, query_weight, key_weight)
+    if any(map(_has_tangent, given)):
+        raise NotImplementedError("norm_rotary has no forward-mode derivative")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        return _NormRotary.apply(*given, positions, frequencies.turns, frequencies.amplitude, frequencies.interleaved, eps)
+    return _norm_forward(query, key, positions, frequencies, query_weight, key_weight, eps)
