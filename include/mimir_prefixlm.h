@@ -630,6 +630,56 @@ int mimir_prefixlm_check_metadata(const int32_t* prefix_lens, const int32_t* cau
 /* Thread-local description of the last failure on this thread ("" if none). */
 const char* mimir_prefixlm_last_error(void);
 
+/* Beam search: of each request's W beams over a vocabulary of V tokens, the `count` best
+ * continuations by scores[r, w] + log_softmax(logits[r, w])[token], ties to the lowest beam,
+ * then token.  Log-probabilities and sums are compared in 64 bits, out_scores rounded once.
+ *
+ * A beam with finished[r, w] != 0 goes on with end_token alone, at its score, and its logits are not
+ * read.  A beam whose score is not finite, or whose logits hold NaN or +inf or nothing above -inf, has
+ * no continuation; nor has a token with logit -inf.  Where a request has fewer than
+ * `count` of them, the rest are the lowest (beam, token) among the others, with score -inf.
+ *
+ * out_rows[r, i] is the beam's row r * W + w, out_finished[r, i] (if not NULL) whether that beam was
+ * finished or the token is end_token (end_token < 0: none).  W <= 32, 1 <= count <= min(64, W * V),
+ * V < 2^30.  The workspace needs no clearing. */
+typedef struct MimirBeamSelectParams {
+  const void* logits;         /* [R, W, V], unit stride on V */
+  const float* scores;        /* [R, W] */
+  const uint8_t* finished;    /* [R, W], or NULL */
+  float* out_scores;          /* [R, count] */
+  int32_t* out_tokens;
+  int32_t* out_rows;
+  uint8_t* out_finished;      /* [R, count], or NULL */
+  int64_t logits_stride_request, logits_stride_beam;  /* elements */
+  int64_t scores_stride_request, scores_stride_beam;
+  int64_t finished_stride_request, finished_stride_beam;
+  int32_t requests, beams, vocab, count;
+  int32_t end_token;
+  int32_t dtype;              /* of the logits: MIMIR_DTYPE_FLOAT32 or MIMIR_DTYPE_BFLOAT16 */
+  void* workspace;            /* >= mimir_prefixlm_beam_select_workspace_bytes(params), 16-byte aligned */
+  size_t workspace_bytes;
+} MimirBeamSelectParams;
+size_t mimir_prefixlm_beam_select_workspace_bytes(const MimirBeamSelectParams* params);
+int mimir_prefixlm_beam_select(const MimirBeamSelectParams* params, void* stream);
+
+/* Reordering of cache rows: row i of each of `count` tensors takes the first
+ * lengths[source[i]] positions of row source[i] as they were before the call, and then (if
+ * update_lengths) lengths[i] that of its source.  Rows form groups of `group` (at most 32) neighbours;
+ * a row whose source lies outside its group stays as it is.  Positions past the length
+ * stay as they are.  A position holds position_bytes (a multiple of 16), side by side in a row; rows lie
+ * stride bytes apart (a multiple of 16, no less than max_length positions, unless there is one row). */
+#define MIMIR_REORDER_TENSORS 16
+typedef struct MimirReorderParams {
+  void* data[MIMIR_REORDER_TENSORS];
+  int64_t stride[MIMIR_REORDER_TENSORS];
+  void* lengths;              /* int32 or int64 (index_int64) [rows] */
+  const void* source;         /* int32 or int64 (source_int64) [rows] */
+  int64_t position_bytes;
+  int32_t count, rows, group, max_length;
+  int32_t index_int64, source_int64, update_lengths;
+} MimirReorderParams;
+int mimir_prefixlm_reorder_rows(const MimirReorderParams* params, void* stream);
+
 /* MIMIR_PREFIXLM_ABI_VERSION of the loaded library. */
 int mimir_prefixlm_abi_version(void);
 

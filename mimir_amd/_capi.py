@@ -177,6 +177,29 @@ class PagesParams(ctypes.Structure):
     ]
 
 
+class BeamSelectParams(ctypes.Structure):
+    _fields_ = [
+        ("logits", _vp), ("scores", _vp), ("finished", _vp), ("out_scores", _vp), ("out_tokens", _vp), ("out_rows", _vp),
+        ("out_finished", _vp),
+        ("logits_stride_request", _i64), ("logits_stride_beam", _i64),
+        ("scores_stride_request", _i64), ("scores_stride_beam", _i64),
+        ("finished_stride_request", _i64), ("finished_stride_beam", _i64),
+        ("requests", _i32), ("beams", _i32), ("vocab", _i32), ("count", _i32), ("end_token", _i32), ("dtype", _i32),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+REORDER_TENSORS = 16  # MIMIR_REORDER_TENSORS
+
+
+class ReorderParams(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp * REORDER_TENSORS), ("stride", _i64 * REORDER_TENSORS), ("lengths", _vp), ("source", _vp),
+        ("position_bytes", _i64), ("count", _i32), ("rows", _i32), ("group", _i32), ("max_length", _i32),
+        ("index_int64", _i32), ("source_int64", _i32), ("update_lengths", _i32),
+    ]
+
+
 PAGE_TOKENS = 64  # MIMIR_PAGE_TOKENS
 
 BWD_STAGE_DELTA = 1
@@ -210,6 +233,9 @@ EXPORTED_SYMBOLS = (
     "mimir_prefixlm_pages_compact",
     "mimir_prefixlm_pages_release",
     "mimir_prefixlm_pages_reserve",
+    "mimir_prefixlm_beam_select",
+    "mimir_prefixlm_beam_select_workspace_bytes",
+    "mimir_prefixlm_reorder_rows",
     "mimir_prefixlm_check_metadata",
     "mimir_prefixlm_last_error",
     "mimir_prefixlm_abi_version",
@@ -285,6 +311,12 @@ def load() -> ctypes.CDLL:
         lib.mimir_prefixlm_pages_release.restype = ctypes.c_int
         lib.mimir_prefixlm_pages_reserve.argtypes = [pages, _vp, _vp]
         lib.mimir_prefixlm_pages_reserve.restype = ctypes.c_int
+        lib.mimir_prefixlm_beam_select.argtypes = [ctypes.POINTER(BeamSelectParams), _vp]
+        lib.mimir_prefixlm_beam_select.restype = ctypes.c_int
+        lib.mimir_prefixlm_beam_select_workspace_bytes.argtypes = [ctypes.POINTER(BeamSelectParams)]
+        lib.mimir_prefixlm_beam_select_workspace_bytes.restype = ctypes.c_size_t
+        lib.mimir_prefixlm_reorder_rows.argtypes = [ctypes.POINTER(ReorderParams), _vp]
+        lib.mimir_prefixlm_reorder_rows.restype = ctypes.c_int
         lib.mimir_prefixlm_check_metadata.argtypes = [_vp, _vp, _vp, _i32, _i32, _vp, _vp]
         lib.mimir_prefixlm_check_metadata.restype = ctypes.c_int
         lib.mimir_prefixlm_last_error.argtypes = []

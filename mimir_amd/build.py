@@ -56,6 +56,7 @@ SOURCES = [
     "prefixlm_noalloc.hip",
     "prefixlm_rotary.hip",
     "prefixlm_norm_rotary.hip",
+    "prefixlm_beams.hip",
     "prefixlm_paged_append.hip",
     "prefixlm_paged_attn.hip",
     "prefixlm_pages.hip",
