@@ -630,6 +630,68 @@ int mimir_prefixlm_check_metadata(const int32_t* prefix_lens, const int32_t* cau
 /* Thread-local description of the last failure on this thread ("" if none). */
 const char* mimir_prefixlm_last_error(void);
 
+/* Cross attention over packed sequences: the queries of sequence s, rows cu_seqlens_q[s] up to
+ * cu_seqlens_q[s + 1] of q, attend all of its states, rows cu_seqlens_k[s] up to cu_seqlens_k[s + 1] of k / v:
+ * out = softmax(softmax_scale q k^T) v.  Both lists hold numseqs + 1 device int32, not decreasing.  A
+ * sequence without states gives O = 0, and rows before the first or behind the last sequence O = 0 and
+ * zero gradients.  lse2 (may be NULL in the forward) is what the backward needs of it: float32 [Hq, total_q],
+ * the base-2 logarithm of the softmax's sum, scale included, -inf without states.  bf16, head_dim
+ * 64 or 128, 16-byte aligned rows.  The workspaces need no clearing. */
+typedef struct MimirCrossParams {
+  const void* q;              /* [total_q, Hq, D] */
+  const void* k;              /* [total_k, Hkv, D] */
+  const void* v;
+  void* out;                  /* [total_q, Hq, D]: written by the forward, read by the backward */
+  float* lse2;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_k;
+  const void* dout;           /* backward */
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t q_stride_token, q_stride_head;
+  int64_t k_stride_token, k_stride_head;
+  int64_t v_stride_token, v_stride_head;
+  int64_t out_stride_token, out_stride_head;
+  int64_t dout_stride_token, dout_stride_head;
+  int64_t dq_stride_token, dq_stride_head;
+  int64_t dk_stride_token, dk_stride_head;
+  int64_t dv_stride_token, dv_stride_head;
+  int32_t total_q, total_k, numseqs, num_q_heads, num_kv_heads, head_dim;
+  int32_t dtype;              /* MIMIR_DTYPE_BFLOAT16 */
+  float softmax_scale;        /* positive */
+  void* workspace;            /* >= mimir_prefixlm_cross_workspace_bytes(params, backward), 256-byte aligned */
+  size_t workspace_bytes;
+} MimirCrossParams;
+size_t mimir_prefixlm_cross_workspace_bytes(const MimirCrossParams* params, int32_t backward);
+int mimir_prefixlm_cross_fwd(const MimirCrossParams* params, void* stream);
+int mimir_prefixlm_cross_bwd(const MimirCrossParams* params, void* stream);
+
+/* Cross attention to rows of a static cache of states: request s is the seq_tokens query rows from
+ * s * seq_tokens on (all tokens of all its beams), over the first lengths[r] (clamped to [0, cache_len]) positions
+ * of cache row r = rows[s] (rows NULL: s).  A row outside [0, cache_rows) has no states; without
+ * states the output is 0.  bf16, head_dim 64 or 128; the workspace needs no clearing. */
+typedef struct MimirStatesParams {
+  const void* q;              /* [requests * seq_tokens, Hq, D] */
+  const void* keys;           /* [cache_rows, cache_len, Hkv, D] */
+  const void* values;
+  void* out;                  /* [requests * seq_tokens, Hq, D] */
+  const void* lengths;        /* device int32 or int64 (lengths_int64) [cache_rows] */
+  const void* rows;           /* device int32 or int64 (rows_int64) [requests], or NULL */
+  int64_t q_stride_token, q_stride_head;
+  int64_t k_stride_row, k_stride_token, k_stride_head;
+  int64_t v_stride_row, v_stride_token, v_stride_head;
+  int64_t out_stride_token, out_stride_head;
+  int32_t requests, seq_tokens, cache_rows, cache_len, num_q_heads, num_kv_heads, head_dim;
+  int32_t dtype;              /* MIMIR_DTYPE_BFLOAT16 */
+  int32_t lengths_int64, rows_int64;
+  float softmax_scale;        /* positive */
+  void* workspace;            /* >= mimir_prefixlm_states_workspace_bytes(params), 256-byte aligned */
+  size_t workspace_bytes;
+} MimirStatesParams;
+size_t mimir_prefixlm_states_workspace_bytes(const MimirStatesParams* params);
+int mimir_prefixlm_states_attn(const MimirStatesParams* params, void* stream);
+
 /* Beam search: of each request's W beams over a vocabulary of V tokens, the `count` best
  * continuations by scores[r, w] + log_softmax(logits[r, w])[token], ties to the lowest beam,
  * then token.  Log-probabilities and sums are compared in 64 bits, out_scores rounded once.

@@ -177,6 +177,33 @@ class PagesParams(ctypes.Structure):
     ]
 
 
+class CrossParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse2", _vp), ("cu_seqlens_q", _vp), ("cu_seqlens_k", _vp),
+        ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("q_stride_token", _i64), ("q_stride_head", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("v_stride_token", _i64), ("v_stride_head", _i64), ("out_stride_token", _i64), ("out_stride_head", _i64),
+        ("dout_stride_token", _i64), ("dout_stride_head", _i64), ("dq_stride_token", _i64), ("dq_stride_head", _i64),
+        ("dk_stride_token", _i64), ("dk_stride_head", _i64), ("dv_stride_token", _i64), ("dv_stride_head", _i64),
+        ("total_q", _i32), ("total_k", _i32), ("numseqs", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32),
+        ("head_dim", _i32), ("dtype", _i32), ("softmax_scale", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class StatesParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("keys", _vp), ("values", _vp), ("out", _vp), ("lengths", _vp), ("rows", _vp),
+        ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("k_stride_row", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
+        ("v_stride_row", _i64), ("v_stride_token", _i64), ("v_stride_head", _i64),
+        ("out_stride_token", _i64), ("out_stride_head", _i64),
+        ("requests", _i32), ("seq_tokens", _i32), ("cache_rows", _i32), ("cache_len", _i32), ("num_q_heads", _i32),
+        ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32), ("lengths_int64", _i32), ("rows_int64", _i32),
+        ("softmax_scale", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class BeamSelectParams(ctypes.Structure):
     _fields_ = [
         ("logits", _vp), ("scores", _vp), ("finished", _vp), ("out_scores", _vp), ("out_tokens", _vp), ("out_rows", _vp),
@@ -233,6 +260,11 @@ EXPORTED_SYMBOLS = (
     "mimir_prefixlm_pages_compact",
     "mimir_prefixlm_pages_release",
     "mimir_prefixlm_pages_reserve",
+    "mimir_prefixlm_cross_fwd",
+    "mimir_prefixlm_cross_bwd",
+    "mimir_prefixlm_cross_workspace_bytes",
+    "mimir_prefixlm_states_attn",
+    "mimir_prefixlm_states_workspace_bytes",
     "mimir_prefixlm_beam_select",
     "mimir_prefixlm_beam_select_workspace_bytes",
     "mimir_prefixlm_reorder_rows",
@@ -311,6 +343,15 @@ def load() -> ctypes.CDLL:
         lib.mimir_prefixlm_pages_release.restype = ctypes.c_int
         lib.mimir_prefixlm_pages_reserve.argtypes = [pages, _vp, _vp]
         lib.mimir_prefixlm_pages_reserve.restype = ctypes.c_int
+        for entry in (lib.mimir_prefixlm_cross_fwd, lib.mimir_prefixlm_cross_bwd):
+            entry.argtypes = [ctypes.POINTER(CrossParams), _vp]
+            entry.restype = ctypes.c_int
+        lib.mimir_prefixlm_cross_workspace_bytes.argtypes = [ctypes.POINTER(CrossParams), _i32]
+        lib.mimir_prefixlm_cross_workspace_bytes.restype = ctypes.c_size_t
+        lib.mimir_prefixlm_states_attn.argtypes = [ctypes.POINTER(StatesParams), _vp]
+        lib.mimir_prefixlm_states_attn.restype = ctypes.c_int
+        lib.mimir_prefixlm_states_workspace_bytes.argtypes = [ctypes.POINTER(StatesParams)]
+        lib.mimir_prefixlm_states_workspace_bytes.restype = ctypes.c_size_t
         lib.mimir_prefixlm_beam_select.argtypes = [ctypes.POINTER(BeamSelectParams), _vp]
         lib.mimir_prefixlm_beam_select.restype = ctypes.c_int
         lib.mimir_prefixlm_beam_select_workspace_bytes.argtypes = [ctypes.POINTER(BeamSelectParams)]

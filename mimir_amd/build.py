@@ -56,6 +56,9 @@ SOURCES = [
     "prefixlm_noalloc.hip",
     "prefixlm_rotary.hip",
     "prefixlm_norm_rotary.hip",
+    "prefixlm_cross_bf16.hip",
+    "prefixlm_cross_bwd_bf16.hip",
+    "prefixlm_states_bf16.hip",
     "prefixlm_beams.hip",
     "prefixlm_paged_append.hip",
     "prefixlm_paged_attn.hip",
