@@ -634,14 +634,16 @@ const char* mimir_prefixlm_last_error(void);
  * cu_seqlens_q[s + 1] of q, attend all of its states, rows cu_seqlens_k[s] up to cu_seqlens_k[s + 1] of k / v:
  * out = softmax(softmax_scale q k^T) v.  Both lists hold numseqs + 1 device int32, not decreasing.  A
  * sequence without states gives O = 0, and rows before the first or behind the last sequence O = 0 and
- * zero gradients.  lse2 (may be NULL in the forward) is what the backward needs of it: float32 [Hq, total_q],
- * the base-2 logarithm of the softmax's sum, scale included, -inf without states.  bf16, head_dim
- * 64 or 128, 16-byte aligned rows.  The workspaces need no clearing. */
+ * zero gradients.  What the backward needs of the forward besides out (both may be NULL in a forward alone):
+ * lse2, float32 [Hq, total_q], the base-2 logarithm of the softmax's sum, scale included, -inf without
+ * states, and out_lo, bf16 [total_q, Hq, D] contiguous, round(O - out), the low half of O.  bf16,
+ * head_dim 64 or 128, 16-byte aligned rows.  The workspaces need no clearing. */
 typedef struct MimirCrossParams {
   const void* q;              /* [total_q, Hq, D] */
   const void* k;              /* [total_k, Hkv, D] */
   const void* v;
   void* out;                  /* [total_q, Hq, D]: written by the forward, read by the backward */
+  void* out_lo;
   float* lse2;
   const int32_t* cu_seqlens_q;
   const int32_t* cu_seqlens_k;

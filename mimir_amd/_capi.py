@@ -179,7 +179,7 @@ class PagesParams(ctypes.Structure):
 
 class CrossParams(ctypes.Structure):
     _fields_ = [
-        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse2", _vp), ("cu_seqlens_q", _vp), ("cu_seqlens_k", _vp),
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("out_lo", _vp), ("lse2", _vp), ("cu_seqlens_q", _vp), ("cu_seqlens_k", _vp),
         ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
         ("q_stride_token", _i64), ("q_stride_head", _i64), ("k_stride_token", _i64), ("k_stride_head", _i64),
         ("v_stride_token", _i64), ("v_stride_head", _i64), ("out_stride_token", _i64), ("out_stride_head", _i64),

@@ -45,9 +45,9 @@ def _check_heads(query: Tensor, key: Tensor, value: Tensor, tail: int) -> None:
 
 # ---------------------------------------------------------------- packed sequences
 
-def _params(query, key, value, out, lse2, cu_q, cu_k, scale, backward=(None, None, None, None)):
+def _params(query, key, value, out, out_lo, lse2, cu_q, cu_k, scale, backward=(None, None, None, None)):
     p = _capi.CrossParams()
-    p.q, p.k, p.v, p.out, p.lse2 = (None if t is None else t.data_ptr() for t in (query, key, value, out, lse2))
+    p.q, p.k, p.v, p.out, p.out_lo, p.lse2 = (None if t is None else t.data_ptr() for t in (query, key, value, out, out_lo, lse2))
     p.cu_seqlens_q, p.cu_seqlens_k = cu_q.data_ptr(), cu_k.data_ptr()
     for name, t in zip(("q", "k", "v", "out", "dout", "dq", "dk", "dv"), (query, key, value, out, *backward)):
         if t is not None:
@@ -73,26 +73,28 @@ def _launch(entry: str, p, backward: bool, device) -> None:
 def _forward(query, key, value, cu_q, cu_k, scale, keep: bool):
     query, key, value = map(P._kernel_layout, (query, key, value))
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out_lo = torch.empty_like(out) if keep else None
     lse2 = torch.empty((query.shape[1], query.shape[0]), dtype=torch.float32, device=query.device) if keep else None
-    _launch("mimir_prefixlm_cross_fwd", _params(query, key, value, out, lse2, cu_q, cu_k, scale), False, query.device)
-    return out, lse2
+    _launch("mimir_prefixlm_cross_fwd", _params(query, key, value, out, out_lo, lse2, cu_q, cu_k, scale), False, query.device)
+    return out, out_lo, lse2
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, cu_q, cu_k, scale):
-        out, lse2 = _forward(query, key, value, cu_q, cu_k, scale, True)
-        ctx.save_for_backward(query, key, value, out, lse2, cu_q, cu_k)
+        out, out_lo, lse2 = _forward(query, key, value, cu_q, cu_k, scale, True)
+        ctx.save_for_backward(query, key, value, out, out_lo, lse2, cu_q, cu_k)
         ctx.scale = scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        query, key, value, out, lse2, cu_q, cu_k = ctx.saved_tensors
+        query, key, value, out, out_lo, lse2, cu_q, cu_k = ctx.saved_tensors
         query, key, value, dout = map(P._kernel_layout, (query, key, value, dout))
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key, value)]
-        _launch("mimir_prefixlm_cross_bwd", _params(query, key, value, out, lse2, cu_q, cu_k, ctx.scale, (dout, *grads)), True, query.device)
+        _launch("mimir_prefixlm_cross_bwd", _params(query, key, value, out, out_lo, lse2, cu_q, cu_k, ctx.scale, (dout, *grads)), True,
+                query.device)
         return (*grads, None, None, None)
 
 
@@ -115,7 +117,8 @@ def cross_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Ten
     (its output is then 0); rows before the first or behind the last sequence give 0 and get zero gradients.  Both lists
     (int32 or int64 [numseqs + 1]) must not decrease (checked with ``mimir_amd.set_validate_metadata(True)``).  ``softmax_scale``
     is positive, 1 / sqrt(D) by default.  P and dS are rounded to bf16 for their products, sums are fp32; results do not
-    depend on timing.
+    depend on timing.  For the backward the output's low half is kept (bf16, as large as the output): the sums
+    rowsum(dO * O) that dS is the difference to would carry the output's rounding without it.
     """
     if query.dim() != 3 or key.dim() != 3 or value.dim() != 3:
         raise ValueError("query, key and value must be [tokens, heads, head_dim]")

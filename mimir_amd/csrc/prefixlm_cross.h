@@ -44,9 +44,9 @@ __device__ __forceinline__ SeqSpan seq_span(const SeqTable& t, int s) {
 
 struct CrossArgs {
   const bf16_t *q, *k, *v, *dout;
-  bf16_t *o, *dq, *dk, *dv;
+  bf16_t *o, *o_lo, *dq, *dk, *dv;  // o_lo: contiguous, or NULL
   float* lse2;   // [Hq, Tq]: log2 of the softmax's sum, scale included; -inf for a row without states
-  float* delta;  // [Hq, Tq]: rowsum(dO * O)
+  float* delta;  // [Hq, Tq]: rowsum(dO * O), O with its low half
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, do_st, do_sh, dq_st, dq_sh, dk_st, dk_sh, dv_st, dv_sh;
   int Tq, Hq, Hkv, group;
   const int4* plan_q;  // query tiles: (first row, rows, first state, states), most states first; no rows: padding
@@ -56,9 +56,29 @@ struct CrossArgs {
 };
 
 inline size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
+// Over at most this many states the forward takes P as two bf16 halves in its product: where few terms make a sum,
+// their roundings do not average out, and they would reach dS through delta (dK of 6 sequences over 3 to 20 states: error
+// against 64 bits 1.52 of that of rounding the exact result, with two halves 1.44).
+constexpr int kSplitStates = 64;
+
 constexpr int kCrossTile = 128;  // query rows or states of a tile
 // Entries of a list for any packing of `total` rows into n sequences.
 inline int cross_capacity(int total, int n) { return total > 0 && n > 0 ? (int)(((int64_t)total + kCrossTile - 1) / kCrossTile + n) : 0; }
+
+// A query tile of the list (rows 0: padding) and its head.  Unit = list entry * Hkv + kv head on XCD unit % 8, its
+// query heads at consecutive slots there: they read the same K and V through one L2.
+struct QueryTile {
+  int4 item;
+  int h, hk;
+};
+__device__ __forceinline__ QueryTile query_tile(const CrossArgs& a) {
+  const int xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  const int unit = (slot / a.group) * kXcds + xcd;
+  const int rank = min(unit / a.Hkv, a.cap_q - 1), hk = unit % a.Hkv;
+  QueryTile t = {load_entry(a.plan_q, rank), hk * a.group + slot % a.group, hk};
+  if (unit >= a.cap_q * a.Hkv) t.item.y = 0;
+  return t;
+}
 
 // The launch in front of the tile kernels: the tile lists, the rows outside every sequence (zeroed), and
 // (backward) the delta rows.
@@ -73,7 +93,7 @@ struct CrossPrologue {
   } fill[3];
   int nfill, D;
   float* lse2;            // of the filled query rows: -inf
-  const bf16_t *o, *dout;
+  const bf16_t *o, *o_lo, *dout;
   int64_t o_st, o_sh, do_st, do_sh;
   float* delta;
   int Hq;

@@ -112,11 +112,13 @@ __device__ __forceinline__ void fill_rows(const CrossPrologue& p, const CrossPro
   }
 }
 
-// delta = rowsum(dO * O), D / 8 lanes a row.
+// delta = rowsum(dO * O), D / 8 lanes a row.  O is taken with its low half: dS = P (dP - delta) is a difference
+// whose rounding errors would else be led by O's (gradients of 2 sequences of 300 over 40: error against 64
+// bits 0.0039 of their size without, 0.0024 with it).
 __device__ __forceinline__ void delta_rows(const CrossPrologue& p, int block) {
   const int lanes = p.D / 8, c = threadIdx.x % lanes, per = kPlanThreads / lanes;
   const int64_t rows = (int64_t)p.seqs.Tq * p.Hq;
-  bf16x8 o[kDeltaPasses], g[kDeltaPasses];
+  bf16x8 o[kDeltaPasses], lo[kDeltaPasses], g[kDeltaPasses];
   int t[kDeltaPasses], h[kDeltaPasses];
 #pragma unroll
   for (int i = 0; i < kDeltaPasses; ++i) {
@@ -126,6 +128,7 @@ __device__ __forceinline__ void delta_rows(const CrossPrologue& p, int block) {
     if (t[i] >= 0) {
       // O is read once: dO, which the tile kernels stream next, keeps its place in the caches
       o[i] = __builtin_nontemporal_load((const bf16x8*)&p.o[t[i] * p.o_st + h[i] * p.o_sh + c * 8]);
+      lo[i] = __builtin_nontemporal_load((const bf16x8*)&p.o_lo[((int64_t)t[i] * p.Hq + h[i]) * p.D + c * 8]);
       g[i] = *(const bf16x8*)&p.dout[t[i] * p.do_st + h[i] * p.do_sh + c * 8];
     }
   }
@@ -134,7 +137,7 @@ __device__ __forceinline__ void delta_rows(const CrossPrologue& p, int block) {
     float acc = 0.f;
     if (t[i] >= 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc += (float)o[i][e] * (float)g[i][e];
+      for (int e = 0; e < 8; ++e) acc += ((float)o[i][e] + (float)lo[i][e]) * (float)g[i][e];
     for (int off = lanes / 2; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
     if (t[i] >= 0 && c == 0) p.delta[(int64_t)h[i] * p.seqs.Tq + t[i]] = acc;
   }
@@ -157,31 +160,37 @@ __global__ __launch_bounds__(kPlanThreads) void cross_prologue_kernel(const Prol
 
 // ---------------------------------------------------------------- forward
 
+// Two LDS stages, the same for both bodies of a kernel.
 template <int D>
-__device__ __forceinline__ void cross_fwd_body(const CrossArgs& a) {
-  constexpr int DT = D / 32;  // 32-row tiles of O^T
-  constexpr int KS = D / 16;  // steps of S^T = K Q^T
+struct FwdStages {
+  bf16_t *k0, *v0, *k1, *v1;
+};
+template <int D>
+__device__ __forceinline__ FwdStages<D> fwd_stages() {
   using L = TileLayout<D>;
   __shared__ __attribute__((aligned(16))) bf16_t sK0[L::kElems];
   __shared__ __attribute__((aligned(16))) bf16_t sV0[L::kElems];
   __shared__ __attribute__((aligned(16))) bf16_t sK1[L::kElems];
   __shared__ __attribute__((aligned(16))) bf16_t sV1[L::kElems];
+  return FwdStages<D>{sK0, sV0, sK1, sV1};
+}
+
+// kSplit: P as two bf16 halves in its product.
+template <int D, bool kSplit>
+__device__ __forceinline__ void cross_fwd_body(const CrossArgs& a, const QueryTile& tile) {
+  constexpr int DT = D / 32;  // 32-row tiles of O^T
+  constexpr int KS = D / 16;  // steps of S^T = K Q^T
+  using L = TileLayout<D>;
+  const FwdStages<D> stages = fwd_stages<D>();
+  bf16_t *const sK0 = stages.k0, *const sV0 = stages.v0, *const sK1 = stages.k1, *const sV1 = stages.v1;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31;
   const int hi = lane >> 5;
 
-  // Unit = list entry * Hkv + kv head on XCD unit % 8, its query heads at consecutive slots there: they read the
-  // same K and V through one L2.
-  const int xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
-  const int unit = (slot / a.group) * kXcds + xcd;
-  if (unit >= a.cap_q * a.Hkv) return;
-  const int rank = unit / a.Hkv, hk = unit - rank * a.Hkv;
-  const int h = hk * a.group + slot % a.group;
-  const int4 item = load_entry(a.plan_q, rank);
-  const int rows = item.y, nk = item.w;
-  if (rows == 0) return;  // list padding
+  const int4 item = tile.item;
+  const int h = tile.h, hk = tile.hk, rows = item.y, nk = item.w;
   const int nkt = (nk + kBlockN - 1) / kBlockN;
   const int qa = wave * 32;
   const bool wave_active = qa < rows;
@@ -262,20 +271,23 @@ __device__ __forceinline__ void cross_fwd_body(const CrossArgs& a) {
         lsum += pr;
       }
     l_run += lsum;
-    bf16x8 pf[4];
+    bf16x8 pf[4], pl[kSplit ? 4 : 1];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       f32x8 t;
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] = st[kk >> 1][(kk & 1) * 8 + e];
       pf[kk] = to_bf16x8(t);
+      if constexpr (kSplit) pl[kk] = lo_half(t, pf[kk]);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const bf16_t* vp = &sV[tl.tr_base + kk * 16 * L::kRowElems + dt * 32];
-        oacc[dt] = mfma32(cat8(lds_read_tr16(vp), lds_read_tr16(vp + L::kTrSecond)), pf[kk], oacc[dt]);
+        const bf16x8 vt = cat8(lds_read_tr16(vp), lds_read_tr16(vp + L::kTrSecond));
+        oacc[dt] = mfma32(vt, pf[kk], oacc[dt]);
+        if constexpr (kSplit) oacc[dt] = mfma32(vt, pl[kk], oacc[dt]);
       }
   };
 
@@ -323,14 +335,49 @@ __device__ __forceinline__ void cross_fwd_body(const CrossArgs& a) {
     const bf16x8 ov = *(const bf16x8*)&stage[r * kPitch + u * 8];
     if (qa + r < rows) *(bf16x8*)&obase[(int64_t)r * a.o_st] = ov;
   }
+  if (a.o_lo == nullptr) return;
+  // The low half, another round through the same rows.
+  __asm__ volatile("" ::: "memory");
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+      f32x4 lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float t = oacc[dt][4 * rg + e] * inv;
+        lo[e] = t - round_to(t, bf16_t());
+      }
+      *(bf16x4*)&stage[l32 * kPitch + 32 * dt + 8 * rg + 4 * hi] = __builtin_convertvector(lo, bf16x4);
+    }
+  __asm__ volatile("" ::: "memory");
+  bf16_t* const lbase = a.o_lo + ((int64_t)(item.x + qa) * a.Hq + h) * D + u * 8;
+#pragma unroll
+  for (int j = 0; j < 32 / kRowsPerInst; ++j) {
+    const int r = j * kRowsPerInst + lane / kUnits;
+    const bf16x8 lv = *(const bf16x8*)&stage[r * kPitch + u * 8];
+    if (qa + r < rows) __builtin_nontemporal_store(lv, (bf16x8*)&lbase[(int64_t)r * a.Hq * D]);
+  }
 }
 
+// The split body in a function of its own, which reads its arguments from the kernel's segment: the plain body keeps
+// the registers of a kernel of its own.
+template <int D>
+__device__ __attribute__((noinline)) void cross_fwd_split(uint64_t seg) {
+  const CrossArgs& a = segment_args<CrossArgs>(uniform_segment(seg));
+  cross_fwd_body<D, true>(a, query_tile(a));
+}
 template <int D>
 constexpr int kFwdWaves = D == 64 ? 4 : 2;  // waves per SIMD = workgroups per CU
 template <int D>
 __global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
                           amdgpu_waves_per_eu(kFwdWaves<D>, kFwdWaves<D>))) void cross_fwd_kernel(const CrossArgs a) {
-  cross_fwd_body<D>(a);
+  const QueryTile tile = query_tile(a);
+  if (tile.item.y == 0) return;
+  if (tile.item.w <= kSplitStates)
+    cross_fwd_split<D>(kernel_segment());
+  else
+    cross_fwd_body<D, false>(a, tile);
 }
 template __global__ void cross_fwd_kernel<64>(const CrossArgs);
 template __global__ void cross_fwd_kernel<128>(const CrossArgs);
@@ -418,7 +465,9 @@ int check_cross(const MimirCrossParams* p, bool backward) {
     if (t.st < p->head_dim || t.st >= (1 << 22) || t.sh < 0)
       return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "token strides must be at least head_dim and below 2^22 elements, head strides not negative");
   }
-  if (p->total_q > 0 && backward && p->lse2 == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "lse2 is NULL");
+  if (p->total_q > 0 && backward && (p->lse2 == nullptr || p->out_lo == nullptr))
+    return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "lse2 or out_lo is NULL");
+  if ((uintptr_t)p->out_lo % 16 != 0) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "out_lo must be 16-byte aligned");
   const size_t need = cross_workspace(*p, backward).total;
   if (need > 0 && (p->workspace == nullptr || (uintptr_t)p->workspace % 256 != 0 || p->workspace_bytes < need))
     return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "cross attention needs a workspace of " + std::to_string(need) + " bytes aligned to 256");
@@ -430,6 +479,7 @@ CrossArgs cross_args(const MimirCrossParams& p, const CrossWorkspace& w) {
   a.q = (const bf16_t*)p.q; a.k = (const bf16_t*)p.k; a.v = (const bf16_t*)p.v;
   a.dout = (const bf16_t*)p.dout;
   a.o = (bf16_t*)p.out; a.dq = (bf16_t*)p.dq; a.dk = (bf16_t*)p.dk; a.dv = (bf16_t*)p.dv;
+  a.o_lo = (bf16_t*)p.out_lo;
   a.lse2 = p.lse2;
   a.delta = (float*)((char*)p.workspace + w.delta);
   a.q_st = p.q_stride_token; a.q_sh = p.q_stride_head;
@@ -492,7 +542,7 @@ extern "C" int mimir_prefixlm_cross_bwd(const MimirCrossParams* p, void* stream)
   CrossPrologue pro = cross_prologue(*p, a);
   if (p->total_q > 0) {
     pro.fill[pro.nfill++] = {a.dq, a.dq_st, a.dq_sh, 0, a.Hq};
-    pro.o = a.o; pro.dout = a.dout;
+    pro.o = a.o; pro.o_lo = a.o_lo; pro.dout = a.dout;
     pro.o_st = a.o_st; pro.o_sh = a.o_sh; pro.do_st = a.do_st; pro.do_sh = a.do_sh;
     pro.delta = a.delta;
   }

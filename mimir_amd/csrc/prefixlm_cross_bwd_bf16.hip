@@ -286,14 +286,9 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31;
   const int hi = lane >> 5;
-  // as in the forward: the query heads of a kv head side by side on one XCD
-  const int xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
-  const int unit = (slot / a.group) * kXcds + xcd;
-  if (unit >= a.cap_q * a.Hkv) return;
-  const int rank = unit / a.Hkv, hk = unit - rank * a.Hkv;
-  const int h = hk * a.group + slot % a.group;
-  const int4 item = load_entry(a.plan_q, rank);
-  const int rows = item.y, nk = item.w;
+  const QueryTile tile = query_tile(a);
+  const int4 item = tile.item;
+  const int h = tile.h, hk = tile.hk, rows = item.y, nk = item.w;
   if (rows == 0) return;  // list padding
   const int nkt = (nk + kBlockK - 1) / kBlockK;
   const int qa = wave * 32;

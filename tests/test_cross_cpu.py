@@ -37,7 +37,7 @@ def test_cpu_tensors_are_refused():
 
 def _cross(**kw):
     p = _capi.CrossParams()
-    values = dict(q=4096, k=8192, v=12288, out=16384, lse2=4096, cu_seqlens_q=64, cu_seqlens_k=64, dout=4096, dq=4096, dk=4096, dv=4096, total_q=4, total_k=5,
+    values = dict(q=4096, k=8192, v=12288, out=16384, out_lo=4096, lse2=4096, cu_seqlens_q=64, cu_seqlens_k=64, dout=4096, dq=4096, dk=4096, dv=4096, total_q=4, total_k=5,
                   numseqs=1, num_q_heads=2, num_kv_heads=1, head_dim=64, dtype=_capi.DTYPE_BFLOAT16, softmax_scale=0.125, workspace=256, workspace_bytes=1 << 20)
     for t in ("q", "k", "v", "out", "dout", "dq", "dk", "dv"):
         values[t + "_stride_token"], values[t + "_stride_head"] = 128, 64
@@ -60,7 +60,7 @@ def test_c_cross_refusals(kw, error, backward):
         _capi.raise_for_status(lib, entry(ctypes.byref(_cross(**kw)), None))
 
 
-@pytest.mark.parametrize("kw", [dict(lse2=None), dict(dout=None), dict(dv=None), dict(dk=4104)])
+@pytest.mark.parametrize("kw", [dict(lse2=None), dict(out_lo=None), dict(out_lo=4104), dict(dout=None), dict(dv=None), dict(dk=4104)])
 def test_c_backward_refusals(kw):
     lib = _capi.load()
     with pytest.raises(ValueError):

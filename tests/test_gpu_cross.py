@@ -3,8 +3,9 @@
 With u = 2^-8, half a step of bf16: P is rounded to bf16 for P V (u of sum p |v|, the size), the scores' fp32 sums and exp2
 add below 2^-12 of P for the inputs here (|s| <= 40 in base 2: 40 * 2^-22 and a few roundings), the sums a few 2^-20; the output
 is rounded once (u |out|).  dV: P again (u of sum p |dO|) and its own rounding.  dS is rounded once (u of its size, which
-takes dP and delta by their magnitudes) and holds delta, which comes from the rounded O (u of sum |dO| |out|, within the
-size's delta part) and P's 2^-12: 2.1 u of the size together; dQ and dK then round once (u)."""
+takes dP and delta by their magnitudes) and holds P's 2^-12 and delta, from O with its low half (u^2 of sum |dO| |out|) but
+with P's rounding in O (u of sum |dO| sum p |v|, within the size's delta part): 2.1 u of the size together; dQ and dK then
+round once (u)."""
 
 import math
 
