@@ -10,8 +10,8 @@
 //   * ranks the few elements that reach it and stores the best `count`, in order.
 // Within a row larger logits are larger scores, so this needs no lse.  beam_merge_kernel, a workgroup per
 // request, joins the pieces' sums in 64 bits, forms the scores of the stored elements in 64 bits (beams
-// meet there, whose scores may lie closer than fp32 tells apart), and ranks those that reach the count-th
-// largest of its threads' best.  Masked logits, ended beams and rows of ties need no case of their own but
+// meet there, whose scores may lie closer than fp32 tells apart), takes the lists whose best reaches the
+// count-th largest of 64 groups' best, and ranks what of them does.  Masked logits, ended beams and rows of ties need no case of their own but
 // for more candidates than the lists hold, which fall back to `count` rounds of a maximum.
 //
 // Reordering.  Rows of a group take each other's place, so every row is read before any is written: a
@@ -60,11 +60,33 @@ __device__ __forceinline__ float wave_reduce(float x, F&& f) {
   return x;
 }
 
-template <typename E, int N>
-struct __attribute__((packed, aligned(sizeof(E)))) Loose {  // N elements at any address of theirs
-  E v[N];
+// 16 bytes of logits at any address of theirs.
+struct __attribute__((packed, aligned(2))) Loose2 {
+  i32x4 v;
 };
+struct __attribute__((packed, aligned(4))) Loose4 {
+  i32x4 v;
+};
+__device__ __forceinline__ i32x4 load_loose(const bf16_t* p) { return ((const Loose2*)p)->v; }
+__device__ __forceinline__ i32x4 load_loose(const float* p) { return ((const Loose4*)p)->v; }
+// Element e of a vector as it lies in registers.
+__device__ __forceinline__ float element(const i32x4& v, int e, bf16_t) {
+  return __int_as_float(e % 2 ? v[e / 2] & (int)0xffff0000 : v[e / 2] << 16);
+}
+__device__ __forceinline__ float element(const i32x4& v, int e, float) { return __int_as_float(v[e]); }
+__device__ __forceinline__ void set_element(i32x4& v, int e, bf16_t x) {
+  const int b = __builtin_bit_cast(uint16_t, x);
+  v[e / 2] = e % 2 ? (v[e / 2] & 0xffff) | b << 16 : (v[e / 2] & (int)0xffff0000) | b;
+}
+__device__ __forceinline__ void set_element(i32x4& v, int e, float x) { v[e] = __float_as_int(x); }
 
+// Between its uses the piece stays in registers as it was loaded: unpacked once for all of them, the bf16 kernel
+// took 162 registers and ran three waves a SIMD.
+template <int NV>
+__device__ __forceinline__ void keep_packed(i32x4 (&v)[NV]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) __asm__ volatile("" : "+v"(v[j]));
+}
 template <typename E, int NV>
 __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   constexpr int kVec = 16 / sizeof(E);
@@ -81,27 +103,39 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   if (ended || !(fabsf(score) < INFINITY)) return;  // the merge does not read this row's pieces
   const E* const x = (const E*)a.logits + r * a.l_sr + w * a.l_sw;
   const int first = chunk * (256 * NV * kVec) + tid * kVec;
-  float v[NV][kVec];
+  // Vector j holds the tokens from token_of(j) on; past the end it is the row's last whole vector, and -inf where another holds
+  // the same tokens.
+  auto at_of = [&](int j) __attribute__((always_inline)) { return first + j * 256 * kVec; };
+  auto token_of = [&](int j) __attribute__((always_inline)) { return max(min(at_of(j), a.V - kVec), 0); };
+  const bool last_chunk = chunk == a.chunks - 1;
+  auto mask_vector = [&](int j, i32x4& u) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = first + j * 256 * kVec;
-    if (at + kVec <= a.V) {
-      const Loose<E, kVec> in = *(const Loose<E, kVec>*)(x + at);
+    for (int e = 0; e < kVec; ++e)
+      if (token_of(j) + e < at_of(j) || token_of(j) + e >= a.V) set_element(u, e, (E)-INFINITY);
+  };
+  i32x4 v[NV];
+  if (a.V >= kVec) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[j][e] = (float)in.v[e];
-    } else {
+    for (int j = 0; j < NV; ++j) v[j] = load_loose(x + token_of(j));
+  } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[j][e] = at + e < a.V ? (float)x[at + e] : -INFINITY;
-    }
+    for (int j = 0; j < NV; ++j) v[j] = i32x4{0, 0, 0, 0};
+    for (int e = 0; e < a.V; ++e) set_element(v[0], e, x[e]);
+  }
+  if (last_chunk) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) mask_vector(j, v[j]);
   }
   float most[NV], top = -INFINITY;  // NaN is left out here and comes back in the sum
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     most[j] = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) most[j] = fmaxf(most[j], v[j][e]);
+    for (int e = 0; e < kVec; e += 2) most[j] = fmaxf(fmaxf(most[j], element(v[j], e, E())), element(v[j], e + 1, E()));
     top = fmaxf(top, most[j]);
+    __builtin_amdgcn_sched_barrier(0);
   }
+  keep_packed(v);
   const float wtop = wave_reduce(top, [](float p, float q) { return fmaxf(p, q); });
   // The count-th largest code of the wave's lane maxima: at least `count` elements reach it.
   const uint32_t code = order_code(top);
@@ -119,12 +153,27 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   if (tid == 0) found = 0;
   __syncthreads();
   const float block_top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-  const float base = block_top == -INFINITY ? 0.f : block_top;
+  // exp(x - top) = exp2(x c - top c): one fma with top c rounded, whose rounding (exact by another fma) is taken
+  // back from the sum; c's own is one of x - top, not of x.  Where top c overflows, the difference first.
+  const bool near = fabsf(block_top) < 1e38f;
+  const float base = block_top == -INFINITY ? 0.f : block_top, shift = near ? base * kLog2e : 0.f;
   float part[4] = {0.f, 0.f, 0.f, 0.f};
+  if (near) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) part[e % 4] += fast_exp2((v[j][e] - base) * kLog2e);
+      for (int e = 0; e < kVec; ++e) part[e % 4] += fast_exp2(__builtin_fmaf(element(v[j], e, E()), kLog2e, -shift));
+      __builtin_amdgcn_sched_barrier(0);  // a vector at a time, for few registers
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part[e % 4] += fast_exp2((element(v[j], e, E()) - base) * kLog2e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  keep_packed(v);
   const float sum = wave_reduce((part[0] + part[1]) + (part[2] + part[3]), [](float p, float q) { return p + q; });
   if ((tid & 63) == 0) wave_sum[wave] = sum;
   const float limit = order_value(max(max(wave_code[0], wave_code[1]), max(wave_code[2], wave_code[3])));
@@ -132,14 +181,20 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   for (int j = 0; j < NV; ++j)
     if (most[j] >= limit) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (v[j][e] >= limit && v[j][e] > -INFINITY) {
+      for (int e = 0; e < kVec; ++e) {
+        const float y = element(v[j], e, E());
+        if (y >= limit && y > -INFINITY) {
           const int n = __hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          if (n < kCap) keys[n] = list_key(v[j][e], first + j * 256 * kVec + e);
+          if (n < kCap) keys[n] = list_key(y, token_of(j) + e);
         }
+      }
     }
   __syncthreads();
-  if (tid == 0) a.sums[blockIdx.x] = f32x2{block_top, (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3])};
+  if (tid == 0) {
+    const float total = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    const float over = near ? __builtin_fmaf(base, kLog2e, -shift) : 0.f;  // of the exponents, in base 2
+    a.sums[blockIdx.x] = f32x2{block_top, total - total * (over * kLn2)};
+  }
   uint64_t* const list = a.lists + (int64_t)blockIdx.x * a.K;
   const int n = found;
   if (n <= kCap) {
@@ -152,19 +207,27 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
     for (int i = n + tid; i < a.K; i += 256) list[i] = 0;
     return;
   }
-  // More than that reach it (long runs of equal logits): the best below the last, `count` times.
+  // More than that reach it (long runs of equal logits): the best below the last, `count` times, from memory (to
+  // serve from the registers as well, these rounds took 60 more of them).
   uint64_t last = ~0ull;
   for (int i = 0; i < a.K; ++i) {
     uint64_t best = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (most[j] >= limit) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const uint64_t k = v[j][e] > -INFINITY ? list_key(v[j][e], first + j * 256 * kVec + e) : 0;
-          if (k < last && k > best) best = k;
-        }
+#pragma unroll 1
+    for (int j = 0; j < NV; ++j) {
+      i32x4 u = v[0];  // a row of less than a vector
+      if (a.V >= kVec) {
+        u = load_loose(x + token_of(j));
+        if (last_chunk) mask_vector(j, u);
+      } else if (j > 0) {
+        break;
       }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float y = element(u, e, E());
+        const uint64_t k = y > -INFINITY ? list_key(y, token_of(j) + e) : 0;
+        if (k < last && k > best) best = k;
+      }
+    }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const uint64_t k = __shfl_xor((unsigned long long)best, off, 64);
@@ -189,86 +252,102 @@ __device__ __forceinline__ bool before(const Choice& p, const Choice& q) {
   return p.score > q.score || (p.score == q.score && p.place < q.place);
 }
 
+constexpr int kBeamLanes = 256 / kMaxBeams;  // threads of a beam while sums are joined
+
 __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
   __shared__ double base[kMaxBeams];  // score - lse
   __shared__ int state[kMaxBeams];    // 0: no continuation, 1: by its lists, 2: ended
+  __shared__ float thread_best[256];
+  __shared__ int reaching[kCap];      // lists whose best reaches the limit
   __shared__ double held_score[kCap];
   __shared__ int64_t held_place[kCap];
-  __shared__ double limit_score;
-  __shared__ int64_t limit_place;
-  __shared__ int found;
+  __shared__ int reached, found;
   __shared__ int64_t chosen[kMaxCount];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x;
   const int r = blockIdx.x;
   const Choice none = {-INFINITY, INT64_MAX};
-  for (int w = wave; w < a.W; w += 4) {
-    const float score = a.scores[r * a.s_sr + w * a.s_sw];
-    const bool ended = a.finished != nullptr && a.finished[r * a.f_sr + w * a.f_sw] != 0;
-    const bool live = fabsf(score) < INFINITY;
-    double lse = 0.0;
-    if (live && !ended) {
-      const f32x2* const sums = a.sums + ((int64_t)r * a.W + w) * a.chunks;
-      float m = -INFINITY;
-      for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, sums[c][0]);
-      m = wave_reduce(m, [](float p, float q) { return fmaxf(p, q); });
-      double s = 0.0;
-      for (int c = lane; c < a.chunks; c += 64) {
-        const f32x2 ms = sums[c];
-        s += ms[0] == -INFINITY && ms[1] == 0.f ? 0.0 : (double)ms[1] * exp((double)ms[0] - (double)m);
-      }
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) s += __shfl_xor(s, off, 64);
-      lse = (double)m + log(s);
-    }
-    if (lane == 0) {
-      base[w] = (double)score - lse;
-      state[w] = !live || !(fabs(lse) < INFINITY) ? 0 : ended ? 2 : 1;
-    }
-  }
-  if (tid == 0) found = 0;
-  __syncthreads();
   const int lists = a.W * a.chunks;
   const uint64_t* const all = a.lists + (int64_t)r * lists * a.K;
-  auto choice = [&](int list, int i) __attribute__((always_inline)) {  // entry i of a list, none past its end
+  // The best of the first lists, the scores and the pieces' sums: one round trip for all.
+  constexpr int kHeads = 4;
+  uint64_t head[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) head[i] = all[(int64_t)min(tid + 256 * i, lists - 1) * a.K];
+  {
+    const int w = min(tid / kBeamLanes, a.W - 1), lane = tid % kBeamLanes;
+    const float score = a.scores[r * a.s_sr + w * a.s_sw];
+    const bool ended = a.finished != nullptr && a.finished[r * a.f_sr + w * a.f_sw] != 0;
+    const f32x2* const sums = a.sums + ((int64_t)r * a.W + w) * a.chunks;
+    // not written for a beam that is not read: what stands there then is not used
+    float m = -INFINITY;
+    for (int c = lane; c < a.chunks; c += kBeamLanes) m = fmaxf(m, sums[c][0]);
+#pragma unroll
+    for (int off = 1; off < kBeamLanes; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    double s = 0.0;
+    for (int c = lane; c < a.chunks; c += kBeamLanes) {
+      const f32x2 ms = sums[c];
+      s += ms[0] == -INFINITY && ms[1] == 0.f ? 0.0 : (double)ms[1] * exp((double)ms[0] - (double)m);
+    }
+#pragma unroll
+    for (int off = 1; off < kBeamLanes; off <<= 1) s += __shfl_xor(s, off, 64);
+    const double lse = (double)m + log(s);
+    const bool live = fabsf(score) < INFINITY;
+    if (lane == 0 && tid / kBeamLanes < a.W) {
+      base[w] = ended ? (double)score : (double)score - lse;
+      state[w] = !live ? 0 : ended ? 2 : fabs(lse) < INFINITY ? 1 : 0;
+    }
+  }
+  if (tid == 0) reached = found = 0;
+  __syncthreads();
+  auto choice = [&](int list, int i, uint64_t k) __attribute__((always_inline)) {  // entry i of a list, key k
     const int w = list / a.chunks;
     if (state[w] == 2) return list == w * a.chunks && i == 0 ? Choice{base[w], (int64_t)w * a.V + a.end} : none;
-    if (state[w] == 0) return none;
-    const uint64_t k = all[(int64_t)list * a.K + i];
-    return k == 0 ? none : Choice{base[w] + (double)key_value(k), (int64_t)w * a.V + key_token(k)};
+    if (state[w] == 0 || k == 0) return none;
+    return Choice{base[w] + (double)key_value(k), (int64_t)w * a.V + key_token(k)};
   };
-  Choice best = none;
-  for (int l = tid; l < lists; l += 256) {
-    const Choice c = choice(l, 0);
-    if (before(c, best)) best = c;
-  }
-  // The count-th best of the threads' best (or the last): what comes before none of them is not chosen.
-  held_score[tid] = best.score;
-  held_place[tid] = best.place;
-  if (tid == 0) {
-    limit_score = -INFINITY;
-    limit_place = INT64_MAX - 1;
-  }
+  auto entry = [&](int list, int i) __attribute__((always_inline)) {
+    return choice(list, i, all[(int64_t)list * a.K + i]);
+  };
+  // At least `count` continuations reach the count-th largest of 64 groups' best; rounding to fp32 keeps the order.
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i)
+    if (tid + 256 * i < lists) best = fmaxf(best, (float)choice(tid + 256 * i, 0, head[i]).score);
+  for (int l = tid + 256 * kHeads; l < lists; l += 256) best = fmaxf(best, (float)entry(l, 0).score);
+  thread_best[tid] = best;
   __syncthreads();
-  if (best.place != none.place) {
-    int rank = 0;
-    for (int m = 0; m < 256; ++m) rank += before({held_score[m], held_place[m]}, best);
-    if (rank == a.K - 1) {
-      limit_score = best.score;
-      limit_place = best.place;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = fmaxf(top, thread_best[(tid & 63) + 64 * i]);
+  const uint32_t code = order_code(top);
+  uint32_t reach = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = reach | 1u << bit;
+    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= next)) >= a.K) reach = next;
+  }
+  const float limit = order_value(reach);
+  auto reaches = [&](const Choice& c) __attribute__((always_inline)) { return c.place != none.place && (float)c.score >= limit; };
+  auto note = [&](int list) __attribute__((always_inline)) {
+    const int n = __hip_atomic_fetch_add(&reached, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (n < kCap) reaching[n] = list;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i)
+    if (tid + 256 * i < lists && reaches(choice(tid + 256 * i, 0, head[i]))) note(tid + 256 * i);
+  for (int l = tid + 256 * kHeads; l < lists; l += 256)
+    if (reaches(entry(l, 0))) note(l);
+  __syncthreads();
+  const int pairs = min(reached, kCap) * a.K;
+  for (int p = tid; p < pairs; p += 256) {
+    const Choice c = entry(reaching[p / a.K], p % a.K);
+    if (!reaches(c)) continue;
+    const int n = __hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (n < kCap) {
+      held_score[n] = c.score;
+      held_place[n] = c.place;
     }
   }
-  __syncthreads();
-  const Choice limit = {limit_score, limit_place};
-  for (int l = tid; l < lists; l += 256)
-    for (int i = 0; i < a.K; ++i) {
-      const Choice c = choice(l, i);
-      if (c.place == none.place || before(limit, c)) break;
-      const int n = __hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      if (n < kCap) {
-        held_score[n] = c.score;
-        held_place[n] = c.place;
-      }
-    }
   __syncthreads();
   auto put = [&](int i, double score, int64_t place) __attribute__((always_inline)) {
     const int w = (int)(place / a.V), token = (int)(place - (int64_t)w * a.V);
@@ -281,7 +360,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
       a.out_finished[at] = (a.finished != nullptr && a.finished[r * a.f_sr + w * a.f_sw] != 0) || token == a.end;
   };
   int n = found;
-  if (n <= kCap) {
+  if (n <= kCap && reached <= kCap) {
     for (int i = tid; i < n; i += 256) {
       const Choice c = {held_score[i], held_place[i]};
       int rank = 0;
@@ -293,26 +372,26 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
     // More than that: the best after the last, `count` times.
     Choice last = {INFINITY, -1};
     for (n = 0; n < a.K; ++n) {
-      best = none;
+      Choice next = none;
       for (int l = tid; l < lists; l += 256)
         for (int i = 0; i < a.K; ++i) {
-          const Choice c = choice(l, i);
+          const Choice c = entry(l, i);
           if (c.place == none.place) break;
           if (!before(last, c)) continue;
-          if (before(c, best)) best = c;
+          if (before(c, next)) next = c;
           break;
         }
       __syncthreads();  // the last round's are read
-      held_score[tid] = best.score;
-      held_place[tid] = best.place;
+      held_score[tid] = next.score;
+      held_place[tid] = next.place;
       __syncthreads();
       for (int m = 0; m < 256; ++m) {
         const Choice c = {held_score[m], held_place[m]};
-        if (before(c, best)) best = c;
+        if (before(c, next)) next = c;
       }
-      if (best.place == none.place) break;
-      if (tid == 0) put(n, best.score, best.place);
-      last = best;
+      if (next.place == none.place) break;
+      if (tid == 0) put(n, next.score, next.place);
+      last = next;
     }
   }
   if (n >= a.K) return;
@@ -350,35 +429,42 @@ __device__ __forceinline__ int source_of(const ReorderArgs& a, int r0, int w) {
   return s >= 0 && s < a.group ? (int)s : w;
 }
 
+// Bytes of a row that a workgroup moves: 16 loads of 16 bytes a thread over the rows of a group.
+constexpr int reorder_chunk(int group) { return 4096 * (group <= 4 ? 4 : group <= 8 ? 2 : 1); }
+
 template <int kGroup>
 __global__ __launch_bounds__(256) void reorder_rows_kernel(const ReorderArgs a) {
-  __shared__ int from[kGroup];
-  __shared__ int64_t bytes[kGroup];  // that row w takes from its source, 0: it stays
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, w = tid & 63;
   const int g = blockIdx.x / a.chunks, chunk = blockIdx.x - g * a.chunks;
   const int r0 = g * a.group;
-  if (tid < kGroup) {
-    int s = tid;
-    int64_t n = 0;
-    if (tid < a.group) {
-      s = source_of(a, r0, tid);
-      const int64_t length = index_at(a.lengths, r0 + s, a.idx64);
-      n = s == tid || length < 0 ? 0 : min(length, (int64_t)a.max_length) * a.position_bytes;
-    }
-    from[tid] = s;
-    bytes[tid] = n;
+  int from = w, take = 0;  // lane w: the source of row w, and the positions it takes from it (0: it stays)
+  if (w < a.group) {
+    from = source_of(a, r0, w);
+    const int64_t length = index_at(a.lengths, r0 + from, a.idx64);
+    take = from == w || length < 0 ? 0 : (int)min(length, (int64_t)a.max_length);
   }
-  __syncthreads();
-  const int64_t at = ((int64_t)chunk * 256 + tid) * 16;
-  char* const base = a.data[blockIdx.y] + r0 * a.stride[blockIdx.y] + at;
-  const int64_t stride = a.stride[blockIdx.y];
-  i32x4 v[kGroup];
+  // Whole buffers of what a row takes of this chunk, so that no load waits for another's condition: past
+  // the end nothing is read, and stores are dropped.
+  const int64_t first = (int64_t)chunk * reorder_chunk(kGroup), stride = a.stride[blockIdx.y];
+  char* const base = a.data[blockIdx.y] + r0 * stride + first;
+  auto rest = [&](int i) __attribute__((always_inline)) {
+    const int64_t n = __builtin_amdgcn_readlane(take, i) * a.position_bytes - first;
+    return (uint32_t)max(min(n, (int64_t)reorder_chunk(kGroup)), (int64_t)0);
+  };
+  constexpr int kVecs = reorder_chunk(kGroup) / 4096;
+  i32x4 v[kGroup][kVecs];
 #pragma unroll
-  for (int w = 0; w < kGroup; ++w)
-    if (at < bytes[w]) v[w] = *(const i32x4*)(base + from[w] * stride);
+  for (int i = 0; i < kGroup; ++i) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + __builtin_amdgcn_readlane(from, i) * stride, rest(i));
 #pragma unroll
-  for (int w = 0; w < kGroup; ++w)
-    if (at < bytes[w]) *(i32x4*)(base + w * stride) = v[w];
+    for (int j = 0; j < kVecs; ++j) v[i][j] = buf_load16(r, (uint32_t)(j * 4096 + tid * 16));
+  }
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base + i * stride, rest(i));
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) __builtin_amdgcn_raw_buffer_store_b128(v[i][j], r, j * 4096 + tid * 16, 0, 0);
+  }
 }
 
 // A wave per group: every lane reads its source's length before one writes.
@@ -518,7 +604,7 @@ extern "C" int mimir_prefixlm_reorder_rows(const MimirReorderParams* p, void* st
   a.position_bytes = p->position_bytes;
   a.rows = p->rows; a.group = p->group; a.max_length = p->max_length;
   a.idx64 = p->index_int64 != 0; a.src64 = p->source_int64 != 0;
-  const int64_t groups = p->rows / p->group, chunks = (row_bytes + 4095) / 4096;
+  const int64_t groups = p->rows / p->group, chunk_bytes = reorder_chunk(p->group), chunks = (row_bytes + chunk_bytes - 1) / chunk_bytes;
   if (groups * chunks > kMaxGroups || chunks > 0x7fffffff) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many positions for one launch");
   a.chunks = (int)chunks;
   const hipStream_t s = (hipStream_t)stream;
