@@ -378,7 +378,7 @@ class _GeneralPath:
     def fwd(*args):
         return None
 
-    bwd = rope = cache_attn = rotary = paged_attn = pages = fwd
+    bwd = rope = cache_attn = rotary = paged_attn = pages = norm_rotary = cross_attention = states = select = reorder = fwd
 
 
 def _load_host():
@@ -410,8 +410,8 @@ _host = None
 def host():
     """The native host calls (csrc/host_calls.cpp), bound to the library.
 
-    ``fwd`` / ``bwd`` / ``rope`` / ``cache_attn`` / ``rotary`` / ``paged_attn`` / ``pages`` check,
-    allocate and launch a well-formed call and return None for any other, which then takes the general path.
+    ``fwd`` / ``bwd`` / ``rope`` / ``cache_attn`` / ``rotary`` / ``paged_attn`` / ``pages`` / ``norm_rotary`` /
+    ``cross_attention`` / ``states`` / ``select`` / ``reorder`` check, allocate and launch a well-formed call and return None for any other, which then takes the general path.
     Where the module is not built, or built for another torch or Python, they serve
     no call.  ImportError if the library itself is not built."""
     global _host

@@ -47,6 +47,11 @@ def select_beams(logits: Tensor, scores: Tensor, count: Optional[int] = None, *,
     a beam whose logits hold NaN or +inf; where fewer than ``count`` continuations are left, the rest have score -inf.
     Scores are compared in 64 bits and rounded once.  W up to 32, ``count`` up to 64.
     """
+    if logits.is_cuda and logits.dim() == 3:
+        out = _capi.host().select(logits, scores, logits.shape[1] if count is None else count, finished, -1 if end_token is None else end_token,
+                                  P._stream(logits.device))
+        if out is not None:
+            return BeamSelection(*out)
     if logits.dim() != 3:
         raise ValueError(f"logits must be [requests, beams, vocab], got shape {tuple(logits.shape)}")
     if logits.dtype not in _DTYPES:
@@ -107,6 +112,8 @@ def reorder_rows(caches: Union[Cache, Sequence[Cache]], lengths: Tensor, source:
     touched.  ``lengths`` has one entry per row of ``source``; caches may have more rows.  W up to 32.
     """
     caches = [caches] if isinstance(caches, Cache) else list(caches)
+    if lengths.is_cuda and not P._validate_metadata and _capi.host().reorder(caches, lengths, source, P._stream(lengths.device)):
+        return
     if source.dim() != 2 or source.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"source must be int32 or int64 [requests, beams], got {tuple(source.shape)} {source.dtype}")
     rows, group = source.numel(), source.shape[1]

@@ -27,7 +27,7 @@ from .cache import Cache
 
 
 def _scale(softmax_scale: Optional[float], d: int) -> float:
-    return 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    return 1.0 / math.sqrt(max(d, 1)) if softmax_scale is None else float(softmax_scale)
 
 
 def _check_heads(query: Tensor, key: Tensor, value: Tensor, tail: int) -> None:
@@ -120,6 +120,11 @@ def cross_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Ten
     depend on timing.  For the backward the output's low half is kept (bf16, as large as the output): the sums
     rowsum(dO * O) that dS is the difference to would carry the output's rounding without it.
     """
+    if query.is_cuda and query.dim() == 3 and not P._validate_metadata:
+        out = _capi.host().cross_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, _scale(softmax_scale, query.shape[2]),
+                                           P._stream(query.device))
+        if out is not None:
+            return out
     if query.dim() != 3 or key.dim() != 3 or value.dim() != 3:
         raise ValueError("query, key and value must be [tokens, heads, head_dim]")
     _check_heads(query, key, value, 3)
@@ -147,6 +152,10 @@ def attention_to_states(query: Tensor, states: Cache, state_lengths: Tensor, sta
     and every query sees all states of its request.  A request whose row lies outside the cache, or is empty, gets 0 (with
     ``mimir_amd.set_validate_metadata(True)`` the first is an IndexError).  Returns [B, S, Hq, D]; not differentiable.
     """
+    if query.is_cuda and query.dim() == 4 and not P._validate_metadata:
+        out = _capi.host().states(query, *states, state_lengths, state_rows, _scale(softmax_scale, query.shape[3]), P._stream(query.device))
+        if out is not None:
+            return out
     if query.dim() != 4 or states.keys.dim() != 4 or states.values.dim() != 4:
         raise ValueError("query must be [batch, tokens, heads, head_dim], states [rows, positions, heads, head_dim]")
     _check_heads(query, states.keys, states.values, 4)

@@ -1,7 +1,8 @@
 // The host side of the common calls in native code: argument checks, output
 // allocation, the parameter struct and the C-ABI launch of the forward, the
 // backward, RoPE and the KV-cache attention, and of rotary positions (with their
-// gradient), the paged attention and its pages' bookkeeping.
+// gradient), the paged attention and its pages' bookkeeping, normed rotary heads and cross
+// attention (with their gradients), attention to cached states, and beam search.
 //
 // Through ctypes these cost 24 us (forward), 32 us (backward) and 17 us (decode) of
 // Python per call, and the backward pays about twice that in a training step: the
@@ -24,9 +25,11 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/mimir_prefixlm.h"
@@ -54,6 +57,17 @@ struct Library {
   decltype(&mimir_prefixlm_pages_compact) pages_compact = nullptr;
   decltype(&mimir_prefixlm_pages_release) pages_release = nullptr;
   decltype(&mimir_prefixlm_pages_reserve) pages_reserve = nullptr;
+  decltype(&mimir_prefixlm_norm_rotary) norm_rotary = nullptr;
+  decltype(&mimir_prefixlm_norm_rotary_bwd) norm_rotary_bwd = nullptr;
+  decltype(&mimir_prefixlm_norm_rotary_workspace_bytes) norm_rotary_workspace = nullptr;
+  decltype(&mimir_prefixlm_cross_fwd) cross_fwd = nullptr;
+  decltype(&mimir_prefixlm_cross_bwd) cross_bwd = nullptr;
+  decltype(&mimir_prefixlm_cross_workspace_bytes) cross_workspace = nullptr;
+  decltype(&mimir_prefixlm_states_attn) states_attn = nullptr;
+  decltype(&mimir_prefixlm_states_workspace_bytes) states_workspace = nullptr;
+  decltype(&mimir_prefixlm_beam_select) beam_select = nullptr;
+  decltype(&mimir_prefixlm_beam_select_workspace_bytes) beam_select_workspace = nullptr;
+  decltype(&mimir_prefixlm_reorder_rows) reorder_rows = nullptr;
   c10::DeviceType device = c10::DeviceType::CUDA;  // of the tensors it takes
 } lib;
 
@@ -439,7 +453,7 @@ bool rotary_operand(const at::Tensor& t, const at::Tensor& q) {
   return t.numel() > 0 && t.size(n - 2) <= 0x7fffffff;
 }
 bool rotary_served(const at::Tensor& q, const at::Tensor* k, const Rotary& r) {
-  if (lib.rotary == nullptr || !on_device(q) || (q.dim() != 3 && q.dim() != 4) ||
+  if (!on_device(q) || (q.dim() != 3 && q.dim() != 4) ||
       (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kFloat) || !rotary_operand(q, q) || (k != nullptr && !rotary_operand(*k, q)))
     return false;
   const int64_t n = q.dim(), d = q.size(n - 1), S = q.size(n - 3);
@@ -546,6 +560,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 // rotary(query, key or None, positions, turns, amplitude, interleaved, inverse, inplace, stream) -> (query, key or None)
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 9, [&](bool& raised) -> PyObject* {
+    NEED(lib.rotary != nullptr);
     TENSOR(q, a[0]);
     const at::Tensor* k = nullptr;
     if (!is_none(a[1])) NEED((k = tensor(a[1])) != nullptr);
@@ -755,6 +770,401 @@ PyObject* py_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------- shared by the calls below
+
+at::Tensor bytes(size_t n, const at::Tensor& like) { return empty({(int64_t)n}, like, at::kByte); }
+
+// A C-ABI call inside an autograd function: a HIP error is a LaunchError, a refusal (nothing launched) another.
+template <typename P>
+void run_or_throw(int (*entry)(const P*, void*), const P& p, void* s) {
+  int status;
+  std::string message;  // (thread-local in the library)
+  {
+    const Unlocked unlocked;
+    status = entry(&p, s);
+    if (status != MIMIR_OK) message = lib.last_error();
+  }
+  if (status == MIMIR_ERR_HIP) throw LaunchError(message);
+  TORCH_CHECK(status == MIMIR_OK, message);
+}
+
+// Gradients from a backward without one of its own: under create_graph they raise when differentiated.
+torch::autograd::variable_list once(torch::autograd::variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list given, out(grads.size());
+  std::vector<size_t> at;
+  for (size_t i = 0; i < grads.size(); ++i)
+    if (grads[i].defined()) {
+      given.push_back(grads[i].detach().requires_grad_(true));
+      at.push_back(i);
+    }
+  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once only", (int64_t)given.size());
+  const auto marked = (*error)(std::move(given));
+  for (size_t i = 0; i < at.size(); ++i) out[at[i]] = marked[i];
+  return out;
+}
+
+// ---------------------------------------------------------------- normed rotary heads
+
+struct NormRotary {
+  at::Tensor q, k, qw, kw, positions, turns;  // k, qw, kw may be undefined
+  double amplitude, eps;
+  bool interleaved;
+};
+
+MimirNormRotaryParams norm_params(const NormRotary& r, const at::Tensor& qo, const at::Tensor& ko, const at::Tensor& dq, const at::Tensor& dk) {
+  const int64_t n = r.q.dim();
+  MimirNormRotaryParams p = {};
+  auto strides = [n](const at::Tensor& t, int64_t& sb, int64_t& st, int64_t& sh) {
+    if (t.defined()) sb = n == 4 ? t.stride(0) : 0, st = t.stride(n - 3), sh = t.stride(n - 2);
+  };
+  auto read = [](const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; };
+  p.q = read(r.q), p.k = read(r.k), p.dq = read(dq), p.dk = read(dk), p.q_weight = read(r.qw), p.k_weight = read(r.kw);
+  p.q_out = qo.mutable_data_ptr(), p.k_out = ko.defined() ? ko.mutable_data_ptr() : nullptr;
+  strides(r.q, p.q_stride_batch, p.q_stride_token, p.q_stride_head);
+  strides(r.k, p.k_stride_batch, p.k_stride_token, p.k_stride_head);
+  strides(qo, p.q_out_stride_batch, p.q_out_stride_token, p.q_out_stride_head);
+  strides(ko, p.k_out_stride_batch, p.k_out_stride_token, p.k_out_stride_head);
+  strides(dq, p.dq_stride_batch, p.dq_stride_token, p.dq_stride_head);
+  strides(dk, p.dk_stride_batch, p.dk_stride_token, p.dk_stride_head);
+  p.turns = r.turns.const_data_ptr<int64_t>(), p.positions = r.positions.const_data_ptr();
+  p.positions_stride_batch = r.positions.dim() == 2 ? r.positions.stride(0) : 0;
+  p.positions_stride_token = r.positions.stride(r.positions.dim() - 1);
+  p.batch = n == 4 ? (int32_t)r.q.size(0) : 1, p.seqlen = (int32_t)r.q.size(n - 3);
+  p.num_q_heads = (int32_t)r.q.size(n - 2), p.num_kv_heads = r.k.defined() ? (int32_t)r.k.size(n - 2) : 0;
+  p.head_dim = (int32_t)r.q.size(n - 1), p.rotary_dim = (int32_t)(2 * r.turns.size(0));
+  p.interleaved = r.interleaved, p.amplitude = (float)r.amplitude, p.eps = (float)r.eps;
+  auto code = [](at::ScalarType t) { return t == at::kBFloat16 ? MIMIR_DTYPE_BFLOAT16 : MIMIR_DTYPE_FLOAT32; };
+  p.dtype = code(r.q.scalar_type());
+  p.weight_dtype = r.qw.defined() ? code(r.qw.scalar_type()) : r.kw.defined() ? code(r.kw.scalar_type()) : p.dtype;
+  p.index_int64 = r.positions.scalar_type() == at::kLong;
+  return p;
+}
+
+at::Tensor like(const at::Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : at::Tensor(); }
+
+struct NormRotaryFunction : torch::autograd::Function<NormRotaryFunction> {
+  using Given = std::optional<at::Tensor>;
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const Given& k, const Given& qw,
+                                                const Given& kw, const at::Tensor& positions, const at::Tensor& turns, double amplitude,
+                                                bool interleaved, double eps, int64_t s) {
+    const at::Tensor none;
+    const NormRotary r = {q, k.value_or(none), qw.value_or(none), kw.value_or(none), positions, turns, amplitude, eps, interleaved};
+    ctx->save_for_backward({r.q, r.k, r.qw, r.kw, positions, turns});
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    const at::Tensor qo = like(r.q), ko = like(r.k);
+    const c10::DeviceGuard guard(q.device());
+    run_or_throw(lib.norm_rotary, norm_params(r, qo, ko, none, none), (void*)s);
+    if (!k.has_value()) return {qo};
+    return {qo, ko};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const NormRotary r = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["amplitude"].toDouble(),
+                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+    torch::autograd::variable_list out(10);
+    auto unit = [](const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); };
+    const at::Tensor dq = unit(grads[0]), dk = r.k.defined() ? unit(grads[1]) : at::Tensor();
+    out[0] = like(r.q), out[1] = like(r.k);
+    size_t edge = r.k.defined() ? 2 : 1;  // an argument that is not given has none
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor& w = i == 0 ? r.qw : r.kw;
+      if (w.defined() && ctx->needs_input_grad(edge++)) out[2 + i] = like(w);
+    }
+    MimirNormRotaryParams p = norm_params(r, out[0], out[1], dq, dk);
+    p.dq_weight = out[2].defined() ? out[2].mutable_data_ptr() : nullptr;
+    p.dk_weight = out[3].defined() ? out[3].mutable_data_ptr() : nullptr;
+    p.workspace_bytes = lib.norm_rotary_workspace(&p);
+    const at::Tensor ws = bytes(p.workspace_bytes, r.q);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(r.q.device());
+    run_or_throw(lib.norm_rotary_bwd, p, stream_of(r.q));
+    return once(out, "norm_rotary");
+  }
+};
+
+// norm_rotary(query, key or None, positions, turns, amplitude, interleaved, query_weight or None, key_weight or None, eps, stream)
+//   -> (query, key or None)
+PyObject* py_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 10, [&](bool& raised) -> PyObject* {
+    NEED(lib.norm_rotary != nullptr && lib.norm_rotary_bwd != nullptr && lib.norm_rotary_workspace != nullptr);
+    TENSOR(q, a[0]);
+    const at::Tensor* given[3] = {nullptr, nullptr, nullptr};  // key, weights
+    const int at[3] = {1, 6, 7};
+    for (int i = 0; i < 3; ++i)
+      if (!is_none(a[at[i]])) NEED((given[i] = tensor(a[at[i]])) != nullptr);
+    const at::Tensor* const k = given[0];
+    TENSOR(positions, a[2]);
+    TENSOR(turns, a[3]);
+    const Rotary checked = {positions, turns, PyFloat_AsDouble(a[4]), truth(a[5]), false};
+    const double eps = PyFloat_AsDouble(a[8]);
+    NEED(PyErr_Occurred() == nullptr && eps >= 0.0 && eps < 1e30 && rotary_served(q, k, checked));
+    NEED(given[2] == nullptr || k != nullptr);
+    for (int i = 1; i < 3; ++i) {
+      if (given[i] == nullptr) continue;
+      const at::Tensor& w = *given[i];
+      NEED(w.dim() == 1 && w.size(0) == q.size(q.dim() - 1) && w.device() == q.device() && (w.size(0) == 1 || w.stride(0) == 1) &&
+           (w.scalar_type() == at::kFloat || w.scalar_type() == q.scalar_type()) &&
+           (given[1] == nullptr || w.scalar_type() == given[1]->scalar_type()));
+    }
+    bool grad = false;
+    for (const at::Tensor* t : {&q, k, given[1], given[2]}) {
+      if (t == nullptr) continue;
+      NEED(!t->_fw_grad(0).defined());  // forward mode: the general path refuses
+      grad = grad || t->requires_grad();
+    }
+    auto or_none = [](const at::Tensor* t) { return t != nullptr ? std::optional<at::Tensor>(*t) : std::nullopt; };
+    auto or_undefined = [](const at::Tensor* t) { return t != nullptr ? *t : at::Tensor(); };
+    at::Tensor qo, ko;
+    if (grad && at::GradMode::is_enabled()) {
+      NEED(current_stream != nullptr);
+      const auto out = NormRotaryFunction::apply(q, or_none(k), or_none(given[1]), or_none(given[2]), positions, turns, checked.amplitude,
+                                                 checked.interleaved, eps, (int64_t)stream(a[9]));
+      qo = out[0];
+      if (k != nullptr) ko = out[1];
+    } else {
+      const NormRotary r = {q, or_undefined(k), or_undefined(given[1]), or_undefined(given[2]), positions, turns, checked.amplitude, eps,
+                            checked.interleaved};
+      qo = like(r.q), ko = like(r.k);
+      const c10::DeviceGuard guard(q.device());
+      NEED(launch(lib.norm_rotary, norm_params(r, qo, ko, at::Tensor(), at::Tensor()), stream(a[9]), raised));
+    }
+    PyObject* second = k != nullptr ? THPVariable_Wrap(ko) : Py_NewRef(Py_None);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(qo), second);
+  });
+}
+
+// ---------------------------------------------------------------- cross attention
+
+MimirCrossParams cross_params(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                              double scale, const at::Tensor& out) {
+  MimirCrossParams p = {};
+  p.q = q.const_data_ptr(), p.k = k.const_data_ptr(), p.v = v.const_data_ptr(), p.out = out.mutable_data_ptr();
+  STRIDES(p, q, q), STRIDES(p, k, k), STRIDES(p, v, v), STRIDES(p, out, out);
+  p.cu_seqlens_q = cu_q.const_data_ptr<int32_t>(), p.cu_seqlens_k = cu_k.const_data_ptr<int32_t>();
+  p.total_q = (int32_t)q.size(0), p.total_k = (int32_t)k.size(0), p.numseqs = (int32_t)(cu_q.size(0) - 1);
+  p.num_q_heads = (int32_t)q.size(1), p.num_kv_heads = (int32_t)k.size(1), p.head_dim = (int32_t)q.size(2);
+  p.dtype = MIMIR_DTYPE_BFLOAT16;
+  p.softmax_scale = (float)scale;
+  return p;
+}
+
+struct CrossFunction : torch::autograd::Function<CrossFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& cu_q, const at::Tensor& cu_k, double scale, int64_t s) {
+    const at::Tensor out = like(q), out_lo = like(q), lse2 = empty({q.size(1), q.size(0)}, q, at::kFloat);
+    MimirCrossParams p = cross_params(q, k, v, cu_q, cu_k, scale, out);
+    p.out_lo = out_lo.mutable_data_ptr(), p.lse2 = lse2.mutable_data_ptr<float>();
+    p.workspace_bytes = lib.cross_workspace(&p, 0);
+    const at::Tensor ws = bytes(p.workspace_bytes, q);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(q.device());
+    run_or_throw(lib.cross_fwd, p, (void*)s);
+    ctx->save_for_backward({q, k, v, cu_q, cu_k, out, out_lo, lse2});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const at::Tensor &q = t[0], &k = t[1], &v = t[2];
+    at::Tensor dout = grads[0];
+    if (!in_place(dout, q)) dout = dout.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor dq = like(q), dk = like(k), dv = like(v);
+    MimirCrossParams p = cross_params(q, k, v, t[3], t[4], ctx->saved_data["scale"].toDouble(), t[5]);
+    p.out_lo = t[6].mutable_data_ptr(), p.lse2 = t[7].mutable_data_ptr<float>();
+    p.dout = dout.const_data_ptr(), p.dq = dq.mutable_data_ptr(), p.dk = dk.mutable_data_ptr(), p.dv = dv.mutable_data_ptr();
+    STRIDES(p, dout, dout), STRIDES(p, dq, dq), STRIDES(p, dk, dk), STRIDES(p, dv, dv);
+    p.workspace_bytes = lib.cross_workspace(&p, 1);
+    const at::Tensor ws = bytes(p.workspace_bytes, q);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(q.device());
+    run_or_throw(lib.cross_bwd, p, stream_of(q));
+    torch::autograd::variable_list out(7);
+    out[0] = dq, out[1] = dk, out[2] = dv;
+    return once(out, "cross_attention");
+  }
+};
+
+// cross_attention(query, key, value, cu_seqlens_q, cu_seqlens_k, softmax_scale, stream) -> out
+PyObject* py_cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 7, [&](bool& raised) -> PyObject* {
+    NEED(lib.cross_fwd != nullptr && lib.cross_bwd != nullptr && lib.cross_workspace != nullptr);
+    TENSOR(q, a[0]);
+    TENSOR(k, a[1]);
+    TENSOR(v, a[2]);
+    TENSOR(cu_q, a[3]);
+    TENSOR(cu_k, a[4]);
+    NEED(on_device(q) && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && k.dim() == 3 && q.size(0) > 0 && k.size(0) > 0 &&
+         q.size(0) <= 0x7fffffff && k.size(0) <= 0x7fffffff && q.size(1) > 0 && k.size(1) > 0 && q.size(1) <= 0x7fffffff);
+    NEED(q.size(2) == k.size(2) && shaped(v, k.size(0), k.size(1), k.size(2)) && in_place(q, q) && in_place(k, q) && in_place(v, q));
+    for (const at::Tensor* t : {&cu_q, &cu_k})
+      NEED(t->dim() == 1 && t->scalar_type() == at::kInt && t->device() == q.device() && t->is_contiguous() && t->size(0) == cu_q.size(0));
+    NEED(cu_q.size(0) >= 2 && cu_q.size(0) <= 0x7fffffff);
+    const double scale = PyFloat_AsDouble(a[5]);
+    NEED(PyErr_Occurred() == nullptr);
+    bool grad = false;
+    for (const at::Tensor* t : {&q, &k, &v}) {
+      NEED(!t->_fw_grad(0).defined());  // forward mode: the general path refuses
+      grad = grad || t->requires_grad();
+    }
+    if (grad && at::GradMode::is_enabled()) {
+      NEED(current_stream != nullptr);
+      return THPVariable_Wrap(CrossFunction::apply(q, k, v, cu_q, cu_k, scale, (int64_t)stream(a[6])));
+    }
+    const at::Tensor out = like(q);
+    MimirCrossParams p = cross_params(q, k, v, cu_q, cu_k, scale, out);
+    p.workspace_bytes = lib.cross_workspace(&p, 0);
+    const at::Tensor ws = bytes(p.workspace_bytes, q);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(q.device());
+    NEED(launch(lib.cross_fwd, p, stream(a[6]), raised));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// A vector of row numbers or lengths that is read as it is.
+bool index_vector(const at::Tensor& t, const at::Tensor& like) {
+  return t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.device() == like.device() && t.is_contiguous();
+}
+
+// states(query, keys, values, lengths, rows or None, softmax_scale, stream) -> out
+PyObject* py_states(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 7, [&](bool& raised) -> PyObject* {
+    NEED(lib.states_attn != nullptr && lib.states_workspace != nullptr);
+    TENSOR(q, a[0]);
+    TENSOR(k, a[1]);
+    TENSOR(v, a[2]);
+    TENSOR(lengths, a[3]);
+    const at::Tensor* rows = nullptr;
+    if (!is_none(a[4])) NEED((rows = tensor(a[4])) != nullptr);
+    NEED(on_device(q) && q.scalar_type() == at::kBFloat16 && q.dim() == 4 && k.dim() == 4 && q.numel() > 0 && k.numel() > 0 && v.sizes() == k.sizes());
+    const int64_t B = q.size(0), S = q.size(1), hq = q.size(2), d = q.size(3), pool = k.size(0), length = k.size(1);
+    NEED(in_place(q, q) && in_place(k, q) && in_place(v, q) && k.size(3) == d && (B == 1 || q.stride(0) == S * q.stride(1)));
+    NEED(index_vector(lengths, q) && lengths.size(0) == pool && (rows == nullptr || index_vector(*rows, q)));
+    const int64_t requests = rows != nullptr ? rows->size(0) : pool;
+    NEED(requests > 0 && B % requests == 0 && B * S <= 0x7fffffff && pool <= 0x7fffffff && length <= 0x7fffffff && hq <= 0x7fffffff);
+    if (at::GradMode::is_enabled())
+      for (const at::Tensor* t : {&q, &k, &v}) NEED(!t->requires_grad());
+    const at::Tensor out = empty({B, S, hq, d}, q, at::kBFloat16);
+    MimirStatesParams p = {};
+    p.q = q.const_data_ptr(), p.keys = k.const_data_ptr(), p.values = v.const_data_ptr(), p.out = out.mutable_data_ptr();
+    p.lengths = lengths.const_data_ptr(), p.rows = rows != nullptr ? rows->const_data_ptr() : nullptr;
+    // a dim of one entry has no stride to speak of
+    auto step = [](const at::Tensor& t, int i, int64_t one) { return t.size(i) == 1 ? one : t.stride(i); };
+    p.q_stride_token = S > 1 ? q.stride(1) : step(q, 0, hq * d), p.q_stride_head = step(q, 2, 0);
+    p.k_stride_row = step(k, 0, 0), p.k_stride_token = step(k, 1, d), p.k_stride_head = step(k, 2, 0);
+    p.v_stride_row = step(v, 0, 0), p.v_stride_token = step(v, 1, d), p.v_stride_head = step(v, 2, 0);
+    p.out_stride_token = hq * d, p.out_stride_head = d;
+    p.requests = (int32_t)requests, p.seq_tokens = (int32_t)(B / requests * S), p.cache_rows = (int32_t)pool, p.cache_len = (int32_t)length;
+    p.num_q_heads = (int32_t)hq, p.num_kv_heads = (int32_t)k.size(2), p.head_dim = (int32_t)d;
+    p.dtype = MIMIR_DTYPE_BFLOAT16;
+    p.lengths_int64 = lengths.scalar_type() == at::kLong, p.rows_int64 = rows != nullptr && rows->scalar_type() == at::kLong;
+    p.softmax_scale = (float)PyFloat_AsDouble(a[5]);
+    p.workspace_bytes = lib.states_workspace(&p);
+    const at::Tensor ws = bytes(p.workspace_bytes, q);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(q.device());
+    NEED(launch(lib.states_attn, p, stream(a[6]), raised));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// ---------------------------------------------------------------- beam search
+
+// select(logits, scores, count, finished or None, end_token or -1, stream) -> (scores, tokens, rows, finished or None)
+PyObject* py_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&](bool& raised) -> PyObject* {
+    NEED(lib.beam_select != nullptr && lib.beam_select_workspace != nullptr);
+    TENSOR(x, a[0]);
+    TENSOR(scores, a[1]);
+    const at::Tensor* done = nullptr;
+    if (!is_none(a[3])) NEED((done = tensor(a[3])) != nullptr);
+    NEED(PyLong_CheckExact(a[2]) && PyLong_CheckExact(a[4]));
+    const int64_t count = PyLong_AsLongLong(a[2]), end = PyLong_AsLongLong(a[4]);
+    NEED(PyErr_Occurred() == nullptr);
+    NEED(on_device(x) && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat) && x.dim() == 3 && x.numel() > 0);
+    const int64_t R = x.size(0), W = x.size(1), V = x.size(2);
+    NEED((V == 1 || x.stride(2) == 1) && R <= 0x7fffffff && W <= 32 && V < (1 << 30) && count >= 1 && count <= 64 && count <= W * V);
+    NEED(end >= -1 && end < V && (done == nullptr || end >= 0));
+    NEED(scores.scalar_type() == at::kFloat && scores.dim() == 2 && scores.size(0) == R && scores.size(1) == W && scores.device() == x.device());
+    NEED(done == nullptr || (done->scalar_type() == at::kBool && done->dim() == 2 && done->size(0) == R && done->size(1) == W &&
+                             done->device() == x.device()));
+    const at::Tensor best = empty({R, count}, x, at::kFloat), tokens = empty({R, count}, x, at::kInt), rows = empty({R, count}, x, at::kInt);
+    const at::Tensor ended = end >= 0 ? empty({R, count}, x, at::kBool) : at::Tensor();
+    MimirBeamSelectParams p = {};
+    p.logits = x.const_data_ptr(), p.scores = scores.const_data_ptr<float>();
+    p.out_scores = best.mutable_data_ptr<float>(), p.out_tokens = tokens.mutable_data_ptr<int32_t>(), p.out_rows = rows.mutable_data_ptr<int32_t>();
+    if (ended.defined()) p.out_finished = (uint8_t*)ended.mutable_data_ptr();
+    p.logits_stride_request = x.stride(0), p.logits_stride_beam = x.stride(1);
+    p.scores_stride_request = scores.stride(0), p.scores_stride_beam = scores.stride(1);
+    if (done != nullptr) {
+      p.finished = (const uint8_t*)done->const_data_ptr();
+      p.finished_stride_request = done->stride(0), p.finished_stride_beam = done->stride(1);
+    }
+    p.requests = (int32_t)R, p.beams = (int32_t)W, p.vocab = (int32_t)V, p.count = (int32_t)count, p.end_token = (int32_t)end;
+    p.dtype = x.scalar_type() == at::kBFloat16 ? MIMIR_DTYPE_BFLOAT16 : MIMIR_DTYPE_FLOAT32;
+    p.workspace_bytes = lib.beam_select_workspace(&p);
+    const at::Tensor ws = bytes(p.workspace_bytes, x);
+    p.workspace = ws.mutable_data_ptr();
+    const c10::DeviceGuard guard(x.device());
+    NEED(launch(lib.beam_select, p, stream(a[5]), raised));
+    PyObject* last = ended.defined() ? THPVariable_Wrap(ended) : Py_NewRef(Py_None);
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(best), THPVariable_Wrap(tokens), THPVariable_Wrap(rows), last);
+  });
+}
+
+// reorder(caches (a list of (keys, values)), lengths, source, stream) -> True
+PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 4, [&](bool& raised) -> PyObject* {
+    NEED(lib.reorder_rows != nullptr && PyList_CheckExact(a[0]));
+    const Py_ssize_t caches = PyList_GET_SIZE(a[0]);
+    NEED(caches > 0 && 2 * caches <= MIMIR_REORDER_TENSORS);  // one launch: past a refusal nothing has run
+    TENSOR(lengths, a[1]);
+    TENSOR(source, a[2]);
+    NEED(on_device(lengths) && index_vector(lengths, lengths) && source.dim() == 2 && source.is_contiguous() && source.device() == lengths.device() &&
+         (source.scalar_type() == at::kInt || source.scalar_type() == at::kLong));
+    const int64_t rows = source.numel(), group = source.size(1);
+    NEED(rows > 0 && rows <= 0x7fffffff && group <= 32 && lengths.size(0) == rows);
+    MimirReorderParams p = {};
+    const at::Tensor* all[MIMIR_REORDER_TENSORS];
+    for (Py_ssize_t i = 0; i < caches; ++i) {
+      PyObject* c = PyList_GET_ITEM(a[0], i);
+      NEED(PyTuple_Check(c) && PyTuple_GET_SIZE(c) == 2);
+      for (int j = 0; j < 2; ++j) {
+        const at::Tensor* const t = tensor(PyTuple_GET_ITEM(c, j));
+        const at::Tensor* const t0 = p.count > 0 ? all[0] : t;
+        NEED(t != nullptr && t->device() == lengths.device() && t->dim() >= 2 && t->sizes() == t0->sizes() && t->scalar_type() == t0->scalar_type());
+        int64_t dense = 1;
+        for (int64_t e = t->dim() - 1; e > 0; --e) {
+          NEED(t->size(e) == 1 || t->stride(e) == dense);
+          dense *= t->size(e);
+        }
+        NEED(dense > 0 && t->size(0) >= rows && t->size(1) <= 0x7fffffff);
+        p.position_bytes = dense / t->size(1) * (int64_t)t->element_size();
+        p.max_length = (int32_t)t->size(1);
+        all[p.count] = t;
+        p.data[p.count] = t->mutable_data_ptr();
+        p.stride[p.count++] = rows > 1 ? t->stride(0) * (int64_t)t->element_size() : 0;
+      }
+    }
+    p.lengths = lengths.mutable_data_ptr(), p.source = source.const_data_ptr();
+    p.rows = (int32_t)rows, p.group = (int32_t)group;
+    p.index_int64 = lengths.scalar_type() == at::kLong, p.source_int64 = source.scalar_type() == at::kLong;
+    p.update_lengths = 1;
+    {
+      const c10::DeviceGuard guard(lengths.device());
+      NEED(launch(lib.reorder_rows, p, stream(a[3]), raised));
+    }
+    // what autograd has saved of them is no longer what it was
+    for (int i = 0; i < p.count; ++i)
+      if (!all[i]->is_inference()) all[i]->unsafeGetTensorImpl()->bump_version();
+    if (!lengths.is_inference()) lengths.unsafeGetTensorImpl()->bump_version();
+    return Py_NewRef(Py_True);
+  });
+}
+
 // streams(function): torch's function from a device index to the raw handle of its current stream.
 PyObject* py_streams(PyObject*, PyObject* f) {
   PyObject* const old = current_stream;
@@ -799,6 +1209,17 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   get(lib.pages_compact, "mimir_prefixlm_pages_compact");
   get(lib.pages_release, "mimir_prefixlm_pages_release");
   get(lib.pages_reserve, "mimir_prefixlm_pages_reserve");
+  get(lib.norm_rotary, "mimir_prefixlm_norm_rotary");
+  get(lib.norm_rotary_bwd, "mimir_prefixlm_norm_rotary_bwd");
+  get(lib.norm_rotary_workspace, "mimir_prefixlm_norm_rotary_workspace_bytes");
+  get(lib.cross_fwd, "mimir_prefixlm_cross_fwd");
+  get(lib.cross_bwd, "mimir_prefixlm_cross_bwd");
+  get(lib.cross_workspace, "mimir_prefixlm_cross_workspace_bytes");
+  get(lib.states_attn, "mimir_prefixlm_states_attn");
+  get(lib.states_workspace, "mimir_prefixlm_states_workspace_bytes");
+  get(lib.beam_select, "mimir_prefixlm_beam_select");
+  get(lib.beam_select_workspace, "mimir_prefixlm_beam_select_workspace_bytes");
+  get(lib.reorder_rows, "mimir_prefixlm_reorder_rows");
   Py_RETURN_NONE;
 }
 
@@ -811,6 +1232,11 @@ PyMethodDef methods[] = {
     {"rotary", (PyCFunction)(void*)py_rotary, METH_FASTCALL, nullptr},
     {"paged_attn", (PyCFunction)(void*)py_paged_attn, METH_FASTCALL, nullptr},
     {"pages", (PyCFunction)(void*)py_pages, METH_FASTCALL, nullptr},
+    {"norm_rotary", (PyCFunction)(void*)py_norm_rotary, METH_FASTCALL, nullptr},
+    {"cross_attention", (PyCFunction)(void*)py_cross_attention, METH_FASTCALL, nullptr},
+    {"states", (PyCFunction)(void*)py_states, METH_FASTCALL, nullptr},
+    {"select", (PyCFunction)(void*)py_select, METH_FASTCALL, nullptr},
+    {"reorder", (PyCFunction)(void*)py_reorder, METH_FASTCALL, nullptr},
     {"streams", py_streams, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -310,6 +310,10 @@ def norm_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequen
     heads' type, both the same.  fp32 arithmetic, one rounding; the weights' gradients are fp32 sums in a fixed
     order.  Positions, frequencies and strides as for :func:`rotary`.
     """
+    if query.is_cuda:
+        res = _capi.host().norm_rotary(query, key, positions, *frequencies, query_weight, key_weight, eps, P._stream(query.device))
+        if res is not None:
+            return res
     positions = _check(query, key, positions, frequencies)
     if query.shape[-1] % 2:
         raise ValueError(f"head_dim must be even, got {query.shape[-1]}")
