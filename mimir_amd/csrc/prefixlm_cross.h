@@ -80,8 +80,7 @@ __device__ __forceinline__ QueryTile query_tile(const CrossArgs& a) {
   return t;
 }
 
-// The launch in front of the tile kernels: the tile lists, the rows outside every sequence (zeroed), and
-// (backward) the delta rows.
+// The launch in front of the tile kernels: the tile lists, and zeros in the rows outside every sequence.
 struct CrossPrologue {
   SeqTable seqs;
   int4 *plan_q, *plan_k;  // NULL: not wanted
@@ -93,10 +92,6 @@ struct CrossPrologue {
   } fill[3];
   int nfill, D;
   float* lse2;            // of the filled query rows: -inf
-  const bf16_t *o, *o_lo, *dout;
-  int64_t o_st, o_sh, do_st, do_sh;
-  float* delta;
-  int Hq;
 };
 hipError_t launch_cross_prologue(const CrossPrologue& p, hipStream_t stream);
 hipError_t launch_cross_fwd(const CrossArgs& a, int head_dim, hipStream_t stream);

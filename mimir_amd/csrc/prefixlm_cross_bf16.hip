@@ -27,11 +27,11 @@ constexpr int kBlockN = 64;  // states of an LDS tile
 // ---------------------------------------------------------------- the launch in front
 
 constexpr int kPlanThreads = 1024, kBuckets = 256;
-constexpr int kFillBlocks = 32, kDeltaPasses = 4;
+constexpr int kFillBlocks = 32;
 
 struct PrologueArgs {
   CrossPrologue p;
-  int plans, delta_blocks;
+  int plans;
 };
 
 // Tiles of one side, those with most rows on the other side first.
@@ -112,37 +112,6 @@ __device__ __forceinline__ void fill_rows(const CrossPrologue& p, const CrossPro
   }
 }
 
-// delta = rowsum(dO * O), D / 8 lanes a row.  O is taken with its low half: dS = P (dP - delta) is a difference
-// whose rounding errors would else be led by O's (gradients of 2 sequences of 300 over 40: error against 64
-// bits 0.0039 of their size without, 0.0024 with it).
-__device__ __forceinline__ void delta_rows(const CrossPrologue& p, int block) {
-  const int lanes = p.D / 8, c = threadIdx.x % lanes, per = kPlanThreads / lanes;
-  const int64_t rows = (int64_t)p.seqs.Tq * p.Hq;
-  bf16x8 o[kDeltaPasses], lo[kDeltaPasses], g[kDeltaPasses];
-  int t[kDeltaPasses], h[kDeltaPasses];
-#pragma unroll
-  for (int i = 0; i < kDeltaPasses; ++i) {
-    const int64_t row = ((int64_t)block * kDeltaPasses + i) * per + threadIdx.x / lanes;
-    t[i] = row < rows ? (int)((uint32_t)row / (uint32_t)p.Hq) : -1;  // host: Tq * Hq below 2^32
-    h[i] = (int)((uint32_t)row - (uint32_t)max(t[i], 0) * (uint32_t)p.Hq);
-    if (t[i] >= 0) {
-      // O is read once: dO, which the tile kernels stream next, keeps its place in the caches
-      o[i] = __builtin_nontemporal_load((const bf16x8*)&p.o[t[i] * p.o_st + h[i] * p.o_sh + c * 8]);
-      lo[i] = __builtin_nontemporal_load((const bf16x8*)&p.o_lo[((int64_t)t[i] * p.Hq + h[i]) * p.D + c * 8]);
-      g[i] = *(const bf16x8*)&p.dout[t[i] * p.do_st + h[i] * p.do_sh + c * 8];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kDeltaPasses; ++i) {
-    float acc = 0.f;
-    if (t[i] >= 0)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc += ((float)o[i][e] + (float)lo[i][e]) * (float)g[i][e];
-    for (int off = lanes / 2; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
-    if (t[i] >= 0 && c == 0) p.delta[(int64_t)h[i] * p.seqs.Tq + t[i]] = acc;
-  }
-}
-
 __global__ __launch_bounds__(kPlanThreads) void cross_prologue_kernel(const PrologueArgs a) {
   int b = blockIdx.x;
   if (b < a.plans) {
@@ -151,11 +120,7 @@ __global__ __launch_bounds__(kPlanThreads) void cross_prologue_kernel(const Prol
     return;
   }
   b -= a.plans;
-  if (b < a.p.nfill * kFillBlocks) {
-    fill_rows(a.p, a.p.fill[b / kFillBlocks], b % kFillBlocks);
-    return;
-  }
-  delta_rows(a.p, b - a.p.nfill * kFillBlocks);
+  fill_rows(a.p, a.p.fill[b / kFillBlocks], b % kFillBlocks);
 }
 
 // ---------------------------------------------------------------- forward
@@ -385,12 +350,8 @@ template __global__ void cross_fwd_kernel<128>(const CrossArgs);
 }  // namespace
 
 hipError_t launch_cross_prologue(const CrossPrologue& p, hipStream_t stream) {
-  PrologueArgs a = {p, (p.plan_q != nullptr) + (p.plan_k != nullptr), 0};
-  if (p.delta != nullptr) {
-    const int64_t rows = (int64_t)p.seqs.Tq * p.Hq, per = (int64_t)kDeltaPasses * kPlanThreads / (p.D / 8);
-    a.delta_blocks = (int)((rows + per - 1) / per);
-  }
-  const int blocks = a.plans + p.nfill * kFillBlocks + a.delta_blocks;
+  const PrologueArgs a = {p, (p.plan_q != nullptr) + (p.plan_k != nullptr)};
+  const int blocks = a.plans + p.nfill * kFillBlocks;
   if (blocks == 0) return hipSuccess;
   hipLaunchKernelGGL(cross_prologue_kernel, dim3((unsigned)blocks), dim3(kPlanThreads), 0, stream, a);
   return hipGetLastError();
@@ -438,6 +399,8 @@ int check_cross(const MimirCrossParams* p, bool backward) {
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "cross attention supports head_dim 64 and 128, got " + std::to_string(p->head_dim));
   if (!(p->softmax_scale > 1e-30f) || !(p->softmax_scale < 1e30f))
     return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and neither below 1e-30 nor above 1e30");
+  if ((int64_t)p->num_q_heads * p->head_dim >= (1 << 22))
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "a token's query heads must hold fewer than 2^22 elements");
   if ((int64_t)p->total_q * p->num_q_heads > 0x7fffffff || (int64_t)p->total_k * p->num_q_heads > 0x7fffffff)
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one call");
   if (p->numseqs > 0 && (p->cu_seqlens_q == nullptr || p->cu_seqlens_k == nullptr))
@@ -507,7 +470,6 @@ CrossPrologue cross_prologue(const MimirCrossParams& p, const CrossArgs& a) {
   if (a.cap_k > 0) pro.plan_k = (int4*)a.plan_k;
   pro.cap_q = a.cap_q; pro.cap_k = a.cap_k;
   pro.D = p.head_dim;
-  pro.Hq = p.num_q_heads;
   return pro;
 }
 
@@ -540,12 +502,7 @@ extern "C" int mimir_prefixlm_cross_bwd(const MimirCrossParams* p, void* stream)
   if (status != MIMIR_OK || (p->total_q == 0 && p->total_k == 0)) return status;
   const CrossArgs a = cross_args(*p, cross_workspace(*p, true));
   CrossPrologue pro = cross_prologue(*p, a);
-  if (p->total_q > 0) {
-    pro.fill[pro.nfill++] = {a.dq, a.dq_st, a.dq_sh, 0, a.Hq};
-    pro.o = a.o; pro.o_lo = a.o_lo; pro.dout = a.dout;
-    pro.o_st = a.o_st; pro.o_sh = a.o_sh; pro.do_st = a.do_st; pro.do_sh = a.do_sh;
-    pro.delta = a.delta;
-  }
+  if (p->total_q > 0) pro.fill[pro.nfill++] = {a.dq, a.dq_st, a.dq_sh, 0, a.Hq};
   if (p->total_k > 0) {
     pro.fill[pro.nfill++] = {a.dk, a.dk_st, a.dk_sh, 1, a.Hkv};
     pro.fill[pro.nfill++] = {a.dv, a.dv_st, a.dv_sh, 1, a.Hkv};

@@ -3,8 +3,10 @@
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q.
 //
 // Two kernels, each the owner of what it sums, so nothing is added atomically and results do not
-// depend on timing: dK / dV per (kv head, 128 states), over all query heads of the group and all
-// queries of the sequence, and dQ per (query head, 128 query rows), which forms S and dP again.
+// depend on timing: dQ per (query head, 128 query rows), which also forms delta, and then dK / dV per (kv head,
+// 128 states), over all query heads of the group and all queries of the sequence, which forms S and dP again.
+// delta takes O with its low half: dS is a difference whose rounding errors would else be led by O's
+// (error of dQ and dK against 64 bits, in units of one rounding of the exact result: up to 2.3 without, 1.4 with it).
 // P and dS are rounded to bf16 for their products.  Both are bound by the matrix units.
 #include "prefixlm_cross.h"
 
@@ -261,12 +263,173 @@ __global__ __attribute__((amdgpu_flat_work_group_size(kKvWaves * 64, kKvWaves * 
     const CrossArgs a) {
   cross_dkdv_body<D>(a);
 }
-template __global__ void cross_dkdv_kernel<64>(const CrossArgs);
 template __global__ void cross_dkdv_kernel<128>(const CrossArgs);
+
+// head_dim 64: K and V fragments both fit the registers, and 4 waves of 32 states each take all 64 rows of
+// a query tile: nothing to add up at the end, and three small workgroups per CU overlap each other's
+// first loads and stores (48 documents of up to 700 queries over up to 1300 states, 8 heads: the scheme above 99 us, with
+// one workgroup of 8 waves per CU).
+constexpr int kSmallWaves = 4, kSmallPerSimd = 3;
+
+__global__ __attribute__((amdgpu_flat_work_group_size(kSmallWaves * 64, kSmallWaves * 64), amdgpu_waves_per_eu(kSmallPerSimd, kSmallPerSimd)))
+void cross_dkdv_d64_kernel(const CrossArgs a) {
+  constexpr int D = 64, DT = D / 32, KS = D / 16;
+  using L = TileLayout<D>;
+  using Loader = TileLoader<D, kSmallWaves>;
+  constexpr int kStageElems = 2 * L::kElems + 2 * kQTile * 2;  // Q, dO, lse2 + delta (fp32)
+  __shared__ __attribute__((aligned(16))) bf16_t sS0[kStageElems];
+  __shared__ __attribute__((aligned(16))) bf16_t sS1[kStageElems];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31;
+  const int hi = lane >> 5;
+  const int rank = blockIdx.x / a.Hkv, hk = blockIdx.x - rank * a.Hkv;
+  const int4 item = load_entry(a.plan_k, rank);
+  const int keys = item.y, nq = item.w;
+  if (keys == 0) return;  // list padding
+  const int ka = wave * 32;
+  const bool wave_active = ka < keys;
+  const int nqt = (nq + kQTile - 1) / kQTile;
+  const int n_iter = nqt * a.group;  // (query head, query tile) steps
+
+  // Per tile the Q copy's last instruction is wave 0's, the dO copy's wave 1's; waves 2 and 3 copy the rows.
+  static_assert(Loader::kInst == (Loader::kPerWave - 1) * kSmallWaves + 1, "one last-round copy per tile");
+  const Loader ldq(a.q_st, wave, lane), ldo(a.do_st, wave, lane, 1);
+  const int qh0 = hk * a.group;
+  const bf16_t* q_head = a.q + (int64_t)item.z * a.q_st + (int64_t)qh0 * a.q_sh;
+  const bf16_t* o_head = a.dout + (int64_t)item.z * a.do_st + (int64_t)qh0 * a.do_sh;
+  const float* r_head = (wave == 2 ? a.lse2 : a.delta) + (int64_t)qh0 * a.Tq + item.z;
+  const bf16_t* i_q = q_head;
+  const bf16_t* i_o = o_head;
+  const float* i_r = r_head;
+  int i_qt = 0, i_rows = nq;
+  auto issue_next = [&](bool valid, bf16_t* stage) {
+    const int rows = valid ? min(i_rows, kQTile) : 0;
+    ldq.issue_at(i_q, rows_bytes32(rows, (uint32_t)a.q_st, D), stage);
+    ldo.issue_at(i_o, rows_bytes32(rows, (uint32_t)a.do_st, D), stage + L::kElems);
+    float* const tr = (float*)(stage + 2 * L::kElems);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(i_r, (uint32_t)rows * 4u);
+    if (wave >= 2)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tr + (wave == 2 ? 0 : kQTile)), 4,
+                                               (uint32_t)lane * 4u, 0, 0, 0);
+    if (++i_qt == nqt) {
+      i_qt = 0;
+      i_rows = nq;
+      q_head += a.q_sh;
+      o_head += a.do_sh;
+      r_head += a.Tq;
+      i_q = q_head;
+      i_o = o_head;
+      i_r = r_head;
+    } else {
+      i_rows -= kQTile;
+      i_q += kQTile * a.q_st;
+      i_o += kQTile * a.do_st;
+      i_r += kQTile;
+    }
+  };
+  issue_next(n_iter > 0, sS0);
+  const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.k + (int64_t)item.x * a.k_st + (int64_t)hk * a.k_sh, rows_bytes(keys, a.k_st, D));
+  const __amdgpu_buffer_rsrc_t rv = make_rsrc(a.v + (int64_t)item.x * a.v_st + (int64_t)hk * a.v_sh, rows_bytes(keys, a.v_st, D));
+  bf16x8 kf[KS], vf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    kf[ks] = __builtin_bit_cast(bf16x8, buf_load16(rk, (uint32_t)(((ka + l32) * a.k_st + 16 * ks + 8 * hi) * 2)));
+    vf[ks] = __builtin_bit_cast(bf16x8, buf_load16(rv, (uint32_t)(((ka + l32) * a.v_st + 16 * ks + 8 * hi) * 2)));
+  }
+  f32x16 dkacc[DT], dvacc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    dkacc[dt] = f32x16{};
+    dvacc[dt] = f32x16{};
+  }
+  const float c2 = a.scale_log2;
+  const TileLanes<D> tl(lane);
+
+  auto compute = [&](const bf16_t* stage, int halves) {
+    const bf16_t* const sQ = stage;
+    const bf16_t* const sdO = stage + L::kElems;
+    const float* const sL = (const float*)(stage + 2 * L::kElems);
+    const float* const sD = sL + kQTile;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {  // 32-row halves of the tile
+      if (mt >= halves) break;
+      f32x16 sc = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int o = tl.op_base + mt * 32 * L::kRowElems + ks * 16;
+        sc = mfma32(*(const bf16x8*)&sQ[o], kf[ks], sc);
+        dp = mfma32(*(const bf16x8*)&sdO[o], vf[ks], dp);
+      }
+      bf16x8 pb[2], db[2];
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        f32x8 tp, tds;
+#pragma unroll
+        for (int rg2 = 0; rg2 < 2; ++rg2) {
+          const int qr0 = 32 * mt + 8 * (2 * s2 + rg2) + 4 * hi;
+          const f32x4 l4 = *(const f32x4*)&sL[qr0], d4 = *(const f32x4*)&sD[qr0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * (2 * s2 + rg2) + e;
+            const float pr = fast_exp2(__builtin_fmaf(sc[r], c2, -l4[e]));
+            tp[4 * rg2 + e] = pr;
+            tds[4 * rg2 + e] = pr * (dp[r] - d4[e]);
+          }
+        }
+        pb[s2] = to_bf16x8(tp);
+        db[s2] = to_bf16x8(tds);
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const int o = tl.tr_base + (2 * mt + s2) * 16 * L::kRowElems + dt * 32;
+          dvacc[dt] = mfma32(cat8(lds_read_tr16(&sdO[o]), lds_read_tr16(&sdO[o + L::kTrSecond])), pb[s2], dvacc[dt]);
+          dkacc[dt] = mfma32(cat8(lds_read_tr16(&sQ[o]), lds_read_tr16(&sQ[o + L::kTrSecond])), db[s2], dkacc[dt]);
+        }
+    }
+  };
+  int s_qt = 0;  // query tile of the next step
+  auto step = [&](const bf16_t* stage) {
+    const int left = nq - s_qt * kQTile;
+    if (++s_qt == nqt) s_qt = 0;
+    if (wave_active) compute(stage, left > 32 ? 2 : 1);
+  };
+  for (int it = 0; it < n_iter; it += 2) {
+    stage_barrier<0>();
+    issue_next(it + 1 < n_iter, sS1);
+    step(sS0);
+    if (it + 1 >= n_iter) break;
+    stage_barrier<0>();
+    issue_next(it + 2 < n_iter, sS0);
+    step(sS1);
+  }
+  wait_vmem();  // copies past the last tile are still in flight
+  if (ka + l32 >= keys) return;
+  const int64_t row = item.x + ka + l32;
+  bf16_t* const krow = a.dk + row * a.dk_st + (int64_t)hk * a.dk_sh;
+  bf16_t* const vrow = a.dv + row * a.dv_st + (int64_t)hk * a.dv_sh;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+      f32x4 tk, tv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        tk[e] = dkacc[dt][4 * rg + e] * a.scale;
+        tv[e] = dvacc[dt][4 * rg + e];
+      }
+      *(bf16x4*)&krow[32 * dt + 8 * rg + 4 * hi] = __builtin_convertvector(tk, bf16x4);
+      *(bf16x4*)&vrow[32 * dt + 8 * rg + 4 * hi] = __builtin_convertvector(tv, bf16x4);
+    }
+}
 
 // ---------------------------------------------------------------------------
 // dQ: the forward's S^T formulation, a query row in a lane, so lse2 and delta are local to it and dS^T is
-// the B operand of dQ^T += K^T dS^T.
+// the B operand of dQ^T += K^T dS^T.  delta comes from the dO fragments that the kernel holds anyway and the same
+// ones of O: a pass of its own over O and dO took 35 us beside the 800 of a training step of 8 x 2048 rows.
 // ---------------------------------------------------------------------------
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
@@ -316,10 +479,22 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
     qf[ks] = __builtin_bit_cast(bf16x8, buf_load16(rq, (uint32_t)((qrow * a.q_st + 16 * ks + 8 * hi) * 2)));
     dof[ks] = __builtin_bit_cast(bf16x8, buf_load16(rdo, (uint32_t)((qrow * a.do_st + 16 * ks + 8 * hi) * 2)));
   }
-  float lse2 = 0.f, dlt = 0.f;
-  if (qrow < rows) {
-    lse2 = a.lse2[(int64_t)h * a.Tq + item.x + qrow];
-    dlt = a.delta[(int64_t)h * a.Tq + item.x + qrow];
+  const int64_t row_at = (int64_t)h * a.Tq + item.x + qrow;
+  const float lse2 = qrow < rows ? a.lse2[row_at] : 0.f;
+  float dlt = 0.f;
+  {
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.o + (int64_t)item.x * a.o_st + (int64_t)h * a.o_sh, rows_bytes(rows, a.o_st, D));
+    const int64_t lo_st = (int64_t)a.Hq * D;
+    const __amdgpu_buffer_rsrc_t rl = make_rsrc(a.o_lo + (int64_t)item.x * lo_st + (int64_t)h * D, rows_bytes(rows, lo_st, D));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const bf16x8 ov = __builtin_bit_cast(bf16x8, buf_load16(ro, (uint32_t)((qrow * a.o_st + 16 * ks + 8 * hi) * 2)));
+      const bf16x8 lv = __builtin_bit_cast(bf16x8, buf_load16(rl, (uint32_t)((qrow * lo_st + 16 * ks + 8 * hi) * 2)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dlt += ((float)ov[e] + (float)lv[e]) * (float)dof[ks][e];
+    }
+    dlt = xor32_sum(dlt);
+    if (hi == 0 && qrow < rows) a.delta[row_at] = dlt;
   }
   f32x16 dqacc[DT];
 #pragma unroll
@@ -418,22 +593,22 @@ template __global__ void cross_dq_kernel<128>(const CrossArgs);
 }  // namespace
 
 hipError_t launch_cross_bwd(const CrossArgs& a, int head_dim, hipStream_t stream) {
-  if (a.cap_k > 0) {
-    const dim3 grid((unsigned)a.cap_k * (unsigned)a.Hkv);
+  const int64_t units = (int64_t)a.cap_q * a.Hkv;
+  if (units > 0) {
+    const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * a.group));
     if (head_dim == 128)
-      hipLaunchKernelGGL(cross_dkdv_kernel<128>, grid, dim3(kKvWaves * 64), 0, stream, a);
+      hipLaunchKernelGGL(cross_dq_kernel<128>, grid, dim3(kThreads), 0, stream, a);
     else
-      hipLaunchKernelGGL(cross_dkdv_kernel<64>, grid, dim3(kKvWaves * 64), 0, stream, a);
+      hipLaunchKernelGGL(cross_dq_kernel<64>, grid, dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  const int64_t units = (int64_t)a.cap_q * a.Hkv;
-  if (units == 0) return hipSuccess;
-  const dim3 grid((unsigned)((units + kXcds - 1) / kXcds * kXcds * a.group));
+  if (a.cap_k == 0) return hipSuccess;
+  const dim3 grid((unsigned)a.cap_k * (unsigned)a.Hkv);
   if (head_dim == 128)
-    hipLaunchKernelGGL(cross_dq_kernel<128>, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(cross_dkdv_kernel<128>, grid, dim3(kKvWaves * 64), 0, stream, a);
   else
-    hipLaunchKernelGGL(cross_dq_kernel<64>, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(cross_dkdv_d64_kernel, grid, dim3(kSmallWaves * 64), 0, stream, a);
   return hipGetLastError();
 }
 

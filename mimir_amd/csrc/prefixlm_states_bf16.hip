@@ -490,7 +490,6 @@ extern "C" int mimir_prefixlm_states_attn(const MimirStatesParams* p, void* stre
     pro.plan_q = (int4*)p->workspace;
     pro.cap_q = plan.cap;
     pro.D = p->head_dim;
-    pro.Hq = p->num_q_heads;
     e = launch_cross_prologue(pro, (hipStream_t)stream);
     if (e == hipSuccess) e = launch_cross_fwd(a, p->head_dim, (hipStream_t)stream);
   } else {
