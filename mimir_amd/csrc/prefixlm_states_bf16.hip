@@ -62,8 +62,16 @@ __device__ __forceinline__ int line_length(const SeqTable& t, Line& line, int la
   }
   return total;
 }
-// First unit of share i of n over a line of `total` units.
-__device__ __forceinline__ int share_start(int i, int n, int total) { return (int)((int64_t)total * i / n); }
+// A line's units dealt to shares: `each`, and one more to the first `more`.
+struct Deal {
+  int each, more;
+  __device__ __forceinline__ Deal(int total, int shares) : each((int)((uint32_t)total / (uint32_t)shares)), more(total - each * shares) {}
+  __device__ __forceinline__ int start(int i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ int share_of(int u) const {  // that holds unit u
+    const int longer = more * (each + 1);
+    return u < longer ? (int)((uint32_t)u / (uint32_t)(each + 1)) : more + (int)((uint32_t)(u - longer) / (uint32_t)max(each, 1));
+  }
+};
 // A share's parts of requests that go on in another: that of its first request, and of its last.
 __device__ __forceinline__ int64_t part_slot(const StatesArgs& a, int tile, int share, bool first, int hk, int tile_rows) {
   return ((((int64_t)tile * a.shares + share) * 2 + !first) * a.Hkv + hk) * tile_rows;
@@ -105,7 +113,8 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
 
   Line line;
   const int total = line_length(a.seqs, line, lane);
-  const int u_begin = share_start(share, a.shares, total), u_end = share_start(share + 1, a.shares, total);
+  const Deal deal(total, a.shares);
+  const int u_begin = deal.start(share), u_end = deal.start(share + 1);
   if (u_begin >= u_end) return;
   if (a.seqs.n > 64) {
     int before = 0;
@@ -142,7 +151,8 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
     const bf16_t* const kbase = a.k + crow * a.k_sb + hk * a.k_sh;
     const bf16_t* const vbase = a.v + crow * a.v_sb + hk * a.v_sh;
     auto issue = [&](int i, bf16_t* tk, bf16_t* tv) __attribute__((always_inline)) {
-      const int key0 = (t0 + i * kShareWaves) * kTile, n = min(keys - key0, kTile);
+      // past the wave's tiles: empty buffers, zeros for a free stage, so that every step waits alike
+      const int key0 = (t0 + min(i, max(n_my - 1, 0)) * kShareWaves) * kTile, n = i < n_my ? min(keys - key0, kTile) : 0;
       const __amdgpu_buffer_rsrc_t rk = make_rsrc(kbase + key0 * a.k_st, rows_bytes32(n, (uint32_t)a.k_st, D));
       const __amdgpu_buffer_rsrc_t rv = make_rsrc(vbase + key0 * a.v_st, rows_bytes32(n, (uint32_t)a.v_st, D));
 #pragma unroll
@@ -161,8 +171,8 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qf[n][ks] = *(const bf16x8*)&qrow[16 * ks];
     }
-    if (n_my > 0) issue(0, mk0, mv0);
-    if (n_my > 1) issue(1, mk1, mv1);
+    issue(0, mk0, mv0);
+    issue(1, mk1, mv1);
     f32x16 oacc[NT][DT];
     float m_run[NT], l_run[NT];
 #pragma unroll
@@ -230,32 +240,26 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
           for (int n = 0; n < NT; ++n) oacc[n][dt] = mfma32(vf, pf[n][kk], oacc[n][dt]);
         }
     };
-    // Tile i has landed once at most the copies of tile i + 1 are outstanding.
+    // Tile i has landed once at most the copies of tile i + 1 are outstanding; a stage is refilled once this wave's
+    // reads of it are done.
     for (int i = 0; i < n_my; i += 2) {
-      if (i + 1 < n_my)
-        wait_vmcnt_wide<2 * kInst>();
-      else
-        wait_vmcnt_wide<0>();
+      wait_vmcnt_wide<2 * kInst>();
       __asm__ volatile("" ::: "memory");
       compute(i, mk0, mv0);
-      if (i + 2 < n_my) {
-        __asm__ volatile("" ::: "memory");
-        wait_lds();  // this wave's reads of the stage are done before it is refilled
-        issue(i + 2, mk0, mv0);
-      }
+      __asm__ volatile("" ::: "memory");
+      wait_lds();
+      issue(i + 2, mk0, mv0);
       if (i + 1 >= n_my) break;
-      if (i + 2 < n_my)
-        wait_vmcnt_wide<2 * kInst>();
-      else
-        wait_vmcnt_wide<0>();
+      wait_vmcnt_wide<2 * kInst>();
       __asm__ volatile("" ::: "memory");
       compute(i + 1, mk1, mv1);
-      if (i + 3 < n_my) {
-        __asm__ volatile("" ::: "memory");
-        wait_lds();
-        issue(i + 3, mk1, mv1);
-      }
+      __asm__ volatile("" ::: "memory");
+      wait_lds();
+      issue(i + 3, mk1, mv1);
     }
+    __asm__ volatile("" ::: "memory");
+    wait_vmcnt_wide<0>();  // the last copies
+    wait_lds();
     // The waves' partial rows meet in LDS.
     auto area = [&](int w) __attribute__((always_inline)) { return (float*)(w == 0 ? sK1 : sV1); };
     auto ml_of = [&](int w, int r) __attribute__((always_inline)) { return (f32x2*)(area(w) + 32 * kPitch) + r; };
@@ -325,32 +329,23 @@ __device__ __forceinline__ void states_merge_body(const StatesArgs& a, int tile_
     if (sub == 0) *(bf16x4*)&orow[col] = bf16x4{};
     return;
   }
-  auto share_of = [&](int u) __attribute__((always_inline)) {
-    int i = (int)((int64_t)u * a.shares / total);
-    while (share_start(i + 1, a.shares, total) <= u) ++i;
-    while (share_start(i, a.shares, total) > u) --i;
-    return i;
-  };
-  const int i0 = share_of(u0), n = share_of(u1 - 1) - i0 + 1;
+  const Deal deal(total, a.shares);
+  // the shares that hold it, none of them empty: a line of fewer units than shares fills the first ones
+  const int i0 = deal.share_of(u0), n = deal.share_of(u1 - 1) - i0 + 1;
   if (n == 1) return;  // finished in its share
   const int tile = r / tile_rows;
   // shares after the first begin inside the request: theirs is the part of their first request
   auto slot = [&](int i) __attribute__((always_inline)) {
-    return part_slot(a, tile, i0 + i, i > 0 || share_start(i0, a.shares, total) == u0, hk, tile_rows) + r - tile * tile_rows;
-  };
-  auto empty = [&](int i) __attribute__((always_inline)) {  // a share of a line with fewer units than shares
-    return share_start(i0 + i, a.shares, total) == share_start(i0 + i + 1, a.shares, total);
+    return part_slot(a, tile, i0 + i, i > 0 || deal.start(i0) == u0, hk, tile_rows) + r - tile * tile_rows;
   };
   float M = -INFINITY;
-  for (int i = lane; i < n; i += 64)
-    if (!empty(i)) M = fmaxf(M, a.part_ml[slot(i) * 2]);
+  for (int i = lane; i < n; i += 64) M = fmaxf(M, a.part_ml[slot(i) * 2]);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float lsum = 0.f;
 #pragma unroll 8
   for (int i = sub; i < n; i += kParts) {
-    if (empty(i)) continue;
     const int64_t at = slot(i);
     const f32x2 ml = *(const f32x2*)&a.part_ml[at * 2];
     const f32x4 o = *(const f32x4*)&a.part_o[at * D + col];
