@@ -6,7 +6,7 @@
 // workgroup of beam_rows_kernel per piece of a row keeps the piece in registers, and from there
 //   * sums exp(x - max) in fp32, a few adds a lane;
 //   * finds a threshold that at least `count` elements reach: the count-th largest of a wave's lane maxima,
-//     bit by bit with ballots (16 steps for bf16), and the largest of that over the waves;
+//     found with ballots two bits at a time (8 steps for bf16), and the largest of that over the waves;
 //   * ranks the few elements that reach it and stores the best `count`, in order.
 // Within a row larger logits are larger scores, so this needs no lse.  beam_merge_kernel, a workgroup per
 // request, joins the pieces' sums in 64 bits, forms the scores of the stored elements in 64 bits (beams
@@ -19,6 +19,7 @@
 // Bound by copying.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "prefixlm_common.h"
 #include "strided_overlap.h"
@@ -53,11 +54,39 @@ __device__ __forceinline__ uint64_t list_key(float x, int token) { return (uint6
 __device__ __forceinline__ float key_value(uint64_t k) { return order_value((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k; }
 
+// Over the wave, on every lane, without LDS round trips.
 template <typename F>
 __device__ __forceinline__ float wave_reduce(float x, F&& f) {
+  auto dpp = [&](auto ctrl) __attribute__((always_inline)) {
+    const int v = __float_as_int(x);
+    return f(x, __int_as_float(__builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  x = dpp(std::integral_constant<int, 0xb1>());   // quad_perm: lane ^ 1
+  x = dpp(std::integral_constant<int, 0x4e>());   // quad_perm: lane ^ 2
+  x = dpp(std::integral_constant<int, 0x141>());  // row_half_mirror: the other quad of eight
+  x = dpp(std::integral_constant<int, 0x140>());  // row_mirror: the other eight of sixteen
+  const int v = __float_as_int(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  const int a = p[0], b = p[1];
+  x = f(__int_as_float(a), __int_as_float(b));
+  float lo, hi;
+  halves(x, lo, hi);
+  return f(lo, hi);
+}
+// The count-th largest of the wave's codes, or less (0) where so many lanes hold none; from the top bit down to
+// `low`, two bits a step.
+template <int kLow>
+__device__ __forceinline__ uint32_t wave_kth(uint32_t code, int count) {
+  uint32_t reach = 0;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x = f(x, __shfl_xor(x, off, 64));
-  return x;
+  for (int bit = 30; bit >= kLow; bit -= 2) {
+    const uint32_t one = 1u << bit;
+    const int n1 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= reach + one));
+    const int n2 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= reach + 2 * one));
+    const int n3 = __builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= reach + 3 * one));
+    reach += n3 >= count ? 3 * one : n2 >= count ? 2 * one : n1 >= count ? one : 0;
+  }
+  return reach;
 }
 
 // 16 bytes of logits at any address of theirs.
@@ -93,7 +122,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   __shared__ uint64_t keys[kCap];
   __shared__ float wave_max[4], wave_sum[4];
   __shared__ uint32_t wave_code[4];
-  __shared__ int found;
+  __shared__ uint16_t vectors[256 * NV];
+  __shared__ int noted, found;
   __shared__ uint64_t round_best[4];
   const int tid = threadIdx.x, wave = tid >> 6;
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
@@ -138,19 +168,13 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   keep_packed(v);
   const float wtop = wave_reduce(top, [](float p, float q) { return fmaxf(p, q); });
   // The count-th largest code of the wave's lane maxima: at least `count` elements reach it.
-  const uint32_t code = order_code(top);
-  uint32_t reach = 0;
-#pragma unroll
-  for (int bit = 31; bit >= (sizeof(E) == 2 ? 16 : 0); --bit) {
-    const uint32_t next = reach | 1u << bit;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= next)) >= a.K) reach = next;
-  }
+  uint32_t reach = wave_kth<sizeof(E) == 2 ? 16 : 0>(order_code(top), a.K);
   if (sizeof(E) == 2 && reach >> 31 == 0) reach |= 0xffffu;  // a negative bf16's code ends in ones
   if ((tid & 63) == 0) {
     wave_max[wave] = wtop;
     wave_code[wave] = reach;
   }
-  if (tid == 0) found = 0;
+  if (tid == 0) noted = found = 0;
   __syncthreads();
   const float block_top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
   // exp(x - top) = exp2(x c - top c): one fma with top c rounded, whose rounding (exact by another fma) is taken
@@ -173,22 +197,28 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  keep_packed(v);
   const float sum = wave_reduce((part[0] + part[1]) + (part[2] + part[3]), [](float p, float q) { return p + q; });
   if ((tid & 63) == 0) wave_sum[wave] = sum;
   const float limit = order_value(max(max(wave_code[0], wave_code[1]), max(wave_code[2], wave_code[3])));
+  // The vectors with an element that reaches the limit are noted, and their elements looked at one a thread, from
+  // memory: tests of all elements in the registers were a third of the instructions.
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (most[j] >= limit) {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const float y = element(v[j], e, E());
-        if (y >= limit && y > -INFINITY) {
-          const int n = __hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          if (n < kCap) keys[n] = list_key(y, token_of(j) + e);
-        }
-      }
+    if (most[j] >= limit && most[j] > -INFINITY) {
+      const int n = __hip_atomic_fetch_add(&noted, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      vectors[n] = (uint16_t)(j * 256 + tid);
     }
+  __syncthreads();
+  const int start = chunk * (256 * NV * kVec);
+  for (int i = tid; i < noted * kVec; i += 256) {
+    const int at = start + vectors[i / kVec] * kVec, token = max(min(at, a.V - kVec), 0) + i % kVec;
+    if (token < at || token >= a.V) continue;  // another vector's, or past the end
+    const float y = (float)x[token];
+    if (y >= limit && y > -INFINITY) {
+      const int n = __hip_atomic_fetch_add(&found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (n < kCap) keys[n] = list_key(y, token);
+    }
+  }
   __syncthreads();
   if (tid == 0) {
     const float total = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
@@ -286,7 +316,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
     double s = 0.0;
     for (int c = lane; c < a.chunks; c += kBeamLanes) {
       const f32x2 ms = sums[c];
-      s += ms[0] == -INFINITY && ms[1] == 0.f ? 0.0 : (double)ms[1] * exp((double)ms[0] - (double)m);
+      s += ms[0] == -INFINITY && ms[1] == 0.f ? 0.0 : (double)ms[1] * (double)fast_exp2((ms[0] - m) * kLog2e);  // 1 for the largest piece
     }
 #pragma unroll
     for (int off = 1; off < kBeamLanes; off <<= 1) s += __shfl_xor(s, off, 64);
@@ -319,13 +349,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = fmaxf(top, thread_best[(tid & 63) + 64 * i]);
-  const uint32_t code = order_code(top);
-  uint32_t reach = 0;
-#pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t next = reach | 1u << bit;
-    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(code >= next)) >= a.K) reach = next;
-  }
+  const uint32_t reach = wave_kth<0>(order_code(top), a.K);
   const float limit = order_value(reach);
   auto reaches = [&](const Choice& c) __attribute__((always_inline)) { return c.place != none.place && (float)c.score >= limit; };
   auto note = [&](int list) __attribute__((always_inline)) {
