@@ -502,46 +502,52 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
   const float c2 = a.scale_log2;
   const TileLanes<D> tl(lane);
 
+  // kSteps 32-state halves at a time: both at head_dim 128, whose MFMAs then run beside more independent work, one
+  // at head_dim 64, where half the scores let four waves share a SIMD.
+  constexpr int kSteps = D == 64 ? 1 : 2;
   auto compute = [&](int kt, const bf16_t* sK, const bf16_t* sV) {
-    f32x16 st[2], dpt[2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      st[mt] = f32x16{};
-      dpt[mt] = f32x16{};
+    for (int m0 = 0; m0 < 2; m0 += kSteps) {
+      f32x16 st[kSteps], dpt[kSteps];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int o = tl.op_base + mt * 32 * L::kRowElems + ks * 16;
-        st[mt] = mfma32(*(const bf16x8*)&sK[o], qf[ks], st[mt]);
-        dpt[mt] = mfma32(*(const bf16x8*)&sV[o], dof[ks], dpt[mt]);
+      for (int mt = 0; mt < kSteps; ++mt) {
+        st[mt] = f32x16{};
+        dpt[mt] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int o = tl.op_base + (m0 + mt) * 32 * L::kRowElems + ks * 16;
+          st[mt] = mfma32(*(const bf16x8*)&sK[o], qf[ks], st[mt]);
+          dpt[mt] = mfma32(*(const bf16x8*)&sV[o], dof[ks], dpt[mt]);
+        }
       }
-    }
-    if (kt * kBlockK + kBlockK > nk) {  // no P past the states: exp2(0 - lse2) may overflow
-      __asm__ volatile("");
-      const int left = nk - kt * kBlockK - 4 * hi;
+      if (kt * kBlockK + kBlockK > nk) {  // no P past the states: exp2(0 - lse2) may overflow
+        __asm__ volatile("");
+        const int left = nk - kt * kBlockK - 32 * m0 - 4 * hi;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < kSteps; ++mt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * mt + 8 * (r >> 2) + (r & 3) >= left) st[mt][r] = -INFINITY;
-    }
-    bf16x8 sf[4];
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      f32x8 t;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int mt = kk >> 1, r = (kk & 1) * 8 + e;
-        t[e] = fast_exp2(__builtin_fmaf(st[mt][r], c2, -lse2)) * (dpt[mt][r] - dlt);
+          for (int r = 0; r < 16; ++r)
+            if (32 * mt + 8 * (r >> 2) + (r & 3) >= left) st[mt][r] = -INFINITY;
       }
-      sf[kk] = to_bf16x8(t);
-    }
+      bf16x8 sf[2 * kSteps];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+      for (int kk = 0; kk < 2 * kSteps; ++kk) {
+        f32x8 t;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const bf16_t* kp = &sK[tl.tr_base + kk * 16 * L::kRowElems + dt * 32];
-        dqacc[dt] = mfma32(cat8(lds_read_tr16(kp), lds_read_tr16(kp + L::kTrSecond)), sf[kk], dqacc[dt]);
+        for (int e = 0; e < 8; ++e) {
+          const int mt = kk >> 1, r = (kk & 1) * 8 + e;
+          t[e] = fast_exp2(__builtin_fmaf(st[mt][r], c2, -lse2)) * (dpt[mt][r] - dlt);
+        }
+        sf[kk] = to_bf16x8(t);
       }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int kk = 0; kk < 2 * kSteps; ++kk) {
+          const bf16_t* kp = &sK[tl.tr_base + (2 * m0 + kk) * 16 * L::kRowElems + dt * 32];
+          dqacc[dt] = mfma32(cat8(lds_read_tr16(kp), lds_read_tr16(kp + L::kTrSecond)), sf[kk], dqacc[dt]);
+        }
+    }
   };
   for (int kt = 0; kt < nkt; kt += 2) {
     wait_vmem();
@@ -584,7 +590,10 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void cross_dq_kernel(const CrossArgs a) {
+constexpr int kDqWaves = D == 64 ? 4 : 2;  // waves per SIMD = workgroups per CU
+template <int D>
+__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads), amdgpu_waves_per_eu(kDqWaves<D>, kDqWaves<D>))) void cross_dq_kernel(
+    const CrossArgs a) {
   cross_dq_body<D>(a);
 }
 template __global__ void cross_dq_kernel<64>(const CrossArgs);
