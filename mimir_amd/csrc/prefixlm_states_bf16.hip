@@ -32,6 +32,8 @@ struct StatesArgs {
   int shares;
   float scale_log2;
   float *part_o, *part_ml;  // [row tile][2 shares][Hkv][rows of a tile](D | maximum in log2, sum)
+  int4* where;              // of each request, by the first workgroup: first share, shares (0: no states), whether it
+                            // begins its first share
 };
 
 // The line of units, 64 requests at a time, one a lane.
@@ -115,6 +117,16 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
   const int total = line_length(a.seqs, line, lane);
   const Deal deal(total, a.shares);
   const int u_begin = deal.start(share), u_end = deal.start(share + 1);
+  if (blockIdx.x == 0 && rt == 0 && wave == 0) {  // for the merge, which would look all this up again
+    int before = 0;
+    for (int s = 0; s < a.seqs.n; s += 64) {
+      if (a.seqs.n > 64) line.load(a.seqs, s, before, lane);
+      before = line.end();
+      const int u0 = line.incl - line.units, i0 = deal.share_of(u0);
+      if (s + lane < a.seqs.n)
+        a.where[s + lane] = line.units > 0 ? make_int4(i0, deal.share_of(line.incl - 1) - i0 + 1, deal.start(i0) == u0, 0) : make_int4(0, 0, 0, 0);
+    }
+  }
   if (u_begin >= u_end) return;
   if (a.seqs.n > 64) {
     int before = 0;
@@ -313,51 +325,57 @@ __device__ __forceinline__ void states_merge_body(const StatesArgs& a, int tile_
   const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = (int)(id / (uint32_t)a.rows), r = (int)(id - pair * (uint32_t)a.rows), s = pair / a.Hkv, hk = pair - s * a.Hkv;
   if (s >= a.seqs.n) return;
-  Line line;
-  int total = 0, u0 = 0, u1 = 0;
-  for (int c = 0; c < a.seqs.n; c += 64) {
-    line.load(a.seqs, c, total, lane);
-    total = line.end();
-    if (s >= c && s < c + 64) {
-      u1 = __builtin_amdgcn_readlane(line.incl, s - c);
-      u0 = u1 - __builtin_amdgcn_readlane(line.units, s - c);
-    }
-  }
+  const int4 where = a.where[s];
+  const int i0 = where.x, n = where.y;
   const int t = r / a.group, col = lane % kLanes * 4, sub = lane / kLanes;
   bf16_t* const orow = a.o + ((int64_t)s * a.seqs.per_seq + t) * a.o_st + (int64_t)(hk * a.group + r - t * a.group) * a.o_sh;
-  if (u0 == u1) {
+  if (n == 0) {
     if (sub == 0) *(bf16x4*)&orow[col] = bf16x4{};
     return;
   }
-  const Deal deal(total, a.shares);
-  // the shares that hold it, none of them empty: a line of fewer units than shares fills the first ones
-  const int i0 = deal.share_of(u0), n = deal.share_of(u1 - 1) - i0 + 1;
   if (n == 1) return;  // finished in its share
   const int tile = r / tile_rows;
-  // shares after the first begin inside the request: theirs is the part of their first request
-  auto slot = [&](int i) __attribute__((always_inline)) {
-    return part_slot(a, tile, i0 + i, i > 0 || deal.start(i0) == u0, hk, tile_rows) + r - tile * tile_rows;
-  };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, a.part_ml[slot(i) * 2]);
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+  // Shares after the first begin inside the request: theirs is the part of their first request.  None is empty: a line
+  // of fewer units than shares fills the first ones.  The parts' maxima are met on the way, so that one round trip
+  // brings all there is to load.
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float lsum = 0.f;
-#pragma unroll 8
-  for (int i = sub; i < n; i += kParts) {
-    const int64_t at = slot(i);
-    const f32x2 ml = *(const f32x2*)&a.part_ml[at * 2];
-    const f32x4 o = *(const f32x4*)&a.part_o[at * D + col];
-    const float w = fast_exp2(ml[0] - M);
-    lsum += ml[1] * w;
-    acc += o * w;
+  float M = -INFINITY, lsum = 0.f;
+  auto add = [&](f32x2 ml, f32x4 o) __attribute__((always_inline)) {
+    const float top = fmaxf(M, ml[0]);
+    const float old = M == -INFINITY ? 0.f : fast_exp2(M - top), w = ml[0] == -INFINITY ? 0.f : fast_exp2(ml[0] - top);
+    lsum = lsum * old + ml[1] * w;
+    acc = acc * old + o * w;
+    M = top;
+  };
+  constexpr int kAhead = 8;
+  for (int i = sub; i < n; i += kAhead * kParts) {
+    f32x2 ml[kAhead];
+    f32x4 o[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int part = min(i + e * kParts, n - 1);  // past the last: that one again
+      const int64_t at = part_slot(a, tile, i0 + part, part > 0 || where.z != 0, hk, tile_rows) + r - tile * tile_rows;
+      ml[e] = *(const f32x2*)&a.part_ml[at * 2];
+      o[e] = *(const f32x4*)&a.part_o[at * D + col];
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      if (i + e * kParts < n) add(ml[e], o[e]);
   }
 #pragma unroll
   for (int off = kLanes; off < 64; off <<= 1) {
-    lsum += __shfl_xor(lsum, off, 64);
+    f32x2 ml = {__shfl_xor(M, off, 64), __shfl_xor(lsum, off, 64)};
+    f32x4 o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], off, 64);
+    for (int e = 0; e < 4; ++e) o[e] = __shfl_xor(acc[e], off, 64);
+    // (max, sum, row) of both groups joined the same way round on either side
+    const bool low = (lane & off) == 0;
+    const f32x2 own = {M, lsum};
+    const f32x4 mine = acc;
+    M = low ? own[0] : ml[0];
+    lsum = low ? own[1] : ml[1];
+    acc = low ? mine : o;
+    add(low ? ml : own, low ? o : mine);
   }
   if (sub == 0) *(bf16x4*)&orow[col] = __builtin_convertvector(acc * (1.f / lsum), bf16x4);
 }
@@ -384,7 +402,7 @@ struct StatesPlan {
   int pitch;   // of a cache row, in positions
   int cap;     // entries of its list
   int rows, tile_rows, row_tiles, shares;
-  size_t ml, total;  // workspace: parts' rows, then maxima and sums
+  size_t ml, where, total;  // workspace: parts' rows, then maxima and sums, then the requests' shares
 };
 StatesPlan states_plan(const MimirStatesParams& p) {
   StatesPlan s = {};
@@ -407,7 +425,8 @@ StatesPlan states_plan(const MimirStatesParams& p) {
   s.shares = (int)std::min<int64_t>(std::max(units, (int64_t)1), std::max(groups / (p.num_kv_heads * s.row_tiles), 1));
   const size_t part_rows = (size_t)s.row_tiles * s.shares * 2 * p.num_kv_heads * s.tile_rows;
   s.ml = align_up(part_rows * p.head_dim * sizeof(float));
-  s.total = s.ml + align_up(part_rows * 2 * sizeof(float));
+  s.where = s.ml + align_up(part_rows * 2 * sizeof(float));
+  s.total = s.where + align_up((size_t)p.requests * sizeof(int4));
   return s;
 }
 bool states_sizes(const MimirStatesParams* p) {
@@ -501,6 +520,7 @@ extern "C" int mimir_prefixlm_states_attn(const MimirStatesParams* p, void* stre
     a.scale_log2 = p->softmax_scale * kLog2e;
     a.part_o = (float*)p->workspace;
     a.part_ml = (float*)((char*)p->workspace + plan.ml);
+    a.where = (int4*)((char*)p->workspace + plan.where);
     const int64_t merge = ((int64_t)p->requests * p->num_kv_heads * plan.rows + 3) / 4, groups = (int64_t)plan.shares * p->num_kv_heads;
     if (merge > kMaxGroups || groups > kMaxGroups || plan.row_tiles > 65535) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one launch");
     const dim3 grid((unsigned)groups, (unsigned)plan.row_tiles), threads(kShareWaves * 64);
