@@ -174,14 +174,17 @@ def attention_to_states(query: Tensor, states: Cache, state_lengths: Tensor, sta
     for name, t in (("keys", states.keys), ("values", states.values)):
         if t.stride(-1) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3)):
             raise ValueError(f"the cached {name} need a unit head_dim stride and 16-byte aligned rows")
+        if length > 1 and t.stride(1) < d:
+            raise ValueError(f"the cached {name} need a position stride of at least head_dim, got {t.stride(1)}")
     if P._validate_metadata and state_rows is not None and requests:
         if bool(((state_rows < 0) | (state_rows >= pool)).any()):
             raise IndexError(f"state_rows must lie in [0, {pool})")
     out = torch.empty((B, S, hq, d), dtype=query.dtype, device=query.device)
     if B == 0 or S == 0:
         return out
-    # all tokens of a request in a row: [B * S, Hq, D]
-    if query.stride(-1) != 1 or query.data_ptr() % 16 or (B > 1 and S > 1 and query.stride(0) != S * query.stride(1)) or any(
+    # all tokens of a request in a row: [B * S, Hq, D], a token's heads no nearer than the head_dim (one expanded to many is copied)
+    token = query.stride(1 if S > 1 else 0)
+    if query.stride(-1) != 1 or query.data_ptr() % 16 or (B > 1 and S > 1 and query.stride(0) != S * token) or (B * S > 1 and token < d) or any(
             query.shape[i] > 1 and query.stride(i) % 8 for i in range(3)):
         query = P._own_copy(query)
     state_lengths = state_lengths.contiguous()

@@ -296,6 +296,19 @@ def test_state_layouts(device):
     _check_states(odd, cache, lens, None)
 
 
+def test_expanded_queries(device):
+    """One query for all batch rows, for all tokens, for all heads: strides of 0 (read as given)."""
+    q, cache, lens, _ = _states(device, 3, 2, 1, 4, 2, 64, 3, 90, [90, 5, 70], None)
+    a = _check_states(q[:1].expand(6, -1, -1, -1), cache, lens, None)
+    assert torch.equal(a, attention_to_states(q[:1].repeat(6, 1, 1, 1), cache, lens))
+    _check_states(q.expand(-1, 5, -1, -1), cache, lens, None)
+    _check_states(q[:1].expand(6, 5, -1, -1), cache, lens, None)
+    _check_states(q[:, :, :1].expand(-1, -1, 4, -1), cache, lens, None)
+    one = Cache(*(t[:, :1].expand(-1, 90, -1, -1) for t in cache))  # one state at all positions
+    with pytest.raises(ValueError, match="position stride"):
+        attention_to_states(q, one, lens)
+
+
 def test_states_agree_with_packed_queries(device):
     q, cache, lens, rows = _states(device, 2, 4, 1, 16, 4, 128, 2, 600, [600, 345], None)
     out = attention_to_states(q, cache, lens)
