@@ -102,6 +102,25 @@ def _cache_rows(name: str, t: Tensor, like: Tensor) -> None:
         raise ValueError(f"the rows of {name} must be contiguous and apart")
 
 
+def _check_all(tensors, rows: int) -> None:
+    """What one launch refuses of its tensors, for all of several: nothing runs before a refusal."""
+    spans = []
+    for t in tensors:
+        row, step = t[0].numel() * t.element_size(), t.stride(0) * t.element_size()
+        if t.data_ptr() % 16 or step % 16:
+            raise ValueError("cache rows must be aligned to 16 bytes")
+        spans.append((t.data_ptr(), row, step))
+    spans.sort()
+    for i, (a, row, step) in enumerate(spans):
+        for b, _, other in spans[i + 1:]:
+            if b >= a + (rows - 1) * step + row:
+                break
+            # rows of equal stride: the one at or before the other's first, and the next
+            at, off = divmod(b - a, step)
+            if step != other or off < row or (step - off < row and at + 1 < rows):
+                raise ValueError("cache tensors must not share memory, and lie in each other's gaps with one stride only")
+
+
 def reorder_rows(caches: Union[Cache, Sequence[Cache]], lengths: Tensor, source: Tensor) -> None:
     """Give row ``i`` of every cache the state of row ``source.flatten()[i]``, in place, as all were before the call:
     the first ``lengths[source[i]]`` positions of its keys and values, and in ``lengths`` (int32 or int64) its length.
@@ -145,6 +164,8 @@ def reorder_rows(caches: Union[Cache, Sequence[Cache]], lengths: Tensor, source:
     p.index_int64, p.source_int64 = int(lengths.dtype == torch.int64), int(source.dtype == torch.int64)
     lib = _capi.load()
     step = _capi.REORDER_TENSORS
+    if len(tensors) > step and rows > 0 and tensors[0].shape[1] > 0:
+        _check_all(tensors, rows)
     with torch.cuda.device(lengths.device):
         for i in range(0, max(len(tensors), 1), step):
             part = tensors[i:i + step]

@@ -250,6 +250,26 @@ def test_reorder_layouts(device):
     assert (lengths[:3] == lengths[0]).all()
 
 
+def test_reorder_of_many_layers(device):
+    """More tensors than one launch takes: nothing has moved where one of the later ones is refused."""
+    gen = torch.Generator().manual_seed(5)
+    lengths, source = torch.tensor([9, 5, 3, 9], device=device), torch.tensor([[1, 0], [2, 2]], device=device)
+    hold = torch.randn(4, 20, 2, 9, 1, 64, generator=gen).to(device)  # all layers' rows side by side
+    caches = [Cache(hold[:, i, 0], hold[:, i, 1]) for i in range(20)]
+    _check_reorder(caches, lengths.clone(), source)
+    caches = _caches(gen, device, 10, 4, 9, 1, 64)
+    before = [t.clone() for c in caches for t in c]
+    wide = torch.zeros(4, 9 * 64 + 4, device=device, dtype=torch.bfloat16)[:, :9 * 64].view(4, 9, 1, 64)  # rows off 16 bytes
+    apart = torch.zeros(2, 4, 9, 1, 64, device=device, dtype=torch.bfloat16)
+    flat = torch.zeros(9 * 4 * 64 + 64, device=device, dtype=torch.bfloat16)
+    half = Cache(*(flat[n:n + 9 * 4 * 64].view(4, 9, 1, 64) for n in (0, 64)))  # a position apart
+    for bad in (caches[0], Cache(apart[0], apart[0]), Cache(wide, apart[1]), half):
+        given = lengths.clone()
+        with pytest.raises(ValueError):
+            reorder_rows([*caches, bad], given, source)
+        assert torch.equal(given, lengths) and all(torch.equal(t, y) for t, y in zip((t for c in caches for t in c), before))
+
+
 def test_reorder_refusals(device):
     from mimir_amd import set_validate_metadata
 
