@@ -3,6 +3,8 @@
 // (prefixlm_states_bf16.hip).
 #pragma once
 
+#include <algorithm>
+
 #include "prefixlm_common.h"
 
 namespace mimir {
@@ -63,7 +65,9 @@ constexpr int kSplitStates = 64;
 
 constexpr int kCrossTile = 128;  // query rows or states of a tile
 // Entries of a list for any packing of `total` rows into n sequences.
-inline int cross_capacity(int total, int n) { return total > 0 && n > 0 ? (int)(((int64_t)total + kCrossTile - 1) / kCrossTile + n) : 0; }
+inline int cross_capacity(int total, int n) {
+  return total > 0 && n > 0 ? (int)std::min<int64_t>(((int64_t)total + kCrossTile - 1) / kCrossTile + n, 0x7fffffff) : 0;
+}
 
 // A query tile of the list (rows 0: padding) and its head.  Unit = list entry * Hkv + kv head on XCD unit % 8, its
 // query heads at consecutive slots there: they read the same K and V through one L2.

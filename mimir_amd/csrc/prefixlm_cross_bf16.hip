@@ -403,6 +403,10 @@ int check_cross(const MimirCrossParams* p, bool backward) {
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "a token's query heads must hold fewer than 2^22 elements");
   if ((int64_t)p->total_q * p->num_q_heads > 0x7fffffff || (int64_t)p->total_k * p->num_q_heads > 0x7fffffff)
     return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one call");
+  // a workgroup of 256 threads per query tile and head, one of up to 512 per tile of states and kv head
+  if ((int64_t)cross_capacity(p->total_q, p->numseqs) * p->num_q_heads > kMaxGroups - kXcds * p->num_q_heads ||
+      (backward && (int64_t)cross_capacity(p->total_k, p->numseqs) * p->num_kv_heads > kMaxGroups / 2))
+    return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many sequences for one launch");
   if (p->numseqs > 0 && (p->cu_seqlens_q == nullptr || p->cu_seqlens_k == nullptr))
     return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "cu_seqlens is NULL");
   struct Tensor {

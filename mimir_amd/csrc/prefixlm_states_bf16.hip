@@ -298,8 +298,8 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
         if (rr >= n_rows) break;
         const f32x2 p = *ml_of(0, rr), q = *ml_of(1, rr);
         const float M = fmaxf(p[0], q[0]);
-        // the second wave may have had no tile: maximum -inf, sum 0
-        const float wp = fast_exp2(p[0] - M), wq = q[0] == -INFINITY ? 0.f : fast_exp2(q[0] - M);
+        // a wave may have had no tile, or only scores of -inf: maximum -inf, sum 0
+        const float wp = p[0] == -INFINITY ? 0.f : fast_exp2(p[0] - M), wq = q[0] == -INFINITY ? 0.f : fast_exp2(q[0] - M);
         const float lsum = p[1] * wp + q[1] * wq;
         const f32x4 acc = *(const f32x4*)&area(0)[rr * kPitch + col] * wp + *(const f32x4*)&area(1)[rr * kPitch + col] * wq;
         if (whole) {
@@ -487,6 +487,8 @@ extern "C" int mimir_prefixlm_states_attn(const MimirStatesParams* p, void* stre
   const int group = p->num_q_heads / p->num_kv_heads;
   hipError_t e;
   if (plan.tiles) {
+    if ((int64_t)plan.cap * p->num_q_heads > kMaxGroups - kXcds * p->num_q_heads)
+      return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one launch");
     CrossArgs a = {};
     a.q = (const bf16_t*)p->q; a.k = (const bf16_t*)p->keys; a.v = (const bf16_t*)p->values;
     a.o = (bf16_t*)p->out;

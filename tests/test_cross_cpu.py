@@ -67,6 +67,22 @@ def test_c_backward_refusals(kw):
         _capi.raise_for_status(lib, lib.mimir_prefixlm_cross_bwd(ctypes.byref(_cross(**kw)), None))
 
 
+@pytest.mark.parametrize("backward,kw", [(False, dict(total_q=1, numseqs=1 << 24)), (False, dict(total_q=0x3fffffff, numseqs=1 << 23)),
+                                         (True, dict(total_q=0, numseqs=1 << 23)), (True, dict(numseqs=0x7fffffff))])
+def test_c_launches_of_2_to_the_32_threads_are_refused(backward, kw):
+    lib = _capi.load()
+    p = _cross(**{**kw, "workspace_bytes": 1 << 40})
+    with pytest.raises(ValueError, match="too many"):
+        _capi.raise_for_status(lib, (lib.mimir_prefixlm_cross_bwd if backward else lib.mimir_prefixlm_cross_fwd)(ctypes.byref(p), None))
+
+
+def test_c_states_launches_of_2_to_the_32_threads_are_refused():
+    lib = _capi.load()
+    p = _states(requests=1 << 23, seq_tokens=130, num_q_heads=1, workspace_bytes=1 << 40)
+    with pytest.raises(ValueError, match="too many"):
+        _capi.raise_for_status(lib, lib.mimir_prefixlm_states_attn(ctypes.byref(p), None))
+
+
 def test_cross_workspace():
     lib = _capi.load()
     size = lambda b, **kw: lib.mimir_prefixlm_cross_workspace_bytes(ctypes.byref(_cross(**kw)), b)  # noqa: E731

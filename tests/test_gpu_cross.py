@@ -296,6 +296,19 @@ def test_state_layouts(device):
     _check_states(odd, cache, lens, None)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lost", [(0, 64), (0, 700), (32, 64), (100, 900), (300, 1000)])
+def test_states_with_scores_of_minus_infinity(device, d, lost):
+    """Keys that give -inf take no part, in one part of the states or over whole parts of them."""
+    q, cache, lens, _ = _states(device, 1, 2, 1, 4, 2, d, 1, 1000, [1000], None)
+    q[..., 0] = 1.0
+    cache.keys[:, lost[0]:lost[1], :, 0] = -float("inf")
+    _check_states(q, cache, lens, None)
+    lists = [torch.tensor([0, n], device=device) for n in (2, 1000)]
+    _near(cross_attention(q[:, 0], cache.keys[0], cache.values[0], *lists),
+          tuple(t[:, 0] for t in O.attention_to_states(q, cache.keys, cache.values, [1000], [0], 1 / math.sqrt(d))), 1.0, "out")
+
+
 def test_expanded_queries(device):
     """One query for all batch rows, for all tokens, for all heads: strides of 0 (read as given)."""
     q, cache, lens, _ = _states(device, 3, 2, 1, 4, 2, 64, 3, 90, [90, 5, 70], None)
