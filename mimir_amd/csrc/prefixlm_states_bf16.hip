@@ -91,7 +91,8 @@ __device__ __forceinline__ void lds_barrier() {  // for LDS data alone: copies a
   __asm__ volatile("" ::: "memory");
 }
 
-template <int D, int NT>
+// kOnce: the states are read past the caches (the builtin's bit for streaming).
+template <int D, int NT, bool kOnce>
 __device__ __forceinline__ void states_body(const StatesArgs& a) {
   constexpr int DT = D / 32, KS = D / 16;
   using L = TileLayout<D>;
@@ -169,10 +170,10 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
       const __amdgpu_buffer_rsrc_t rv = make_rsrc(vbase + key0 * a.v_st, rows_bytes32(n, (uint32_t)a.v_st, D));
 #pragma unroll
       for (int e = 0; e < kInst; ++e)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(tk + e * 512), 16, voffk[e], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(tk + e * 512), 16, voffk[e], 0, 0, kOnce ? 2 : 0);
 #pragma unroll
       for (int e = 0; e < kInst; ++e)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(tv + e * 512), 16, voffv[e], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(tv + e * 512), 16, voffv[e], 0, 0, kOnce ? 2 : 0);
     };
     // Q^T B-operand fragments; lanes past the rows take the last row: their columns are not read
     bf16x8 qf[NT][KS];
@@ -380,28 +381,35 @@ __device__ __forceinline__ void states_merge_body(const StatesArgs& a, int tile_
   if (sub == 0) *(bf16x4*)&orow[col] = __builtin_convertvector(acc * (1.f / lsum), bf16x4);
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kOnce>
 __global__ __launch_bounds__(kShareWaves * 64, 1) void states_kernel(const StatesArgs a) {
-  states_body<D, NT>(a);
+  states_body<D, NT, kOnce>(a);
 }
 template <int D>
 __global__ __launch_bounds__(256) void states_merge_kernel(const StatesArgs a, int tile_rows) {
   states_merge_body<D>(a, tile_rows);
 }
 // By name: of several instantiations launched below, this toolchain drops host stubs.
-template __global__ void states_kernel<64, 1>(const StatesArgs);
-template __global__ void states_kernel<64, 2>(const StatesArgs);
-template __global__ void states_kernel<128, 1>(const StatesArgs);
-template __global__ void states_kernel<128, 2>(const StatesArgs);
+template __global__ void states_kernel<64, 1, false>(const StatesArgs);
+template __global__ void states_kernel<64, 1, true>(const StatesArgs);
+template __global__ void states_kernel<64, 2, false>(const StatesArgs);
+template __global__ void states_kernel<128, 1, false>(const StatesArgs);
+template __global__ void states_kernel<128, 1, true>(const StatesArgs);
+template __global__ void states_kernel<128, 2, false>(const StatesArgs);
 template __global__ void states_merge_kernel<64>(const StatesArgs, int);
 template __global__ void states_merge_kernel<128>(const StatesArgs, int);
 
+// States of a launch that read past the caches where one row tile reads them, once: more than the 256 MiB in front of
+// memory cannot be found there by the next step.  48 requests of 300 to 4096 states, 4 kv heads of 128, other states each
+// time: 60.2 us with the caches, 54.2 past them (the same states each time: 48.9 and 53.9).  Two row tiles: 99 and 108.
+constexpr int64_t kOnceBytes = (int64_t)256 << 20;
 constexpr int kManyRows = 128;  // more rows per kv head than this: the tile kernel
 struct StatesPlan {
   bool tiles;  // the tile kernel
   int pitch;   // of a cache row, in positions
   int cap;     // entries of its list
   int rows, tile_rows, row_tiles, shares;
+  bool once;   // the states are read past the caches
   size_t ml, where, total;  // workspace: parts' rows, then maxima and sums, then the requests' shares
 };
 StatesPlan states_plan(const MimirStatesParams& p) {
@@ -423,6 +431,7 @@ StatesPlan states_plan(const MimirStatesParams& p) {
   const int64_t units = (int64_t)p.requests * ((p.cache_len + kUnit - 1) / kUnit);
   const int groups = p.head_dim == 64 ? 2 * kShareGroups : kShareGroups;
   s.shares = (int)std::min<int64_t>(std::max(units, (int64_t)1), std::max(groups / (p.num_kv_heads * s.row_tiles), 1));
+  s.once = s.tile_rows == 32 && (int64_t)p.requests * p.cache_len * p.num_kv_heads * p.head_dim * 4 >= kOnceBytes;
   const size_t part_rows = (size_t)s.row_tiles * s.shares * 2 * p.num_kv_heads * s.tile_rows;
   s.ml = align_up(part_rows * p.head_dim * sizeof(float));
   s.where = s.ml + align_up(part_rows * 2 * sizeof(float));
@@ -527,11 +536,13 @@ extern "C" int mimir_prefixlm_states_attn(const MimirStatesParams* p, void* stre
     if (merge > kMaxGroups || groups > kMaxGroups || plan.row_tiles > 65535) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many rows for one launch");
     const dim3 grid((unsigned)groups, (unsigned)plan.row_tiles), threads(kShareWaves * 64);
     const hipStream_t s = (hipStream_t)stream;
-    const bool two = plan.tile_rows == 64;
-    if (p->head_dim == 128 && two) hipLaunchKernelGGL((states_kernel<128, 2>), grid, threads, 0, s, a);
-    else if (p->head_dim == 128) hipLaunchKernelGGL((states_kernel<128, 1>), grid, threads, 0, s, a);
-    else if (two) hipLaunchKernelGGL((states_kernel<64, 2>), grid, threads, 0, s, a);
-    else hipLaunchKernelGGL((states_kernel<64, 1>), grid, threads, 0, s, a);
+    const bool two = plan.tile_rows == 64, wide = p->head_dim == 128;
+    if (two && wide) hipLaunchKernelGGL((states_kernel<128, 2, false>), grid, threads, 0, s, a);
+    else if (two) hipLaunchKernelGGL((states_kernel<64, 2, false>), grid, threads, 0, s, a);
+    else if (wide && plan.once) hipLaunchKernelGGL((states_kernel<128, 1, true>), grid, threads, 0, s, a);
+    else if (wide) hipLaunchKernelGGL((states_kernel<128, 1, false>), grid, threads, 0, s, a);
+    else if (plan.once) hipLaunchKernelGGL((states_kernel<64, 1, true>), grid, threads, 0, s, a);
+    else hipLaunchKernelGGL((states_kernel<64, 1, false>), grid, threads, 0, s, a);
     e = hipGetLastError();
     if (e == hipSuccess) {
       if (p->head_dim == 128) hipLaunchKernelGGL(states_merge_kernel<128>, dim3((unsigned)merge), dim3(256), 0, s, a, plan.tile_rows);

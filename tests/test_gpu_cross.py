@@ -309,6 +309,21 @@ def test_states_with_scores_of_minus_infinity(device, d, lost):
           tuple(t[:, 0] for t in O.attention_to_states(q, cache.keys, cache.values, [1000], [0], 1 / math.sqrt(d))), 1.0, "out")
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("requests", [1, 700])
+def test_states_past_the_caches(device, d, requests):
+    """A cache of 2^28 bytes and more (by its rows and positions) of which little is held, or all by one request."""
+    length = (1 << 28) // (requests * 4 * d) + 1
+    if requests == 1:
+        q, cache, lens, _ = _states(device, 1, 1, 1, 1, 1, d, 1, length, [length], None)
+        keys, values = cache.keys[0, :, 0].double().cpu(), cache.values[0, :, 0].double().cpu()
+        p = torch.softmax(keys @ q[0, 0, 0].double().cpu() / math.sqrt(d), dim=0)
+        _near(attention_to_states(q, cache, lens)[0, 0, 0], (p @ values, p @ values.abs()), 1.0, "out")
+        return
+    lens = [min(length, (37 * i) % 300) for i in range(requests)]
+    _check_states(*_states(device, requests, 2, 1, 2, 1, d, requests, length, lens, None))
+
+
 def test_expanded_queries(device):
     """One query for all batch rows, for all tokens, for all heads: strides of 0 (read as given)."""
     q, cache, lens, _ = _states(device, 3, 2, 1, 4, 2, 64, 3, 90, [90, 5, 70], None)
