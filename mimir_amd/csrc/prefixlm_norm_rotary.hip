@@ -292,16 +292,17 @@ __global__ __launch_bounds__(256) void norm_rotary_bwd_kernel(const NormRotaryAr
     for (int n = (int)threadIdx.x; n < a.lanes * 2 * V; n += 256) {
       const int e = n / a.lanes, lane = n % a.lanes;
       if (lane >= a.items) continue;
-      float s = 0.f;
+      double s = 0.0;
       for (int j = 0; j < per_block; ++j) s += sums[e * 256 + j * a.lanes + lane];
       Item<V, kInterleaved> o;
       o.place(a, lane);
-      out[e < V ? o.d1 + e : o.d2 + e - V] = s;
+      out[e < V ? o.d1 + e : o.d2 + e - V] = (float)s;
     }
   }
 }
 
-// The weights' gradients: the rows of partial sums added up, 16 columns a workgroup.
+// The weights' gradients: the rows of partial sums added up, 16 columns a workgroup, in 64 bits (in 32 the error of
+// 8 x 2048 tokens of 16 heads was 1.9e-7, three times that of one rounding).
 constexpr int kSumCols = 16, kSumRows = 1024 / kSumCols;
 struct WeightSumArgs {
   const float* part;
@@ -309,10 +310,10 @@ struct WeightSumArgs {
   int rows, D, w32;
 };
 __global__ __launch_bounds__(1024) void norm_weight_sum_kernel(const WeightSumArgs a) {
-  __shared__ float sums[kSumRows][kSumCols + 1];
+  __shared__ double sums[kSumRows][kSumCols + 1];
   const int c = threadIdx.x % kSumCols, r0 = threadIdx.x / kSumCols;
   const int col = blockIdx.x * kSumCols + c;
-  float s = 0.f;
+  double s = 0.0;
   if (col < 2 * a.D) {
 #pragma unroll 8
     for (int r = r0; r < a.rows; r += kSumRows) s += a.part[(int64_t)r * 2 * a.D + col];
@@ -327,9 +328,9 @@ __global__ __launch_bounds__(1024) void norm_weight_sum_kernel(const WeightSumAr
   void* const out = a.out[col / a.D];
   if (out == nullptr) return;
   if (a.w32)
-    ((float*)out)[col % a.D] = sums[0][c];
+    ((float*)out)[col % a.D] = (float)sums[0][c];
   else
-    ((bf16_t*)out)[col % a.D] = (bf16_t)sums[0][c];
+    ((bf16_t*)out)[col % a.D] = (bf16_t)(float)sums[0][c];
 }
 
 // By name: of several instantiations launched below, this toolchain drops host stubs.

@@ -307,8 +307,8 @@ def norm_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, frequen
     ``turn(x / sqrt(mean(x^2) + eps) * weight)`` with the mean over all of the head.
 
     Returns ``(query, key)``, new tensors; gradients for the heads and the weights, which are float32 or of the
-    heads' type, both the same.  fp32 arithmetic, one rounding; the weights' gradients are fp32 sums in a fixed
-    order.  Positions, frequencies and strides as for :func:`rotary`.
+    heads' type, both the same.  fp32 arithmetic, one rounding; the weights' gradients are summed in a fixed order,
+    across workgroups in 64 bits.  Positions, frequencies and strides as for :func:`rotary`.
     """
     if query.is_cuda:
         res = _capi.host().norm_rotary(query, key, positions, *frequencies, query_weight, key_weight, eps, P._stream(query.device))
