@@ -250,6 +250,22 @@ def test_reorder_layouts(device):
     assert (lengths[:3] == lengths[0]).all()
 
 
+def test_reorder_of_large_caches(device):
+    """Caches of 2^28 bytes and more, little of which is moved: stored past the caches, read by the next reordering."""
+    gen = torch.Generator().manual_seed(6)
+    length = (1 << 28) // (2 * 6 * 64 * 2) + 1
+    cache = Cache.create(6, length, 1, 64, dtype=torch.bfloat16, device=device)
+    for t in cache:
+        t[:, :700] = torch.randn(6, 700, 1, 64, generator=gen).to(device)
+    lengths = torch.tensor([700, 0, 333, 1, 699, 64], device=device)
+    for source in ([[2, 0, 0], [4, 5, 3]], [[1, 2, 0], [5, 5, 4]]):
+        source = torch.tensor(source, device=device)
+        heads = [t[:, :701].clone() for t in cache]
+        want, lens = O.reorder_rows(heads, lengths, source.cpu())
+        reorder_rows(cache, lengths, source)
+        assert all(torch.equal(t[:, :701].cpu(), y) for t, y in zip(cache, want)) and torch.equal(lengths.cpu(), lens)
+
+
 def test_reorder_of_many_layers(device):
     """More tensors than one launch takes: nothing has moved where one of the later ones is refused."""
     gen = torch.Generator().manual_seed(5)
