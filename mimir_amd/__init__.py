@@ -7,8 +7,10 @@ layer's core around it (``gated_attention``: gqkv split, RoPE, the operator and
 the sigmoid output gate of src/mimir/model/layers.py:182-239).
 
 Submodules for serving: ``mimir_amd.cache`` (attention against a static bf16 cache),
-``mimir_amd.paged`` (the same against 8-bit pages, and their bookkeeping) and
-``mimir_amd.rotary`` (rotary positions without tables, for training too).
+``mimir_amd.paged`` (the same against 8-bit pages, and their bookkeeping),
+``mimir_amd.rotary`` (rotary positions without tables, with normed heads too, for training as well),
+``mimir_amd.cross`` (attention to states of another length, packed for training or in a cache) and
+``mimir_amd.beams`` (beam search: selection, and the caches' rows in its order).
 """
 
 from .metadata import (
