@@ -462,7 +462,8 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
   const __amdgpu_buffer_rsrc_t rdo = make_rsrc(a.dout + (int64_t)item.x * a.do_st + (int64_t)h * a.do_sh, rows_bytes(rows, a.do_st, D));
   const TileLoader<D, kWaves> ldk(a.k_st, wave, lane), ldv(a.v_st, wave, lane);
   const bf16_t* i_k = a.k + (int64_t)item.z * a.k_st + (int64_t)hk * a.k_sh;
-  const bf16_t* i_v = a.v + (int64_t)item.z * a.v_st + (int64_t)hk * a.v_sh;
+  const bf16_t* const i_v0 = a.v + (int64_t)item.z * a.v_st + (int64_t)hk * a.v_sh;
+  const bf16_t* i_v = i_v0;
   int i_rows = nk;
   auto issue_next = [&](bf16_t* tk, bf16_t* tv) {
     const int n = min(i_rows, kBlockK);
@@ -494,6 +495,16 @@ __device__ __forceinline__ void cross_dq_body(const CrossArgs& a) {
       for (int e = 0; e < 8; ++e) dlt += ((float)ov[e] + (float)lv[e]) * (float)dof[ks][e];
     }
     dlt = xor32_sum(dlt);
+    if (nk == 1) {
+      // One state: O is its value and delta is dP, so dS = 0.  Taken from the product that dP comes from, here and in the
+      // dK / dV kernel, that holds exactly, and not to the rounding of two sums.
+      const __amdgpu_buffer_rsrc_t rv = make_rsrc(i_v0, rows_bytes(1, a.v_st, D));
+      f32x16 one = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        one = mfma32(__builtin_bit_cast(bf16x8, buf_load16(rv, (uint32_t)((l32 * a.v_st + 16 * ks + 8 * hi) * 2))), dof[ks], one);
+      dlt = __shfl(one[0], l32, 64);  // state 0 is the first half's
+    }
     if (hi == 0 && qrow < rows) a.delta[row_at] = dlt;
   }
   f32x16 dqacc[DT];

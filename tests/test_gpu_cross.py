@@ -117,6 +117,19 @@ def test_low_scores_do_not_overflow_past_the_end(device):
         _near(g, w, rel, name)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (8, 2, 64), (2, 2, 128), (16, 4, 128)])
+def test_one_state_has_no_score_gradient(device, hq, hkv, d):
+    """P is 1 whatever the score: dQ and dK are exactly 0, beside sequences with more states too."""
+    pairs = [(300, 1), (1, 1), (130, 1), (70, 129), (64, 2)]
+    q, k, v, do, cu_q, cu_k = _make(device, pairs, hq, hkv, d, lead=(3, 5), pad=(9, 4))
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves, *(torch.tensor(c, device=device) for c in (cu_q, cu_k)))
+    dq, dk, dv = torch.autograd.grad(out, leaves, do)
+    assert not dq[:cu_q[3]].any() and not dk[:cu_k[3]].any()
+    assert dq[cu_q[3]:cu_q[5]].any() and dk[cu_k[3]:cu_k[5]].any() and dv[5:8].any()
+    _check(device, pairs, hq, hkv, d, lead=(3, 5), pad=(9, 4))
+
+
 def test_nan_and_inf_stay_in_their_sequence(device):
     pairs = [(70, 90), (70, 90), (70, 90)]
     q, k, v, do, cu_q, cu_k = _make(device, pairs, 4, 2, 64, pad=(10, 10))
