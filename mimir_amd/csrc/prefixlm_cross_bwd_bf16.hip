@@ -7,7 +7,8 @@
 // 128 states), over all query heads of the group and all queries of the sequence, which forms S and dP again.
 // delta takes O with its low half: dS is a difference whose rounding errors would else be led by O's
 // (error of dQ and dK against 64 bits, in units of one rounding of the exact result: up to 2.3 without, 1.4 with it).
-// P and dS are rounded to bf16 for their products.  Both are bound by the matrix units.
+// P and dS are rounded to bf16 for their products.  Both are bound by the matrix units: 8 sequences of 1500 to 2048 queries over
+// 1024 to 2048 states, 16 / 4 heads of 128, dQ 279 us (0.94 PFLOP/s executed), dK / dV 402 (0.87, a fifth of it the tail).
 #include "prefixlm_cross.h"
 
 namespace mimir {

@@ -8,7 +8,8 @@
 // 32-state tile of a request in two LDS stages of its own, waiting only for its own copies.  S^T = K Q^T leaves a row in a
 // lane, P^T is the B operand of O^T += V^T P^T (prefixlm_fwd_bf16.hip); one or two sets of 32 rows
 // take part in each tile.  The waves meet in LDS; a request inside one share is finished there,
-// the parts of the others go to the workspace and states_merge_kernel adds them in order.
+// the parts of the others go to the workspace and states_merge_kernel adds them in order.  48 requests of 8 beams over 300 to
+// 4096 states, 16 / 4 heads of 128: 48.9 us (4.4 TB/s) and 6.5; one request of 1500 states 7.3 and 5.4, round trips.
 //
 // Requests of more than 128 rows go to the tile kernel of prefixlm_cross_bf16.hip instead.
 #include <algorithm>
