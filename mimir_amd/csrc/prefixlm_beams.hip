@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kMaxBeams = 32, kMaxCount = 64;
 constexpr int kCap = 1024;  // candidates ranked at once
+constexpr float kFusedTop = 4096.f;  // log2(e) times it is below 2^13, whose fp32 neighbours are 2^-11 apart
 
 struct SelectArgs {
   const void* logits;
@@ -179,8 +180,10 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const SelectArgs a) {
   __syncthreads();
   const float block_top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
   // exp(x - top) = exp2(x c - top c): one fma with top c rounded, whose rounding (exact by another fma) is taken
-  // back from the sum; c's own is one of x - top, not of x.  Where top c overflows, the difference first.
-  const bool near = fabsf(block_top) < 1e38f;
+  // back from the sum to first order; c's own is one of x - top, not of x.  That rounding grows with top: below
+  // kFusedTop it is at most 2^-12 and what the first order leaves (its half square) 2^-26 of the sum.  From there on, as in
+  // a piece that is masked with a large finite value, the difference first, which is exact for what counts in the sum.
+  const bool near = fabsf(block_top) < kFusedTop;
   const float base = block_top == -INFINITY ? 0.f : block_top, shift = near ? base * kLog2e : 0.f;
   float part[4] = {0.f, 0.f, 0.f, 0.f};
   if (near) {
@@ -286,7 +289,10 @@ __device__ __forceinline__ bool before(const Choice& p, const Choice& q) {
 constexpr int kBeamLanes = 256 / kMaxBeams;  // threads of a beam while sums are joined
 
 __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
-  __shared__ double base[kMaxBeams];  // score - lse
+  // A continuation's score is (logit - maximum) + (score - log of the sum), not through the sum of the last two: of large
+  // logits that would leave none of the score.
+  __shared__ double base[kMaxBeams];  // score - log of the sum of exp(x - maximum)
+  __shared__ float row_max[kMaxBeams];
   __shared__ int state[kMaxBeams];    // 0: no continuation, 1: by its lists, 2: ended
   __shared__ float thread_best[256];
   __shared__ int reaching[kCap];      // lists whose best reaches the limit
@@ -321,11 +327,12 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
     }
 #pragma unroll
     for (int off = 1; off < kBeamLanes; off <<= 1) s += __shfl_xor(s, off, 64);
-    const double lse = (double)m + log(s);
+    const double log_sum = log(s);
     const bool live = fabsf(score) < INFINITY;
     if (lane == 0 && tid / kBeamLanes < a.W) {
-      base[w] = ended ? (double)score : (double)score - lse;
-      state[w] = !live ? 0 : ended ? 2 : fabs(lse) < INFINITY ? 1 : 0;
+      base[w] = ended ? (double)score : (double)score - log_sum;
+      row_max[w] = m;
+      state[w] = !live ? 0 : ended ? 2 : fabsf(m) < INFINITY && fabs(log_sum) < INFINITY ? 1 : 0;
     }
   }
   if (tid == 0) reached = found = 0;
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const SelectArgs a) {
     const int w = list / a.chunks;
     if (state[w] == 2) return list == w * a.chunks && i == 0 ? Choice{base[w], (int64_t)w * a.V + a.end} : none;
     if (state[w] == 0 || k == 0) return none;
-    return Choice{base[w] + (double)key_value(k), (int64_t)w * a.V + key_token(k)};
+    return Choice{base[w] + ((double)key_value(k) - (double)row_max[w]), (int64_t)w * a.V + key_token(k)};
   };
   auto entry = [&](int list, int i) __attribute__((always_inline)) {
     return choice(list, i, all[(int64_t)list * a.K + i]);

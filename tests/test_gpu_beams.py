@@ -328,3 +328,44 @@ def test_reorder_captured(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(t.cpu(), y) for t, y in zip(tensors, want)) and torch.equal(lengths.cpu(), lens)
+
+
+# ---------------------------------------------------------------- logits of any finite size
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("mask", [-1e4, -1e5, -1e9, -1e10, -1e20, -1e30, -1e37])
+def test_finite_masks_over_whole_pieces(device, dtype, wide, mask):
+    """A piece of a row is at most 16384 tokens from a multiple of them: masked whole at the start, in the middle, up to the end, all
+    but a few tokens, and a row of nothing else (where the sums of exp(x - max) are exact: all are 1)."""
+    requests, beams, vocab = (70, 4, 50000) if wide else (2, 4, 50000)
+    gen = torch.Generator().manual_seed(int(wide))
+    x, s = _logits(gen, requests, beams, vocab, dtype, device)
+    value = torch.tensor(mask, dtype=dtype)
+    x[0, 0, 16384:32768] = value
+    x[0, 1, :16384] = value
+    x[0, 2, 300:] = value
+    x[0, 3, :49990] = value
+    x[1] = value
+    if wide:
+        x[5:, :, 32768:] = value
+    got = _check(x, s, 6)
+    best = (s[0].double() + torch.log_softmax(x[0].double(), -1).amax(-1)).cpu().max()
+    assert (got.scores[0, 0].cpu().double() - best).abs() <= OFF + 2.0 ** -24 * best.abs()
+    first = int(s[1].argmax())  # of the row of nothing else: its best beam's first tokens
+    assert got.tokens[1].tolist() == list(range(6)) and got.rows[1].tolist() == [beams + first] * 6
+    assert torch.isfinite(got.scores).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("top", [1e3, 4095.0, 4097.0, -4095.0, -4097.0, 1e5, 1e6, -1e6, 1e7, -1e8, 1e9, -1e9, 1e20, -1e30])
+def test_rows_far_from_zero(device, dtype, wide, top):
+    """Logits around `top`, some of them equal to their neighbours by their type's spacing there."""
+    requests, beams, vocab = (70, 4, 20000) if wide else (2, 4, 20000)
+    gen = torch.Generator().manual_seed(3)
+    x, s = _logits(gen, requests, beams, vocab, torch.float32, device)
+    x = (x + top).to(dtype)
+    x[0, 1] = (x[0, 1].float() - 1e3).to(dtype)  # beams far from each other: their scores are not
+    got = _check(x, s, 8)
+    assert torch.isfinite(got.scores).all() and (got.scores <= 0).all()
