@@ -48,8 +48,8 @@ def select_beams(logits: Tensor, scores: Tensor, count: Optional[int] = None, *,
     Scores are compared in 64 bits and rounded once.  W up to 32, ``count`` up to 64.
     """
     if logits.is_cuda and logits.dim() == 3:
-        out = _capi.host().select(logits, scores, logits.shape[1] if count is None else count, finished, -1 if end_token is None else end_token,
-                                  P._stream(logits.device))
+        end = -1 if end_token is None else None if end_token == -1 else end_token  # (a given -1 is refused below)
+        out = _capi.host().select(logits, scores, logits.shape[1] if count is None else count, finished, end, P._stream(logits.device))
         if out is not None:
             return BeamSelection(*out)
     if logits.dim() != 3:

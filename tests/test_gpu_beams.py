@@ -369,3 +369,33 @@ def test_rows_far_from_zero(device, dtype, wide, top):
     x[0, 1] = (x[0, 1].float() - 1e3).to(dtype)  # beams far from each other: their scores are not
     got = _check(x, s, 8)
     assert torch.isfinite(got.scores).all() and (got.scores <= 0).all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_select_refusals(device, monkeypatch, native):
+    """The same calls, whether the native host calls are there or not."""
+    from mimir_amd import _capi
+
+    if not native:
+        monkeypatch.setattr(_capi, "_host", _capi._GeneralPath)
+    x, s = torch.zeros(2, 3, 20, device=device), torch.zeros(2, 3, device=device)
+    done = torch.zeros(2, 3, dtype=torch.bool, device=device)
+    for end in (-1, -2, 20, 1 << 40, -(1 << 40)):
+        with pytest.raises(ValueError, match="end_token"):
+            select_beams(x, s, end_token=end)
+        with pytest.raises(ValueError, match="end_token"):
+            select_beams(x, s, finished=done, end_token=end)
+    with pytest.raises(ValueError, match="end_token"):
+        select_beams(x, s, finished=done)
+    for count in (0, -1, 61, 65):
+        with pytest.raises(ValueError, match="count"):
+            select_beams(x, s, count)
+    with pytest.raises(ValueError, match="beams"):
+        select_beams(torch.zeros(1, 33, 20, device=device), torch.zeros(1, 33, device=device))
+    for scores in (s.double(), s[:1], s[:, :2], s.cpu()):
+        with pytest.raises(ValueError, match="scores"):
+            select_beams(x, scores)
+    for ended in (done.int(), done[:, :2], done.cpu()):
+        with pytest.raises(ValueError, match="finished"):
+            select_beams(x, s, finished=ended, end_token=0)
+    assert select_beams(x, s).finished is None and select_beams(x, s, end_token=0).finished.dtype == torch.bool
