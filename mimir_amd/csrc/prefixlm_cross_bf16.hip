@@ -37,24 +37,35 @@ struct PrologueArgs {
 
 // Tiles of one side, those with most rows on the other side first.
 __device__ __forceinline__ void plan_tiles(const SeqTable& t, bool by_key, int4* list, int cap) {
-  __shared__ int counts[kBuckets], most, total;
+  __shared__ int counts[kBuckets], most, all, total;
   __shared__ int4 span[kPlanThreads];
   __shared__ int slot[kPlanThreads];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  if (tid == 0) most = total = 0;
+  if (tid == 0) most = all = total = 0;
   for (int i = tid; i < kBuckets; i += kPlanThreads) counts[i] = 0;
   __syncthreads();
   auto at = [&](int s) __attribute__((always_inline)) {  // (own first, own rows, other first, other rows)
     const SeqSpan g = seq_span(t, s);
     return by_key ? make_int4(g.k0, g.nk, g.q0, g.nq) : make_int4(g.q0, g.nq, g.k0, g.nk);
   };
+  auto tiles = [](const int4& g) { return (g.y + kCrossTile - 1) / kCrossTile; };
+  // Sequences that do not overlap have no more tiles than the list has entries.  Lists that decrease may name any number:
+  // counted up to one more than the entries (host: below 2^24), where the sums below would wrap, and then none is listed.
+  const int over = cap + 1;
+  int own = 0;
   for (int s = tid; s < t.n; s += kPlanThreads) {
     const int4 g = at(s);
     if (g.y > 0) atomicMax(&most, g.w);
+    own = min(own + tiles(g), over);
   }
+  own = wave_inclusive_sum(own);
+  if (lane == 63) atomicAdd(&all, min(own, over));
   __syncthreads();
+  if (all > cap) {
+    for (int i = tid; i < cap; i += kPlanThreads) list[i] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const int step = most / kBuckets + 1;
-  auto tiles = [](const int4& g) { return (g.y + kCrossTile - 1) / kCrossTile; };
   auto bucket = [&](const int4& g) __attribute__((always_inline)) { return max(kBuckets - 1 - g.w / step, 0); };
   for (int s = tid; s < t.n; s += kPlanThreads) {
     const int4 g = at(s);
@@ -88,7 +99,7 @@ __device__ __forceinline__ void plan_tiles(const SeqTable& t, bool by_key, int4*
     for (int i = wave; i < min(t.n - s0, kPlanThreads); i += kPlanThreads / 64) {
       const int4 g = span[i];
       for (int j = lane; j < tiles(g); j += 64)
-        if (slot[i] + j < cap) list[slot[i] + j] = make_int4(g.x + j * kCrossTile, min(g.y - j * kCrossTile, kCrossTile), g.z, g.w);
+        list[slot[i] + j] = make_int4(g.x + j * kCrossTile, min(g.y - j * kCrossTile, kCrossTile), g.z, g.w);
     }
     __syncthreads();
   }

@@ -398,3 +398,38 @@ def test_states_refusals(device):
             attention_to_states(q, cache, lens, torch.tensor([0, 3], device=device))
     finally:
         set_validate_metadata(False)
+
+
+def test_lists_that_decrease_stay_in_their_workspace(device):
+    """Lists up and down name more tiles than 32 bits count (2^18 sequences of 2^20 rows, 8192 tiles each): nothing is listed,
+    nothing around the workspace is written, and calls after it are right."""
+    import ctypes
+
+    from mimir_amd import _capi
+
+    total, n = 1 << 20, (1 << 19) + 2
+    q = torch.zeros(total, 1, 64, dtype=torch.bfloat16, device=device)
+    k, v = (torch.randn(200, 1, 64, device=device).bfloat16() for _ in range(2))
+    up_down = torch.arange(n + 1, device=device) % 2
+    cu_q, cu_k = (total * up_down).int(), (200 * up_down).int()
+    out, lo = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.zeros(1, total, device=device)
+    p = _capi.CrossParams()
+    grads = [torch.zeros_like(t) for t in (q, k, v)]
+    for name, t in zip(("q", "k", "v", "out", "dout", "dq", "dk", "dv"), (q, k, v, out, q, *grads)):
+        setattr(p, name, t.data_ptr())
+        setattr(p, name + "_stride_token", 64)
+    p.out_lo, p.lse2, p.cu_seqlens_q, p.cu_seqlens_k = lo.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr()
+    p.total_q, p.total_k, p.numseqs, p.num_q_heads, p.num_kv_heads, p.head_dim = total, 200, n, 1, 1, 64
+    p.dtype, p.softmax_scale = _capi.DTYPE_BFLOAT16, 0.125
+    lib = _capi.load()
+    for backward, entry in ((0, lib.mimir_prefixlm_cross_fwd), (1, lib.mimir_prefixlm_cross_bwd)):
+        size = lib.mimir_prefixlm_cross_workspace_bytes(ctypes.byref(p), backward)
+        hold = torch.full((size + (1 << 21),), 0x5a, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = hold.data_ptr() + (1 << 20), size
+        _capi.raise_for_status(lib, entry(ctypes.byref(p), torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert (hold[:1 << 20] == 0x5a).all() and (hold[(1 << 20) + size:] == 0x5a).all()
+        assert not hold[1 << 20:(1 << 20) + 16 * (total // 128 + n)].any()  # the list of query tiles: nothing
+    assert not out.any()
+    _check(device, [(1100, 1500), (513, 2049)], 4, 4, 64)
