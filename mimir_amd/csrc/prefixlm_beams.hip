@@ -647,7 +647,8 @@ extern "C" int mimir_prefixlm_reorder_rows(const MimirReorderParams* p, void* st
   a.rows = p->rows; a.group = p->group; a.max_length = p->max_length;
   a.idx64 = p->index_int64 != 0; a.src64 = p->source_int64 != 0;
   const int64_t groups = p->rows / p->group, chunk_bytes = reorder_chunk(p->group), chunks = (row_bytes + chunk_bytes - 1) / chunk_bytes;
-  if (groups * chunks > kMaxGroups || chunks > 0x7fffffff) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many positions for one launch");
+  // workgroups of 256 threads, and for the lengths one of 64 a group
+  if (groups * chunks > kMaxGroups || chunks > 0x7fffffff || groups > 0xffffffffll / 64) return fail_with(MIMIR_ERR_UNSUPPORTED_SHAPE, "too many positions for one launch");
   a.chunks = (int)chunks;
   a.past = (int64_t)p->count * row_bytes >= kPastBytes / p->rows;
   const hipStream_t s = (hipStream_t)stream;

@@ -107,3 +107,11 @@ def test_structs_match_the_header():
         size, offsets = _c_layout(name, fields)
         assert ctypes.sizeof(cls) == size
         assert [getattr(cls, f).offset for f in fields] == offsets
+
+
+def test_c_reorder_launches_of_2_to_the_32_threads_are_refused():
+    """The lengths' launch has a wave for each group; without caches there is no other that would be too large."""
+    lib = _capi.load()
+    for kw in (dict(rows=1 << 26, group=1), dict(rows=1 << 30, group=16)):
+        with pytest.raises(ValueError, match="too many"):
+            _capi.raise_for_status(lib, lib.mimir_prefixlm_reorder_rows(ctypes.byref(_reorder((), (), update_lengths=1, max_length=0, **kw)), None))
