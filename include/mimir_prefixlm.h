@@ -632,7 +632,8 @@ const char* mimir_prefixlm_last_error(void);
 
 /* Cross attention over packed sequences: the queries of sequence s, rows cu_seqlens_q[s] up to
  * cu_seqlens_q[s + 1] of q, attend all of its states, rows cu_seqlens_k[s] up to cu_seqlens_k[s + 1] of k / v:
- * out = softmax(softmax_scale q k^T) v.  Both lists hold numseqs + 1 device int32, not decreasing.  A
+ * out = softmax(softmax_scale q k^T) v.  Both lists hold numseqs + 1 device int32, not decreasing and within the rows
+ * there are (others address nothing outside, but what is then written is not defined).  A
  * sequence without states gives O = 0, and rows before the first or behind the last sequence O = 0 and
  * zero gradients.  What the backward needs of the forward besides out (both may be NULL in a forward alone):
  * lse2, float32 [Hq, total_q], the base-2 logarithm of the softmax's sum, scale included, -inf without
@@ -696,7 +697,8 @@ int mimir_prefixlm_states_attn(const MimirStatesParams* params, void* stream);
 
 /* Beam search: of each request's W beams over a vocabulary of V tokens, the `count` best
  * continuations by scores[r, w] + log_softmax(logits[r, w])[token], ties to the lowest beam,
- * then token.  Log-probabilities and sums are compared in 64 bits, out_scores rounded once.
+ * then token.  Sums of exponentials are fp32 (a beam's scores are all off by the same, less than 2^-19: beams
+ * whose scores lie closer than twice that may change places), scores are formed and compared in 64 bits, out_scores rounded once.
  *
  * A beam with finished[r, w] != 0 goes on with end_token alone, at its score, and its logits are not
  * read.  A beam whose score is not finite, or whose logits hold NaN or +inf or nothing above -inf, has

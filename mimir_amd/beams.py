@@ -45,7 +45,8 @@ def select_beams(logits: Tensor, scores: Tensor, count: Optional[int] = None, *,
     in use, as all but the first at the first step).  A beam that is ``finished`` (bool [requests, W]) goes on with
     ``end_token`` alone, at its score, and its logits are not read.  Tokens with logit -inf are never chosen, nor is
     a beam whose logits hold NaN or +inf; where fewer than ``count`` continuations are left, the rest have score -inf.
-    Scores are compared in 64 bits and rounded once.  W up to 32, ``count`` up to 64.
+    Sums of exponentials are fp32, the rest is 64 bits and rounded once: a beam's scores are all off by the same,
+    less than 2^-19, so beams whose scores lie closer than twice that may change places.  Not differentiable.  W up to 32, ``count`` up to 64.
     """
     if logits.is_cuda and logits.dim() == 3:
         end = -1 if end_token is None else None if end_token == -1 else end_token  # (a given -1 is refused below)

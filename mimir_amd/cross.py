@@ -115,7 +115,8 @@ def cross_attention(query: Tensor, key: Tensor, value: Tensor, cu_seqlens_q: Ten
 
     Returns [total_q, Hq, D], with gradients for query, key and value.  A sequence may have no queries or no states
     (its output is then 0); rows before the first or behind the last sequence give 0 and get zero gradients.  Both lists
-    (int32 or int64 [numseqs + 1]) must not decrease (checked with ``mimir_amd.set_validate_metadata(True)``).  ``softmax_scale``
+    (int32 or int64 [numseqs + 1]) must not decrease and stay within the rows there are (checked with
+    ``mimir_amd.set_validate_metadata(True)``).  The backward computes all three gradients, whichever are needed.  ``softmax_scale``
     is positive, 1 / sqrt(D) by default.  P and dS are rounded to bf16 for their products, sums are fp32; results do not
     depend on timing.  For the backward the output's low half is kept (bf16, as large as the output): the sums
     rowsum(dO * O) that dS is the difference to would carry the output's rounding without it.

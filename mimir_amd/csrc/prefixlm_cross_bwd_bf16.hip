@@ -8,7 +8,9 @@
 // delta takes O with its low half: dS is a difference whose rounding errors would else be led by O's
 // (error of dQ and dK against 64 bits, in units of one rounding of the exact result: up to 2.3 without, 1.4 with it).
 // P and dS are rounded to bf16 for their products.  Both are bound by the matrix units: 8 sequences of 1500 to 2048 queries over
-// 1024 to 2048 states, 16 / 4 heads of 128, dQ 279 us (0.94 PFLOP/s executed), dK / dV 402 (0.87, a fifth of it the tail).
+// 1024 to 2048 states, 16 / 4 heads of 128, dQ 270 to 290 us (0.94 PFLOP/s executed at 279), dK / dV 375 to 410 (0.87 at 402, a fifth of it the tail).
+// No tile is split over workgroups, so few tiles leave the chip idle: forward and backward of 4096 queries over 77 states (one tile of
+// states, 16 / 4 heads) take 402 us, of 16 queries over 8192 states 340.
 #include "prefixlm_cross.h"
 
 namespace mimir {

@@ -11,7 +11,8 @@
 // the parts of the others go to the workspace and states_merge_kernel adds them in order.  48 requests of 8 beams over 300 to
 // 4096 states, 16 / 4 heads of 128: 48.9 us (4.4 TB/s) and 6.5; one request of 1500 states 7.3 and 5.4, round trips.
 //
-// Requests of more than 128 rows go to the tile kernel of prefixlm_cross_bf16.hip instead.
+// Requests of more than 128 rows go to the tile kernel of prefixlm_cross_bf16.hip instead, whatever their number: it splits no
+// states and reads them once for each query head (one request of 16384 states, 64 / 8 heads of 128: 128 rows 38 us, 256 rows 281).
 #include <algorithm>
 
 #include "prefixlm_cross.h"
@@ -98,7 +99,7 @@ __device__ __forceinline__ void states_body(const StatesArgs& a) {
   constexpr int DT = D / 32, KS = D / 16;
   // P enters its product as two bf16 halves where one row tile takes part, which leaves the matrix units idle: error
   // against 64 bits 0.0021 -> 0.0017 of the output, one rounding's, at 54.4 us where 54.2 were spent (48 requests of 300 to 4096
-  // states, 32 rows).  Two row tiles: 107 us where 99 were spent, so P is rounded to bf16 there.
+  // states, 32 rows).  Two row tiles (96 rows): 107 us where 99 were spent, so P is rounded to bf16 there.
   constexpr bool kSplit = NT == 1;
   using L = TileLayout<D>;
   constexpr int kInst = (kTile * L::kRowUnits + 63) / 64;  // wave copy instructions per tile
@@ -409,8 +410,9 @@ template __global__ void states_merge_kernel<64>(const StatesArgs, int);
 template __global__ void states_merge_kernel<128>(const StatesArgs, int);
 
 // States of a launch that read past the caches where one row tile reads them, once: more than the 256 MiB in front of
-// memory cannot be found there by the next step.  48 requests of 300 to 4096 states, 4 kv heads of 128, other states each
-// time: 60.2 us with the caches, 54.2 past them (the same states each time: 48.9 and 53.9).  Two row tiles: 99 and 108.
+// memory cannot be found there by the next step.  It goes by the positions there are, as the lengths are on the device, so that
+// large rows with little in them lose what the caches would hold.  48 requests of 300 to 4096 states, 4 kv heads of 128, other states each
+// time: 60.2 us with the caches, 54.2 past them (the same states each time: 48.9 and 53.9).  Two row tiles (96 rows): 99 and 108.
 constexpr int64_t kOnceBytes = (int64_t)256 << 20;
 constexpr int kManyRows = 128;  // more rows per kv head than this: the tile kernel
 struct StatesPlan {
