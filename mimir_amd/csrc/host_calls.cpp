@@ -865,8 +865,16 @@ struct NormRotaryFunction : torch::autograd::Function<NormRotaryFunction> {
     const NormRotary r = {saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["amplitude"].toDouble(),
                           ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
     torch::autograd::variable_list out(10);
-    auto unit = [](const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); };
-    const at::Tensor dq = unit(grads[0]), dk = r.k.defined() ? unit(grads[1]) : at::Tensor();
+    // A head takes at most 64 lanes of 2 accesses, so past 128 columns they must be wide: a gradient, whose layout is
+    // not the caller's choice, is copied where its rows do not allow that.
+    auto laid = [](const at::Tensor& t) {
+      int64_t columns = 1;
+      while (t.size(-1) > 128 * columns) columns *= 2;
+      bool fits = t.stride(-1) == 1 && (uintptr_t)t.const_data_ptr() % (columns * t.element_size()) == 0;
+      for (int64_t i = 0; i < t.dim() - 1; ++i) fits = fits && t.stride(i) % columns == 0;
+      return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+    };
+    const at::Tensor dq = laid(grads[0]), dk = r.k.defined() ? laid(grads[1]) : at::Tensor();
     out[0] = like(r.q), out[1] = like(r.k);
     size_t edge = r.k.defined() ? 2 : 1;  // an argument that is not given has none
     for (int i = 0; i < 2; ++i) {

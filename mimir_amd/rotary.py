@@ -274,6 +274,19 @@ def _norm_forward(query, key, positions, frequencies, query_weight, key_weight, 
     return out
 
 
+def _gradient(t: Optional[Tensor]) -> Optional[Tensor]:
+    """A head takes at most 64 lanes of 2 accesses, so past 128 columns they must be wide: a gradient, whose layout
+    is not the caller's choice, is copied where its rows do not allow that."""
+    if t is None:
+        return None
+    columns = 1
+    while t.shape[-1] > 128 * columns:
+        columns *= 2
+    if t.stride(-1) != 1 or t.data_ptr() % (columns * t.element_size()) or any(s % columns for s in t.stride()[:-1]):
+        t = P._own_copy(t)
+    return t
+
+
 class _NormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, query_weight, key_weight, positions, turns, amplitude, interleaved, eps):
@@ -286,7 +299,8 @@ class _NormRotary(torch.autograd.Function):
     def backward(ctx, dquery, dkey):
         query, key, query_weight, key_weight, positions, turns = ctx.saved_tensors
         amplitude, interleaved, eps = ctx.meta
-        query, key, dquery, dkey = map(_unit, (query, key, dquery, dkey if key is not None else None))
+        query, key = _unit(query), _unit(key)
+        dquery, dkey = _gradient(dquery), _gradient(dkey if key is not None else None)
         out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key))
         p = _norm_params(query, key, positions, RotaryFrequencies(turns, amplitude, interleaved), query_weight, key_weight, eps,
                          out, (dquery, dkey))

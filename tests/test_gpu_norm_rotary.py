@@ -202,3 +202,29 @@ def test_misaligned_heads_past_the_lanes_are_refused(device):
     x = torch.randn(4, 2, 256, device=device, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="columns at a time"):
         norm_rotary(x, None, torch.arange(4, device=device), RotaryFrequencies.create(2, device=device))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 256), (torch.bfloat16, 640), (torch.float32, 256), (torch.float32, 512), (torch.bfloat16, 128)])
+def test_gradients_off_their_alignment(device, monkeypatch, native, dtype, d):
+    """A forward that ran has a backward, whatever the layout of the gradients that come."""
+    from mimir_amd import _capi
+
+    if not native:
+        monkeypatch.setattr(_capi, "_host", _capi._GeneralPath)
+    gen = torch.Generator(device=device).manual_seed(d)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=device).to(dtype)  # noqa: E731
+    leaves = [rand(7, 3, d).requires_grad_(True), rand(7, 1, d).requires_grad_(True), rand(d).requires_grad_(True)]
+    table, pos = RotaryFrequencies.create(d, device=device), torch.arange(7, device=device)
+    out = norm_rotary(leaves[0], leaves[1], pos, table, leaves[2], leaves[2])
+    dout = [rand(*y.shape) for y in out]
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    odd = [torch.zeros(1 + 7 * (y.shape[1] * d + 3), dtype=dtype, device=device)[1:].view(7, -1)[:, :y.shape[1] * d].view(y.shape) for y in out]
+    fine = [torch.zeros(7, d, y.shape[1], dtype=dtype, device=device).transpose(1, 2) for y in out]  # no unit stride
+    # Past 128 columns the copies are read as the aligned gradients were.  Up to there they are read by other accesses, whose sums
+    # add in another order: 2^-18 of sizes below 16 either way, and each rounded once, to neighbours 2^-7 apart at most.
+    for views in (odd, fine):
+        for view, g in zip(views, dout):
+            view.copy_(g)
+        got = torch.autograd.grad(out, leaves, views, retain_graph=True)
+        assert all(torch.equal(a, b) if d > 128 else torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -13) for a, b in zip(got, want))
