@@ -871,7 +871,7 @@ struct NormRotaryFunction : torch::autograd::Function<NormRotaryFunction> {
       int64_t columns = 1;
       while (t.size(-1) > 128 * columns) columns *= 2;
       bool fits = t.stride(-1) == 1 && (uintptr_t)t.const_data_ptr() % (columns * t.element_size()) == 0;
-      for (int64_t i = 0; i < t.dim() - 1; ++i) fits = fits && t.stride(i) % columns == 0;
+      for (int64_t i = 0; i < t.dim() - 1; ++i) fits = fits && (t.size(i) == 1 || t.stride(i) % columns == 0);
       return fits ? t : t.clone(at::MemoryFormat::Contiguous);
     };
     const at::Tensor dq = laid(grads[0]), dk = r.k.defined() ? laid(grads[1]) : at::Tensor();

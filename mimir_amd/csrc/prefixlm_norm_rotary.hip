@@ -389,9 +389,20 @@ int access_columns(const MimirNormRotaryParams& p, bool bwd) {
 // Workgroups of the gradient: each group of lanes walks its share of the tokens.
 int64_t bwd_blocks(int64_t groups, int lanes) { return std::min<int64_t>((groups * lanes + 255) / 256, kMaxBlocks); }
 
-int run_norm_rotary(const MimirNormRotaryParams* p, bool bwd, void* stream) {
+int run_norm_rotary(const MimirNormRotaryParams* given, bool bwd, void* stream) {
   fail_with(MIMIR_OK, "");
-  if (p == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (given == nullptr) return fail_with(MIMIR_ERR_INVALID_ARGUMENT, "params is NULL");
+  // A dim of one entry has a stride, but no step: none that would keep accesses narrow.
+  MimirNormRotaryParams own = *given;
+  for (int64_t* s : {&own.q_stride_batch, &own.k_stride_batch, &own.q_out_stride_batch, &own.k_out_stride_batch, &own.dq_stride_batch, &own.dk_stride_batch})
+    if (own.batch == 1) *s = 0;
+  for (int64_t* s : {&own.q_stride_token, &own.k_stride_token, &own.q_out_stride_token, &own.k_out_stride_token, &own.dq_stride_token, &own.dk_stride_token})
+    if (own.seqlen == 1) *s = 0;
+  for (int64_t* s : {&own.q_stride_head, &own.q_out_stride_head, &own.dq_stride_head})
+    if (own.num_q_heads == 1) *s = 0;
+  for (int64_t* s : {&own.k_stride_head, &own.k_out_stride_head, &own.dk_stride_head})
+    if (own.num_kv_heads == 1) *s = 0;
+  const MimirNormRotaryParams* const p = &own;
   if (p->dtype != MIMIR_DTYPE_FLOAT32 && p->dtype != MIMIR_DTYPE_BFLOAT16)
     return fail_with(MIMIR_ERR_UNSUPPORTED_DTYPE, "normed rotary heads support float32 and bfloat16 tensors only (dtype code " +
                                                       std::to_string(p->dtype) + ")");

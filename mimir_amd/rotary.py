@@ -282,7 +282,8 @@ def _gradient(t: Optional[Tensor]) -> Optional[Tensor]:
     columns = 1
     while t.shape[-1] > 128 * columns:
         columns *= 2
-    if t.stride(-1) != 1 or t.data_ptr() % (columns * t.element_size()) or any(s % columns for s in t.stride()[:-1]):
+    if t.stride(-1) != 1 or t.data_ptr() % (columns * t.element_size()) or any(
+            n > 1 and s % columns for n, s in zip(t.shape[:-1], t.stride())):
         t = P._own_copy(t)
     return t
 

@@ -228,3 +228,21 @@ def test_gradients_off_their_alignment(device, monkeypatch, native, dtype, d):
             view.copy_(g)
         got = torch.autograd.grad(out, leaves, views, retain_graph=True)
         assert all(torch.equal(a, b) if d > 128 else torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -13) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_of_one_entry(device, dtype):
+    """[tokens, D, 1] transposed, and any stride for a dim of one entry: read as if it were contiguous."""
+    gen = torch.Generator(device=device).manual_seed(2)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=device).to(dtype)  # noqa: E731
+    table = RotaryFrequencies.create(256, device=device)
+    for tokens, strides in ((5, (256, 1, 1)), (5, (264, 3, 1)), (1, (1, 7, 1))):
+        q, k, dq, dk = (rand(tokens, 1, 256) for _ in range(4))
+        odd = [torch.zeros(1 << 12, dtype=dtype, device=device).as_strided(q.shape, strides).copy_(t) for t in (q, k, dq, dk)]
+        pos = torch.arange(tokens, device=device)
+        results = []
+        for a, b, da, db in ((q, k, dq, dk), odd):
+            leaves = [a.detach().requires_grad_(True), b.detach().requires_grad_(True)]
+            out = norm_rotary(*leaves, pos, table)
+            results.append([*out, *torch.autograd.grad(out, leaves, (da, db))])
+        assert all(torch.equal(x, y) for x, y in zip(*results))

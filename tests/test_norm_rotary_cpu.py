@@ -86,3 +86,25 @@ def test_struct_matches_the_header():
     size, offsets = _c_layout("MimirNormRotaryParams", fields)
     assert ctypes.sizeof(_capi.NormRotaryParams) == size
     assert [getattr(_capi.NormRotaryParams, f).offset for f in fields] == offsets
+
+
+def _status(p, bwd):
+    lib = _capi.load()
+    entry = lib.mimir_prefixlm_norm_rotary_bwd if bwd else lib.mimir_prefixlm_norm_rotary
+    return entry(ctypes.byref(p), None), lib.mimir_prefixlm_last_error().decode()
+
+
+@pytest.mark.parametrize("bwd", [False, True])
+@pytest.mark.parametrize("kw", [dict(q_stride_head=1), dict(q_stride_batch=3), dict(q_stride_token=1, q_out_stride_batch=1, q_out_stride_head=3),
+                                dict(dq_stride_token=5, dq_stride_head=1), dict(seqlen=1, k_stride_head=1, dk_stride_batch=1, num_kv_heads=1)])
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what is not refused would be launched, on addresses that are none")
+def test_strides_of_one_entry_refuse_nothing(kw, bwd):
+    """256 columns need accesses of two: strides of dims of one entry (here all) do not stand in their way.  Past all
+    refusals there is no device here."""
+    at = dict(head_dim=256, rotary_dim=256, q=1 << 20, q_out=2 << 20, dq=3 << 20, k=4 << 20, k_out=5 << 20, dk=6 << 20)
+    for t in ("q", "q_out", "dq", "k", "k_out", "dk"):
+        at[t + "_stride_token"] = at[t + "_stride_head"] = at[t + "_stride_batch"] = 256
+    status, message = _status(_params(**{**at, **kw}), bwd)
+    assert "columns at a time" not in message and status == _capi.ERR_HIP
+    status, message = _status(_params(**{**at, **kw, "num_q_heads": 2, "q_stride_head": 257}), bwd)
+    assert "columns at a time" in message
