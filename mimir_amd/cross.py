@@ -26,6 +26,16 @@ from . import prefixlm as P
 from .cache import Cache
 
 
+_MAX_STRIDE = 1 << 22  # elements: the kernels address a tile's 128 rows in 31 bits
+
+
+def _rows(t: Tensor) -> Tensor:
+    """Rows of tokens as the kernels read them; copied where they lie otherwise, or too far apart (the last tokens of long
+    sequences, one of each)."""
+    t = P._kernel_layout(t)
+    return t if t.stride(0) < _MAX_STRIDE else P._own_copy(t)
+
+
 def _scale(softmax_scale: Optional[float], d: int) -> float:
     return 1.0 / math.sqrt(max(d, 1)) if softmax_scale is None else float(softmax_scale)
 
@@ -71,7 +81,7 @@ def _launch(entry: str, p, backward: bool, device) -> None:
 
 
 def _forward(query, key, value, cu_q, cu_k, scale, keep: bool):
-    query, key, value = map(P._kernel_layout, (query, key, value))
+    query, key, value = map(_rows, (query, key, value))
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     out_lo = torch.empty_like(out) if keep else None
     lse2 = torch.empty((query.shape[1], query.shape[0]), dtype=torch.float32, device=query.device) if keep else None
@@ -91,7 +101,7 @@ class _CrossAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         query, key, value, out, out_lo, lse2, cu_q, cu_k = ctx.saved_tensors
-        query, key, value, dout = map(P._kernel_layout, (query, key, value, dout))
+        query, key, value, dout = map(_rows, (query, key, value, dout))
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (query, key, value)]
         _launch("mimir_prefixlm_cross_bwd", _params(query, key, value, out, out_lo, lse2, cu_q, cu_k, ctx.scale, (dout, *grads)), True,
                 query.device)
@@ -184,8 +194,9 @@ def attention_to_states(query: Tensor, states: Cache, state_lengths: Tensor, sta
     if B == 0 or S == 0:
         return out
     # all tokens of a request in a row: [B * S, Hq, D], a token's heads no nearer than the head_dim (one expanded to many is copied)
+    # and no further than the kernels reach
     token = query.stride(1 if S > 1 else 0)
-    if query.stride(-1) != 1 or query.data_ptr() % 16 or (B > 1 and S > 1 and query.stride(0) != S * token) or (B * S > 1 and token < d) or any(
+    if query.stride(-1) != 1 or query.data_ptr() % 16 or (B > 1 and S > 1 and query.stride(0) != S * token) or (B * S > 1 and not d <= token < _MAX_STRIDE) or any(
             query.shape[i] > 1 and query.stride(i) % 8 for i in range(3)):
         query = P._own_copy(query)
     state_lengths = state_lengths.contiguous()

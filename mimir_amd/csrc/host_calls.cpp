@@ -978,7 +978,8 @@ struct CrossFunction : torch::autograd::Function<CrossFunction> {
     const auto t = ctx->get_saved_variables();
     const at::Tensor &q = t[0], &k = t[1], &v = t[2];
     at::Tensor dout = grads[0];
-    if (!in_place(dout, q)) dout = dout.clone(at::MemoryFormat::Contiguous);
+    // (as cross.py: rows further apart than 2^22 elements are more than the kernels reach)
+    if (!in_place(dout, q) || dout.stride(0) >= (1 << 22)) dout = dout.clone(at::MemoryFormat::Contiguous);
     const at::Tensor dq = like(q), dk = like(k), dv = like(v);
     MimirCrossParams p = cross_params(q, k, v, t[3], t[4], ctx->saved_data["scale"].toDouble(), t[5]);
     p.out_lo = t[6].mutable_data_ptr(), p.lse2 = t[7].mutable_data_ptr<float>();

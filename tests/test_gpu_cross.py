@@ -433,3 +433,33 @@ def test_lists_that_decrease_stay_in_their_workspace(device):
         assert not hold[1 << 20:(1 << 20) + 16 * (total // 128 + n)].any()  # the list of query tiles: nothing
     assert not out.any()
     _check(device, [(1100, 1500), (513, 2049)], 4, 4, 64)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_rows_far_apart(device, monkeypatch, native):
+    """The last tokens of sequences of 2^22 elements and more, one of each: queries, states and gradients 2^22 apart and further."""
+    from mimir_amd import _capi
+
+    if not native:
+        monkeypatch.setattr(_capi, "_host", _capi._GeneralPath)
+    gen = torch.Generator().manual_seed(8)
+    hold = torch.zeros(4, 2 << 22, dtype=torch.bfloat16, device=device)
+
+    def far(n, heads, step):
+        t = hold.as_strided((n, heads, 64), (step, 64, 1), 64 * far.used)
+        far.used += heads
+        return t.copy_(torch.randn(n, heads, 64, generator=gen).bfloat16())
+
+    for step, n in ((1 << 22, 5), ((1 << 22) + 64, 5), (1 << 23, 1)):
+        far.used = 0
+        q, k, v, do = (far(n, h, step).detach().requires_grad_(True) for h in (4, 2, 2, 4))
+        near = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True) for t in (q, k, v, do)]
+        cu = torch.tensor([0, n // 2, n], dtype=torch.int32, device=device)
+        results = []
+        for leaves in ((q, k, v, do), near, (*near[:3], do)):
+            out = cross_attention(*leaves[:3], cu, cu)
+            results.append([out, *torch.autograd.grad(out, leaves[:3], leaves[3])])
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*results))
+        states = Cache(torch.randn(n, 40, 2, 64, device=device).bfloat16(), torch.randn(n, 40, 2, 64, device=device).bfloat16())
+        lens = torch.full((n,), 33, device=device)
+        assert torch.equal(*(attention_to_states(t.detach()[:, None], states, lens) for t in (q, near[0])))
